@@ -321,6 +321,52 @@ int w4a16_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, 
 int w4a16_moe_silu_split(const float* y, int64_t ldy, const int32_t* inv_pos, int64_t T, int top_k, int64_t inter,
                          int dtype, uint8_t* a_fp8, int64_t lda, float* a_scales, void* h, int64_t ldh, void* stream);
 
+/* ---- A paged cache of keys and values in 4 bits, and attention over it. No counterpart in the reference, whose
+ * cache holds 16 or 8 bits.
+ *
+ * A vector of one token and key/value head is D codes (D = 64, 128 or 256) with a step s and a least value m in the
+ * model's type (bf16 or fp16), and stands for s * code + m:
+ *   m = min x, s = max((max x - min x) / 15, 2^-14 max |x|) rounded to the type and at least its smallest positive
+ *   value (2^-24 for fp16, 2^-126 for bf16), code = clamp(rint((x - m) / s), 0, 15), in f32.
+ * A vector with an infinity or a NaN in it is stored as s = m = NaN.
+ * The cache's arrays, contiguous, for pages of page_size tokens (a power of two, 16 to 65536):
+ *   k_codes (pages, H, page_size, D/2) bytes, code d in nibble d % 8 of the row's 32-bit word d / 8;
+ *   v_codes (pages, H, page_size/8, D) 32-bit words, nibble j the code of token 8 i + j;
+ *   k_scale, v_scale (pages, H, page_size, 2): s and m.
+ * Which tokens: sequence b of B has seq_lens[b] tokens on pages table[b * ldt + i], i < width; its last cu[b+1] - cu[b]
+ * ones are rows cu[b] .. cu[b+1]-1 of the call's T. cu (B + 1, ascending), seq_lens and table are read on the device,
+ * so a captured call replays with new ones. Rows outside cu[0] .. cu[B]-1 are left as they are. A table entry outside
+ * 0 .. pages-1, or a token past the table's width, is no fault: nothing is written for it, and what would read it is
+ * NaN. */
+
+/* Quantizes rows of k and v (T, H, D) (ldk, hk: elements between tokens and heads; multiples of 8) into the cache. V's words
+ * hold 8 tokens: the 8 tokens of a block are one sequence's (pages are not shared where tokens are still added). */
+int w4a8_kv4_append(const void* k, int64_t ldk, int64_t hk, const void* v, int64_t ldv, int64_t hv, int dtype, int64_t T,
+                    int64_t H, int64_t D, void* k_codes, void* v_codes, void* k_scale, void* v_scale, int64_t pages,
+                    int64_t page_size, const int32_t* table, int64_t ldt, int64_t width, const int32_t* cu,
+                    const int32_t* seq_lens, int64_t B, void* stream);
+
+/* The values that the cache holds for these rows, rounded to the type, into k and v (T, H, D), contiguous. */
+int w4a8_kv4_read(const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, int dtype,
+                  int64_t pages, int64_t page_size, int64_t H, int64_t D, const int32_t* table, int64_t ldt, int64_t width,
+                  const int32_t* cu, const int32_t* seq_lens, int64_t B, int64_t T, void* k, void* v, void* stream);
+
+/* Bytes of w4a8_kv4_attention's workspace for a call of these sizes (0: none is needed); -1 on bad sizes. */
+int64_t w4a8_kv4_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t B, int64_t max_q,
+                                           int64_t max_kv);
+
+/* out[i] = softmax over the keys that row i sees of (scale q k), times v: q, out (T, Hq, D) with strides, Hq a
+ * multiple of H (query head h reads key/value head h / (Hq/H)). causal: row i, at position pos, sees keys up to pos
+ * (else all of its sequence's); window > 0: only those after pos - window. A row that sees none is 0, its lse -inf.
+ * lse: (T, Hq) f32, the natural logarithm of the sum of exp(scale q k), or null. max_q and max_kv bound the new tokens
+ * and the length of a sequence: they size the grid and the workspace, and a bound that is too low costs time only. */
+int w4a8_kv4_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_t T, int64_t Hq, int64_t H, int64_t D,
+                       const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, int64_t pages,
+                       int64_t page_size, const int32_t* table, int64_t ldt, int64_t width, const int32_t* cu,
+                       const int32_t* seq_lens, int64_t B, float scale, int causal, int64_t window, int64_t max_q,
+                       int64_t max_kv, void* out, int64_t ldo, int64_t ho, float* lse, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

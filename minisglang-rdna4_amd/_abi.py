@@ -80,6 +80,14 @@ SIGNATURES = {
                               _vp, _c_i64, _c_int, _vp, _c_i64, _c_int, _vp]),
     "w4a16_moe_silu_split": (_c_int, [_vp, _c_i64, _vp, _c_i64, _c_int, _c_i64, _c_int, _vp, _c_i64, _vp, _vp,
                                       _c_i64, _vp]),
+    "w4a8_kv4_append": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_int, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp,
+                                 _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp]),
+    "w4a8_kv4_read": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp,
+                               _c_i64, _c_i64, _vp, _vp, _vp]),
+    "w4a8_kv4_attention_workspace_bytes": (_c_i64, [_c_i64] * 7),
+    "w4a8_kv4_attention": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _vp,
+                                    _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, ctypes.c_float, _c_int,
+                                    _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp]),
 }
 
 _lock = threading.Lock()
