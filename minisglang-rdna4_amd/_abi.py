@@ -80,6 +80,9 @@ SIGNATURES = {
                               _vp, _c_i64, _c_int, _vp, _c_i64, _c_int, _vp]),
     "w4a16_moe_silu_split": (_c_int, [_vp, _c_i64, _vp, _c_i64, _c_int, _c_i64, _c_int, _vp, _c_i64, _vp, _vp,
                                       _c_i64, _vp]),
+    "w4a8_lora_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_int]),
+    "w4a8_lora_add": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _vp, _c_int, _vp, _vp,
+                               _c_int, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp]),
     "w4a8_kv4_append": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_int, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp,
                                  _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp]),
     "w4a8_kv4_read": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp,

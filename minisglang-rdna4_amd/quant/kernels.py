@@ -304,13 +304,27 @@ def _dense_prep(x, w_packed, scales, w_zeros, group_size, weight_is_e2m1, what):
     return M, K, N, sfmt, w_zeros, scales
 
 
-def _dense(x, w_packed, scales, w_zeros, group_size, weight_is_e2m1, x_fp8, act_scales, silu, arm):
+def _dense_arm(x, w_packed, group_size, kernel, weight_is_e2m1, x_fp8):
+    """(the C ABI's kernel choice, the arm's name) for a dense call's ``kernel`` argument."""
+    if kernel is None:
+        kernel = _pick_dense_kernel(x.shape[0], weight_is_e2m1, group_size, k=x.shape[-1], n=_n_of(w_packed))
+    if kernel == "decode_gemv":
+        return _abi.KERNEL_DECODE, kernel
+    if kernel not in _PREFILL_NAMES and kernel not in _IN_PROLOGUE_NAMES:
+        raise ValueError(f"w4a8_linear: unknown kernel {kernel!r}")
+    if kernel in _IN_PROLOGUE_NAMES and x_fp8 is not None:
+        raise RuntimeError(f"w4a8_linear: kernel={kernel} quantizes activations in-prologue and refuses a "
+                           f"pre-quantized (x_fp8, act_scales) pair")
+    return _abi.KERNEL_PREFILL, kernel
+
+
+def _dense(x, w_packed, scales, w_zeros, group_size, weight_is_e2m1, x_fp8, act_scales, silu, arm, out_dtype=None):
     what = "w4a8_linear_silu" if silu else "w4a8_linear"
     M, K, N, sfmt, w_zeros, scales = _dense_prep(x, w_packed, scales, w_zeros, group_size, weight_is_e2m1, what)
     xq, xs = _check_producer_pair(x, x_fp8, act_scales, what)
     tiles = _as_tiles(w_packed, K, weight_is_e2m1, 2, what)
     nout = N // 2 if silu else N
-    out = torch.empty((M, nout), dtype=x.dtype, device=x.device)
+    out = torch.empty((M, nout), dtype=out_dtype or x.dtype, device=x.device)
     lib = _abi.load()
     zeros = _abi.ptr(w_zeros.contiguous() if w_zeros is not None else None)
     wfmt = _abi.W_E2M1 if weight_is_e2m1 else _abi.W_INT4
@@ -324,7 +338,7 @@ def _dense(x, w_packed, scales, w_zeros, group_size, weight_is_e2m1, x_fp8, act_
         ws = torch.empty((max(ws_bytes, 1),), dtype=torch.uint8, device=x.device)
         _abi.check(
             lib.w4a8_linear(_abi.ptr(x), _abi.dtype_code(x.dtype), M, K, K, _abi.ptr(tiles), N, _abi.ptr(sc),
-                            sfmt, zeros, wfmt, group_size, _abi.ptr(out), _abi.dtype_code(x.dtype), nout, int(silu),
+                            sfmt, zeros, wfmt, group_size, _abi.ptr(out), _abi.dtype_code(out.dtype), nout, int(silu),
                             _abi.ptr(ws), ws_bytes, arm, _abi.stream_of(x)),
             what,
         )
@@ -334,7 +348,7 @@ def _dense(x, w_packed, scales, w_zeros, group_size, weight_is_e2m1, x_fp8, act_
         ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=x.device) if ws_bytes > 0 else None
         _abi.check(
             lib.w4a8_gemm(_abi.ptr(xq), K, _abi.ptr(xs), M, _abi.ptr(tiles), N, K, _abi.ptr(sc), sfmt, zeros, wfmt,
-                          group_size, _abi.ptr(out), _abi.dtype_code(x.dtype), nout, int(silu), _abi.ptr(ws),
+                          group_size, _abi.ptr(out), _abi.dtype_code(out.dtype), nout, int(silu), _abi.ptr(ws),
                           max(ws_bytes, 0), arm, _abi.stream_of(x)),
             what,
         )
@@ -362,19 +376,7 @@ def w4a8_linear(
         if r is not None:
             engaged(_LINEAR_LEDGER[r[1], bool(weight_is_e2m1), x_fp8 is not None])
             return r[0]
-    N = _n_of(w_packed)
-    K = x.shape[-1]
-    if kernel is None:
-        kernel = _pick_dense_kernel(x.shape[0], weight_is_e2m1, group_size, k=K, n=N)
-    if kernel == "decode_gemv":
-        arm = _abi.KERNEL_DECODE
-    elif kernel in _PREFILL_NAMES or kernel in _IN_PROLOGUE_NAMES:
-        if kernel in _IN_PROLOGUE_NAMES and x_fp8 is not None:
-            raise RuntimeError(f"w4a8_linear: kernel={kernel} quantizes activations in-prologue and refuses a "
-                               f"pre-quantized (x_fp8, act_scales) pair")
-        arm = _abi.KERNEL_PREFILL
-    else:
-        raise ValueError(f"w4a8_linear: unknown kernel {kernel!r}")
+    arm, kernel = _dense_arm(x, w_packed, group_size, kernel, weight_is_e2m1, x_fp8)
     out, repacked = _dense(x, w_packed, scales, w_zeros, group_size, weight_is_e2m1, x_fp8, act_scales, False, arm)
     engaged(f"w4a8_mi355x.gemm({kernel}{'+e2m1' if weight_is_e2m1 else ''}"
             f"{'+prequant' if x_fp8 is not None else ''}{'+repack' if repacked else ''})")

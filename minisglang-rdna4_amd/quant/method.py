@@ -25,6 +25,7 @@ import torch
 import torch.nn.functional as F
 
 from . import kernels
+from . import lora as _lora
 from .config import QuantConfig
 
 
@@ -130,13 +131,17 @@ def apply_ct_sign(t: torch.Tensor, conv: CtSignConvention) -> torch.Tensor:
 # ------------------------------------------------------------------------------------------------
 # methods
 # ------------------------------------------------------------------------------------------------
+# the low-rank adapters of a batch: a projection's adapters and each row's, (M,) int32
+LoraBatch = tuple[_lora.LoraAdapters, torch.Tensor]
+
+
 class LinearMethod(Protocol):
     """How a linear layer allocates its weights and computes its matmul
-    (python/minisgl/quant/method.py:352-364)."""
+    (python/minisgl/quant/method.py:352-364). ``lora``: adds each row's low-rank adapter."""
 
     def create_weights(self, layer, out_features: int, in_features: int) -> None: ...
 
-    def apply(self, layer, x: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor: ...
+    def apply(self, layer, x: torch.Tensor, bias: torch.Tensor | None, *, lora: LoraBatch | None = None) -> torch.Tensor: ...
 
 
 class UnquantizedLinearMethod:
@@ -145,8 +150,20 @@ class UnquantizedLinearMethod:
     def create_weights(self, layer, out_features: int, in_features: int) -> None:
         layer.weight = torch.empty(out_features, in_features)
 
-    def apply(self, layer, x: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor:
-        return F.linear(x, layer.weight, bias)
+    def apply(self, layer, x: torch.Tensor, bias: torch.Tensor | None, *, lora: LoraBatch | None = None) -> torch.Tensor:
+        out = F.linear(x, layer.weight, bias)
+        return out if lora is None else _lora.lora_add(out, x, *lora)
+
+
+def _quantized_apply(x, w, scales, zeros, group_size, e2m1, x_fp8, act_scales, lora) -> torch.Tensor:
+    """The quantized linear of the W4A16 arm where it is on, else W4A8, with a batch's adapters."""
+    if _w4a16():
+        out = kernels.w4a16_linear(x, w, scales, zeros, group_size, kernels._n_of(w), weight_is_e2m1=e2m1)
+        return out if lora is None else _lora.lora_add(out, x, *lora)
+    if lora is None:
+        return kernels.w4a8_linear(x, w, scales, zeros, group_size, weight_is_e2m1=e2m1, x_fp8=x_fp8, act_scales=act_scales)
+    return _lora.w4a8_linear_lora(x, w, scales, zeros, group_size, *lora, weight_is_e2m1=e2m1, x_fp8=x_fp8,
+                                  act_scales=act_scales)
 
 
 def _to_kernel_layout(w_op: torch.Tensor, weight_is_e2m1: bool) -> torch.Tensor:
@@ -239,23 +256,21 @@ class W4A8LinearMethod:
             del layer.qzeros
 
     def apply(self, layer, x: torch.Tensor, bias: torch.Tensor | None, *,
-              x_fp8: torch.Tensor | None = None, act_scales: torch.Tensor | None = None) -> torch.Tensor:
-        if _w4a16():
-            out = kernels.w4a16_linear(x, layer._w_packed_op, layer._scales_op, layer._zeros_op, self.quant.group_size,
-                                       kernels._n_of(layer._w_packed_op))
-        else:
-            out = kernels.w4a8_linear(x, layer._w_packed_op, layer._scales_op, layer._zeros_op, self.quant.group_size,
-                                      x_fp8=x_fp8, act_scales=act_scales)
+              x_fp8: torch.Tensor | None = None, act_scales: torch.Tensor | None = None,
+              lora: LoraBatch | None = None) -> torch.Tensor:
+        out = _quantized_apply(x, layer._w_packed_op, layer._scales_op, layer._zeros_op, self.quant.group_size, False, x_fp8,
+                               act_scales, lora)
         out = out.to(x.dtype)
         if bias is not None:
             out = out + bias
         return out
 
-    def apply_swiglu(self, layer, x: torch.Tensor) -> torch.Tensor | None:
+    def apply_swiglu(self, layer, x: torch.Tensor, *, lora: LoraBatch | None = None) -> torch.Tensor | None:
         """Fused gate_up + silu at decode on a merged gate_up layer; None -> the caller runs the
-        unfused pair. Bit-exact to the unfused pair when it fires."""
+        unfused pair, as it does with adapters, which add to gate and up before the product. Bit-exact to the
+        unfused pair when it fires."""
         w = layer._w_packed_op
-        if not _fused_swiglu_ok(x, w, self.quant.group_size):
+        if lora is not None or not _fused_swiglu_ok(x, w, self.quant.group_size):
             return None
         fn = kernels.w4a16_linear_silu if _w4a16() else kernels.w4a8_linear_silu
         return fn(x, w, layer._scales_op, layer._zeros_op, self.quant.group_size).to(x.dtype)
@@ -291,21 +306,18 @@ class MxFp4LinearMethod:
         del layer.weight_packed, layer.weight_scale
 
     def apply(self, layer, x: torch.Tensor, bias: torch.Tensor | None, *,
-              x_fp8: torch.Tensor | None = None, act_scales: torch.Tensor | None = None) -> torch.Tensor:
-        if _w4a16():
-            out = kernels.w4a16_linear(x, layer._w_packed_op, layer._scales_op, None, self.quant.group_size,
-                                       kernels._n_of(layer._w_packed_op), weight_is_e2m1=True)
-        else:
-            out = kernels.w4a8_linear(x, layer._w_packed_op, layer._scales_op, None, self.quant.group_size,
-                                      weight_is_e2m1=True, x_fp8=x_fp8, act_scales=act_scales)
+              x_fp8: torch.Tensor | None = None, act_scales: torch.Tensor | None = None,
+              lora: LoraBatch | None = None) -> torch.Tensor:
+        out = _quantized_apply(x, layer._w_packed_op, layer._scales_op, None, self.quant.group_size, True, x_fp8, act_scales,
+                               lora)
         out = out.to(x.dtype)
         if bias is not None:
             out = out + bias
         return out
 
-    def apply_swiglu(self, layer, x: torch.Tensor) -> torch.Tensor | None:
+    def apply_swiglu(self, layer, x: torch.Tensor, *, lora: LoraBatch | None = None) -> torch.Tensor | None:
         w = getattr(layer, "_w_packed_op", None)
-        if w is None or not _fused_swiglu_ok(x, w, self.quant.group_size, weight_is_e2m1=True):
+        if w is None or lora is not None or not _fused_swiglu_ok(x, w, self.quant.group_size, weight_is_e2m1=True):
             return None
         fn = kernels.w4a16_linear_silu if _w4a16() else kernels.w4a8_linear_silu
         return fn(x, w, layer._scales_op, None, self.quant.group_size, weight_is_e2m1=True).to(x.dtype)
@@ -346,21 +358,17 @@ class NvFp4LinearMethod:
         del layer.weight_packed, layer.weight_scale, layer.weight_global
 
     def apply(self, layer, x: torch.Tensor, bias: torch.Tensor | None, *,
-              x_fp8: torch.Tensor | None = None, act_scales: torch.Tensor | None = None) -> torch.Tensor:
-        if _w4a16():
-            out = kernels.w4a16_linear(x, layer._w_packed_op, layer._scales_op, layer._global_op, 16,
-                                       kernels._n_of(layer._w_packed_op), weight_is_e2m1=True)
-        else:
-            out = kernels.w4a8_linear(x, layer._w_packed_op, layer._scales_op, layer._global_op, 16,
-                                      weight_is_e2m1=True, x_fp8=x_fp8, act_scales=act_scales)
+              x_fp8: torch.Tensor | None = None, act_scales: torch.Tensor | None = None,
+              lora: LoraBatch | None = None) -> torch.Tensor:
+        out = _quantized_apply(x, layer._w_packed_op, layer._scales_op, layer._global_op, 16, True, x_fp8, act_scales, lora)
         out = out.to(x.dtype)
         if bias is not None:
             out = out + bias
         return out
 
-    def apply_swiglu(self, layer, x: torch.Tensor) -> torch.Tensor | None:
+    def apply_swiglu(self, layer, x: torch.Tensor, *, lora: LoraBatch | None = None) -> torch.Tensor | None:
         w = getattr(layer, "_w_packed_op", None)
-        if w is None or not _fused_swiglu_ok(x, w, 16, weight_is_e2m1=True):
+        if w is None or lora is not None or not _fused_swiglu_ok(x, w, 16, weight_is_e2m1=True):
             return None
         fn = kernels.w4a16_linear_silu if _w4a16() else kernels.w4a8_linear_silu
         return fn(x, w, layer._scales_op, layer._global_op, 16, weight_is_e2m1=True).to(x.dtype)

@@ -4,7 +4,8 @@ the cache's contents against the formulas and attention against 64-bit attention
 Tolerances. Codes, steps and least values follow from exact f32 steps and are compared for equality.
 Attention's output is rounded once (2^-8 of the value for bf16, 2^-11 for fp16). Before that: scores are f32
 sums of four (D = 128) MFMA steps of at most 31 sum|q| s, about 3e-5 on a score of these sizes, and p s
-enters its product within 2^-18; together below 2e-4 of the largest cached value."""
+enters its product within 2^-18; together below 2e-4 of the largest cached value. (fp16's 2^-25 for results
+below 2^-14 is far inside that, but for cached values below 1e-4, where it is allowed on top.)"""
 import math
 
 import pytest
@@ -132,7 +133,7 @@ class Setup:
         ref, rl = ref_attention(q, kv, self.table, self.page, self.lens, self.news, kw.get("sm_scale", D ** -0.5), causal, window)
         eps = 2.0 ** (-8 if q.dtype == torch.bfloat16 else -11)
         vmax = self.v.float().abs().max().item() if self.v.numel() else 0.0
-        err = (out.cpu().double() - ref).abs() - eps * ref.abs() - 2e-4 * vmax
+        err = (out.cpu().double() - ref).abs() - eps * ref.abs() - 2e-4 * vmax - 2.0 ** -25
         assert not torch.isnan(out).any(), what
         assert err.max().item() <= 0 if err.numel() else True, f"{what}: off by {err.max().item():.3e} past the tolerance"
         lf = torch.isfinite(rl)
