@@ -24,6 +24,8 @@ _ENTRY_POINTS = (
     "w4a8_rms_norm", "w4a8_moe_padded_capacity", "w4a8_moe_route_gemm1", "w4a8_moe_route_slots",
     "w4a8_moe_route_align", "w4a8_moe_gemm_workspace_bytes", "w4a8_moe_gemm", "w4a8_moe_gemm2_combine_supported",
     "w4a8_moe_gemm2_combine", "w4a8_moe_gemm_quant_workspace_bytes", "w4a8_moe_gemm_quant", "w4a8_moe_combine",
+    "w4a8_kv4_append", "w4a8_kv4_read", "w4a8_kv4_attention_workspace_bytes", "w4a8_kv4_attention",
+    "w4a8_lora_workspace_bytes", "w4a8_lora_add",
 )
 
 _lock = threading.Lock()
@@ -34,6 +36,7 @@ class _Absent:
     """In the extension's place: takes no call."""
 
     linear = rms_norm = moe = staticmethod(lambda *a: None)
+    kv4_append = kv4_read = kv4_attention = lora_add = linear_lora = staticmethod(lambda *a: None)
 
 
 def _running() -> str:

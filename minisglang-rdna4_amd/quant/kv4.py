@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import torch
 
-from .. import _abi
+from .. import _abi, _host
 from .._hip_engage import engaged
 
 _DTYPES = (torch.bfloat16, torch.float16)
@@ -129,6 +129,9 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, page_table: to
     pages may be shared. Rows outside cu_q, before a sequence's first token or on a page that does not
     exist write nothing."""
     what = "kv4_append"
+    if _host.load().kv4_append(cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, cu_q, seq_lens, k, v):
+        engaged("w4a8_mi355x.kv4_append")
+        return
     k = _rows(k, cache, cache.num_kv_heads, "k", what)
     v = _rows(v, cache, cache.num_kv_heads, "v", what)
     if v.shape[0] != k.shape[0]:
@@ -149,6 +152,10 @@ def kv4_read(cache: KV4Cache, page_table: torch.Tensor, cu_q: torch.Tensor, seq_
     reads. With cu_q the running sum of seq_lens, whole sequences. Rows outside cu_q are not written; a
     row without a place in the cache is NaN. One launch."""
     what = "kv4_read"
+    r = _host.load().kv4_read(cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, cu_q, seq_lens, num_rows)
+    if r is not None:
+        engaged("w4a8_mi355x.kv4_read")
+        return r
     table, ldt, width, cu, lens, B = _batch(cache, page_table, cu_q, seq_lens, what)
     if num_rows < 0:
         raise ValueError(f"{what}: num_rows={num_rows}")
@@ -191,6 +198,13 @@ def kv4_attention(
     low a one as well; neither changes which keys are read. One launch, and a second that joins the
     parts where the keys are split over workgroups."""
     what = "kv4_attention"
+    if sm_scale is None:
+        sm_scale = cache.head_dim ** -0.5
+    r = _host.load().kv4_attention(cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, cu_q, seq_lens, q, max_q,
+                                   max_kv, sm_scale, causal, window, out, return_lse)
+    if r is not None:
+        engaged("w4a8_mi355x.kv4_attention")
+        return r if return_lse else r[0]
     q = _rows(q, cache, None, "q", what)
     T, Hq, D = q.shape
     if Hq < cache.num_kv_heads or Hq % cache.num_kv_heads:
@@ -219,7 +233,7 @@ def kv4_attention(
         _abi.check(lib.w4a8_kv4_attention(
             q.data_ptr(), _abi.dtype_code(q.dtype), q.stride(0), q.stride(1), T, Hq, cache.num_kv_heads, D, *cache._ptrs(),
             cache.num_pages, cache.page_size, table, ldt, width, cu, lens, B,
-            float(D ** -0.5 if sm_scale is None else sm_scale), int(bool(causal)), int(window), max_q, max_kv,
+            float(sm_scale), int(bool(causal)), int(window), max_q, max_kv,
             out.data_ptr(), out.stride(0), out.stride(1), _abi.ptr(lse), _abi.ptr(ws), max(ws_bytes, 0),
             _abi.stream_of(q)), what)
     engaged("w4a8_mi355x.kv4_attention")

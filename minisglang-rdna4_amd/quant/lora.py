@@ -17,7 +17,7 @@ from typing import Sequence
 
 import torch
 
-from .. import _abi
+from .. import _abi, _host
 from .._hip_engage import engaged
 from . import kernels
 
@@ -27,6 +27,7 @@ _MAX_RANK, _MAX_SLICES = 256, 8
 # Rows up to which w4a8_linear_lora keeps the projection's output in f32 until the adapters' part is added,
 # for one rounding of the sum; above, the projection's output is rounded to the type in between.
 _F32_BASE_MAX_ROWS = 128
+_LEDGER = {False: "w4a8_mi355x.linear_lora(int4)", True: "w4a8_mi355x.linear_lora(e2m1)"}
 
 
 class LoraAdapters:
@@ -105,6 +106,9 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora: LoraAdapters, adapters: tor
     output for x (M, K), both in the adapters' type, their rows strided or not. Rows without an adapter
     keep y's values. The sum is in f32 and rounded once."""
     what = "lora_add"
+    if _host.load().lora_add(lora.a, lora.b, lora.scaling, lora.slices, adapters, y, x, y if out is None else out):
+        engaged("w4a8_mi355x.lora_add")
+        return y if out is None else out
     _check(x, lora, adapters, what)
     out = y if out is None else out
     for name, t in (("y", y), ("out", out)):
@@ -133,6 +137,14 @@ def w4a8_linear_lora(
     unquantized, also where the producer pair is given for the projection. Up to 128 rows the sum is
     rounded once; above, the projection's output is rounded before."""
     what = "w4a8_linear_lora"
+    if x.is_cuda and (kernel is None or kernel == "decode_gemv"):
+        r = _host.load().linear_lora(lora.a, lora.b, lora.scaling, lora.slices, adapters, x, w_packed, scales, w_zeros,
+                                     group_size, weight_is_e2m1, x_fp8, act_scales,
+                                     _abi.KERNEL_AUTO if kernel is None else _abi.KERNEL_DECODE,
+                                     x.shape[0] <= _F32_BASE_MAX_ROWS)
+        if r is not None:
+            engaged(_LEDGER[bool(weight_is_e2m1)])
+            return r
     _check(x, lora, adapters, what)
     if kernels._n_of(w_packed) != lora.out_features:
         raise ValueError(f"{what}: the weight has {kernels._n_of(w_packed)} output channels, the adapters "
@@ -145,5 +157,5 @@ def w4a8_linear_lora(
     else:
         out = base = kernels.w4a8_linear(x, w_packed, scales, w_zeros, group_size, kernel, weight_is_e2m1, x_fp8, act_scales)
     _add(base, x, lora, adapters, out, what)
-    engaged(f"w4a8_mi355x.linear_lora({'e2m1' if weight_is_e2m1 else 'int4'})")
+    engaged(_LEDGER[bool(weight_is_e2m1)])
     return out
