@@ -52,6 +52,7 @@ struct Kv4Attn {
   Kv4Cache c;
   Kv4Batch s;
   int G;            // query heads per key/value head
+  uint32_t gmul;    // ceil(2^31 / G): x / G is the high half of 2 x gmul for x below 2^31 / G
   float scale;      // softmax scale times log2(e)
   int causal;
   int window;       // keys before position - window + 1 are not seen; 0: all are

@@ -126,6 +126,8 @@ int w4a8_kv4_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_
   if (rc) return rc;
   if (Hq < H || Hq % H || Hq > 65535)
     return fail(kErrInvalid, "%s: %lld query heads for %lld key/value heads", who, (long long)Hq, (long long)H);
+  if (T * Hq > 0x3fffffff)  // queries times heads are columns, indexed in 32 bits
+    return fail(kErrUnsupported, "%s: past its index ranges (T=%lld, %lld query heads)", who, (long long)T, (long long)Hq);
   if (window < 0 || window > 0x7fffffff || max_q < 0 || max_kv < 0 || max_q > 0x7fffffff || max_kv > 0x7fffffff)
     return fail(kErrInvalid, "%s: window=%lld max_q=%lld max_kv=%lld", who, (long long)window, (long long)max_q,
                 (long long)max_kv);
@@ -147,9 +149,10 @@ int w4a8_kv4_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_
   p.ldo = ldo; p.ho = ho;
   p.lse = lse;
   p.G = (int)(Hq / H);
+  p.gmul = (uint32_t)((((uint64_t)1 << 31) + p.G - 1) / p.G);
   p.scale = scale * 1.4426950408889634f;
   p.causal = causal != 0;
-  p.window = (int)window;
+  p.window = (int)(window < (1 << 30) ? window : 1 << 30);
   return launched(launch_kv4_attention(p, (int)D, dtype, pl, workspace, (hipStream_t)stream), who);
 }
 

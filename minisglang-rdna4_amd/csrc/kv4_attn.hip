@@ -76,36 +76,26 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
-// what one lane reads of a tile: its two rows of K, its 8 tokens of V's channels, and those tokens' scales
-template <int D>
-struct Tile {
-  uint32_t k[2][D / 32], v[D / 16], ks[8], vs[8];
+// The page numbers of a tile, wave-uniform: those of its tokens 0..15 and 16..31 (a page holds at least 16),
+// as the table has them, -1 where it has none. Looked up a tile before they are used: the scalar loads
+// then have nobody waiting. (Nothing writes the table during a launch: constant address space.)
+typedef const int32_t __attribute__((address_space(4))) * Table;
+struct Pages {
+  int a, b;
 };
-
-// of a tile's blocks: the one with this lane's K rows, and the one of its group (-1: no such page)
-struct Blocks {
-  int k, g;
-};
-
-template <int D>
-__device__ __forceinline__ Blocks find_blocks(const Kv4Attn& p, int b, int h, int64_t t0, int len, int lane) {
-  const int gk = (lane & 15) >> 2, g = lane >> 4;
-  const int64_t tk = t0 + 8 * gk, tg = t0 + 8 * g;
-  const int pk = tk < len ? kv4_page(p.c, p.s, b, tk) : -1;
-  const int pg = tg < len ? kv4_page(p.c, p.s, b, tg) : -1;
-  return {pk < 0 ? 0 : kv4_block(p.c, pk, h, (int)(tk & 0x7fffffff)), pg < 0 ? -1 : kv4_block(p.c, pg, h, (int)(tg & 0x7fffffff))};
+__device__ __forceinline__ Pages look_up(const Kv4Attn& p, Table table, int t, int len) {
+  Pages r = {-1, -1};
+  const int i = t >> p.c.shift, j = (t + 16) >> p.c.shift;
+  if (t < len && i < p.s.width) r.a = table[i];
+  if (t + 16 < len && j < p.s.width) r.b = table[j];
+  return r;
 }
-
-template <int D>
-__device__ __forceinline__ void load_tile(const Kv4Attn& p, const Blocks& at, int lane, Tile<D>& t) {
-  const int g = lane >> 4, r = lane & 3;
-  const int bg = at.g < 0 ? 0 : at.g;  // block 0 is there to be read; what it gives is not used
-  const uint8_t* kp = p.c.k + (int64_t)at.k * (4 * D) + r * (D / 2) + g * (D / 8);
-  load_words(kp, t.k[0]);
-  load_words(kp + 4 * (D / 2), t.k[1]);
-  load_words(p.c.v + (int64_t)bg * (4 * D) + (lane & 15) * (D / 4), t.v);
-  load_words(reinterpret_cast<const uint8_t*>(p.c.ks + (int64_t)bg * 8), t.ks);
-  load_words(reinterpret_cast<const uint8_t*>(p.c.vs + (int64_t)bg * 8), t.vs);
+__device__ __forceinline__ bool exists(const Kv4Attn& p, int page) { return (uint32_t)page < (uint32_t)p.c.pages; }
+// block `i` of 4 of the tile at t: this lane's; a missing page reads block 0, which is there, and its values
+// are not used
+__device__ __forceinline__ uint32_t pick(const Kv4Attn& p, const Pages& pg, int h, int t, int i) {
+  const int a = exists(p, pg.a) ? kv4_block(p.c, pg.a, h, t) : 0, b = exists(p, pg.b) ? kv4_block(p.c, pg.b, h, t + 16) : 0;
+  return (uint32_t)((i < 2 ? a : b) + (i & 1));
 }
 
 template <int DT>
@@ -117,18 +107,20 @@ __device__ __forceinline__ float hi16(uint32_t w) {
   return DT == kBF16 ? __uint_as_float(w & 0xffff0000u) : f16_to_f32((uint16_t)(w >> 16));
 }
 
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  return (uint32_t)f32_to_bf16(a) | ((uint32_t)f32_to_bf16(b) << 16);
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2bf));
 }
 
 // D: channels; DT: the model's type; NQ: blocks of 16 columns per wave; WKV: 4 waves over the tokens, or 1:
 // 4 waves over the columns
 template <int D, int DT, int NQ, int WKV>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, WKV == 1 ? 1 : D == 256 ? 2 : 3)
 kv4_attn_kernel(const Kv4Attn p) {
   constexpr int KS = D / 32, DB = D / 16;  // products per S tile, blocks of 16 channels
   constexpr int kCols = 16 * NQ * (WKV == 1 ? 4 : 1);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
   const int h = blockIdx.y, b = blockIdx.z;
   const int split = blockIdx.x % p.splits;
@@ -136,52 +128,91 @@ kv4_attn_kernel(const Kv4Attn p) {
   int64_t start;
   int n;
   kv4_rows(p.s, b, start, n);
-  const int64_t cols = (int64_t)n * p.G;
+  const int cols = n * p.G;
   const int64_t cap = (int64_t)p.s.width << p.c.shift;
   // one token past the table's end stands for all of them: its page is missing
   const int len0 = p.s.lens[b];
   const int len = len0 > cap ? (int)(cap + 1 < 0x7fffffff ? cap + 1 : 0x7fffffff) : len0 < 0 ? 0 : len0;
   const int first_pos = len0 - n;  // position of the first new token
 
-  __shared__ float red_o[WKV == 1 ? 1 : 3 * 16 * NQ * D];
-  __shared__ float red_ml[WKV == 1 ? 1 : 4 * 16 * NQ * 2];
+  const float slack = 8.f / p.scale;
+  __shared__ float red_o[WKV == 1 ? 1 : 4 * 16 * D];
+  __shared__ float red_ml[WKV == 1 ? 1 : 4 * 16 * 2];
 
   // the last tiles of columns have the most keys: first
-  const int64_t qtiles = (cols + kCols - 1) / kCols;
-  const int64_t gq = gridDim.x / p.splits;
-  for (int64_t qi = blockIdx.x / p.splits; qi < qtiles; qi += gq) {
-    const int64_t c0 = (qtiles - 1 - qi) * kCols + (WKV == 1 ? wave * 16 * NQ : 0);
-    // per block of columns: the query's token and head, and the keys [klo, khi) that it sees
+  const int qtiles = (cols + kCols - 1) / kCols;
+  const int gq = gridDim.x / p.splits;
+  for (int qi = blockIdx.x / p.splits; qi < qtiles; qi += gq) {
+    const int c0 = (qtiles - 1 - qi) * kCols + (WKV == 1 ? wave * 16 * NQ : 0);
+    // Columns are queries in order, so the keys that all of them and that any of them sees, [lo_all, hi_all) and
+    // [lo, hi), follow from the first and the last one.
+    const int cend = c0 + 16 * NQ < cols ? c0 + 16 * NQ : cols;
+    const int i0 = c0 / p.G, r0 = c0 - i0 * p.G, i1 = (cend - 1) / p.G;
+    auto upto = [&](int i) { return p.causal ? min(max(first_pos + i + 1, 0), len) : len; };
+    auto from = [&](int i) { return p.window ? min(max(first_pos + i - p.window + 1, 0), len) : 0; };
+    const int lo = from(i0), lo_all = from(i1), hi_all = upto(i0), hi = c0 < cols ? upto(i1) : 0;
+    const int t_first = lo < hi ? lo >> 5 : 0;
+    const int nt = lo < hi ? ((hi + 31) >> 5) - t_first : 0;
+    const int hop = (p.splits - 1) * p.ct;
+    auto next = [&](int t) {
+      t += WKV;
+      return (t & (p.ct - 1)) < WKV ? t + hop : t;
+    };
+    const Table table = (Table)(uintptr_t)(p.s.table + b * p.s.ldt);
+    // Each part of the next tile is loaded into the registers of this one's as soon as they are free.
+    uint32_t kw[2][KS], vw[DB], ksw[8], vsw[8];
+    auto load_k = [&](const Pages& pg, int t) {
+      const uint8_t* kp = p.c.k + (uint64_t)pick(p, pg, h, t, (lane & 15) >> 2) * (4 * D) + ((lane & 3) * (D / 2) + g * (D / 8));
+      load_words(kp, kw[0]);
+      load_words(kp + 4 * (D / 2), kw[1]);
+    };
+    auto load_v = [&](const Pages& pg, int t) {
+      load_words(p.c.v + (uint64_t)pick(p, pg, h, t, g) * (4 * D) + (lane & 15) * (D / 4), vw);
+    };
+    auto load_s = [&](const Pages& pg, int t) {
+      const uint64_t o = (uint64_t)pick(p, pg, h, t, g) * 32;
+      load_words(reinterpret_cast<const uint8_t*>(p.c.ks) + o, ksw);
+      load_words(reinterpret_cast<const uint8_t*>(p.c.vs) + o, vsw);
+    };
+    int t = split * p.ct + (WKV == 1 ? 0 : wave);
+    int tn = next(t);
+    auto token = [&](int t) { return (t_first + t) * 32; };
+    Pages at = {-1, -1}, nat = {-1, -1};
+    if (t < nt) at = look_up(p, table, token(t), hi);
+    if (tn < nt) nat = look_up(p, table, token(tn), hi);
+
+    // this lane's query of column 16 j + col
+    auto query = [&](int j, int& head) {
+      const int x = r0 + 16 * j + col, i = (int)__umulhi((uint32_t)x << 1, p.gmul);
+      head = h * p.G + x - i * p.G;
+      return i0 + i;
+    };
+    uint4 qr[NQ][KS];
     int klo[NQ], khi[NQ];
-    v4w qf[NQ][KS];
-    float qs[NQ];
-    int64_t row[NQ];
-    int head[NQ];
-    int lo = 0x7fffffff, hi = 0, lo_all = 0, hi_all = 0x7fffffff;
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
-      const int64_t c = c0 + 16 * j + col;
-      const bool on = c < cols;
-      const int64_t i = on ? c / p.G : 0;
-      head[j] = h * p.G + (int)(on ? c - i * p.G : 0);
-      row[j] = on ? start + i : -1;
-      const int64_t pos = first_pos + i;
-      const int64_t e = p.causal ? pos + 1 : len, a = p.window ? pos - p.window + 1 : 0;
-      khi[j] = on ? (int)(e < 0 ? 0 : e < len ? e : len) : 0;
-      klo[j] = (int)(a < 0 ? 0 : a < len ? a : len);
-      if (on && klo[j] < khi[j]) {
-        lo = klo[j] < lo ? klo[j] : lo;
-        hi = khi[j] > hi ? khi[j] : hi;
-      }
-      if (on) {
-        lo_all = klo[j] > lo_all ? klo[j] : lo_all;
-        hi_all = khi[j] < hi_all ? khi[j] : hi_all;
-      }
-      const uint16_t* qp = p.q + (on ? start + i : start) * p.ldq + head[j] * p.hq + g * (D / 4);
+      int head;
+      const int i = query(j, head);
+      const bool on = c0 + 16 * j + col < cols;
+      khi[j] = on ? upto(i) : 0;
+      klo[j] = from(i);
+      const uint16_t* qp = p.q + (start + (on ? i : 0)) * p.ldq + (on ? head : 0) * p.hq + g * (D / 4);
+#pragma unroll
+      for (int w = 0; w < KS; ++w) qr[j][w] = on ? *reinterpret_cast<const uint4*>(qp + 8 * w) : make_uint4(0, 0, 0, 0);
+    }
+    if (t < nt) {
+      load_k(at, token(t));
+      load_s(at, token(t));
+      load_v(at, token(t));
+    }
+    v4w qf[NQ][KS];
+    float qs[NQ];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < KS; ++w) {
-        const uint4 u = on ? *reinterpret_cast<const uint4*>(qp + 8 * w) : make_uint4(0, 0, 0, 0);
+        const uint4 u = qr[j][w];
         // the codes' order: elements 0 4, 1 5, 2 6, 3 7
         qf[j][w][0] = (u.x & 0xffffu) | (u.z << 16);
         qf[j][w][1] = (u.x >> 16) | (u.z & 0xffff0000u);
@@ -193,102 +224,81 @@ kv4_attn_kernel(const Kv4Attn p) {
       }
       qs[j] = col_sum(sum);
     }
-    // over the wave
-#pragma unroll
-    for (int s = 1; s < 16; s <<= 1) {
-      lo = min(lo, __shfl_xor(lo, s));
-      hi = max(hi, __shfl_xor(hi, s));
-      lo_all = max(lo_all, __shfl_xor(lo_all, s));
-      hi_all = min(hi_all, __shfl_xor(hi_all, s));
-    }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    hi = __builtin_amdgcn_readfirstlane(hi);
-    lo_all = __builtin_amdgcn_readfirstlane(lo_all);
-    hi_all = __builtin_amdgcn_readfirstlane(hi_all);
 
     v4f o[NQ][DB];
-    float m[NQ], l[NQ], cc[NQ];
+    float m[NQ], mu[NQ], l[NQ], cc[NQ];  // mu: m in powers of two, 0 while no key was seen
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
       m[j] = -__builtin_inff();
-      l[j] = cc[j] = 0.f;
+      mu[j] = l[j] = cc[j] = 0.f;
 #pragma unroll
       for (int d = 0; d < DB; ++d) o[j][d] = v4f{0.f, 0.f, 0.f, 0.f};
     }
 
-    const int t_first = lo < hi ? lo >> 5 : 0;
-    const int nt = lo < hi ? ((hi + 31) >> 5) - t_first : 0;
-    const int hop = (p.splits - 1) * p.ct;
-    auto next = [&](int t) {
-      t += WKV;
-      return (t & (p.ct - 1)) < WKV ? t + hop : t;
-    };
-    int t = split * p.ct + (WKV == 1 ? 0 : wave);
-    Tile<D> cur;
-    Blocks at = {0, -1};
-    if (t < nt) {
-      at = find_blocks<D>(p, b, h, (int64_t)(t_first + t) * 32, hi, lane);
-      load_tile<D>(p, at, lane, cur);
-    }
-    int tn = next(t);
-    Blocks nat = {0, -1};
-    if (tn < nt) nat = find_blocks<D>(p, b, h, (int64_t)(t_first + tn) * 32, hi, lane);
     while (t < nt) {
-      const Tile<D> x = cur;
-      const bool missing = at.g < 0;
-      const int t0 = (t_first + t) * 32;
-      at = nat;
-      if (tn < nt) load_tile<D>(p, at, lane, cur);
+      const int t0 = token(t);
       const int tnn = next(tn);
-      if (tnn < nt) nat = find_blocks<D>(p, b, h, (int64_t)(t_first + tnn) * 32, hi, lane);
+      Pages nnat = {-1, -1};
+      if (tnn < nt) nnat = look_up(p, table, token(tnn), hi);
 
       v4f s[NQ][2];
 #pragma unroll
-      for (int j = 0; j < NQ; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[j][0][r] = s[j][1][r] = -16.f * qs[j];
+      for (int j = 0; j < NQ; ++j) {
+        const float q16 = -16.f * qs[j];
+        s[j][0] = s[j][1] = v4f{q16, q16, q16, q16};
+      }
 #pragma unroll
       for (int w = 0; w < KS; ++w) {
-        const v4w a0 = widen<DT>(x.k[0][w]), a1 = widen<DT>(x.k[1][w]);
+        const v4w a0 = widen<DT>(kw[0][w]), a1 = widen<DT>(kw[1][w]);
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
           s[j][0] = mfma16<DT>(a0, qf[j][w], s[j][0]);
           s[j][1] = mfma16<DT>(a1, qf[j][w], s[j][1]);
         }
       }
-      const int tb = t0 + 8 * g;  // this lane's first token
-      const bool whole = t0 >= lo_all && t0 + 32 <= hi_all;
+      if (tn < nt) load_k(nat, token(tn));
+
+      const bool whole = t0 >= lo_all && t0 + 32 <= hi_all && exists(p, at.a) && exists(p, at.b);
       v4w ph[NQ], pl[NQ];
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
-        float y[8], top = -__builtin_inff();
+        float y[8], sv[8], mv[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          y[i] = __builtin_fmaf(lo16<DT>(x.ks[i]), s[j][i >> 2][i & 3], hi16<DT>(x.ks[i]) * qs[j]) * p.scale;
-          if (missing) y[i] = __builtin_nanf("");
-          if (!whole && !(tb + i >= klo[j] && tb + i < khi[j])) y[i] = -__builtin_inff();
-          top = fmaxf(top, y[i]);
+          y[i] = __builtin_fmaf(lo16<DT>(ksw[i]), s[j][i >> 2][i & 3], hi16<DT>(ksw[i]) * qs[j]);
+          sv[i] = lo16<DT>(vsw[i]);
+          mv[i] = __builtin_fmaf(-16.f, sv[i], hi16<DT>(vsw[i]));
         }
-        if (__ballot(top > m[j] + 8.f)) {
+        if (!whole) {
+          // an unseen token's scale may be anything, and 0 times it is not 0; a missing page is NaN to whoever sees it
+          const int a = klo[j] - (t0 + 8 * g), e = khi[j] - (t0 + 8 * g);
+          const bool missing = !exists(p, g < 2 ? at.a : at.b);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const bool see = i >= a && i < e;
+            y[i] = !see ? -__builtin_inff() : missing ? __builtin_nanf("") : y[i];
+            sv[i] = see ? sv[i] : 0.f;
+            mv[i] = see ? mv[i] : 0.f;
+          }
+        }
+        const float top = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+        if (__ballot(top > m[j] + slack)) {
           const float mn = fmaxf(m[j], col_max(top));
-          const float f = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m[j] - mn);
+          const float f = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((m[j] - mn) * p.scale);
           m[j] = mn;
+          mu[j] = mn == -__builtin_inff() ? 0.f : mn * p.scale;
           l[j] *= f;
           cc[j] *= f;
 #pragma unroll
           for (int d = 0; d < DB; ++d) o[j][d] *= f;
         }
-        const float mu = m[j] == -__builtin_inff() ? 0.f : m[j];
         float ps[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float pr = __builtin_amdgcn_exp2f(y[i] - mu);
-          const float sv = lo16<DT>(x.vs[i]), mv = hi16<DT>(x.vs[i]);
+          const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(y[i], p.scale, -mu[j]));
           l[j] += pr;
-          // an unseen token's scale may be anything: 0 times it is not 0
-          const bool off = !whole && y[i] == -__builtin_inff();
-          ps[i] = off ? 0.f : pr * sv;
-          cc[j] = off ? cc[j] : __builtin_fmaf(pr, __builtin_fmaf(-16.f, sv, mv), cc[j]);
+          ps[i] = pr * sv[i];
+          cc[j] = __builtin_fmaf(pr, mv[i], cc[j]);
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -296,124 +306,140 @@ kv4_attn_kernel(const Kv4Attn p) {
           pl[j][r] = pack_bf16(ps[r] - __uint_as_float(ph[j][r] << 16), ps[r + 4] - __uint_as_float(ph[j][r] & 0xffff0000u));
         }
       }
+      if (tn < nt) load_s(nat, token(tn));
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        const v4w a = widen<kBF16>(x.v[d]);
+        const v4w a = widen<kBF16>(vw[d]);
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
           o[j][d] = mfma16<kBF16>(a, ph[j], o[j][d]);
           o[j][d] = mfma16<kBF16>(a, pl[j], o[j][d]);
         }
       }
+      if (tn < nt) load_v(nat, token(tn));
+      at = nat;
+      nat = nnat;
       t = tn;
       tn = tnn;
     }
 
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
+      m[j] *= p.scale;
       l[j] = col_sum(l[j]);
       cc[j] = col_sum(cc[j]);
 #pragma unroll
       for (int d = 0; d < DB; ++d) o[j][d] += cc[j];
     }
-    if (WKV > 1) {
-      // join the waves: all to the common maximum, waves 1 to 3 through LDS to wave 0
+    // a lane's channels: DB (4 g + r) + d of its column, r = 0..3
+    auto store = [&](int j, int r, const float (&v)[DB], float mx, float sum) {
+      if (c0 + 16 * j + col >= cols) return;
+      int head;
+      const int64_t row = start + query(j, head);
+      const bool first = g == 0 && r == 0;
+      if (p.splits > 1) {
+        const int64_t at_o = ((int64_t)split * p.s.T + row) * Hq + head;
+        float* op = p.po + at_o * D + (4 * g + r) * DB;
+#pragma unroll
+        for (int d = 0; d < DB; d += 4) *reinterpret_cast<v4f*>(op + d) = v4f{v[d], v[d + 1], v[d + 2], v[d + 3]};
+        if (first) {
+          p.pml[at_o * 2] = mx;
+          p.pml[at_o * 2 + 1] = sum;
+        }
+      } else {
+        // no key seen: the sum is 0, the output 0
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        uint16_t* op = p.out + row * p.ldo + head * p.ho + (4 * g + r) * DB;
+#pragma unroll
+        for (int d = 0; d < DB; d += 4) {
+          uint2 u;
+          u.x = (uint32_t)to_dtype(v[d] * inv, DT) | ((uint32_t)to_dtype(v[d + 1] * inv, DT) << 16);
+          u.y = (uint32_t)to_dtype(v[d + 2] * inv, DT) | ((uint32_t)to_dtype(v[d + 3] * inv, DT) << 16);
+          *reinterpret_cast<uint2*>(op + d) = u;
+        }
+        if (p.lse && first) p.lse[row * Hq + head] = sum == 0.f ? -__builtin_inff() : mx * 0.69314718055994531f + logf(sum);
+      }
+    };
+    if constexpr (WKV == 1) {
 #pragma unroll
       for (int j = 0; j < NQ; ++j)
-        if (g == 0) {
-          red_ml[((wave * NQ + j) * 16 + col) * 2] = m[j];
-          red_ml[((wave * NQ + j) * 16 + col) * 2 + 1] = l[j];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float v[DB];
+#pragma unroll
+          for (int d = 0; d < DB; ++d) v[d] = o[j][d][r];
+          store(j, r, v, m[j], l[j]);
         }
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-        float mn = -__builtin_inff(), sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) mn = fmaxf(mn, red_ml[((w * NQ + j) * 16 + col) * 2]);
-        const float mu = mn == -__builtin_inff() ? 0.f : mn;
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          sum += red_ml[((w * NQ + j) * 16 + col) * 2 + 1] * __builtin_amdgcn_exp2f(red_ml[((w * NQ + j) * 16 + col) * 2] - mu);
-        const float f = __builtin_amdgcn_exp2f(m[j] - mu);
-        m[j] = mn;
-        l[j] = sum;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          o[j][d] *= f;
-          if (wave)
-            *reinterpret_cast<v4f*>(&red_o[((((wave - 1) * NQ + j) * DB + d) * 64 + lane) * 4]) = o[j][d];
-        }
+    } else {
+      // join the waves through LDS, each to the common maximum; wave r then sums and writes the channels of r
+      static_assert(NQ == 1, "one block of columns");
+      if (g == 0) {
+        red_ml[(wave * 16 + col) * 2] = m[0];
+        red_ml[(wave * 16 + col) * 2 + 1] = l[0];
       }
+#pragma unroll
+      for (int d = 0; d < DB; ++d) *reinterpret_cast<v4f*>(&red_o[((wave * DB + d) * 64 + lane) * 4]) = o[0][d];
       __syncthreads();
-      if (wave == 0)
+      float mw[4], mx = -__builtin_inff(), sum = 0.f, v[DB];
 #pragma unroll
-        for (int j = 0; j < NQ; ++j)
+      for (int w = 0; w < 4; ++w) mx = fmaxf(mx, mw[w] = red_ml[(w * 16 + col) * 2]);
 #pragma unroll
-          for (int d = 0; d < DB; ++d)
+      for (int d = 0; d < DB; ++d) v[d] = 0.f;
 #pragma unroll
-            for (int w = 0; w < 3; ++w)
-              o[j][d] += *reinterpret_cast<const v4f*>(&red_o[(((w * NQ + j) * DB + d) * 64 + lane) * 4]);
+      for (int w = 0; w < 4; ++w) {
+        const float f = mx == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mw[w] - mx);
+        sum += f * red_ml[(w * 16 + col) * 2 + 1];
+#pragma unroll
+        for (int d = 0; d < DB; ++d) v[d] += f * red_o[((w * DB + d) * 64 + lane) * 4 + wave];
+      }
+      store(0, wave, v, mx, sum);
+      __syncthreads();  // before the next tile of columns writes LDS
     }
-    // lane: channels DB * 4 g + DB r + d of its column
-    if (WKV == 1 || wave == 0)
-#pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-        if (row[j] < 0) continue;
-        if (p.splits > 1) {
-          const int64_t at_o = ((int64_t)split * p.s.T + row[j]) * Hq + head[j];
-          float* op = p.po + at_o * D + g * (DB * 4);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int d = 0; d < DB; d += 4)
-              *reinterpret_cast<v4f*>(op + r * DB + d) = v4f{o[j][d][r], o[j][d + 1][r], o[j][d + 2][r], o[j][d + 3][r]};
-          if (g == 0) {
-            p.pml[at_o * 2] = m[j];
-            p.pml[at_o * 2 + 1] = l[j];
-          }
-        } else {
-          // no key seen: the sum is 0, the output 0
-          const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];
-          uint16_t* op = p.out + row[j] * p.ldo + head[j] * p.ho + g * (DB * 4);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int d = 0; d < DB; d += 4) {
-              uint2 u;
-              u.x = (uint32_t)to_dtype(o[j][d][r] * inv, DT) | ((uint32_t)to_dtype(o[j][d + 1][r] * inv, DT) << 16);
-              u.y = (uint32_t)to_dtype(o[j][d + 2][r] * inv, DT) | ((uint32_t)to_dtype(o[j][d + 3][r] * inv, DT) << 16);
-              *reinterpret_cast<uint2*>(op + r * DB + d) = u;
-            }
-          if (p.lse && g == 0)
-            p.lse[row[j] * Hq + head[j]] = l[j] == 0.f ? -__builtin_inff() : m[j] * 0.69314718055994531f + logf(l[j]);
-        }
-      }
-    if (WKV > 1) __syncthreads();  // before the next tile of columns writes LDS
   }
 }
 
-// The splits of one row and head: 64 lanes, D / 64 channels each, a wave per (row, head).
+// The splits of one row and head: a wave, first a lane per split (at most 64) for the maxima and sums, then
+// D / 64 channels per lane. Splits that saw no key are not read.
 template <int D, int DT>
 __global__ void __launch_bounds__(256)
 kv4_join_kernel(const Kv4Attn p) {
   constexpr int E = D / 64;
   const int lane = threadIdx.x & 63;
   const int Hq = p.c.H * p.G;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (id >= p.s.T * Hq) return;
-  const int64_t row = id / Hq, head = id - row * Hq, step = p.s.T * Hq;
+  const int rows = (int)p.s.T * Hq;
+  const int id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  if (id >= rows) return;
+  const int row = id / Hq, head = id - row * Hq;
   if (row >= p.s.cu[p.s.B] || row < p.s.cu[0]) return;  // rows of no sequence stay as they are
-  float mn = -__builtin_inff();
-  for (int s = 0; s < p.splits; ++s) mn = fmaxf(mn, p.pml[(s * step + id) * 2]);
-  const float mu = mn == -__builtin_inff() ? 0.f : mn;
-  float l = 0.f, o[E];
+  float ms = -__builtin_inff(), ls = 0.f;
+  if (lane < p.splits) {
+    const v2f ml = *reinterpret_cast<const v2f*>(p.pml + ((int64_t)lane * rows + id) * 2);
+    ms = ml.x;
+    ls = ml.y;
+  }
+  const float mn = wave_max(ms);
+  const float f = mn == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ms - mn);
+  const float l = wave_sum(ls == 0.f ? 0.f : ls * f);
+  uint64_t todo = __ballot(!(ls == 0.f));
+  float o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float f = __builtin_amdgcn_exp2f(p.pml[(s * step + id) * 2] - mu);
-    l += f * p.pml[(s * step + id) * 2 + 1];
+  const float* po = p.po + (int64_t)id * D + lane * E;
+  while (todo) {
+    // four at a time, all loaded before the first is used
+    float v[4][E], w[4];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] += f * p.po[(s * step + id) * D + lane * E + e];
+    for (int u = 0; u < 4; ++u) {
+      const int s = todo ? __builtin_ctzll(todo) : 0;
+      w[u] = todo ? lane_f(f, s) : 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[u][e] = todo ? po[(int64_t)s * rows * D + e] : 0.f;
+      todo &= todo - 1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(w[u], v[u][e], o[e]);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* op = p.out + row * p.ldo + head * p.ho + lane * E;
