@@ -57,15 +57,17 @@ struct Kv4Attn {
   int causal;
   int window;       // keys before position - window + 1 are not seen; 0: all are
   int splits;       // of the tokens, over the grid
-  int ct;           // tiles per split step, a power of two, at least WKV
   float* po;        // (splits, T, Hq, D) partial outputs
   float* pml;       // (splits, T, Hq, 2) their maximum and sum
 };
 
-// How a call is cut: columns per wave, waves over the tokens, splits.
+// How a call is cut. few: 16 columns and the waves of a workgroup over the tokens; else nq * 16 columns per
+// wave, the waves side by side.
 struct Kv4Plan {
-  int nq, wkv, splits, ct;
-  int64_t qgrid;
+  bool few;
+  int nq;
+  int splits;      // of the tokens, over the grid
+  int64_t qgrid;   // tiles of columns per sequence and head
 };
 
 // rows [start, start + n) of sequence b, kept inside the call's rows whatever cu holds

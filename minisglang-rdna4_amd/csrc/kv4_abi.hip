@@ -126,6 +126,7 @@ int w4a8_kv4_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_
   if (rc) return rc;
   if (Hq < H || Hq % H || Hq > 65535)
     return fail(kErrInvalid, "%s: %lld query heads for %lld key/value heads", who, (long long)Hq, (long long)H);
+  if (!(scale > 0.f && scale < 1e30f)) return fail(kErrInvalid, "%s: the softmax scale must be positive", who);
   if (T * Hq > 0x3fffffff)  // queries times heads are columns, indexed in 32 bits
     return fail(kErrUnsupported, "%s: past its index ranges (T=%lld, %lld query heads)", who, (long long)T, (long long)Hq);
   if (window < 0 || window > 0x7fffffff || max_q < 0 || max_kv < 0 || max_q > 0x7fffffff || max_kv > 0x7fffffff)
