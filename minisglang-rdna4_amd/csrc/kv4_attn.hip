@@ -3,49 +3,218 @@
 // Per key/value head, the queries that share it are the columns of the matrix products: column c is
 // query c / G, query head h * G + c % G. A wave takes 16 NQ columns and walks tiles of 32 tokens, with
 // one pass over the cache and the running maximum and sum of the softmax in f32:
-//   S = U Q^T      U = 16 + c: the codes as bf16/fp16 numbers 16..31, made by a shift and an and-or for
-//                  two codes, exact in either type. The accumulators start at -16 sum(q), so S is q c;
-//   x = s S + m sum(q)                       the score, with nothing rounded but f32 sums;
-//   O += (p s)^T U, C += p (m - 16 s)        out = (O + C) / sum p.
-// p s enters its product as the sum of two bf16 terms (rounded by at most 2^-18 of itself: one term would
-// cost as much accuracy as the output's own rounding), with U in bf16 whatever the model's type, so that
-// a small V step does not fall below fp16's range.
+//   S = c Q^T,   x = s S + m sum(q),   p = 2^(x scale - M),   O += (p s)^T c,   C += p m,   out = (O + C) / sum p.
+// Codes. A code in an fp16 number's lowest bits is the subnormal c 2^-24, four bits higher c 2^-20: a shift
+// and four ands turn the 8 codes of a word into an fp16 operand, with no offset and no rounding (the matrix
+// units keep subnormals). The other operand carries the 2^-4 of the higher codes, the sums the 2^24.
+// Queries enter in fp16 for either model type: a power of two per row puts their largest value at 2^14, so
+// values down to 2^-28 of it are exact.
+// p s enters in fp16: for fp16 models as two terms (22 bits), for bf16 models as one, w, rounded by 2^-12
+// of itself. So that this error meets c - 7.5, and not the whole of c, bf16 models sum
+// O - 7.5 sum w + sum p (m + 7.5 s), sum w by one more product with a row of ones: the error is within 2^-12
+// of half a V vector's range, an eighth of the output's own rounding. So that p s stays in fp16's range
+// whatever V's steps are, p carries 2^-e, 2^e about the largest step so far over 64: it moves with the running
+// maximum and drops out of the quotient.
 // The row of S that a lane of group g = lane / 16 holds is chosen to be the token whose V codes that
 // lane holds (tokens 8 g + r in the first 16 rows' register r, 8 g + 4 + r in the second's), so p goes
 // from one product into the next in its lane, and nothing passes through LDS.
 // The running maximum is raised only when a score passes it by 8 (in powers of two): p stays below 2^8,
 // and most tiles need no exchange between lanes and no rescaling.
 //
-// Split: WKV waves of a workgroup (and the splits of the grid) walk the same columns over different
-// tiles; their (O, C, sum, max) are joined through LDS, and those of the splits through the workspace
-// by kv4_join_kernel.
-#include "kv4_attn.h"
+// WKV = 4 (decode): the waves of a workgroup walk the same 16 columns over different tiles and join through
+// LDS. WKV = 1 (more than 16 columns): each wave has columns of its own; the waves read the same tiles at about
+// the same time, and share them in the caches. Where that leaves the card empty the grid splits the tokens
+// too, and kv4_join_kernel joins the parts.
+#include "kv4.h"
 
 namespace w4a8 {
 
-void launch_kv4_prompt(const Kv4Attn& p, int D, int dtype, int nq, dim3 grid, hipStream_t st);
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef uint32_t v4w __attribute__((ext_vector_type(4)));
 
-// Decode: 16 columns, the 4 waves of a workgroup (and the splits of the grid) over the tokens.
+__device__ __forceinline__ v4f mfma16(const v4w& a, const v4w& b, const v4f& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// The codes of a word as fp16 subnormals: register r holds codes r and r + 4, times 2^-24 for even r, 2^-20 for odd
+__device__ __forceinline__ v4w widen(uint32_t w) {
+  const uint32_t u = w >> 8;
+  return v4w{w & 0x000f000fu, w & 0x00f000f0u, u & 0x000f000fu, u & 0x00f000f0u};
+}
+
+// the same value over the four lanes that hold a column (xor 16 and xor 32)
+__device__ __forceinline__ float col_max(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float col_sum(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    w[0] = u.x; w[1] = u.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p + 4 * i);
+      w[i] = u.x; w[i + 1] = u.y; w[i + 2] = u.z; w[i + 3] = u.w;
+    }
+  }
+}
+
+// The page numbers of a tile, wave-uniform: those of its tokens 0..15 and 16..31 (a page holds at least 16),
+// as the table has them, -1 where it has none. Looked up a tile before they are used: the scalar loads
+// then have nobody waiting. (Nothing writes the table during a launch: constant address space.)
+typedef const int32_t __attribute__((address_space(4))) * Table;
+struct Pages {
+  int a, b;
+};
+__device__ __forceinline__ Pages look_up(const Kv4Attn& p, Table table, int t, int len) {
+  Pages r = {-1, -1};
+  const int i = t >> p.c.shift, j = (t + 16) >> p.c.shift;
+  if (t < len && i < p.s.width) r.a = table[i];
+  if (t + 16 < len && j < p.s.width) r.b = table[j];
+  return r;
+}
+__device__ __forceinline__ bool exists(const Kv4Attn& p, int page) { return (uint32_t)page < (uint32_t)p.c.pages; }
+// block `i` of 4 of the tile at t: this lane's; a missing page reads block 0, which is there, and its values
+// are not used
+__device__ __forceinline__ uint32_t pick(const Kv4Attn& p, const Pages& pg, int h, int t, int i) {
+  const int a = exists(p, pg.a) ? kv4_block(p.c, pg.a, h, t) : 0, b = exists(p, pg.b) ? kv4_block(p.c, pg.b, h, t + 16) : 0;
+  return (uint32_t)((i < 2 ? a : b) + (i & 1));
+}
+
+template <int DT>
+__device__ __forceinline__ float lo16(uint32_t w) {
+  return DT == kBF16 ? __uint_as_float(w << 16) : f16_to_f32((uint16_t)(w & 0xffffu));
+}
+template <int DT>
+__device__ __forceinline__ float hi16(uint32_t w) {
+  return DT == kBF16 ? __uint_as_float(w & 0xffff0000u) : f16_to_f32((uint16_t)(w >> 16));
+}
+
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2h));
+}
+
+// A sequence of the call: its rows and its length. Columns are its queries in order, G heads each.
+struct Span {
+  int64_t start;
+  int n, cols, len, first_pos;  // new tokens, columns, length, position of the first new token
+};
+__device__ __forceinline__ Span kv4_span(const Kv4Attn& p, int b) {
+  Span s;
+  kv4_rows(p.s, b, s.start, s.n);
+  s.cols = s.n * p.G;
+  const int64_t cap = (int64_t)p.s.width << p.c.shift;
+  const int len = p.s.lens[b];
+  // one token past the table's end stands for all of them: its page is missing
+  s.len = len > cap ? (int)(cap + 1 < 0x7fffffff ? cap + 1 : 0x7fffffff) : len < 0 ? 0 : len;
+  s.first_pos = len - s.n;
+  return s;
+}
+// the keys [from, upto) that query i of the span sees
+__device__ __forceinline__ int seen_from(const Kv4Attn& p, const Span& s, int i) {
+  return p.window ? min(max(s.first_pos + i - p.window + 1, 0), s.len) : 0;
+}
+__device__ __forceinline__ int seen_upto(const Kv4Attn& p, const Span& s, int i) {
+  return p.causal ? min(max(s.first_pos + i + 1, 0), s.len) : s.len;
+}
+// The keys that some, [lo, hi), and that all, [lo_all, hi_all), of columns c0 .. c1 - 1 see: columns are queries
+// in order, so the first and the last one tell.
+struct Keys {
+  int lo, hi, lo_all, hi_all;
+};
+__device__ __forceinline__ Keys kv4_keys(const Kv4Attn& p, const Span& s, int c0, int c1) {
+  if (c0 >= c1) return {0, 0, 0, 0};
+  const int i0 = c0 / p.G, i1 = (c1 - 1) / p.G;
+  return {seen_from(p, s, i0), seen_upto(p, s, i1), seen_from(p, s, i1), seen_upto(p, s, i0)};
+}
+// Of the wave's columns c0 .. : the query, from its first column's i0 = c0 / G, r0 = c0 % G, and its head
+__device__ __forceinline__ int kv4_query(const Kv4Attn& p, int i0, int r0, int x, int& head) {
+  const int c = r0 + x, i = (int)__umulhi((uint32_t)c << 1, p.gmul);
+  head = c - i * p.G;
+  return i0 + i;
+}
+
+template <int DT>
+__device__ __forceinline__ void unpack_query(const uint4& u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = lo16<DT>(w[i]);
+    f[2 * i + 1] = hi16<DT>(w[i]);
+  }
+}
+
+// One lane's DB neighbouring channels of a column, from channel `d0` of (row, head): the output, or the split's
+// part for kv4_join_kernel. m: the maximum in powers of two; first: this lane writes the column's statistics.
 template <int D, int DT>
-__global__ void __launch_bounds__(256, D == 256 ? 2 : 3)
-kv4_decode_kernel(const Kv4Attn p) {
+__device__ __forceinline__ void kv4_store(const Kv4Attn& p, int split, int64_t row, int head, int d0, const float (&v)[D / 16],
+                                          float m, float sum, bool first) {
+  constexpr int DB = D / 16;
+  const int Hq = p.c.H * p.G;
+  if (p.splits > 1) {
+    const int64_t at = ((int64_t)split * p.s.T + row) * Hq + head;
+    float* op = p.po + at * D + d0;
+#pragma unroll
+    for (int d = 0; d < DB; d += 4) *reinterpret_cast<v4f*>(op + d) = v4f{v[d], v[d + 1], v[d + 2], v[d + 3]};
+    if (first) {
+      p.pml[at * 2] = m;
+      p.pml[at * 2 + 1] = sum;
+    }
+    return;
+  }
+  // no key seen: the sum is 0, the output 0
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* op = p.out + row * p.ldo + head * p.ho + d0;
+#pragma unroll
+  for (int d = 0; d < DB; d += 4) {
+    uint2 u;
+    u.x = (uint32_t)to_dtype(v[d] * inv, DT) | ((uint32_t)to_dtype(v[d + 1] * inv, DT) << 16);
+    u.y = (uint32_t)to_dtype(v[d + 2] * inv, DT) | ((uint32_t)to_dtype(v[d + 3] * inv, DT) << 16);
+    *reinterpret_cast<uint2*>(op + d) = u;
+  }
+  if (p.lse && first) p.lse[row * Hq + head] = sum == 0.f ? -__builtin_inff() : m * 0.69314718055994531f + logf(sum);
+}
+
+// D: channels; DT: the model's type; NQ: blocks of 16 columns per wave; WKV: waves of a workgroup that share
+// their columns
+template <int D, int DT, int NQ, int WKV>
+__global__ void __launch_bounds__(256, WKV == 1 ? 2 : D == 256 ? 2 : 3)
+kv4_attn_kernel(const Kv4Attn p) {
+  static_assert(WKV == 1 || (WKV == 4 && NQ == 1), "side by side, or one block of columns");
   constexpr int KS = D / 32, DB = D / 16;  // products per S tile, blocks of 16 channels
+  constexpr int W = DT == kF16 ? 2 : 1;    // fp16 terms of p s
+  constexpr int kCols = 16 * NQ * (WKV == 1 ? 4 : 1);
+  constexpr float kInf = __builtin_inff();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
   const int h = blockIdx.y, b = blockIdx.z;
   const int split = blockIdx.x % p.splits;
   const Span sp = kv4_span(p, b);
-  const float slack = 8.f / p.scale;
-  __shared__ float red_o[4 * 16 * D];
-  __shared__ float red_ml[4 * 16 * 2];
+  const Table table = (Table)(uintptr_t)(p.s.table + b * p.s.ldt);
+  __shared__ float red_o[WKV == 1 ? 1 : 4 * 16 * D];
+  __shared__ float red_ml[WKV == 1 ? 1 : 4 * 16 * 2];
 
-  const int qtiles = (sp.cols + 15) / 16;
+  const int qtiles = (sp.cols + kCols - 1) / kCols;
   const int gq = gridDim.x / p.splits;
   for (int qi = blockIdx.x / p.splits; qi < qtiles; qi += gq) {
-    const int c0 = qi * 16;
-    const Keys ks = kv4_keys(p, sp, c0, min(c0 + 16, sp.cols));
+    // the last columns have the most keys: first
+    const int c0 = (qtiles - 1 - qi) * kCols + (WKV == 1 ? wave * 16 * NQ : 0);
+    const Keys ks = kv4_keys(p, sp, c0, min(c0 + 16 * NQ, sp.cols));
     const int t_first = ks.lo >> 5, nt = ks.lo < ks.hi ? ((ks.hi + 31) >> 5) - t_first : 0;
-    const Table table = (Table)(uintptr_t)(p.s.table + b * p.s.ldt);
+    auto token = [&](int t) { return (t_first + t) * 32; };
     // Each part of the next tile is loaded into the registers of this one's as soon as they are free.
     uint32_t kw[2][KS], vw[DB], ksw[8], vsw[8];
     auto load_k = [&](const Pages& pg, int t) {
@@ -62,45 +231,78 @@ kv4_decode_kernel(const Kv4Attn p) {
       load_words(reinterpret_cast<const uint8_t*>(p.c.vs) + o, vsw);
     };
     // tiles are dealt out one by one, over the splits and their waves: all have the same share of a sequence
-    const int step = p.splits * 4;
-    int t = split * 4 + wave;
+    const int step = p.splits * WKV;
+    int t = split * WKV + (WKV == 1 ? 0 : wave);
     int tn = t + step;
-    auto token = [&](int t) { return (t_first + t) * 32; };
     Pages at = {-1, -1}, nat = {-1, -1};
     if (t < nt) at = look_up(p, table, token(t), ks.hi);
     if (tn < nt) nat = look_up(p, table, token(tn), ks.hi);
 
-    // this lane's query
-    const int i0 = c0 / p.G;
-    int head;
-    const int qry = kv4_query(p, i0, c0 - i0 * p.G, col, head);
-    head += h * p.G;
-    const bool on = c0 + col < sp.cols;
-    const int klo = seen_from(p, sp, qry), khi = on ? seen_upto(p, sp, qry) : 0;
-    uint4 qr[KS];
-    {
-      const uint16_t* qp = p.q + (sp.start + (on ? qry : 0)) * p.ldq + (on ? head : 0) * p.hq + g * (D / 4);
+    // this lane's queries: columns 16 j + col
+    const int i0 = c0 / p.G, r0 = c0 - i0 * p.G;
+    int klo[NQ], khi[NQ];
+    uint4 qr[NQ][KS];
 #pragma unroll
-      for (int w = 0; w < KS; ++w) qr[w] = on ? *reinterpret_cast<const uint4*>(qp + 8 * w) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < NQ; ++j) {
+      int head;
+      const int i = kv4_query(p, i0, r0, 16 * j + col, head);
+      const bool on = c0 + 16 * j + col < sp.cols;
+      khi[j] = on ? seen_upto(p, sp, i) : 0;
+      klo[j] = seen_from(p, sp, i);
+      const uint16_t* qp = p.q + (sp.start + (on ? i : 0)) * p.ldq + (h * p.G + (on ? head : 0)) * p.hq + g * (D / 4);
+#pragma unroll
+      for (int w = 0; w < KS; ++w) qr[j][w] = on ? *reinterpret_cast<const uint4*>(qp + 8 * w) : make_uint4(0, 0, 0, 0);
     }
     if (t < nt) {
       load_k(at, token(t));
       load_s(at, token(t));
       load_v(at, token(t));
     }
-    v4w qf[KS];
-    float qs = 0.f;
+    v4w qf[NQ][KS];
+    float qs[NQ], sc[NQ], slack[NQ];  // sum(q) and x's factor, in the products' units, and 8 powers of two there
 #pragma unroll
-    for (int w = 0; w < KS; ++w) {
-      qf[w] = query_operand(qr[w]);
-      qs += sum8<DT>(qr[w]);
+    for (int j = 0; j < NQ; ++j) {
+      float sum = 0.f, top = 0.f;
+#pragma unroll
+      for (int w = 0; w < KS; ++w) {
+        float f[8];
+        unpack_query<DT>(qr[j][w], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          sum += f[e];
+          top = fmaxf(top, fabsf(f[e]));
+        }
+      }
+      top = col_max(top);
+      // 2^eq puts the largest value into [2^14, 2^15)
+      const int eq = max(141 - (int)(__float_as_uint(top) >> 23), -100);
+      qs[j] = __builtin_ldexpf(col_sum(sum), eq - 24);
+      sc[j] = __builtin_ldexpf(p.scale, 24 - eq);
+      slack[j] = 8.f / sc[j];
+#pragma unroll
+      for (int w = 0; w < KS; ++w) {
+        float f[8];
+        unpack_query<DT>(qr[j][w], f);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int er = r & 1 ? eq - 4 : eq;
+          qf[j][w][r] = pack_f16(__builtin_ldexpf(f[r], er), __builtin_ldexpf(f[r + 4], er));
+        }
+      }
     }
-    qs = col_sum(qs);
 
-    v4f o[DB];
-    float m = -__builtin_inff(), mu = 0.f, l = 0.f, cc = 0.f;  // mu: m in powers of two, 0 while no key was seen
+    v4f o[NQ][DB], ws[NQ];                // ws: sum w (bf16 models), in every register
+    float m[NQ], mu[NQ], l[NQ], cc[NQ];   // mu: M, the maximum in powers of two (0 while no key was seen) plus e
+    int ex = -46;                         // e
+    float lim = -1.f;                     // steps up to here are in e's range; none was seen yet
 #pragma unroll
-    for (int d = 0; d < DB; ++d) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NQ; ++j) {
+      m[j] = -kInf;
+      mu[j] = l[j] = cc[j] = 0.f;
+      ws[j] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[j][d] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
 
     while (t < nt) {
       const int t0 = token(t);
@@ -108,65 +310,106 @@ kv4_decode_kernel(const Kv4Attn p) {
       Pages nnat = {-1, -1};
       if (tnn < nt) nnat = look_up(p, table, token(tnn), ks.hi);
 
-      const float q16 = -16.f * qs;
-      v4f s[2] = {v4f{q16, q16, q16, q16}, v4f{q16, q16, q16, q16}};
+      v4f s[NQ][2];
 #pragma unroll
-      for (int w = 0; w < KS; ++w) {
-        s[0] = mfma16<DT>(widen<DT>(kw[0][w]), qf[w], s[0]);
-        s[1] = mfma16<DT>(widen<DT>(kw[1][w]), qf[w], s[1]);
-      }
+      for (int j = 0; j < NQ; ++j) s[j][0] = s[j][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < KS; ++w)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const v4w a = widen(kw[z][w]);
+#pragma unroll
+          for (int j = 0; j < NQ; ++j) s[j][z] = mfma16(a, qf[j][w], s[j][z]);
+        }
       if (tn < nt) load_k(nat, token(tn));
 
-      float y[8], sv[8], mv[8];
+      float y[NQ][8], sv[8], mv[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        y[i] = __builtin_fmaf(lo16<DT>(ksw[i]), s[i >> 2][i & 3], hi16<DT>(ksw[i]) * qs);
+        const float sk = lo16<DT>(ksw[i]), mk = hi16<DT>(ksw[i]);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) y[j][i] = __builtin_fmaf(sk, s[j][i >> 2][i & 3], mk * qs[j]);
         sv[i] = lo16<DT>(vsw[i]);
-        mv[i] = __builtin_fmaf(-16.f, sv[i], hi16<DT>(vsw[i]));
+        mv[i] = W == 1 ? __builtin_fmaf(7.5f, sv[i], hi16<DT>(vsw[i])) : hi16<DT>(vsw[i]);
       }
       if (!(t0 >= ks.lo_all && t0 + 32 <= ks.hi_all && exists(p, at.a) && exists(p, at.b))) {
-        // an unseen token's scale may be anything, and 0 times it is not 0; a missing page is NaN to whoever sees it
-        const int a = klo - (t0 + 8 * g), e = khi - (t0 + 8 * g);
+        // An unseen token's scale may be anything, and 0 times it is not 0: what is not finite, and a missing page,
+        // is NaN in the score of whoever sees it, and 0 here.
         const bool missing = !exists(p, g < 2 ? at.a : at.b);
+        const int tb = t0 + 8 * g;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const bool see = i >= a && i < e;
-          y[i] = !see ? -__builtin_inff() : missing ? __builtin_nanf("") : y[i];
-          sv[i] = see ? sv[i] : 0.f;
-          mv[i] = see ? mv[i] : 0.f;
+          const bool bad = missing || !__builtin_isfinite(sv[i]) || !__builtin_isfinite(mv[i]);
+          sv[i] = bad ? 0.f : sv[i];
+          mv[i] = bad ? 0.f : mv[i];
+          if (tb + i < ks.lo || tb + i >= ks.hi) sv[i] = 0.f;  // not a step to scale by
+#pragma unroll
+          for (int j = 0; j < NQ; ++j)
+            y[j][i] = tb + i >= klo[j] && tb + i < khi[j] ? (bad ? __builtin_nanf("") : y[j][i]) : -kInf;
         }
       }
-      const float top = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
-      if (__ballot(top > m + slack)) {
-        const float mn = fmaxf(m, col_max(top));
-        const float f = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((m - mn) * p.scale);
-        m = mn;
-        mu = mn == -__builtin_inff() ? 0.f : mn * p.scale;
-        l *= f;
-        cc *= f;
+      auto top8 = [](const float (&v)[8]) {
+        return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+      };
+      const float ts = top8(sv);
+      float top[NQ];
+      bool up = ts > lim;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) o[d] *= f;
+      for (int j = 0; j < NQ; ++j) {
+        top[j] = top8(y[j]);
+        up = up || top[j] > m[j] + slack[j];
       }
-      float ps[8];
+      if (__ballot(up)) {
+        // 2^-e takes the largest step to [2^5, 2^6); steps that 2^-40 bounds stay below
+        const int te = (int)((__float_as_uint(wave_max(ts)) >> 23) & 255u) - 132;
+        const int en = __builtin_amdgcn_readfirstlane(min(max(te, ex), 94));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(y[i], p.scale, -mu));
-        l += pr;
-        ps[i] = pr * sv[i];
-        cc = __builtin_fmaf(pr, mv[i], cc);
+        for (int j = 0; j < NQ; ++j) {
+          const float mn = fmaxf(m[j], col_max(top[j]));
+          const float mun = (mn == -kInf ? 0.f : mn * sc[j]) + (float)en;
+          const float f = m[j] == -kInf ? 1.f : __builtin_amdgcn_exp2f(mu[j] - mun);  // nothing summed yet: any
+          m[j] = mn;
+          mu[j] = mun;
+          l[j] *= f;
+          cc[j] *= f;
+          ws[j] *= f;
+#pragma unroll
+          for (int d = 0; d < DB; ++d) o[j][d] *= f;
+        }
+        ex = en;
+        lim = __uint_as_float((uint32_t)(ex + 6 + 127) << 23);
       }
-      v4w ph, pl;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        ph[r] = pack_bf16(ps[r], ps[r + 4]);
-        pl[r] = pack_bf16(ps[r] - __uint_as_float(ph[r] << 16), ps[r + 4] - __uint_as_float(ph[r] & 0xffff0000u));
+      for (int i = 1; i < 8; i += 2) sv[i] *= 0.0625f;  // the higher codes
+      v4w ph[NQ], pl[NQ];
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        float ps[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j][i], sc[j], -mu[j]));
+          l[j] += pr;
+          cc[j] = __builtin_fmaf(pr, mv[i], cc[j]);
+          ps[i] = pr * sv[i];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          ph[j][r] = pack_f16(ps[r], ps[r + 4]);
+          if (W == 2)
+            pl[j][r] = pack_f16(ps[r] - f16_to_f32((uint16_t)(ph[j][r] & 0xffffu)), ps[r + 4] - f16_to_f32((uint16_t)(ph[j][r] >> 16)));
+        }
+        // sum w: ones, sixteens against the higher codes' 1/16
+        if (W == 1) ws[j] = mfma16(v4w{0x3c003c00u, 0x4c004c00u, 0x3c003c00u, 0x4c004c00u}, ph[j], ws[j]);
       }
       if (tn < nt) load_s(nat, token(tn));
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        const v4w a = widen<kBF16>(vw[d]);
-        o[d] = mfma16<kBF16>(a, ph, o[d]);
-        o[d] = mfma16<kBF16>(a, pl, o[d]);
+        const v4w a = widen(vw[d]);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+          o[j][d] = mfma16(a, ph[j], o[j][d]);
+          if (W == 2) o[j][d] = mfma16(a, pl[j], o[j][d]);
+        }
       }
       if (tn < nt) load_v(nat, token(tn));
       at = nat;
@@ -175,31 +418,58 @@ kv4_decode_kernel(const Kv4Attn p) {
       tn = tnn;
     }
 
-    l = col_sum(l);
-    cc = col_sum(cc);
-    // join the waves through LDS, each to the common maximum; wave r then sums and writes the channels of r
-    if (g == 0) {
-      red_ml[(wave * 16 + col) * 2] = m * p.scale;
-      red_ml[(wave * 16 + col) * 2 + 1] = l;
+    // O in the codes' units is 2^24 times the products' sum
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+      l[j] = col_sum(l[j]);
+      cc[j] = col_sum(cc[j]) - (W == 1 ? 7.5f * ws[j][0] : 0.f);
+      if (m[j] == -kInf) mu[j] = -kInf;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[j][d][r] = __builtin_fmaf(o[j][d][r], 16777216.f, cc[j]);
     }
+    auto store = [&](int j, int r, const float (&v)[DB], float mx, float sum) {
+      int head;
+      const int i = kv4_query(p, i0, r0, 16 * j + col, head);
+      // a lane's channels: DB (4 g + r) + d of its column
+      if (c0 + 16 * j + col < sp.cols)
+        kv4_store<D, DT>(p, split, sp.start + i, h * p.G + head, (4 * g + r) * DB, v, mx, sum, g == 0 && r == 0);
+    };
+    if constexpr (WKV == 1) {
 #pragma unroll
-    for (int d = 0; d < DB; ++d) *reinterpret_cast<v4f*>(&red_o[((wave * DB + d) * 64 + lane) * 4]) = o[d] + cc;
-    __syncthreads();
-    float mw[4], mx = -__builtin_inff(), sum = 0.f, v[DB];
+      for (int j = 0; j < NQ; ++j)
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, mw[w] = red_ml[(w * 16 + col) * 2]);
+        for (int r = 0; r < 4; ++r) {
+          float v[DB];
 #pragma unroll
-    for (int d = 0; d < DB; ++d) v[d] = 0.f;
+          for (int d = 0; d < DB; ++d) v[d] = o[j][d][r];
+          store(j, r, v, mu[j], l[j]);
+        }
+    } else {
+      // join the waves through LDS, each to the common maximum; wave r then sums and writes the channels of r
+      if (g == 0) {
+        red_ml[(wave * 16 + col) * 2] = mu[0];
+        red_ml[(wave * 16 + col) * 2 + 1] = l[0];
+      }
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = mx == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mw[w] - mx);
-      sum += f * red_ml[(w * 16 + col) * 2 + 1];
+      for (int d = 0; d < DB; ++d) *reinterpret_cast<v4f*>(&red_o[((wave * DB + d) * 64 + lane) * 4]) = o[0][d];
+      __syncthreads();
+      float mw[4], mx = -kInf, sum = 0.f, v[DB];
 #pragma unroll
-      for (int d = 0; d < DB; ++d) v[d] += f * red_o[((w * DB + d) * 64 + lane) * 4 + wave];
+      for (int w = 0; w < 4; ++w) mx = fmaxf(mx, mw[w] = red_ml[(w * 16 + col) * 2]);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) v[d] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = mx == -kInf ? 0.f : __builtin_amdgcn_exp2f(mw[w] - mx);
+        sum += f * red_ml[(w * 16 + col) * 2 + 1];
+#pragma unroll
+        for (int d = 0; d < DB; ++d) v[d] += f * red_o[((w * DB + d) * 64 + lane) * 4 + wave];
+      }
+      store(0, wave, v, mx, sum);
+      __syncthreads();  // before the next tile of columns writes LDS
     }
-    // a lane's channels: DB (4 g + r) + d of its column
-    if (on) kv4_store<D, DT>(p, split, sp.start + qry, head, (4 * g + wave) * DB, v, mx, sum, g == 0 && wave == 0);
-    __syncthreads();  // before the next tile of columns writes LDS
   }
 }
 
@@ -281,8 +551,9 @@ int64_t kv4_workspace(int64_t T, int Hq, int D, int splits) {
 template <int D, int DT>
 static int launch_dt(Kv4Attn& p, const Kv4Plan& pl, hipStream_t st) {
   const dim3 g((unsigned)(pl.qgrid * pl.splits), (unsigned)p.c.H, (unsigned)p.s.B), b(256);
-  if (pl.few) hipLaunchKernelGGL((kv4_decode_kernel<D, DT>), g, b, 0, st, p);
-  else launch_kv4_prompt(p, D, DT, pl.nq, g, st);
+  if (pl.few) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 4>), g, b, 0, st, p);
+  else if (pl.nq == 1) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 1>), g, b, 0, st, p);
+  else hipLaunchKernelGGL((kv4_attn_kernel<D, DT, D == 256 ? 1 : 2, 1>), g, b, 0, st, p);
   if (hipGetLastError() != hipSuccess) return kErrHip;
   if (pl.splits > 1) {
     const int64_t rows = p.s.T * p.c.H * p.G;
