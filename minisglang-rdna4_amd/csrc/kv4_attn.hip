@@ -523,24 +523,34 @@ kv4_join_kernel(const Kv4Attn p) {
   if (p.lse && lane == 0) p.lse[id] = l == 0.f ? -__builtin_inff() : mn * 0.69314718055994531f + logf(l);
 }
 
+// Splits of the tokens. Decode (3 workgroups of 4 waves per CU, 768 on the card): one round of the card, and up to
+// four per sequence and head where that many more workgroups even out sequences of different lengths; a split has
+// 8 tiles, two for each wave, and the first 8 are not worth the join's launch. us, with the splits that
+// this gives / without: 64 sequences of up to 8192 tokens x 8 heads 77 / 139, 16 of 4000 21 / 34, one of 8000
+// 13 / 40, two of 131072 64 / 800; 48 of 500 11 (unsplit) / 14 in two.
+// More columns (2 workgroups of 32-column waves per CU, 512; 16-column waves 1024): as many rounds, up to four
+// splits below one round. us: 512 new tokens on 8192 127 / 265, 7 chunks of 257 on up to 6001 137 / 194, 16 x 8 new
+// tokens on 4096 37 / 134; one prompt of 2048 fills the card, 112 (unsplit) / 120 in two.
 Kv4Plan kv4_plan(int64_t T, int B, int H, int G, int D, int64_t max_q, int64_t max_kv) {
   Kv4Plan pl;
   // a bound below the mean is wrong; the workspace would grow with it
   if (max_q < (T + B - 1) / B) max_q = (T + B - 1) / B;
   const int64_t cols = max_q * G;
   pl.few = cols <= 16;
-  // the prompt kernel's columns per wave: 32, or 16 where those of a workgroup cover a sequence's, and for 256
-  // channels, whose 32 would not fit the registers of two waves per SIMD
-  pl.nq = D == 256 || cols <= 64 ? 1 : 2;
+  // 32 columns a wave, or 16 where those of a workgroup cover a sequence's, and for 256 channels, whose 32 would
+  // not fit the registers of two waves per SIMD
+  pl.nq = pl.few || D == 256 || cols <= 64 ? 1 : 2;
   const int64_t per = pl.few ? 16 : 64 * pl.nq;
   pl.qgrid = (cols + per - 1) / per;
   const int64_t pairs = pl.qgrid * H * B, tiles = (max_kv + 31) / 32;
-  // a tile per wave at least
-  const int64_t most = pl.few ? (tiles + 3) / 4 : tiles;
-  int64_t s = pl.few ? 2048 / pairs : 512 / pairs;
-  if (s > (pl.few ? 48 : 8)) s = pl.few ? 48 : 8;
-  if (s > most) s = most;
-  pl.splits = s < 1 ? 1 : (int)s;
+  auto most = [](int64_t a, int64_t b) { return a > b ? a : b; };
+  auto least = [](int64_t a, int64_t b) { return a < b ? a : b; };
+  const int64_t round = pl.few ? 768 : pl.nq == 2 ? 512 : 1024;
+  int64_t s = round / pairs;
+  if (pl.few || pairs < round) s = most(s, least(4, 2048 / pairs));
+  s = least(s, pl.few ? tiles / 8 - 1 : tiles / 8);
+  s = least(s, least(64, most(16, tiles / 64)));  // kv4_join_kernel has a lane per split
+  pl.splits = (int)most(s, 1);
   return pl;
 }
 
