@@ -70,26 +70,40 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
-// The page numbers of a tile, wave-uniform: those of its tokens 0..15 and 16..31 (a page holds at least 16),
-// as the table has them, -1 where it has none. Looked up a tile before they are used: the scalar loads
-// then have nobody waiting. (Nothing writes the table during a launch: constant address space.)
+// The page numbers of a tile, wave-uniform: those of its tokens 0..15 and 16..31 (a page holds at least 16), as
+// the table has them, -1 past its end. Looked up a tile before they are used: the scalar loads then have
+// nobody waiting. (Nothing writes the table during a launch: constant address space.)
 typedef const int32_t __attribute__((address_space(4))) * Table;
 struct Pages {
   int a, b;
 };
 __device__ __forceinline__ Pages look_up(const Kv4Attn& p, Table table, int t, int len) {
-  Pages r = {-1, -1};
-  const int i = t >> p.c.shift, j = (t + 16) >> p.c.shift;
-  if (t < len && i < p.s.width) r.a = table[i];
-  if (t + 16 < len && j < p.s.width) r.b = table[j];
+  const int i = t >> p.c.shift;
+  Pages r;
+  r.a = r.b = i < p.s.width ? table[i] : -1;
+  // a tile of longer pages lies in one; slots past the sequence's end may be read there, not used
+  if (p.c.shift == 4) r.b = t + 16 < len && i + 1 < p.s.width ? table[i + 1] : -1;
   return r;
 }
-__device__ __forceinline__ bool exists(const Kv4Attn& p, int page) { return (uint32_t)page < (uint32_t)p.c.pages; }
-// block `i` of 4 of the tile at t: this lane's; a missing page reads block 0, which is there, and its values
-// are not used
-__device__ __forceinline__ uint32_t pick(const Kv4Attn& p, const Pages& pg, int h, int t, int i) {
-  const int a = exists(p, pg.a) ? kv4_block(p.c, pg.a, h, t) : 0, b = exists(p, pg.b) ? kv4_block(p.c, pg.b, h, t + 16) : 0;
-  return (uint32_t)((i < 2 ? a : b) + (i & 1));
+// The tile's blocks: of tokens 0..15 and of 16..31, each with the next one. A missing page reads block 0, which is
+// there, and its values are not used.
+struct Blocks {
+  uint32_t a, b;
+  bool has_a, has_b;
+};
+__device__ __forceinline__ Blocks blocks_of(const Kv4Attn& p, const Pages& pg, int h, int t) {
+  Blocks r;
+  r.has_a = (uint32_t)pg.a < (uint32_t)p.c.pages;
+  r.has_b = (uint32_t)pg.b < (uint32_t)p.c.pages;
+  r.a = r.has_a ? (uint32_t)kv4_block(p.c, pg.a, h, t) : 0;
+  r.b = r.has_b ? (p.c.shift == 4 ? (uint32_t)kv4_block(p.c, pg.b, h, t + 16) : r.a + 2) : 0;
+  return r;
+}
+// block `i` of 4 of the tile: this lane's
+// (values, not b's members: a choice of members is one of addresses, which the compiler would make in LDS)
+__device__ __forceinline__ uint32_t pick(const Blocks& b, int i) {
+  const uint32_t x = b.a, y = b.b;
+  return (i < 2 ? x : y) + (i & 1);
 }
 
 template <int DT>
@@ -217,16 +231,14 @@ kv4_attn_kernel(const Kv4Attn p) {
     auto token = [&](int t) { return (t_first + t) * 32; };
     // Each part of the next tile is loaded into the registers of this one's as soon as they are free.
     uint32_t kw[2][KS], vw[DB], ksw[8], vsw[8];
-    auto load_k = [&](const Pages& pg, int t) {
-      const uint8_t* kp = p.c.k + (uint64_t)pick(p, pg, h, t, (lane & 15) >> 2) * (4 * D) + ((lane & 3) * (D / 2) + g * (D / 8));
+    auto load_k = [&](const Blocks& bl) {
+      const uint8_t* kp = p.c.k + (uint64_t)pick(bl, (lane & 15) >> 2) * (4 * D) + ((lane & 3) * (D / 2) + g * (D / 8));
       load_words(kp, kw[0]);
       load_words(kp + 4 * (D / 2), kw[1]);
     };
-    auto load_v = [&](const Pages& pg, int t) {
-      load_words(p.c.v + (uint64_t)pick(p, pg, h, t, g) * (4 * D) + (lane & 15) * (D / 4), vw);
-    };
-    auto load_s = [&](const Pages& pg, int t) {
-      const uint64_t o = (uint64_t)pick(p, pg, h, t, g) * 32;
+    auto load_v = [&](const Blocks& bl) { load_words(p.c.v + (uint64_t)pick(bl, g) * (4 * D) + (lane & 15) * (D / 4), vw); };
+    auto load_s = [&](const Blocks& bl) {
+      const uint64_t o = (uint64_t)pick(bl, g) * 32;
       load_words(reinterpret_cast<const uint8_t*>(p.c.ks) + o, ksw);
       load_words(reinterpret_cast<const uint8_t*>(p.c.vs) + o, vsw);
     };
@@ -234,8 +246,8 @@ kv4_attn_kernel(const Kv4Attn p) {
     const int step = p.splits * WKV;
     int t = split * WKV + (WKV == 1 ? 0 : wave);
     int tn = t + step;
-    Pages at = {-1, -1}, nat = {-1, -1};
-    if (t < nt) at = look_up(p, table, token(t), ks.hi);
+    Pages first = {-1, -1}, nat = {-1, -1};
+    if (t < nt) first = look_up(p, table, token(t), ks.hi);
     if (tn < nt) nat = look_up(p, table, token(tn), ks.hi);
 
     // this lane's queries: columns 16 j + col
@@ -253,10 +265,11 @@ kv4_attn_kernel(const Kv4Attn p) {
 #pragma unroll
       for (int w = 0; w < KS; ++w) qr[j][w] = on ? *reinterpret_cast<const uint4*>(qp + 8 * w) : make_uint4(0, 0, 0, 0);
     }
+    Blocks at = blocks_of(p, first, h, token(t));
     if (t < nt) {
-      load_k(at, token(t));
-      load_s(at, token(t));
-      load_v(at, token(t));
+      load_k(at);
+      load_s(at);
+      load_v(at);
     }
     v4w qf[NQ][KS];
     float qs[NQ], sc[NQ], slack[NQ];  // sum(q) and x's factor, in the products' units, and 8 powers of two there
@@ -307,8 +320,9 @@ kv4_attn_kernel(const Kv4Attn p) {
     while (t < nt) {
       const int t0 = token(t);
       const int tnn = tn + step;
-      Pages nnat = {-1, -1};
-      if (tnn < nt) nnat = look_up(p, table, token(tnn), ks.hi);
+      const bool more = tn < nt;
+      const Blocks next = blocks_of(p, nat, h, token(tn));
+      if (tnn < nt) nat = look_up(p, table, token(tnn), ks.hi);
 
       v4f s[NQ][2];
 #pragma unroll
@@ -321,7 +335,7 @@ kv4_attn_kernel(const Kv4Attn p) {
 #pragma unroll
           for (int j = 0; j < NQ; ++j) s[j][z] = mfma16(a, qf[j][w], s[j][z]);
         }
-      if (tn < nt) load_k(nat, token(tn));
+      if (more) load_k(next);
 
       float y[NQ][8], sv[8], mv[8];
 #pragma unroll
@@ -332,10 +346,10 @@ kv4_attn_kernel(const Kv4Attn p) {
         sv[i] = lo16<DT>(vsw[i]);
         mv[i] = W == 1 ? __builtin_fmaf(7.5f, sv[i], hi16<DT>(vsw[i])) : hi16<DT>(vsw[i]);
       }
-      if (!(t0 >= ks.lo_all && t0 + 32 <= ks.hi_all && exists(p, at.a) && exists(p, at.b))) {
+      if (!(t0 >= ks.lo_all && t0 + 32 <= ks.hi_all && at.has_a && at.has_b)) {
         // An unseen token's scale may be anything, and 0 times it is not 0: what is not finite, and a missing page,
         // is NaN in the score of whoever sees it, and 0 here.
-        const bool missing = !exists(p, g < 2 ? at.a : at.b);
+        const bool ha = at.has_a, hb = at.has_b, missing = !(g < 2 ? ha : hb);
         const int tb = t0 + 8 * g;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -401,7 +415,7 @@ kv4_attn_kernel(const Kv4Attn p) {
         // sum w: ones, sixteens against the higher codes' 1/16
         if (W == 1) ws[j] = mfma16(v4w{0x3c003c00u, 0x4c004c00u, 0x3c003c00u, 0x4c004c00u}, ph[j], ws[j]);
       }
-      if (tn < nt) load_s(nat, token(tn));
+      if (more) load_s(next);
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
         const v4w a = widen(vw[d]);
@@ -411,9 +425,8 @@ kv4_attn_kernel(const Kv4Attn p) {
           if (W == 2) o[j][d] = mfma16(a, pl[j], o[j][d]);
         }
       }
-      if (tn < nt) load_v(nat, token(tn));
-      at = nat;
-      nat = nnat;
+      if (more) load_v(next);
+      at = next;
       t = tn;
       tn = tnn;
     }
