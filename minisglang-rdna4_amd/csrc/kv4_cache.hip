@@ -1,192 +1,265 @@
 // Writing new tokens into the 4-bit cache and reading tokens back (layout and formulas: kv4.h).
 //
-// A wave per (block of 8 tokens, head), found from the rows: the wave of the first new token in a block
-// does that block's new tokens, the waves of the others return. V's words hold 8 tokens each, so this
-// wave is the only writer of its words; tokens of the block that are not new keep their nibbles.
-// Each lane holds E neighbouring channels of up to 8 tokens, all loaded before the first is used; the
-// minimum and the maximum of a vector are wave reductions. Both are exact, so the codes do not depend
-// on any order.
+// A vector of D channels is D / 8 lanes with 8 neighbouring channels each, so a wave has 8, 4 or 2 vectors
+// side by side (D = 64, 128, 256) and the minimum and maximum of each are 3 to 5 steps between lanes. Both
+// are exact, so the codes do not depend on any order.
+//
+// Append: a wave per block of 8 tokens and head, V's words hold 8 tokens each, so this wave is the only writer
+// of its words; tokens of the block that are not new keep their nibbles. Blocks are found from the rows: a row
+// leads its block when it is the first new token in it. A wave looks at `rows` rows, 8 of a prompt, which lead one
+// block as a rule, or one of a decode step, which leads its own.
+// All loads of a block are in flight before the first is used. 7000 prompt tokens x 4 heads of 128 (18 MB in and
+// out): see DESIGN for the times; bound by the launch and the chain row -> sequence -> page -> block.
 #include "kv4.h"
 
 namespace w4a8 {
 
-__device__ __forceinline__ float wave_min(float v) { return -wave_max(-v); }
-
-// the sequence whose rows hold row i: the last b with cu[b] <= i
-__device__ __forceinline__ int kv4_sequence(const Kv4Batch& s, int64_t i) {
-  int lo = 0, hi = s.B - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (s.cu[mid] <= i) lo = mid; else hi = mid - 1;
+// the last sequence b with cu[b] <= i, 64 candidates at a time; i is wave-uniform
+__device__ __forceinline__ int kv4_sequence(const Kv4Batch& s, int64_t i, int lane) {
+  int lo = 0, n = s.B;
+  while (n > 1) {
+    const int stride = (n + 63) / 64, at = lane * stride;
+    const uint64_t below = __ballot(at < n && s.cu[lo + (at < n ? at : 0)] <= i);
+    const int k = below ? 63 - __builtin_clzll(below) : 0;
+    lo += k * stride;
+    n = n - k * stride < stride ? n - k * stride : stride;
   }
   return lo;
 }
 
-template <int E>
-__device__ __forceinline__ void load_e(const uint16_t* p, uint32_t (&w)[E / 2]) {
-  if constexpr (E == 2) w[0] = *reinterpret_cast<const uint32_t*>(p);
-  else { const uint2 u = *reinterpret_cast<const uint2*>(p); w[0] = u.x; w[1] = u.y; }
+// the place of row i (a lane's own), given the wave's first row's sequence: its position, whether it is its
+// sequence's first row, and how many rows follow it there, itself included. False: no sequence has it.
+struct Place {
+  int b;
+  int64_t pos;
+  bool first;
+  int left;
+};
+__device__ __forceinline__ bool kv4_place(const Kv4Batch& s, int b, int64_t i, Place& p) {
+  while (b + 1 < s.B && s.cu[b + 1] <= i) ++b;
+  int64_t start;
+  int n;
+  kv4_rows(s, b, start, n);
+  if (i < start || i >= start + n) return false;
+  p.b = b;
+  p.left = (int)(start + n - i);
+  p.pos = (int64_t)s.lens[b] - p.left;
+  p.first = i == start;
+  return true;
 }
 
-// codes of the wave's vector (x in this lane's channels), step and least value packed as stored
-template <int E>
-__device__ __forceinline__ void quantize(const uint32_t (&w)[E / 2], int dtype, bool on, uint32_t (&c)[E], uint32_t& sm) {
-  float f[E];
+// maximum over the L lanes of a vector
+template <int L>
+__device__ __forceinline__ float vector_max(float v) {
+  v = fmaxf(v, dpp_f<kDppXor1>(v));
+  v = fmaxf(v, dpp_f<kDppXor2>(v));
+  v = fmaxf(v, dpp_f<kDppHalfMirror>(v));
+  if (L >= 16) v = fmaxf(v, dpp_f<kDppRowMirror>(v));
+  if (L == 32) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  }
+  return v;
+}
+// or over the wave's vectors (lanes L apart)
+template <int L>
+__device__ __forceinline__ uint32_t vectors_or(uint32_t v) {
+  if (L == 8) v |= (uint32_t)dpp_i<0x128>((int)v);  // 8 lanes round in a row of 16
+  if (L <= 16) {
+    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = a[0] | a[1];
+  }
+  auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return b[0] | b[1];
+}
+
+// codes of the lane's 8 channels of its vector, with step and least value as stored
+template <int L, int dtype>
+__device__ __forceinline__ void quantize(const uint4& u, uint32_t (&c)[8], uint32_t& sm) {
+  float f[8];
+  unpack8(u, dtype, f);
+  float lo = f[0], hi = f[0], far = 0.f;
 #pragma unroll
-  for (int i = 0; i < E; ++i) f[i] = from_dtype((uint16_t)(w[i / 2] >> (16 * (i & 1))), dtype);
-  float lo = f[0], hi = f[0];
-  bool fin = true;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
+  for (int i = 0; i < 8; ++i) {
     lo = fminf(lo, f[i]);
     hi = fmaxf(hi, f[i]);
-    fin = fin && __builtin_isfinite(f[i]);
+    far = fmaxf(far, __builtin_isfinite(f[i]) ? 0.f : 1.f);
   }
-  const float kInf = __builtin_inff();
-  lo = wave_min(on ? lo : kInf);
-  hi = wave_max(on ? hi : -kInf);
+  lo = -vector_max<L>(-lo);
+  hi = vector_max<L>(hi);
+  far = vector_max<L>(far);
   // the type's own rounding of the step: codes are chosen for the step that readers see
   const float tiny = dtype == kF16 ? 5.9604644775390625e-08f : 1.1754943508222875e-38f;
   const float raw = fmaxf((hi - lo) / 15.0f, fmaxf(hi, -lo) * 6.103515625e-05f);
   const float s = fmaxf(from_dtype(to_dtype(raw, dtype), dtype), tiny);
-  const bool good = __ballot(on && !fin) == 0 && __builtin_isfinite(s) && __builtin_isfinite(raw);
+  const bool good = far == 0.f && __builtin_isfinite(s) && __builtin_isfinite(raw);
+  // rint of the correctly rounded quotient. The product with 1 / s is within 2^-21 of it, so it rounds alike
+  // wherever it is not that near to a half; the wave divides where a lane is.
+  const float inv = __builtin_amdgcn_rcpf(s);
+  float r[8];
+  bool near = false;
 #pragma unroll
-  for (int i = 0; i < E; ++i)
-    c[i] = good ? (uint32_t)fminf(fmaxf(__builtin_rintf((f[i] - lo) / s), 0.0f), 15.0f) : 0u;
+  for (int i = 0; i < 8; ++i) {
+    const float q = (f[i] - lo) * inv;
+    r[i] = __builtin_rintf(q);
+    near = near || !(fabsf(q - r[i]) < 0.4999f);
+  }
+  if (__ballot(near))
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = __builtin_rintf((f[i] - lo) / s);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = good ? (uint32_t)fminf(fmaxf(r[i], 0.0f), 15.0f) : 0u;
   const uint32_t nan = dtype == kF16 ? 0x7e007e00u : 0x7fc07fc0u;
   sm = good ? (uint32_t)to_dtype(s, dtype) | ((uint32_t)to_dtype(lo, dtype) << 16) : nan;
 }
 
-template <int D>
+template <int D, int DT>
 __global__ void __launch_bounds__(256)
 kv4_append_kernel(const uint16_t* __restrict__ k, int64_t ldk, int64_t hk, const uint16_t* __restrict__ v, int64_t ldv,
-                  int64_t hv, int dtype, Kv4Cache c, Kv4Batch s) {
-  constexpr int E = D == 256 ? 4 : 2, NL = D / E;
+                  int64_t hv, Kv4Cache c, Kv4Batch s, int rows) {
+  constexpr int L = D / 8, VP = 64 / L, PASS = 8 / VP;  // lanes per vector, vectors per wave, passes for 8 tokens
   const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t i = id / c.H;
-  const int h = (int)(id - i * c.H);
-  if (i >= s.T) return;
-  const int b = kv4_sequence(s, i);
-  int64_t start;
-  int n;
-  kv4_rows(s, b, start, n);
-  if (i < start || i >= start + n) return;
-  const int64_t pos = s.lens[b] - (start + n - i);
-  if (pos < 0 || !((pos & 7) == 0 || i == start)) return;
-  const int page = kv4_page(c, s, b, pos);
-  if (page < 0) return;
-  const int j0 = (int)(pos & 7);
-  const int cnt = (int)(start + n - i < 8 - j0 ? start + n - i : 8 - j0);
-  const bool on = lane < NL;
-  const int ch = (on ? lane : 0) * E;
-
-  uint32_t kw[8][E / 2], vw[8][E / 2];
-  const uint16_t* kp = k + i * ldk + h * hk + ch;
-  const uint16_t* vp = v + i * ldv + h * hv + ch;
+  const uint32_t id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t i0 = (int64_t)(id / (uint32_t)c.H) * rows;
+  const int h = (int)(id % (uint32_t)c.H);
+  if (i0 >= s.T) return;
+  Place pl = {};
+  const int64_t i = i0 + lane;
+  const int b0 = kv4_sequence(s, i0, lane);
+  const bool leads = lane < rows && i < s.T && kv4_place(s, b0, i, pl) && pl.pos >= 0 &&
+                     ((pl.pos & 7) == 0 || pl.first);
+  const int page = leads ? kv4_page(c, s, pl.b, pl.pos) : -1;
+  uint64_t todo = __ballot(leads && page >= 0);
+  const int tok0 = lane / L, ch = (lane & (L - 1)) * 8;
+  for (; todo; todo &= todo - 1) {
+    const int x = __builtin_ctzll(todo);
+    const int pos = __builtin_amdgcn_readlane((int)pl.pos, x);
+    const int left = __builtin_amdgcn_readlane(pl.left, x);
+    const int64_t blk = kv4_block(c, __builtin_amdgcn_readlane(page, x), h, pos & ~7);
+    const int j0 = pos & 7, cnt = left < 8 - j0 ? left : 8 - j0;
+    const uint16_t* kp = k + (i0 + x) * ldk + h * hk + ch;
+    const uint16_t* vp = v + (i0 + x) * ldv + h * hv + ch;
+    uint32_t* vd = reinterpret_cast<uint32_t*>(c.v + blk * (4 * D)) + ch;
+    uint4 kr[PASS], vr[PASS], old[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < cnt) {
-      load_e<E>(kp + j * ldk, kw[j]);
-      load_e<E>(vp + j * ldv, vw[j]);
+    for (int p = 0; p < PASS; ++p) {
+      const int tok = p * VP + tok0;  // lanes of tokens that are not there hold the first one's
+      kr[p] = *reinterpret_cast<const uint4*>(kp + (tok < cnt ? tok : 0) * ldk);
+      vr[p] = *reinterpret_cast<const uint4*>(vp + (tok < cnt ? tok : 0) * ldv);
     }
-  const int64_t blk = kv4_block(c, page, h, (int)(pos & ~(int64_t)7 & ((1 << c.shift) - 1)));
-  uint8_t* kd = c.k + blk * (4 * D);
-  uint32_t* vd = reinterpret_cast<uint32_t*>(c.v + blk * (4 * D)) + ch;
-  uint32_t words[E];
+    if (cnt < 8 && tok0 == 0) {
+      old[0] = *reinterpret_cast<const uint4*>(vd);
+      old[1] = *reinterpret_cast<const uint4*>(vd + 4);
+    }
+    uint32_t words[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-  for (int e = 0; e < E; ++e) words[e] = cnt < 8 && on ? vd[e] : 0u;
+    for (int p = 0; p < PASS; ++p)
+      if (p * VP < cnt) {
+        const int tok = p * VP + tok0;
+        const bool on = tok < cnt;
+        uint32_t cc[8], sm, w = 0;
+        quantize<L, DT>(kr[p], cc, sm);
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < cnt) {
-      uint32_t cc[E], sm;
-      quantize<E>(kw[j], dtype, on, cc, sm);
-      uint8_t* row = kd + (j0 + j) * (D / 2) + ch / 2;
-      if (on) {
-        if constexpr (E == 2) *row = (uint8_t)(cc[0] | (cc[1] << 4));
-        else *reinterpret_cast<uint16_t*>(row) = (uint16_t)(cc[0] | (cc[1] << 4) | (cc[2] << 8) | (cc[3] << 12));
+        for (int e = 0; e < 8; ++e) w |= cc[e] << (4 * e);
+        if (on) {
+          *reinterpret_cast<uint32_t*>(c.k + blk * (4 * D) + (j0 + tok) * (D / 2) + ch / 2) = w;
+          if (ch == 0) c.ks[blk * 8 + j0 + tok] = sm;
+        }
+        quantize<L, DT>(vr[p], cc, sm);
+        if (on) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) words[e] |= cc[e] << (4 * (j0 + tok));
+          if (ch == 0) c.vs[blk * 8 + j0 + tok] = sm;
+        }
       }
-      if (lane == 0) c.ks[blk * 8 + j0 + j] = sm;
-      quantize<E>(vw[j], dtype, on, cc, sm);
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        words[e] = (words[e] & ~(15u << (4 * (j0 + j)))) | (cc[e] << (4 * (j0 + j)));
-      if (lane == 0) c.vs[blk * 8 + j0 + j] = sm;
+    for (int e = 0; e < 8; ++e) words[e] = vectors_or<L>(words[e]);
+    if (tok0 == 0) {
+      const uint32_t keep = ~((cnt == 8 ? ~0u : (1u << (4 * cnt)) - 1) << (4 * j0));
+      const uint32_t o[8] = {old[0].x, old[0].y, old[0].z, old[0].w, old[1].x, old[1].y, old[1].z, old[1].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) words[e] |= o[e] & keep;
+      *reinterpret_cast<uint4*>(vd) = make_uint4(words[0], words[1], words[2], words[3]);
+      *reinterpret_cast<uint4*>(vd + 4) = make_uint4(words[4], words[5], words[6], words[7]);
     }
-  if (on)
-#pragma unroll
-    for (int e = 0; e < E; ++e) vd[e] = words[e];
+  }
 }
 
 // Rows of the cache as values in the model's type: s c + m with one rounding to f32 (the product is
 // exact) and one to the type. A row without a place in the cache (before the sequence's first token,
-// on a page that does not exist) is NaN.
-template <int D>
+// on a page that does not exist) is NaN. A vector per D / 8 lanes, heads of a row side by side.
+template <int D, int DT>
 __global__ void __launch_bounds__(256)
-kv4_read_kernel(Kv4Cache c, Kv4Batch s, int dtype, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
-  constexpr int E = D == 256 ? 4 : 2, NL = D / E;
+kv4_read_kernel(Kv4Cache c, Kv4Batch s, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
+  constexpr int L = D / 8, VP = 64 / L;
   const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t i = id / c.H;
-  const int h = (int)(id - i * c.H);
-  if (i >= s.T || lane >= NL) return;
-  const int b = kv4_sequence(s, i);
-  int64_t start;
-  int n;
-  kv4_rows(s, b, start, n);
-  if (i < start || i >= start + n) return;
-  const int64_t pos = s.lens[b] - (start + n - i);
-  const int page = kv4_page(c, s, b, pos);
-  const int ch = lane * E;
-  uint32_t kc[E], vc[E], ks, vs;
-  if (page < 0) {
-    ks = vs = dtype == kF16 ? 0x7e007e00u : 0x7fc07fc0u;
-#pragma unroll
-    for (int e = 0; e < E; ++e) kc[e] = vc[e] = 0;
-  } else {
-    const int j = (int)(pos & 7);
-    const int64_t blk = kv4_block(c, page, h, (int)(pos & ~(int64_t)7 & ((1 << c.shift) - 1)));
-    const uint8_t* row = c.k + blk * (4 * D) + j * (D / 2) + ch / 2;
-    const uint32_t* vd = reinterpret_cast<const uint32_t*>(c.v + blk * (4 * D)) + ch;
+  const uint32_t id0 = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * VP;
+  if (id0 >= s.T * c.H) return;
+  const int b0 = kv4_sequence(s, id0 / (uint32_t)c.H, lane);
+  const uint32_t id = id0 + lane / L;
+  const int64_t i = id / (uint32_t)c.H;
+  const int h = (int)(id % (uint32_t)c.H), ch = (lane & (L - 1)) * 8;
+  Place pl;
+  if (i >= s.T || !kv4_place(s, b0, i, pl)) return;
+  const int page = kv4_page(c, s, pl.b, pl.pos);
+  uint32_t ks = DT == kF16 ? 0x7e007e00u : 0x7fc07fc0u, vs = ks, kc = 0, vc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  const int j = (int)(pl.pos & 7);
+  if (page >= 0) {
+    const int64_t blk = kv4_block(c, page, h, (int)(pl.pos & ~(int64_t)7));
+    const uint4* vd = reinterpret_cast<const uint4*>(c.v + blk * (4 * D) + ch * 4);
+    kc = *reinterpret_cast<const uint32_t*>(c.k + blk * (4 * D) + j * (D / 2) + ch / 2);
+    const uint4 a = vd[0], b = vd[1];
+    vc[0] = a.x; vc[1] = a.y; vc[2] = a.z; vc[3] = a.w;
+    vc[4] = b.x; vc[5] = b.y; vc[6] = b.z; vc[7] = b.w;
     ks = c.ks[blk * 8 + j];
     vs = c.vs[blk * 8 + j];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      kc[e] = (row[e / 2] >> (4 * (e & 1))) & 15u;
-      vc[e] = (vd[e] >> (4 * j)) & 15u;
-    }
   }
-  const int64_t at = (i * c.H + h) * D + ch;
-  auto put = [&](uint16_t* o, const uint32_t (&cc)[E], uint32_t sm) {
-    const float st = from_dtype((uint16_t)(sm & 0xffffu), dtype), m = from_dtype((uint16_t)(sm >> 16), dtype);
-    uint32_t w[E / 2];
-#pragma unroll
-    for (int e = 0; e < E; e += 2)
-      w[e / 2] = (uint32_t)to_dtype(__builtin_fmaf((float)cc[e], st, m), dtype) |
-                 ((uint32_t)to_dtype(__builtin_fmaf((float)cc[e + 1], st, m), dtype) << 16);
-    if constexpr (E == 2) *reinterpret_cast<uint32_t*>(o + at) = w[0];
-    else *reinterpret_cast<uint2*>(o + at) = make_uint2(w[0], w[1]);
+  auto value = [&](uint32_t code, uint32_t sm) {
+    return (uint32_t)to_dtype(__builtin_fmaf((float)code, from_dtype((uint16_t)(sm & 0xffffu), DT),
+                                             from_dtype((uint16_t)(sm >> 16), DT)), DT);
   };
-  put(k, kc, ks);
-  put(v, vc, vs);
+  uint32_t kw[4], vw[4];
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    kw[e / 2] = value((kc >> (4 * e)) & 15u, ks) | (value((kc >> (4 * e + 4)) & 15u, ks) << 16);
+    vw[e / 2] = value((vc[e] >> (4 * j)) & 15u, vs) | (value((vc[e + 1] >> (4 * j)) & 15u, vs) << 16);
+  }
+  *reinterpret_cast<uint4*>(k + (int64_t)id * D + ch) = make_uint4(kw[0], kw[1], kw[2], kw[3]);
+  *reinterpret_cast<uint4*>(v + (int64_t)id * D + ch) = make_uint4(vw[0], vw[1], vw[2], vw[3]);
+}
+
+template <int DT>
+static void append(int D, dim3 g, const uint16_t* k, int64_t ldk, int64_t hk, const uint16_t* v, int64_t ldv, int64_t hv,
+                   const Kv4Cache& c, const Kv4Batch& s, int rows, hipStream_t st) {
+  if (D == 64) hipLaunchKernelGGL((kv4_append_kernel<64, DT>), g, dim3(256), 0, st, k, ldk, hk, v, ldv, hv, c, s, rows);
+  else if (D == 128) hipLaunchKernelGGL((kv4_append_kernel<128, DT>), g, dim3(256), 0, st, k, ldk, hk, v, ldv, hv, c, s, rows);
+  else hipLaunchKernelGGL((kv4_append_kernel<256, DT>), g, dim3(256), 0, st, k, ldk, hk, v, ldv, hv, c, s, rows);
 }
 
 int launch_kv4_append(const void* k, int64_t ldk, int64_t hk, const void* v, int64_t ldv, int64_t hv, int dtype, int D,
                       const Kv4Cache& c, const Kv4Batch& s, hipStream_t st) {
-  const dim3 g((unsigned)((s.T * c.H + 3) / 4));
+  // one row per wave while that many waves (8192) fill the card no more than once
+  const int rows = s.T * c.H <= 8192 ? 1 : 8;
+  const dim3 g((unsigned)(((s.T + rows - 1) / rows * c.H + 3) / 4));
   auto kp = reinterpret_cast<const uint16_t*>(k), vp = reinterpret_cast<const uint16_t*>(v);
-  if (D == 64) hipLaunchKernelGGL(kv4_append_kernel<64>, g, dim3(256), 0, st, kp, ldk, hk, vp, ldv, hv, dtype, c, s);
-  else if (D == 128) hipLaunchKernelGGL(kv4_append_kernel<128>, g, dim3(256), 0, st, kp, ldk, hk, vp, ldv, hv, dtype, c, s);
-  else hipLaunchKernelGGL(kv4_append_kernel<256>, g, dim3(256), 0, st, kp, ldk, hk, vp, ldv, hv, dtype, c, s);
+  if (dtype == kBF16) append<kBF16>(D, g, kp, ldk, hk, vp, ldv, hv, c, s, rows, st);
+  else append<kF16>(D, g, kp, ldk, hk, vp, ldv, hv, c, s, rows, st);
   return hipGetLastError() == hipSuccess ? kOk : kErrHip;
 }
 
+template <int DT>
+static void read(int D, dim3 g, const Kv4Cache& c, const Kv4Batch& s, uint16_t* k, uint16_t* v, hipStream_t st) {
+  if (D == 64) hipLaunchKernelGGL((kv4_read_kernel<64, DT>), g, dim3(256), 0, st, c, s, k, v);
+  else if (D == 128) hipLaunchKernelGGL((kv4_read_kernel<128, DT>), g, dim3(256), 0, st, c, s, k, v);
+  else hipLaunchKernelGGL((kv4_read_kernel<256, DT>), g, dim3(256), 0, st, c, s, k, v);
+}
+
 int launch_kv4_read(const Kv4Cache& c, const Kv4Batch& s, int dtype, int D, void* k, void* v, hipStream_t st) {
-  const dim3 g((unsigned)((s.T * c.H + 3) / 4));
+  const int per = 4 * 512 / D;  // vectors per workgroup
+  const dim3 g((unsigned)((s.T * c.H + per - 1) / per));
   auto kp = reinterpret_cast<uint16_t*>(k), vp = reinterpret_cast<uint16_t*>(v);
-  if (D == 64) hipLaunchKernelGGL(kv4_read_kernel<64>, g, dim3(256), 0, st, c, s, dtype, kp, vp);
-  else if (D == 128) hipLaunchKernelGGL(kv4_read_kernel<128>, g, dim3(256), 0, st, c, s, dtype, kp, vp);
-  else hipLaunchKernelGGL(kv4_read_kernel<256>, g, dim3(256), 0, st, c, s, dtype, kp, vp);
+  if (dtype == kBF16) read<kBF16>(D, g, c, s, kp, vp, st);
+  else read<kF16>(D, g, c, s, kp, vp, st);
   return hipGetLastError() == hipSuccess ? kOk : kErrHip;
 }
 

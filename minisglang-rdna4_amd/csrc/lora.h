@@ -17,7 +17,7 @@ struct LoraArgs {
   int L, rank, slices;
   int64_t N;
   int64_t col[kLoraMaxSlices + 1];    // first column of each slice, then N
-  int64_t chunk[kLoraMaxSlices + 1];  // its first 64-column chunk, then all of them
+  int64_t chunk[kLoraMaxSlices + 1];  // its first chunk of 256 columns, then all of them
   const void* base;  // (M, ldb): the projection's output, in the model's type or f32
   int64_t ldb;
   int base_f32;

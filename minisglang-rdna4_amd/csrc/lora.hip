@@ -111,114 +111,208 @@ lora_down_kernel(const LoraArgs p) {
   }
 }
 
-// grid: (4 chunks of 64 columns of one slice * blocks of 16 rows, 1, slots). A wave per chunk: row (4 q + i) of
-// its j-th product is column 16 q + 4 j + i of the chunk, so a lane ends with 16 neighbouring columns.
-template <int DT>
-__global__ void __launch_bounds__(256)
+// grid: (4 chunks of 64 columns of one slice * blocks of 16 RB rows, 1, slots). A wave per chunk: row (4 q + i) of
+// its j-th product is column 16 q + 4 j + i of the chunk, so a lane ends with 16 neighbouring columns. The
+// workgroup first sums the parts of v for its rows and slice, once for its four chunks, into LDS. (The chunks
+// of a workgroup are of one slice: launch_lora counts them so.) An adapter's B stays in registers over the RB
+// blocks of 16 rows, where its rank is up to 64.
+template <int DT, int RB, bool F32>
+__global__ void __launch_bounds__(256, RB == 4 ? 2 : 4)
 lora_up_kernel(const LoraArgs p) {
-  const int lane = threadIdx.x & 63;
+  constexpr int kPad = 4;  // floats between rows: the rows of a read start 16 bytes apart, modulo the banks
+  extern __shared__ float vs[];  // (16 RB, rank + kPad), then the rows' largest |v|
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
-  const uint32_t quads = (uint32_t)((p.chunk[p.slices] + 3) / 4);
-  const int64_t chunk = (int64_t)(blockIdx.x % quads) * 4 + (threadIdx.x >> 6);
-  if (chunk >= p.chunk[p.slices]) return;
+  const uint32_t quads = (uint32_t)p.chunk[p.slices];
+  const uint32_t quad = blockIdx.x % quads;
   int s = 0;
-  while (chunk >= p.chunk[s + 1]) ++s;
-  const int64_t n0 = p.col[s] + (chunk - p.chunk[s]) * 64;
+  while (quad >= p.chunk[s + 1]) ++s;
   const int64_t nend = p.col[s + 1];
-  const int64_t m0 = (int64_t)(blockIdx.x / quads) * 16;
-  const int R = p.slices * p.rank;
-  Rows rows = row_adapters(p, m0, lane);
-  v4f acc[4];
+  const int64_t n0 = p.col[s] + (int64_t)(quad - p.chunk[s]) * 256 + wave * 64;
+  const int64_t m0 = (int64_t)(blockIdx.x / quads) * (16 * RB);
+  const int R = p.slices * p.rank, ld = p.rank + kPad;
+  const bool work = n0 < nend;  // this wave's columns exist (the last workgroup of a slice may have fewer)
+
+  Rows rows[RB];
+  uint4 base[RB][F32 ? 4 : 2];
+  const int64_t n = n0 + 16 * g;
+  const bool cols = work && n < nend;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
-  // rows without an adapter are the base itself, the first slot's
-  bool write = rows.id < 0 && blockIdx.z == 0;
-  for (int i = 0; rows.left; ++i) {
-    const int a = next_adapter(rows);
-    if (i % (int)gridDim.z != (int)blockIdx.z) continue;
-    const bool mine = rows.id == a;
-    write |= mine;
+  for (int b = 0; b < RB; ++b) {
+    rows[b] = row_adapters(p, m0 + 16 * b, lane);
+    const int64_t m = m0 + 16 * b + c;
+    if (cols && m < p.M) {
+      const uint4* bp = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.base) + (m * p.ldb + n) * (F32 ? 4 : 2));
+#pragma unroll
+      for (int j = 0; j < (F32 ? 4 : 2); ++j) base[b][j] = bp[j];
+    }
+  }
+  // v of the rows that this workgroup's slot does: the i-th adapter of the rows is slot i's, modulo the slots
+  v4f acc[RB][4];
+  bool write[RB], mine_any = false;
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[b][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    write[b] = rows[b].id < 0 && blockIdx.z == 0;  // rows without an adapter are the base itself, the first slot's
+  }
+  // a row is done by this slot when its adapter's place among the rows' adapters is the slot's
+  bool todo[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) todo[b] = false;
+  {
+    Rows r[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) r[b] = rows[b];
+    for (int i = 0;; ++i) {
+      int a = -1;
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+        if (a < 0 && r[b].left) a = __builtin_amdgcn_readlane(r[b].id, __builtin_ctz(r[b].left));
+      if (a < 0) break;
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        const bool m = r[b].id == a;
+        r[b].left &= ~((uint32_t)__ballot(m) & 0xffffu);
+        if (i % (int)gridDim.z == (int)blockIdx.z) todo[b] = todo[b] || m;
+      }
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    rows[b].left &= (uint32_t)__ballot(todo[b]) & 0xffffu;
+    mine_any = mine_any || rows[b].left != 0;
+    write[b] = write[b] || todo[b];
+  }
+  if (mine_any) {
+    // four ranks a thread, parts of K in order; rows of other slots are skipped
+    const int per = p.rank / 4;
+    for (int t = threadIdx.x; t < 16 * RB * per; t += 256) {
+      const int row = t / per, r = (t - row * per) * 4;
+      uint32_t left = 0;
+#pragma unroll
+      for (int b = 0; b < RB; ++b) left = row / 16 == b ? rows[b].left : left;
+      v4f v = {0.f, 0.f, 0.f, 0.f};
+      if ((left >> (row & 15)) & 1) {
+        const float* vp = p.v + (m0 + row) * R + s * p.rank + r;
+        const int64_t part = p.M * R;
+        int q = 0;
+        for (; q + 4 <= p.kc; q += 4) {
+          const v4f a0 = *reinterpret_cast<const v4f*>(vp + q * part), a1 = *reinterpret_cast<const v4f*>(vp + (q + 1) * part),
+                    a2 = *reinterpret_cast<const v4f*>(vp + (q + 2) * part), a3 = *reinterpret_cast<const v4f*>(vp + (q + 3) * part);
+          v = (((v + a0) + a1) + a2) + a3;
+        }
+        for (; q < p.kc; ++q) v += *reinterpret_cast<const v4f*>(vp + q * part);
+      }
+      *reinterpret_cast<v4f*>(&vs[row * ld + r]) = v;
+    }
+    __syncthreads();
+  }
+  if (!work) return;
+
+  bool some = mine_any;
+  while (some) {
+    int a = -1;
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+      if (a < 0 && rows[b].left) a = __builtin_amdgcn_readlane(rows[b].id, __builtin_ctz(rows[b].left));
     const float scale = p.scaling[a];
-    const float* vp = p.v + (m0 + (mine ? c : 0)) * R + s * p.rank;
-    float top = 0.f;
-    for (int r = 8 * g; r < p.rank; r += 32) {
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (mine)
-        for (int q = 0; q < p.kc; ++q)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += vp[(int64_t)q * p.M * R + r + e];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
-    }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    // 2^-e with 2^e the power of two at or below the largest |v|; NaN and infinity pass through as they are
-    const uint32_t ex = (__float_as_uint(top) >> 23) & 255u;
-    const bool plain = ex > 1 && ex < 253;
-    const float down = plain ? __uint_as_float((254u - ex) << 23) : 1.f;
-    const float up = (plain ? __uint_as_float(ex << 23) : 1.f) * scale;
-    v4f d[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) d[j] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int rr = 0; rr < p.rank; rr += 32) {
+    const uint16_t* bp = p.b + (int64_t)a * p.N * p.rank;
+    auto load_b = [&](int rr, v4w (&bw)[4]) {
       const int r = rr + 8 * g;
-      const bool in = r < p.rank;
-      v4w bw[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int64_t n = n0 + (c >> 2) * 16 + j * 4 + (c & 3);
-        bw[j] = load16(p.b + ((int64_t)a * p.N + (n < nend ? n : n0)) * p.rank + (in ? r : 0), in && n < nend);
+        const int64_t nn = n0 + (c >> 2) * 16 + j * 4 + (c & 3);
+        const bool in = r < p.rank && nn < nend;
+        bw[j] = load16(bp + (in ? nn * p.rank + r : 0), in);
       }
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (mine && in)
-        for (int q = 0; q < p.kc; ++q)
+    };
+    v4w b0[4], b1[4];
+    load_b(0, b0);
+    if (p.rank > 32) load_b(32, b1);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += vp[(int64_t)q * p.M * R + r + e];
-      v4w hi, lo;
+    for (int b = 0; b < RB; ++b) {
+      const bool mine = rows[b].id == a && todo[b];
+      const uint32_t which = (uint32_t)__ballot(mine) & 0xffffu;
+      if (!which) continue;
+      rows[b].left &= ~which;
+      const float* vr = vs + (16 * b + c) * ld;
+      float top = 0.f;
+      for (int r = 8 * g; r < p.rank; r += 32)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v0 = v[2 * e] * down, v1 = v[2 * e + 1] * down;
-        const uint16_t h0 = to_dtype(v0, DT), h1 = to_dtype(v1, DT);
-        hi[e] = (uint32_t)h0 | ((uint32_t)h1 << 16);
-        lo[e] = (uint32_t)to_dtype(v0 - from_dtype(h0, DT), DT) | ((uint32_t)to_dtype(v1 - from_dtype(h1, DT), DT) << 16);
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(vr[r + e]));
+      top = mine ? top : 0.f;
+      auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+      auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+      // 2^-e with 2^e the power of two at or below the largest |v|; NaN and infinity pass through as they are
+      const uint32_t ex = (__float_as_uint(top) >> 23) & 255u;
+      const bool plain = ex > 1 && ex < 253;
+      const float down = plain ? __uint_as_float((254u - ex) << 23) : 1.f;
+      const float up = (plain ? __uint_as_float(ex << 23) : 1.f) * scale;
+      v4f d[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[j] = v4f{0.f, 0.f, 0.f, 0.f};
+      auto product = [&](int rr, const v4w (&bw)[4]) {
+        const int r = rr + 8 * g;
+        const bool in = mine && r < p.rank;
+        v4w hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v0 = in ? vr[r + 2 * e] * down : 0.f, v1 = in ? vr[r + 2 * e + 1] * down : 0.f;
+          const uint16_t h0 = to_dtype(v0, DT), h1 = to_dtype(v1, DT);
+          hi[e] = (uint32_t)h0 | ((uint32_t)h1 << 16);
+          lo[e] = (uint32_t)to_dtype(v0 - from_dtype(h0, DT), DT) | ((uint32_t)to_dtype(v1 - from_dtype(h1, DT), DT) << 16);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          d[j] = mfma16<DT>(bw[j], hi, d[j]);
+          d[j] = mfma16<DT>(bw[j], lo, d[j]);
+        }
+      };
+      product(0, b0);
+      if (p.rank > 32) product(32, b1);
+      for (int rr = 64; rr < p.rank; rr += 32) {
+        v4w bw[4];
+        load_b(rr, bw);
+        product(rr, bw);
       }
+      if (mine)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[b][j] = d[j] * up;
+    }
+    some = false;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) some = some || rows[b].left != 0;
+  }
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int64_t m = m0 + 16 * b + c;
+    if (!write[b] || m >= p.M || !cols) continue;
+    uint32_t w[8];
+    if constexpr (F32) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        d[j] = mfma16<DT>(bw[j], hi, d[j]);
-        d[j] = mfma16<DT>(bw[j], lo, d[j]);
+        const v4f y = __builtin_bit_cast(v4f, base[b][j]) + acc[b][j];
+        w[2 * j] = (uint32_t)to_dtype(y[0], DT) | ((uint32_t)to_dtype(y[1], DT) << 16);
+        w[2 * j + 1] = (uint32_t)to_dtype(y[2], DT) | ((uint32_t)to_dtype(y[3], DT) << 16);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float f[8];
+        unpack8(base[b][t], DT, f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[4 * t + e] = (uint32_t)to_dtype(f[2 * e] + acc[b][2 * t + e / 2][(2 * e) & 3], DT) |
+                         ((uint32_t)to_dtype(f[2 * e + 1] + acc[b][2 * t + e / 2][(2 * e + 1) & 3], DT) << 16);
       }
     }
-    if (mine)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = d[j] * up;
+    uint16_t* op = p.out + m * p.ldo + n;
+    *reinterpret_cast<uint4*>(op) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(op + 8) = make_uint4(w[4], w[5], w[6], w[7]);
   }
-  const int64_t m = m0 + c, n = n0 + 16 * g;
-  if (!write || m >= p.M || n >= nend) return;
-  uint32_t w[8];
-  if (p.base_f32) {
-    const float* bp = reinterpret_cast<const float*>(p.base) + m * p.ldb + n;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const v4f y = *reinterpret_cast<const v4f*>(bp + 4 * j) + acc[j];
-      w[2 * j] = (uint32_t)to_dtype(y[0], DT) | ((uint32_t)to_dtype(y[1], DT) << 16);
-      w[2 * j + 1] = (uint32_t)to_dtype(y[2], DT) | ((uint32_t)to_dtype(y[3], DT) << 16);
-    }
-  } else {
-    const uint16_t* bp = reinterpret_cast<const uint16_t*>(p.base) + m * p.ldb + n;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint4 u = *reinterpret_cast<const uint4*>(bp + 8 * t);
-      float f[8];
-      unpack8(u, DT, f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[4 * t + e] = (uint32_t)to_dtype(f[2 * e] + acc[2 * t + e / 2][(2 * e) & 3], DT) |
-                       ((uint32_t)to_dtype(f[2 * e + 1] + acc[2 * t + e / 2][(2 * e + 1) & 3], DT) << 16);
-    }
-  }
-  uint16_t* op = p.out + m * p.ldo + n;
-  *reinterpret_cast<uint4*>(op) = make_uint4(w[0], w[1], w[2], w[3]);
-  *reinterpret_cast<uint4*>(op + 8) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 // parts of K: enough workgroups for a few rows, one part for many
@@ -241,14 +335,20 @@ int launch_lora(LoraArgs& p, int dtype, hipStream_t st) {
   const int rb = R <= 16 ? 1 : R <= 32 ? 2 : 4;
   const int64_t groups = (R + 16 * rb - 1) / (16 * rb);
   const dim3 gd((unsigned)(blocks * groups * p.kc), 1, (unsigned)p.slots), bl(256);
-  const dim3 gu((unsigned)((p.chunk[p.slices] + 3) / 4 * blocks), 1, (unsigned)p.slots);
+  // blocks of 64 rows where they fill the card (prompts), of 16 else
+  const int64_t quads = p.chunk[p.slices];
+  const int up_rows = p.slots == 1 && !p.base_f32 && p.rank <= 128 && quads * ((p.M + 63) / 64) >= 1024 ? 64 : 16;
+  const dim3 gu((unsigned)(quads * ((p.M + up_rows - 1) / up_rows)), 1, (unsigned)p.slots);
+  const unsigned lds = (unsigned)(up_rows * (p.rank + 4) * 4);
 #define W4A8_LORA(DT_)                                                                        \
   do {                                                                                        \
     if (rb == 1) hipLaunchKernelGGL((lora_down_kernel<DT_, 1>), gd, bl, 0, st, p);            \
     else if (rb == 2) hipLaunchKernelGGL((lora_down_kernel<DT_, 2>), gd, bl, 0, st, p);       \
     else hipLaunchKernelGGL((lora_down_kernel<DT_, 4>), gd, bl, 0, st, p);                    \
     if (hipGetLastError() != hipSuccess) return kErrHip;                                      \
-    hipLaunchKernelGGL(lora_up_kernel<DT_>, gu, bl, 0, st, p);                                \
+    if (up_rows == 64) hipLaunchKernelGGL((lora_up_kernel<DT_, 4, false>), gu, bl, lds, st, p);    \
+    else if (p.base_f32) hipLaunchKernelGGL((lora_up_kernel<DT_, 1, true>), gu, bl, lds, st, p);   \
+    else hipLaunchKernelGGL((lora_up_kernel<DT_, 1, false>), gu, bl, lds, st, p);                  \
   } while (0)
   if (dtype == kBF16) W4A8_LORA(kBF16);
   else W4A8_LORA(kF16);

@@ -54,14 +54,14 @@ int w4a8_lora_add(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, c
     p.col[i] = n;
     p.chunk[i] = chunks;
     n += slice_cols[i];
-    chunks += (slice_cols[i] + 63) / 64;
+    chunks += (slice_cols[i] + 255) / 256;
   }
   for (int i = slices; i <= kLoraMaxSlices; ++i) {
     p.col[i] = n;
     p.chunk[i] = chunks;
   }
   if (M == 0) return kOk;
-  if ((M + 15) / 16 * ((chunks + 3) / 4) > 0x7fffffff || M > 0x7fffffff)
+  if ((M + 15) / 16 * chunks > 0x7fffffff || M > 0x7fffffff)
     return fail(kErrUnsupported, "%s: past its index ranges (M=%lld, N=%lld)", who, (long long)M, (long long)n);
   if (!x || !a || !b || !scaling || !adapters || !base || !out || !aligned16(x) || !aligned16(a) || !aligned16(b) ||
       !aligned16(base) || !aligned16(out))
