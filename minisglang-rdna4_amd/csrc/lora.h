@@ -17,7 +17,8 @@ struct LoraArgs {
   int L, rank, slices;
   int64_t N;
   int64_t col[kLoraMaxSlices + 1];    // first column of each slice, then N
-  int64_t chunk[kLoraMaxSlices + 1];  // its first chunk of 256 columns, then all of them
+  int64_t span;                       // columns per workgroup of the second product, a multiple of 256
+  int64_t chunk[kLoraMaxSlices + 1];  // each slice's first span, then all of them
   const void* base;  // (M, ldb): the projection's output, in the model's type or f32
   int64_t ldb;
   int base_f32;
@@ -26,7 +27,6 @@ struct LoraArgs {
   float* v;          // (kc, M, slices * rank) partial x A^T
   int kc;            // parts of K
   int64_t kstep;     // its length, a multiple of 512
-  int slots;         // adapters of a block of 16 rows that run side by side
 };
 
 }  // namespace w4a8

@@ -111,248 +111,231 @@ lora_down_kernel(const LoraArgs p) {
   }
 }
 
-// grid: (4 chunks of 64 columns of one slice * blocks of 16 RB rows, 1, slots). A wave per chunk: row (4 q + i) of
-// its j-th product is column 16 q + 4 j + i of the chunk, so a lane ends with 16 neighbouring columns. The
-// workgroup first sums the parts of v for its rows and slice, once for its four chunks, into LDS. (The chunks
-// of a workgroup are of one slice: launch_lora counts them so.) An adapter's B stays in registers over the RB
-// blocks of 16 rows, where its rank is up to 64.
-template <int DT, int RB, bool F32>
-__global__ void __launch_bounds__(256, RB == 4 ? 2 : 4)
+// grid: (spans of p.span columns of one slice * blocks of 16 rows, 1, slots). The workgroup first sums the parts of v
+// for its rows and slice into LDS. Then, adapter by adapter, its waves walk the span, 64 columns each at a time: row
+// (4 q + i) of the j-th product is column 16 q + 4 j + i of them, so a lane ends with 16 neighbouring columns of its
+// row, of which only the adapter's rows are read and written. The next columns' base is loaded while these are
+// computed. NS: steps of 32 ranks whose v operands stay in registers over the span; 0: any rank, from LDS each time.
+template <int DT, bool F32, int NS>
+__global__ void __launch_bounds__(256)
 lora_up_kernel(const LoraArgs p) {
-  constexpr int kPad = 4;  // floats between rows: the rows of a read start 16 bytes apart, modulo the banks
-  extern __shared__ float vs[];  // (16 RB, rank + kPad), then the rows' largest |v|
+  extern __shared__ float vs[];  // (16, rank + 4)
+  constexpr int NB = F32 ? 4 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
-  const uint32_t quads = (uint32_t)p.chunk[p.slices];
-  const uint32_t quad = blockIdx.x % quads;
+  const uint32_t spans = (uint32_t)p.chunk[p.slices], span = blockIdx.x % spans;
   int s = 0;
-  while (quad >= p.chunk[s + 1]) ++s;
-  const int64_t nend = p.col[s + 1];
-  const int64_t n0 = p.col[s] + (int64_t)(quad - p.chunk[s]) * 256 + wave * 64;
-  const int64_t m0 = (int64_t)(blockIdx.x / quads) * (16 * RB);
-  const int R = p.slices * p.rank, ld = p.rank + kPad;
-  const bool work = n0 < nend;  // this wave's columns exist (the last workgroup of a slice may have fewer)
+  while (span >= p.chunk[s + 1]) ++s;
+  const int64_t m0 = (int64_t)(blockIdx.x / spans) * 16, m = m0 + c;
+  const int64_t first = p.col[s] + (span - p.chunk[s]) * p.span;
+  const int64_t end = first + p.span < p.col[s + 1] ? first + p.span : p.col[s + 1];
+  const int R = p.slices * p.rank, ld = p.rank + 4;
+  const Rows rows = row_adapters(p, m0, lane);
 
-  Rows rows[RB];
-  uint4 base[RB][F32 ? 4 : 2];
-  const int64_t n = n0 + 16 * g;
-  const bool cols = work && n < nend;
+  const uint8_t* brow = reinterpret_cast<const uint8_t*>(p.base) + (m < p.M ? m : m0) * p.ldb * (F32 ? 4 : 2);
+  uint16_t* orow = p.out + (m < p.M ? m : m0) * p.ldo;
+  uint4 base[NB];
+  auto load_base = [&](int64_t n, bool on) {
+    if (on && n < end)
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    rows[b] = row_adapters(p, m0 + 16 * b, lane);
-    const int64_t m = m0 + 16 * b + c;
-    if (cols && m < p.M) {
-      const uint4* bp = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.base) + (m * p.ldb + n) * (F32 ? 4 : 2));
+      for (int j = 0; j < NB; ++j) base[j] = reinterpret_cast<const uint4*>(brow + n * (F32 ? 4 : 2))[j];
+  };
+  // base (f32 or the type's) plus d, rounded, at column n of this lane's row
+  auto store = [&](const uint4 (&y)[NB], const v4f (&d)[4], float up, int64_t n) {
+    uint32_t w[8];
 #pragma unroll
-      for (int j = 0; j < (F32 ? 4 : 2); ++j) base[b][j] = bp[j];
+    for (int j = 0; j < 4; ++j) {
+      v4f f;
+      if constexpr (F32) f = __builtin_bit_cast(v4f, y[j]);
+      else {
+        const uint32_t a = j & 1 ? y[j / 2].z : y[j / 2].x, b = j & 1 ? y[j / 2].w : y[j / 2].y;
+        f = v4f{from_dtype((uint16_t)(a & 0xffffu), DT), from_dtype((uint16_t)(a >> 16), DT),
+                from_dtype((uint16_t)(b & 0xffffu), DT), from_dtype((uint16_t)(b >> 16), DT)};
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = __builtin_fmaf(d[j][e], up, f[e]);
+      w[2 * j] = (uint32_t)to_dtype(f[0], DT) | ((uint32_t)to_dtype(f[1], DT) << 16);
+      w[2 * j + 1] = (uint32_t)to_dtype(f[2], DT) | ((uint32_t)to_dtype(f[3], DT) << 16);
     }
-  }
-  // v of the rows that this workgroup's slot does: the i-th adapter of the rows is slot i's, modulo the slots
-  v4f acc[RB][4];
-  bool write[RB], mine_any = false;
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[b][j] = v4f{0.f, 0.f, 0.f, 0.f};
-    write[b] = rows[b].id < 0 && blockIdx.z == 0;  // rows without an adapter are the base itself, the first slot's
-  }
-  // a row is done by this slot when its adapter's place among the rows' adapters is the slot's
-  bool todo[RB];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) todo[b] = false;
+    uint4* op = reinterpret_cast<uint4*>(orow + n);
+    op[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    op[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  };
+
+  // the rows of this workgroup's adapters: the i-th of the block is slot i's, modulo the slots
+  uint32_t todo = 0;
   {
-    Rows r[RB];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) r[b] = rows[b];
-    for (int i = 0;; ++i) {
-      int a = -1;
-#pragma unroll
-      for (int b = 0; b < RB; ++b)
-        if (a < 0 && r[b].left) a = __builtin_amdgcn_readlane(r[b].id, __builtin_ctz(r[b].left));
-      if (a < 0) break;
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        const bool m = r[b].id == a;
-        r[b].left &= ~((uint32_t)__ballot(m) & 0xffffu);
-        if (i % (int)gridDim.z == (int)blockIdx.z) todo[b] = todo[b] || m;
-      }
+    Rows r = rows;
+    for (int i = 0; r.left; ++i) {
+      const uint32_t before = r.left;
+      next_adapter(r);
+      if (i % (int)gridDim.z == (int)blockIdx.z) todo |= before & ~r.left;
     }
   }
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    rows[b].left &= (uint32_t)__ballot(todo[b]) & 0xffffu;
-    mine_any = mine_any || rows[b].left != 0;
-    write[b] = write[b] || todo[b];
-  }
-  if (mine_any) {
-    // four ranks a thread, parts of K in order; rows of other slots are skipped
-    const int per = p.rank / 4;
-    for (int t = threadIdx.x; t < 16 * RB * per; t += 256) {
-      const int row = t / per, r = (t - row * per) * 4;
-      uint32_t left = 0;
-#pragma unroll
-      for (int b = 0; b < RB; ++b) left = row / 16 == b ? rows[b].left : left;
-      v4f v = {0.f, 0.f, 0.f, 0.f};
-      if ((left >> (row & 15)) & 1) {
-        const float* vp = p.v + (m0 + row) * R + s * p.rank + r;
-        const int64_t part = p.M * R;
-        int q = 0;
-        for (; q + 4 <= p.kc; q += 4) {
-          const v4f a0 = *reinterpret_cast<const v4f*>(vp + q * part), a1 = *reinterpret_cast<const v4f*>(vp + (q + 1) * part),
-                    a2 = *reinterpret_cast<const v4f*>(vp + (q + 2) * part), a3 = *reinterpret_cast<const v4f*>(vp + (q + 3) * part);
-          v = (((v + a0) + a1) + a2) + a3;
-        }
-        for (; q < p.kc; ++q) v += *reinterpret_cast<const v4f*>(vp + q * part);
-      }
-      *reinterpret_cast<v4f*>(&vs[row * ld + r]) = v;
-    }
-    __syncthreads();
-  }
-  if (!work) return;
+  const bool bare = blockIdx.z == 0 && rows.id < 0 && m < p.M && (F32 || p.base != p.out);
+  if (!todo && !__ballot(bare)) return;
 
-  bool some = mine_any;
-  while (some) {
-    int a = -1;
+  // four ranks a thread, the parts of K in their order
+  const int per = p.rank / 4;
+  for (int t = threadIdx.x; t < 16 * per; t += 256) {
+    const int row = t / per, r = (t - row * per) * 4;
+    if (!((todo >> row) & 1)) continue;
+    const float* vp = p.v + (m0 + row) * R + s * p.rank + r;
+    const int64_t part = p.M * R;
+    v4f v = {0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < p.kc; q += 8) {
+      v4f x[8];
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
-      if (a < 0 && rows[b].left) a = __builtin_amdgcn_readlane(rows[b].id, __builtin_ctz(rows[b].left));
+      for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const v4f*>(vp + (q + u < p.kc ? q + u : 0) * part);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v += q + u < p.kc ? x[u] : v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    *reinterpret_cast<v4f*>(&vs[row * ld + r]) = v;
+  }
+  // rows without an adapter are the base, rounded to the type
+  if (__ballot(bare)) {
+    const v4f zero[4] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+    for (int64_t n = first + wave * 64 + 16 * g; n < end; n += 256) {
+      load_base(n, bare);
+      if (bare) store(base, zero, 0.f, n);
+    }
+  }
+  __syncthreads();
+
+  Rows r = rows;
+  while (r.left) {
+    const int a = next_adapter(r);
+    const bool mine = rows.id == a && ((todo >> c) & 1);
+    if (!__ballot(mine)) continue;
+    load_base(first + wave * 64 + 16 * g, mine);
     const float scale = p.scaling[a];
-    const uint16_t* bp = p.b + (int64_t)a * p.N * p.rank;
-    auto load_b = [&](int rr, v4w (&bw)[4]) {
-      const int r = rr + 8 * g;
+    const float* vr = vs + c * ld + 8 * g;
+    float top = 0.f;
+    for (int q = 0; q + 8 * g < p.rank; q += 32)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t nn = n0 + (c >> 2) * 16 + j * 4 + (c & 3);
-        const bool in = r < p.rank && nn < nend;
-        bw[j] = load16(bp + (in ? nn * p.rank + r : 0), in);
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(vr[q + e]));
+    top = mine ? top : 0.f;
+    auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+    top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+    auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+    top = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+    // 2^-e with 2^e the power of two at or below the largest |v|; NaN and infinity pass through as they are
+    const uint32_t ex = (__float_as_uint(top) >> 23) & 255u;
+    const bool plain = ex > 1 && ex < 253;
+    const float down = plain ? __uint_as_float((254u - ex) << 23) : 1.f;
+    const float up = (plain ? __uint_as_float(ex << 23) : 1.f) * scale;
+    // v of ranks q .. q + 31 as two terms
+    auto operand = [&](int q, v4w& hi, v4w& lo) {
+      const bool in = mine && q + 8 * g < p.rank;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v0 = in ? vr[q + 2 * e] * down : 0.f, v1 = in ? vr[q + 2 * e + 1] * down : 0.f;
+        const uint16_t h0 = to_dtype(v0, DT), h1 = to_dtype(v1, DT);
+        hi[e] = (uint32_t)h0 | ((uint32_t)h1 << 16);
+        lo[e] = (uint32_t)to_dtype(v0 - from_dtype(h0, DT), DT) | ((uint32_t)to_dtype(v1 - from_dtype(h1, DT), DT) << 16);
       }
     };
-    v4w b0[4], b1[4];
-    load_b(0, b0);
-    if (p.rank > 32) load_b(32, b1);
+    v4w hi[NS + 1], lo[NS + 1];
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const bool mine = rows[b].id == a && todo[b];
-      const uint32_t which = (uint32_t)__ballot(mine) & 0xffffu;
-      if (!which) continue;
-      rows[b].left &= ~which;
-      const float* vr = vs + (16 * b + c) * ld;
-      float top = 0.f;
-      for (int r = 8 * g; r < p.rank; r += 32)
+    for (int q = 0; q < NS; ++q) operand(32 * q, hi[q], lo[q]);
+    const uint16_t* bp = p.b + (int64_t)a * p.N * p.rank;
+    for (int64_t n0 = first + wave * 64; n0 < end; n0 += 256) {
+      uint4 cur[NB];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(vr[r + e]));
-      top = mine ? top : 0.f;
-      auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-      top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-      auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-      top = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
-      // 2^-e with 2^e the power of two at or below the largest |v|; NaN and infinity pass through as they are
-      const uint32_t ex = (__float_as_uint(top) >> 23) & 255u;
-      const bool plain = ex > 1 && ex < 253;
-      const float down = plain ? __uint_as_float((254u - ex) << 23) : 1.f;
-      const float up = (plain ? __uint_as_float(ex << 23) : 1.f) * scale;
+      for (int j = 0; j < NB; ++j) cur[j] = base[j];
       v4f d[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) d[j] = v4f{0.f, 0.f, 0.f, 0.f};
-      auto product = [&](int rr, const v4w (&bw)[4]) {
-        const int r = rr + 8 * g;
-        const bool in = mine && r < p.rank;
-        v4w hi, lo;
+      const int64_t nb = n0 + (c >> 2) * 16 + (c & 3);
+      const bool in = nb - (c & 3) < end;  // slices are multiples of 16 columns
+      const uint16_t* bn = bp + (in ? nb : n0) * p.rank;
+      auto product = [&](int q, const v4w& h, const v4w& l) {
+        const int rk = q + 8 * g;
+        v4w bw[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v0 = in ? vr[r + 2 * e] * down : 0.f, v1 = in ? vr[r + 2 * e + 1] * down : 0.f;
-          const uint16_t h0 = to_dtype(v0, DT), h1 = to_dtype(v1, DT);
-          hi[e] = (uint32_t)h0 | ((uint32_t)h1 << 16);
-          lo[e] = (uint32_t)to_dtype(v0 - from_dtype(h0, DT), DT) | ((uint32_t)to_dtype(v1 - from_dtype(h1, DT), DT) << 16);
-        }
+        for (int j = 0; j < 4; ++j) bw[j] = load16(bn + 4 * j * p.rank + (rk < p.rank ? rk : 0), in && rk < p.rank);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          d[j] = mfma16<DT>(bw[j], hi, d[j]);
-          d[j] = mfma16<DT>(bw[j], lo, d[j]);
+          d[j] = mfma16<DT>(bw[j], h, d[j]);
+          d[j] = mfma16<DT>(bw[j], l, d[j]);
         }
       };
-      product(0, b0);
-      if (p.rank > 32) product(32, b1);
-      for (int rr = 64; rr < p.rank; rr += 32) {
-        v4w bw[4];
-        load_b(rr, bw);
-        product(rr, bw);
-      }
-      if (mine)
+      if constexpr (NS > 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[b][j] = d[j] * up;
+        for (int q = 0; q < NS; ++q) product(32 * q, hi[q], lo[q]);
+      } else {
+        for (int q = 0; q < p.rank; q += 32) {
+          operand(q, hi[0], lo[0]);
+          product(q, hi[0], lo[0]);
+        }
+      }
+      load_base(n0 + 256 + 16 * g, mine);
+      if (mine && n0 + 16 * g < end) store(cur, d, up, n0 + 16 * g);
     }
-    some = false;
-#pragma unroll
-    for (int b = 0; b < RB; ++b) some = some || rows[b].left != 0;
-  }
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int64_t m = m0 + 16 * b + c;
-    if (!write[b] || m >= p.M || !cols) continue;
-    uint32_t w[8];
-    if constexpr (F32) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const v4f y = __builtin_bit_cast(v4f, base[b][j]) + acc[b][j];
-        w[2 * j] = (uint32_t)to_dtype(y[0], DT) | ((uint32_t)to_dtype(y[1], DT) << 16);
-        w[2 * j + 1] = (uint32_t)to_dtype(y[2], DT) | ((uint32_t)to_dtype(y[3], DT) << 16);
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        float f[8];
-        unpack8(base[b][t], DT, f);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          w[4 * t + e] = (uint32_t)to_dtype(f[2 * e] + acc[b][2 * t + e / 2][(2 * e) & 3], DT) |
-                         ((uint32_t)to_dtype(f[2 * e + 1] + acc[b][2 * t + e / 2][(2 * e + 1) & 3], DT) << 16);
-      }
-    }
-    uint16_t* op = p.out + m * p.ldo + n;
-    *reinterpret_cast<uint4*>(op) = make_uint4(w[0], w[1], w[2], w[3]);
-    *reinterpret_cast<uint4*>(op + 8) = make_uint4(w[4], w[5], w[6], w[7]);
   }
 }
 
-// parts of K: enough workgroups for a few rows, one part for many
-int lora_parts(int64_t M, int64_t K) {
-  const int64_t blocks = (M + 15) / 16, most = (K + 511) / 512;
-  int64_t kc = 256 / (blocks > 0 ? blocks : 1);
+// How a call is cut. Few rows (up to 64): every adapter of a block of 16 rows has a workgroup of its own (slots), and
+// 16 ranks; more rows: 64 ranks and a block's adapters one after another. Parts of K, of at least 512 inputs, to
+// about 1024 workgroups; up to 8, since the second kernel sums them in one round of loads.
+struct LoraPlan {
+  int slots, rb, kc;
+  int64_t kstep;
+};
+static LoraPlan lora_plan(int64_t M, int64_t K, int64_t R) {
+  LoraPlan pl;
+  const bool few = M <= 64;
+  pl.slots = few ? (int)(M < 16 ? M : 16) : 1;
+  pl.rb = few || R <= 16 ? 1 : R <= 32 ? 2 : 4;
+  const int64_t tiles = (few ? M : (M + 15) / 16) * ((R + 16 * pl.rb - 1) / (16 * pl.rb));
+  int64_t kc = (1024 + tiles - 1) / tiles, most = (K + 511) / 512;
   if (kc > most) kc = most;
-  if (kc > 16) kc = 16;
-  return kc < 1 ? 1 : (int)kc;
+  if (kc > 8) kc = 8;
+  pl.kc = (int)kc;
+  pl.kstep = (K + kc * 512 - 1) / (kc * 512) * 512;
+  return pl;
 }
 
-int64_t lora_workspace(int64_t M, int64_t K, int64_t R) { return lora_parts(M, K) * M * R * 4; }
+int64_t lora_workspace(int64_t M, int64_t K, int64_t R) { return lora_plan(M, K, R).kc * M * R * 4; }
 
 int launch_lora(LoraArgs& p, int dtype, hipStream_t st) {
   const int R = p.slices * p.rank;
-  p.kc = lora_parts(p.M, p.K);
-  p.kstep = (p.K + p.kc * 512 - 1) / (p.kc * 512) * 512;
-  const int64_t blocks = (p.M + 15) / 16;
-  p.slots = p.M <= 64 ? (int)(p.M < 16 ? p.M : 16) : 1;
-  const int rb = R <= 16 ? 1 : R <= 32 ? 2 : 4;
-  const int64_t groups = (R + 16 * rb - 1) / (16 * rb);
-  const dim3 gd((unsigned)(blocks * groups * p.kc), 1, (unsigned)p.slots), bl(256);
-  // blocks of 64 rows where they fill the card (prompts), of 16 else
-  const int64_t quads = p.chunk[p.slices];
-  const int up_rows = p.slots == 1 && !p.base_f32 && p.rank <= 128 && quads * ((p.M + 63) / 64) >= 1024 ? 64 : 16;
-  const dim3 gu((unsigned)(quads * ((p.M + up_rows - 1) / up_rows)), 1, (unsigned)p.slots);
-  const unsigned lds = (unsigned)(up_rows * (p.rank + 4) * 4);
-#define W4A8_LORA(DT_)                                                                        \
-  do {                                                                                        \
-    if (rb == 1) hipLaunchKernelGGL((lora_down_kernel<DT_, 1>), gd, bl, 0, st, p);            \
-    else if (rb == 2) hipLaunchKernelGGL((lora_down_kernel<DT_, 2>), gd, bl, 0, st, p);       \
-    else hipLaunchKernelGGL((lora_down_kernel<DT_, 4>), gd, bl, 0, st, p);                    \
-    if (hipGetLastError() != hipSuccess) return kErrHip;                                      \
-    if (up_rows == 64) hipLaunchKernelGGL((lora_up_kernel<DT_, 4, false>), gu, bl, lds, st, p);    \
-    else if (p.base_f32) hipLaunchKernelGGL((lora_up_kernel<DT_, 1, true>), gu, bl, lds, st, p);   \
-    else hipLaunchKernelGGL((lora_up_kernel<DT_, 1, false>), gu, bl, lds, st, p);                  \
+  const LoraPlan pl = lora_plan(p.M, p.K, R);
+  p.kc = pl.kc;
+  p.kstep = pl.kstep;
+  const int64_t blocks = (p.M + 15) / 16, groups = (R + 16 * pl.rb - 1) / (16 * pl.rb);
+  const dim3 gd((unsigned)(blocks * groups * p.kc), 1, (unsigned)pl.slots), bl(256);
+  // the second product's spans: one step of the four waves, or up to 8 where the rows fill the card
+  const int64_t quads = (p.N + 255) / 256;
+  int64_t steps = quads * blocks / 2048;
+  steps = steps < 1 ? 1 : steps > 8 ? 8 : steps;
+  p.span = 256 * steps;
+  int64_t spans = 0;
+  for (int i = 0; i <= kLoraMaxSlices; ++i) {
+    p.chunk[i] = spans;
+    if (i < p.slices) spans += (p.col[i + 1] - p.col[i] + p.span - 1) / p.span;
+  }
+  const dim3 gu((unsigned)(spans * blocks), 1, (unsigned)pl.slots);
+  const unsigned lds = (unsigned)(16 * (p.rank + 4) * 4);
+#define W4A8_LORA_UP(DT_, F32_)                                                                       \
+  do {                                                                                                \
+    if (p.rank <= 32) hipLaunchKernelGGL((lora_up_kernel<DT_, F32_, 1>), gu, bl, lds, st, p);         \
+    else if (p.rank <= 64) hipLaunchKernelGGL((lora_up_kernel<DT_, F32_, 2>), gu, bl, lds, st, p);    \
+    else hipLaunchKernelGGL((lora_up_kernel<DT_, F32_, 0>), gu, bl, lds, st, p);                      \
+  } while (0)
+#define W4A8_LORA(DT_)                                                                                \
+  do {                                                                                                \
+    if (pl.rb == 1) hipLaunchKernelGGL((lora_down_kernel<DT_, 1>), gd, bl, 0, st, p);                 \
+    else if (pl.rb == 2) hipLaunchKernelGGL((lora_down_kernel<DT_, 2>), gd, bl, 0, st, p);            \
+    else hipLaunchKernelGGL((lora_down_kernel<DT_, 4>), gd, bl, 0, st, p);                            \
+    if (hipGetLastError() != hipSuccess) return kErrHip;                                              \
+    if (p.base_f32) W4A8_LORA_UP(DT_, true);                                                          \
+    else W4A8_LORA_UP(DT_, false);                                                                    \
   } while (0)
   if (dtype == kBF16) W4A8_LORA(kBF16);
   else W4A8_LORA(kF16);
 #undef W4A8_LORA
+#undef W4A8_LORA_UP
   return hipGetLastError() == hipSuccess ? kOk : kErrHip;
 }
 

@@ -52,14 +52,10 @@ int w4a8_lora_add(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, c
     if (slice_cols[i] <= 0 || slice_cols[i] % 16 || slice_cols[i] > 0x7fffffff)
       return fail(kErrInvalid, "%s: slice %d has %lld columns (multiples of 16)", who, i, (long long)slice_cols[i]);
     p.col[i] = n;
-    p.chunk[i] = chunks;
     n += slice_cols[i];
     chunks += (slice_cols[i] + 255) / 256;
   }
-  for (int i = slices; i <= kLoraMaxSlices; ++i) {
-    p.col[i] = n;
-    p.chunk[i] = chunks;
-  }
+  for (int i = slices; i <= kLoraMaxSlices; ++i) p.col[i] = n;
   if (M == 0) return kOk;
   if ((M + 15) / 16 * chunks > 0x7fffffff || M > 0x7fffffff)
     return fail(kErrUnsupported, "%s: past its index ranges (M=%lld, N=%lld)", who, (long long)M, (long long)n);
