@@ -25,8 +25,8 @@ __device__ __forceinline__ v4f mfma16(const v4w& a, const v4w& b, const v4f& c) 
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ v4w load16(const uint16_t* p, bool on) {
-  const uint4 u = on ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+__device__ __forceinline__ v4w load16(const uint16_t* p) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
   return v4w{u.x, u.y, u.z, u.w};
 }
 
@@ -68,27 +68,40 @@ lora_down_kernel(const LoraArgs p) {
   for (int i = 0; rows.left; ++i) {
     const int a = next_adapter(rows);
     if (i % (int)gridDim.z != (int)blockIdx.z) continue;
+    // Rows of other adapters and ranks past R are loaded as some row that is there, and their sums dropped below:
+    // a column of the product is one row's, a row of it one rank's.
     const bool mine = rows.id == a;
-    const uint16_t* xp = p.x + (m0 + (mine ? c : 0)) * p.ldx;
+    const int some = __builtin_ctz((uint32_t)__ballot(mine));
+    const uint16_t* xp = p.x + (m0 + (mine ? c : some)) * p.ldx;
     const uint16_t* ap[RB];
-    bool ron[RB];
 #pragma unroll
     for (int t = 0; t < RB; ++t) {
       const int r = r0 + 16 * t + c;
-      ron[t] = r < R;
-      ap[t] = p.a + ((int64_t)a * R + (ron[t] ? r : 0)) * p.K;
+      ap[t] = p.a + ((int64_t)a * R + (r < R ? r : R - 1)) * p.K;
     }
     v4f acc[RB];
 #pragma unroll
     for (int t = 0; t < RB; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int64_t k = k0 + wave * 128 + g * 32; k < k1 + g * 32; k += 512) {
+    for (int64_t kb = k0 + wave * 128; kb < k1; kb += 512) {
+      const int64_t k = kb + g * 32;
       v4w xv[4], av[RB][4];
+      if (kb + 128 <= k1) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool in = k + 8 * j < k1;
-        xv[j] = load16(xp + k + 8 * j, in && mine);
+        for (int j = 0; j < 4; ++j) {
+          xv[j] = load16(xp + k + 8 * j);
 #pragma unroll
-        for (int t = 0; t < RB; ++t) av[t][j] = load16(ap[t] + k + 8 * j, in && ron[t]);
+          for (int t = 0; t < RB; ++t) av[t][j] = load16(ap[t] + k + 8 * j);
+        }
+      } else {
+        // K's last inputs: past them x and A are zeros
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool in = k + 8 * j < k1;
+          const v4w zero = {0, 0, 0, 0};
+          xv[j] = in ? load16(xp + k + 8 * j) : zero;
+#pragma unroll
+          for (int t = 0; t < RB; ++t) av[t][j] = in ? load16(ap[t] + k + 8 * j) : zero;
+        }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -247,13 +260,13 @@ lora_up_kernel(const LoraArgs p) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) d[j] = v4f{0.f, 0.f, 0.f, 0.f};
       const int64_t nb = n0 + (c >> 2) * 16 + (c & 3);
-      const bool in = nb - (c & 3) < end;  // slices are multiples of 16 columns
-      const uint16_t* bn = bp + (in ? nb : n0) * p.rank;
+      // slices are multiples of 16 columns: those past the end are the first 16 again, and not stored
+      const uint16_t* bn = bp + (nb - (c & 3) < end ? nb : n0 + (c & 3)) * p.rank;
       auto product = [&](int q, const v4w& h, const v4w& l) {
         const int rk = q + 8 * g;
         v4w bw[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) bw[j] = load16(bn + 4 * j * p.rank + (rk < p.rank ? rk : 0), in && rk < p.rank);
+        for (int j = 0; j < 4; ++j) bw[j] = load16(bn + 4 * j * p.rank + (rk < p.rank ? rk : 0));  // v is 0 past the rank
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           d[j] = mfma16<DT>(bw[j], h, d[j]);
