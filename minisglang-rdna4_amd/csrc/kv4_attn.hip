@@ -14,7 +14,7 @@
 // O - 7.5 sum w + sum p (m + 7.5 s), sum w by one more product with a row of ones: the error is within 2^-12
 // of half a V vector's range, an eighth of the output's own rounding. So that p s stays in fp16's range
 // whatever V's steps are, p carries 2^-e, 2^e about the largest step so far over 64: it moves with the running
-// maximum and drops out of the quotient.
+// maximum, column by column, and drops out of the quotient.
 // The row of S that a lane of group g = lane / 16 holds is chosen to be the token whose V codes that
 // lane holds (tokens 8 g + r in the first 16 rows' register r, 8 g + 4 + r in the second's), so p goes
 // from one product into the next in its lane, and nothing passes through LDS.
@@ -306,10 +306,12 @@ kv4_attn_kernel(const Kv4Attn p) {
 
     v4f o[NQ][DB], ws[NQ];                // ws: sum w (bf16 models), in every register
     float m[NQ], mu[NQ], l[NQ], cc[NQ];   // mu: M, the maximum in powers of two (0 while no key was seen) plus e
-    int ex = -46;                         // e
-    float lim = -1.f;                     // steps up to here are in e's range; none was seen yet
+    int ex[NQ];                           // e
+    float lim[NQ];                        // steps up to here are in e's range; none was seen yet
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
+      ex[j] = -46;
+      lim[j] = -1.f;
       m[j] = -kInf;
       mu[j] = l[j] = cc[j] = 0.f;
       ws[j] = v4f{0.f, 0.f, 0.f, 0.f};
@@ -337,6 +339,9 @@ kv4_attn_kernel(const Kv4Attn p) {
         }
       if (more) load_k(next);
 
+      // the vector unit is what bounds a wave here: it goes before the other wave's products (prompts of 8192 1428 ->
+      // 1391 us)
+      __builtin_amdgcn_s_setprio(1);
       float y[NQ][8], sv[8], mv[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -346,41 +351,51 @@ kv4_attn_kernel(const Kv4Attn p) {
         sv[i] = lo16<DT>(vsw[i]);
         mv[i] = W == 1 ? __builtin_fmaf(7.5f, sv[i], hi16<DT>(vsw[i])) : hi16<DT>(vsw[i]);
       }
+      auto top8 = [](const float (&v)[8]) {
+        return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+      };
+      float ts[NQ];  // the largest V step that the column sees
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) ts[j] = top8(sv);
       if (!(t0 >= ks.lo_all && t0 + 32 <= ks.hi_all && at.has_a && at.has_b)) {
         // An unseen token's scale may be anything, and 0 times it is not 0: what is not finite, and a missing page,
         // is NaN in the score of whoever sees it, and 0 here.
         const bool ha = at.has_a, hb = at.has_b, missing = !(g < 2 ? ha : hb);
         const int tb = t0 + 8 * g;
 #pragma unroll
+        for (int j = 0; j < NQ; ++j) ts[j] = 0.f;
+#pragma unroll
         for (int i = 0; i < 8; ++i) {
           const bool bad = missing || !__builtin_isfinite(sv[i]) || !__builtin_isfinite(mv[i]);
           sv[i] = bad ? 0.f : sv[i];
           mv[i] = bad ? 0.f : mv[i];
-          if (tb + i < ks.lo || tb + i >= ks.hi) sv[i] = 0.f;  // not a step to scale by
 #pragma unroll
-          for (int j = 0; j < NQ; ++j)
-            y[j][i] = tb + i >= klo[j] && tb + i < khi[j] ? (bad ? __builtin_nanf("") : y[j][i]) : -kInf;
+          for (int j = 0; j < NQ; ++j) {
+            const bool see = tb + i >= klo[j] && tb + i < khi[j];
+            y[j][i] = see ? (bad ? __builtin_nanf("") : y[j][i]) : -kInf;
+            ts[j] = see ? fmaxf(ts[j], sv[i]) : ts[j];
+          }
         }
       }
-      auto top8 = [](const float (&v)[8]) {
-        return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
-      };
-      const float ts = top8(sv);
       float top[NQ];
-      bool up = ts > lim;
+      bool up = false;
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
         top[j] = top8(y[j]);
-        up = up || top[j] > m[j] + slack[j];
+        up = up || top[j] > m[j] + slack[j] || ts[j] > lim[j];
       }
       if (__ballot(up)) {
-        // 2^-e takes the largest step to [2^5, 2^6); steps that 2^-40 bounds stay below
-        const int te = (int)((__float_as_uint(wave_max(ts)) >> 23) & 255u) - 132;
-        const int en = __builtin_amdgcn_readfirstlane(min(max(te, ex), 94));
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
-          const float mn = fmaxf(m[j], col_max(top[j]));
-          const float mun = (mn == -kInf ? 0.f : mn * sc[j]) + (float)en;
+          // a column that has no need keeps its bits, whatever its neighbours do
+          const float tt = col_max(ts[j]), tp = col_max(top[j]);
+          const bool need = tp > m[j] + slack[j] || tt > lim[j];
+          // 2^-e takes the column's largest step to [2^5, 2^6); steps that 2^-40 bounds stay below
+          const int te = (int)((__float_as_uint(tt) >> 23) & 255u) - 132;
+          ex[j] = need ? min(max(te, ex[j]), 94) : ex[j];
+          lim[j] = need ? __uint_as_float((uint32_t)(ex[j] + 6 + 127) << 23) : lim[j];
+          const float mn = need ? fmaxf(m[j], tp) : m[j];
+          const float mun = need ? (mn == -kInf ? 0.f : mn * sc[j]) + (float)ex[j] : mu[j];
           const float f = m[j] == -kInf ? 1.f : __builtin_amdgcn_exp2f(mu[j] - mun);  // nothing summed yet: any
           m[j] = mn;
           mu[j] = mun;
@@ -390,8 +405,6 @@ kv4_attn_kernel(const Kv4Attn p) {
 #pragma unroll
           for (int d = 0; d < DB; ++d) o[j][d] *= f;
         }
-        ex = en;
-        lim = __uint_as_float((uint32_t)(ex + 6 + 127) << 23);
       }
 #pragma unroll
       for (int i = 1; i < 8; i += 2) sv[i] *= 0.0625f;  // the higher codes
@@ -415,6 +428,7 @@ kv4_attn_kernel(const Kv4Attn p) {
         // sum w: ones, sixteens against the higher codes' 1/16
         if (W == 1) ws[j] = mfma16(v4w{0x3c003c00u, 0x4c004c00u, 0x3c003c00u, 0x4c004c00u}, ph[j], ws[j]);
       }
+      __builtin_amdgcn_s_setprio(0);
       if (more) load_s(next);
 #pragma unroll
       for (int d = 0; d < DB; ++d) {

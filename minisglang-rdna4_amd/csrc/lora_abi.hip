@@ -57,7 +57,7 @@ int w4a8_lora_add(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, c
   }
   for (int i = slices; i <= kLoraMaxSlices; ++i) p.col[i] = n;
   if (M == 0) return kOk;
-  if ((M + 15) / 16 * chunks > 0x7fffffff || M > 0x7fffffff)
+  if ((M + 15) / 16 * chunks > 0x7fffffff || M > (1 << 26))
     return fail(kErrUnsupported, "%s: past its index ranges (M=%lld, N=%lld)", who, (long long)M, (long long)n);
   if (!x || !a || !b || !scaling || !adapters || !base || !out || !aligned16(x) || !aligned16(a) || !aligned16(b) ||
       !aligned16(base) || !aligned16(out))

@@ -141,9 +141,10 @@ class Setup:
         lf = torch.isfinite(rl)
         assert torch.equal(torch.isfinite(lse.cpu()), lf), what
         if lf.any():
-            # A score is s (q c) + m sum(q): both terms may be far larger than it. Each passes about eight f32 roundings
-            # (the products' four steps, the two terms, the scale, M and the logarithm of the sum), 2^-24 of it each.
-            most = self.k.double().abs().max().item() * q.double().sum(-1).abs().max().item() * kw.get("sm_scale", D ** -0.5)
+            # A score is s (q c) + m sum(q): both terms may be far larger than it, up to a key's range times sum|q|, and
+            # that is at most twice the largest key value times sum|q|. Each passes about eight f32 roundings (the
+            # products' four steps, the two terms, the scale, M and the logarithm of the sum), 2^-24 of it each.
+            most = 2 * self.k.double().abs().max().item() * q.double().abs().sum(-1).max().item() * kw.get("sm_scale", D ** -0.5)
             assert (lse.cpu().double() - rl)[lf].abs().max().item() < 2e-4 + 2.0 ** -21 * most, what
         return out
 
@@ -197,9 +198,9 @@ def test_abi_refuses_before_any_launch():
     P = 1 << 20
 
     def attend(dtype=0, ldq=4096, hq=128, T=4, Hq=32, H=8, D=128, kc=P, pages=16, page=16, table=P, ldt=4, width=4, cu=P,
-               B=2, window=0, max_q=1, max_kv=64, out=P, ws=None, ws_bytes=0):
+               B=2, window=0, max_q=1, max_kv=64, out=P, ws=None, ws_bytes=0, scale=1.0):
         rc = lib.w4a8_kv4_attention(P, dtype, ldq, hq, T, Hq, H, D, kc, P, P, P, pages, page, table, ldt, width, cu, P, B,
-                                    1.0, 1, window, max_q, max_kv, out, 4096, 128, None, ws, ws_bytes, None)
+                                    scale, 1, window, max_q, max_kv, out, 4096, 128, None, ws, ws_bytes, None)
         return rc, lib.w4a8_last_error()
 
     for kw, code, msg in ((dict(dtype=2), 1, b"bf16 or fp16"), (dict(D=96), 2, b"64, 128 or 256"),
@@ -207,7 +208,9 @@ def test_abi_refuses_before_any_launch():
                           (dict(Hq=12, H=8), 1, b"query heads"), (dict(Hq=4, H=8), 1, b"query heads"),
                           (dict(T=-1), 1, b"sizes"), (dict(pages=0), 1, b"sizes"), (dict(B=65536), 2, b"index ranges"),
                           (dict(pages=1 << 28), 2, b"index ranges"), (dict(width=1 << 28), 2, b"index ranges"),
-                          (dict(window=-1), 1, b"window"), (dict(max_kv=-1), 1, b"max_kv"),
+                          (dict(scale=0.0), 1, b"positive"), (dict(scale=-1.0), 1, b"positive"),
+                          (dict(scale=float("nan")), 1, b"positive"), (dict(scale=float("inf")), 1, b"positive"),
+                          (dict(T=1 << 26), 2, b"index ranges"), (dict(window=-1), 1, b"window"), (dict(max_kv=-1), 1, b"max_kv"),
                           (dict(kc=P + 8), 1, b"aligned"), (dict(kc=None), 1, b"aligned"), (dict(cu=None), 1, b"cu"),
                           (dict(table=None), 1, b"page table"), (dict(ldt=3), 1, b"page table"),
                           (dict(ldq=4100), 1, b"multiples of 8"), (dict(hq=4), 1, b"multiples of 8"),
@@ -378,7 +381,7 @@ def test_bad_pages_and_lengths_touch_nothing(dev):
 # ------------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("D,H,G,page", [(128, 2, 4, 16), (128, 1, 1, 64), (64, 2, 3, 32), (256, 1, 2, 16), (128, 1, 16, 128), (64, 1, 17, 16)])
+@pytest.mark.parametrize("D,H,G,page", [(128, 2, 4, 16), (128, 1, 1, 64), (64, 2, 3, 32), (256, 1, 2, 16), (128, 1, 16, 128), (64, 1, 17, 16), (128, 1, 128, 32)])
 def test_decode(dev, dtype, D, H, G, page):
     lens = [1, 2, 31, 32, 33, 64, 100, 257, 1000, 0, 5]
     s = Setup(dev, dtype, D, H, page, lens, [1] * len(lens))
@@ -439,6 +442,56 @@ def test_unseen_tokens_do_not_reach_the_output(dev):
     seen = torch.zeros(60, dtype=torch.bool)
     seen[40:45] = seen[50:55] = True
     assert torch.equal(torch.isnan(out.cpu()).all(-1).all(-1), seen) and torch.equal(torch.isnan(out.cpu()).any(-1).any(-1), seen)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_do_not_depend_on_what_they_do_not_see(dev, dtype):
+    """A later token with huge values (its V step 2^25 times the others') in the same tile and the same block of
+    columns: the rows before it keep every bit, the rows after it are right."""
+    kv4 = _kv4()
+    s = Setup(dev, dtype, 128, 1, 16, [60], [60], seed=21)
+    s.v *= 1e-3
+    kv4.kv4_append(s.cache, s.k.to(dev), s.v.to(dev), s.d_table, s.cu_all.to(dev), s.d_seq)
+    q = s.q(2)
+    before = s.attend(q)
+    s.v[45] *= 2.0 ** 25
+    s.k[52] *= 100.0
+    kv4.kv4_append(s.cache, s.k.to(dev), s.v.to(dev), s.d_table, s.cu_all.to(dev), s.d_seq)
+    after = s.check(q, "outlier")
+    assert torch.equal(before[:45], after[:45])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,page", [(65, 16), (300, 32)])
+def test_many_sequences(dev, dtype, B, page):
+    """More sequences than lanes, empty ones and ones without new tokens among them, in calls of one row and of many."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 25, (B,), generator=g).tolist()
+    lens[7:20] = [0] * 13
+    s = Setup(dev, dtype, 64, 1, page, lens, [min(n, i % 3) for i, n in enumerate(lens)], seed=B)
+    k, v = _kv4().kv4_read(s.cache, s.d_table, s.cu_all.to(dev), s.d_seq, sum(lens))
+    assert torch.equal(k.cpu(), ref_values(s.k).float().to(dtype)) and torch.equal(v.cpu(), ref_values(s.v).float().to(dtype))
+    s.check(s.q(2), "decode", max_q=2)
+    # the whole again through the few-rows path, one call per sequence
+    for b in (0, 6, 21, B - 1):
+        if lens[b]:
+            at = sum(lens[:b])
+            cu = torch.tensor([0, lens[b]], dtype=torch.int32, device=dev)
+            k1, v1 = _kv4().kv4_read(s.cache, s.d_table[b:b + 1], cu, s.d_seq[b:b + 1], lens[b])
+            assert torch.equal(k1, k[at:at + lens[b]]) and torch.equal(v1, v[at:at + lens[b]])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_append_of_prompts(dev, dtype):
+    """Enough rows that a wave looks at 8 of them, prompts that start and end anywhere in a block."""
+    lens = [1003, 2, 777, 4001, 13, 8, 1]
+    s = Setup(dev, dtype, 128, 2, 16, lens, [1] * 7, seed=3)
+    assert sum(lens) * 2 > 8192
+    k, v = _kv4().kv4_read(s.cache, s.d_table, s.cu_all.to(dev), s.d_seq, sum(lens))
+    assert torch.equal(k.cpu(), ref_values(s.k).float().to(dtype)) and torch.equal(v.cpu(), ref_values(s.v).float().to(dtype))
 
 
 @pytest.mark.gpu
