@@ -205,7 +205,7 @@ __device__ __forceinline__ void kv4_store(const Kv4Attn& p, int split, int64_t r
 // D: channels; DT: the model's type; NQ: blocks of 16 columns per wave; WKV: waves of a workgroup that share
 // their columns
 template <int D, int DT, int NQ, int WKV>
-__global__ void __launch_bounds__(256, WKV == 1 ? 2 : D == 256 ? 2 : 3)
+__global__ void __launch_bounds__(256, D == 256 || (NQ == 2 && D == 128) ? 2 : 3)
 kv4_attn_kernel(const Kv4Attn p) {
   static_assert(WKV == 1 || (WKV == 4 && NQ == 1), "side by side, or one block of columns");
   constexpr int KS = D / 32, DB = D / 16;  // products per S tile, blocks of 16 channels
@@ -252,15 +252,12 @@ kv4_attn_kernel(const Kv4Attn p) {
 
     // this lane's queries: columns 16 j + col
     const int i0 = c0 / p.G, r0 = c0 - i0 * p.G;
-    int klo[NQ], khi[NQ];
     uint4 qr[NQ][KS];
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
       int head;
       const int i = kv4_query(p, i0, r0, 16 * j + col, head);
       const bool on = c0 + 16 * j + col < sp.cols;
-      khi[j] = on ? seen_upto(p, sp, i) : 0;
-      klo[j] = seen_from(p, sp, i);
       const uint16_t* qp = p.q + (sp.start + (on ? i : 0)) * p.ldq + (h * p.G + (on ? head : 0)) * p.hq + g * (D / 4);
 #pragma unroll
       for (int w = 0; w < KS; ++w) qr[j][w] = on ? *reinterpret_cast<const uint4*>(qp + 8 * w) : make_uint4(0, 0, 0, 0);
@@ -272,7 +269,7 @@ kv4_attn_kernel(const Kv4Attn p) {
       load_v(at);
     }
     v4w qf[NQ][KS];
-    float qs[NQ], sc[NQ], slack[NQ];  // sum(q) and x's factor, in the products' units, and 8 powers of two there
+    float qs[NQ], sc[NQ];  // sum(q) and x's factor, in the products' units
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
       float sum = 0.f, top = 0.f;
@@ -291,7 +288,6 @@ kv4_attn_kernel(const Kv4Attn p) {
       const int eq = max(141 - (int)(__float_as_uint(top) >> 23), -100);
       qs[j] = __builtin_ldexpf(col_sum(sum), eq - 24);
       sc[j] = __builtin_ldexpf(p.scale, 24 - eq);
-      slack[j] = 8.f / sc[j];
 #pragma unroll
       for (int w = 0; w < KS; ++w) {
         float f[8];
@@ -305,14 +301,13 @@ kv4_attn_kernel(const Kv4Attn p) {
     }
 
     v4f o[NQ][DB], ws[NQ];                // ws: sum w (bf16 models), in every register
+    float thr[NQ];                        // scores up to here leave the maximum as it is: m and 8 powers of two
     float m[NQ], mu[NQ], l[NQ], cc[NQ];   // mu: M, the maximum in powers of two (0 while no key was seen) plus e
-    int ex[NQ];                           // e
-    float lim[NQ];                        // steps up to here are in e's range; none was seen yet
+    float lim[NQ];                        // 2^(e + 6): steps up to here are in its range; 0: none was seen yet
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
-      ex[j] = -46;
-      lim[j] = -1.f;
-      m[j] = -kInf;
+      lim[j] = 0.f;
+      m[j] = thr[j] = -kInf;
       mu[j] = l[j] = cc[j] = 0.f;
       ws[j] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -339,9 +334,6 @@ kv4_attn_kernel(const Kv4Attn p) {
         }
       if (more) load_k(next);
 
-      // the vector unit is what bounds a wave here: it goes before the other wave's products (prompts of 8192 1428 ->
-      // 1391 us)
-      __builtin_amdgcn_s_setprio(1);
       float y[NQ][8], sv[8], mv[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -361,9 +353,15 @@ kv4_attn_kernel(const Kv4Attn p) {
         // An unseen token's scale may be anything, and 0 times it is not 0: what is not finite, and a missing page,
         // is NaN in the score of whoever sees it, and 0 here.
         const bool ha = at.has_a, hb = at.has_b, missing = !(g < 2 ? ha : hb);
-        const int tb = t0 + 8 * g;
+        int klo[NQ], khi[NQ];  // the column's keys, from this lane's first token
 #pragma unroll
-        for (int j = 0; j < NQ; ++j) ts[j] = 0.f;
+        for (int j = 0; j < NQ; ++j) {
+          int head;
+          const int i = kv4_query(p, i0, r0, 16 * j + col, head);
+          khi[j] = (c0 + 16 * j + col < sp.cols ? seen_upto(p, sp, i) : 0) - (t0 + 8 * g);
+          klo[j] = seen_from(p, sp, i) - (t0 + 8 * g);
+          ts[j] = 0.f;
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const bool bad = missing || !__builtin_isfinite(sv[i]) || !__builtin_isfinite(mv[i]);
@@ -371,7 +369,7 @@ kv4_attn_kernel(const Kv4Attn p) {
           mv[i] = bad ? 0.f : mv[i];
 #pragma unroll
           for (int j = 0; j < NQ; ++j) {
-            const bool see = tb + i >= klo[j] && tb + i < khi[j];
+            const bool see = i >= klo[j] && i < khi[j];
             y[j][i] = see ? (bad ? __builtin_nanf("") : y[j][i]) : -kInf;
             ts[j] = see ? fmaxf(ts[j], sv[i]) : ts[j];
           }
@@ -382,23 +380,24 @@ kv4_attn_kernel(const Kv4Attn p) {
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
         top[j] = top8(y[j]);
-        up = up || top[j] > m[j] + slack[j] || ts[j] > lim[j];
+        up = up || top[j] > thr[j] || ts[j] > lim[j];
       }
       if (__ballot(up)) {
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
           // a column that has no need keeps its bits, whatever its neighbours do
           const float tt = col_max(ts[j]), tp = col_max(top[j]);
-          const bool need = tp > m[j] + slack[j] || tt > lim[j];
+          const bool need = tp > thr[j] || tt > lim[j];
           // 2^-e takes the column's largest step to [2^5, 2^6); steps that 2^-40 bounds stay below
-          const int te = (int)((__float_as_uint(tt) >> 23) & 255u) - 132;
-          ex[j] = need ? min(max(te, ex[j]), 94) : ex[j];
-          lim[j] = need ? __uint_as_float((uint32_t)(ex[j] + 6 + 127) << 23) : lim[j];
+          const int old = (int)(__float_as_uint(lim[j]) >> 23), le = (int)((__float_as_uint(tt) >> 23) & 255u) + 1;
+          const int nl = need ? min(max(max(le, old), 87), 227) : old;  // lim's exponent
+          lim[j] = __uint_as_float((uint32_t)nl << 23);
           const float mn = need ? fmaxf(m[j], tp) : m[j];
-          const float mun = need ? (mn == -kInf ? 0.f : mn * sc[j]) + (float)ex[j] : mu[j];
+          const float mun = need ? (mn == -kInf ? 0.f : mn * sc[j]) + (float)(nl - 133) : mu[j];
           const float f = m[j] == -kInf ? 1.f : __builtin_amdgcn_exp2f(mu[j] - mun);  // nothing summed yet: any
           m[j] = mn;
           mu[j] = mun;
+          thr[j] = mn + 8.f / sc[j];
           l[j] *= f;
           cc[j] *= f;
           ws[j] *= f;
@@ -428,7 +427,6 @@ kv4_attn_kernel(const Kv4Attn p) {
         // sum w: ones, sixteens against the higher codes' 1/16
         if (W == 1) ws[j] = mfma16(v4w{0x3c003c00u, 0x4c004c00u, 0x3c003c00u, 0x4c004c00u}, ph[j], ws[j]);
       }
-      __builtin_amdgcn_s_setprio(0);
       if (more) load_s(next);
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
