@@ -576,11 +576,11 @@ PyObject* lora_add(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// linear_lora(a, b, scaling, slices, adapters, x, w, scales, zeros, group, e2m1, x_fp8, act_scales, arm, f32 base)
-// -> out or None: linear() above with arm 0, 1 or 2, its output in f32 until the adapters are added, or not
+// linear_lora(a, b, scaling, slices, adapters, x, w, scales, zeros, group, e2m1, x_fp8, act_scales, arm)
+// -> out or None: linear() above with arm 0, 1 or 2, its output in f32 until the adapters are added
 PyObject* linear_lora(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 15 || !bound) {
-    PyErr_SetString(PyExc_TypeError, "linear_lora: 15 arguments, after bind()");
+  if (n != 14 || !bound) {
+    PyErr_SetString(PyExc_TypeError, "linear_lora: 14 arguments, after bind()");
     return nullptr;
   }
   return guarded([&]() -> PyObject* {
@@ -589,7 +589,6 @@ PyObject* linear_lora(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (PyErr_Occurred()) return nullptr;
       Py_RETURN_NONE;
     }
-    const bool f32 = PyObject_IsTrue(a[14]) == 1;
     Dense d;
     if (!dense(a + 5, false, a[13], d)) {
       if (PyErr_Occurred()) return nullptr;
@@ -603,17 +602,16 @@ PyObject* linear_lora(PyObject*, PyObject* const* a, Py_ssize_t n) {
     // the projection's workspace, the adapters' one and the f32 output in one allocation
     const int64_t at1 = (std::max<int64_t>(d.wsb, 0) + 255) / 256 * 256, at2 = at1 + (lwb + 255) / 256 * 256;
     at::Tensor out = empty(*d.x, {d.M, d.N}, d.x->scalar_type());
-    at::Tensor mem = empty(*d.x, {at2 + (f32 ? d.M * d.N * 4 : 0)}, at::kByte);
+    at::Tensor mem = empty(*d.x, {at2 + d.M * d.N * 4}, at::kByte);
     uint8_t* m = static_cast<uint8_t*>(mem.data_ptr());
-    void* base = f32 ? static_cast<void*>(m + at2) : out.data_ptr();
-    const int bdt = f32 ? kF32 : d.dt;
+    void* base = m + at2;
     void* st = stream_of(*d.x);
     const char* what = "w4a8_linear";
     const int rc = unlocked([&] {
-      const int r = d.launch(base, bdt, d.N, m, st);
+      const int r = d.launch(base, kF32, d.N, m, st);
       if (r) return r;
       what = "w4a8_linear_lora";
-      return add_adapters(*d.x, l, base, bdt, d.N, out.data_ptr(), d.N, m + at1, lwb, st);
+      return add_adapters(*d.x, l, base, kF32, d.N, out.data_ptr(), d.N, m + at1, lwb, st);
     });
     if (rc) return failed(rc, what);
     return THPVariable_Wrap(std::move(out));

@@ -49,7 +49,7 @@ def _check_step(half, x, ids, lens, news, table, outs):
         base = kernels.w4a8_linear(inp.to(half.dev), layer._w_packed_op, layer._scales_op, None, 128).cpu().double()
         d, mag = delta(inp, *raw, slices, ids)
         want = base + d
-        # the projection alone is rounded to the type too, which the operator does once less up to 128 rows
+        # here the projection alone is rounded to the type too; the operator rounds the sum only
         assert ((got.double() - want).abs() <= eps * (want.abs() + base.abs()) + 2.0 ** -14 * mag + 2.0 ** -24).all()
     ref, _ = ref_attention(qkv[:, :HQ * D].reshape(-1, HQ, D), cache_values(half.att.cache), table, PAGE, lens, news, D ** -0.5)
     vmax = qkv[:, HQ * D + KV:].double().abs().max().item() + 4

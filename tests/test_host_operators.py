@@ -6,7 +6,7 @@ import torch
 import synth
 from conftest import pkg
 
-NEW = {"kv4_append": 9, "kv4_read": 8, "kv4_attention": 15, "lora_add": 8, "linear_lora": 15}
+NEW = {"kv4_append": 9, "kv4_read": 8, "kv4_attention": 15, "lora_add": 8, "linear_lora": 14}
 
 
 def test_cpu_tensors_and_wrong_counts_are_left_alone():
