@@ -8,8 +8,10 @@
 // of its words; tokens of the block that are not new keep their nibbles. Blocks are found from the rows: a row
 // leads its block when it is the first new token in it. A wave looks at `rows` rows, 8 of a prompt, which lead one
 // block as a rule, or one of a decode step, which leads its own.
-// All loads of a block are in flight before the first is used. 7000 prompt tokens x 4 heads of 128 (18 MB in and
-// out): see DESIGN for the times; bound by the launch and the chain row -> sequence -> page -> block.
+// All loads of a block are in flight before the first is used. 6900 prompt tokens x 4 heads of 128 (14 MB in, 4 MB
+// out) 14 us, and 7 us to read them back (a wave per token and head, with wave-wide reductions of one vector at a
+// time, 35 and 17); 64 decode tokens x 8 heads 5 and 3.3 us. Bound by the chain row -> sequence -> page -> block,
+// one dependent read each, and for prompts by the quantizing, 16 vectors a wave at 3.5 waves per SIMD.
 #include "kv4.h"
 
 namespace w4a8 {

@@ -9,6 +9,11 @@
 //   up:   y[m, n] = base + scaling sum_r v[m, slice * rank + r] B[a, n, r], rounded once
 // v keeps f32: it enters the second product as two terms of the model's type (v's first 16 bits for bf16,
 // 22 for fp16), scaled by a power of two per row so that neither fp16's range nor its subnormals matter.
+//
+// Measured, first and second kernel: one row, K = N = 4096, rank 16: 2.3 and 4.8 us, latency; 48 rows of 40 adapters,
+// K = 14336, N = 4096, rank 64 (A 73 MB, B 21 MB): 16.7 (4.4 TB/s) and 10.4 us; 4096 rows, K = 4096, N = 28672 in two
+// slices, rank 16: 18.6 and 126 us (y in and out, 470 MB, 3.7 TB/s). The second kernel with 64 rows a workgroup and
+// all their sums in registers took 161 us there: 240 registers a wave, and less of y in flight.
 #include "lora.h"
 
 namespace w4a8 {
