@@ -26,11 +26,11 @@
 // the same time, and share them in the caches. Where that leaves the card empty the grid splits the tokens
 // too, and kv4_join_kernel joins the parts.
 //
-// Measured. Decode is bound by HBM: two sequences of 131072 tokens x 8 heads of 128 (280 MB) 64 us, 4.4 TB/s, at 3
-// waves per SIMD (at 4, 128 registers, spills make it 70 to 77). Prompts by the vector unit: 8192 + 5690 + 3190 tokens,
+// Measured. Decode is bound by HBM: two sequences of 131072 tokens x 8 heads of 128 (280 MB) 64 us, 4.4 TB/s, with
+// cold caches, at 3 waves per SIMD (warm 57; at 4 waves, whose 128 registers spill, 70). Prompts by the vector unit: 8192 + 5690 + 3190 tokens,
 // 32 heads of 128 (898 GFLOP) 1.46 ms, 615 TFLOP/s: 330 vector instructions a tile and wave, 80 of them to widen
 // codes and 180 for the softmax of 32 columns, beside 34 MFMA of 16 cycles; 2 waves per SIMD (16 columns a wave, 3
-// waves: 1.69 ms; 64 columns, one wave: 3.4).
+// waves: 1.69 ms).
 #include "kv4.h"
 
 namespace w4a8 {
@@ -557,8 +557,8 @@ kv4_join_kernel(const Kv4Attn p) {
 // Splits of the tokens. Decode (3 workgroups of 4 waves per CU, 768 on the card): one round of the card, and up to
 // four per sequence and head where that many more workgroups even out sequences of different lengths; a split has
 // 8 tiles, two for each wave, and the first 8 are not worth the join's launch. us, with the splits that
-// this gives / without: 64 sequences of up to 8192 tokens x 8 heads 77 / 139, 16 of 4000 21 / 34, one of 8000
-// 13 / 40, two of 131072 64 / 800; 48 of 500 11 (unsplit) / 14 in two.
+// this gives / without: 64 sequences of up to 8192 tokens x 8 heads 73 / 81, 16 of 4000 21 / 37, one of 8000
+// 13 / 61, two of 131072 57 / 1060; 48 of 500 10 (unsplit) / 14 in two.
 // More columns (2 workgroups of 32-column waves per CU, 512; 16-column waves 1024): as many rounds, up to four
 // splits below one round. us: 512 new tokens on 8192 127 / 265, 7 chunks of 257 on up to 6001 137 / 194, 16 x 8 new
 // tokens on 4096 37 / 134; one prompt of 2048 fills the card, 112 (unsplit) / 120 in two.
