@@ -153,7 +153,7 @@ int w4a8_kv4_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_
   p.gmul = (uint32_t)((((uint64_t)1 << 31) + p.G - 1) / p.G);
   p.scale = scale * 1.4426950408889634f;
   p.causal = causal != 0;
-  p.window = (int)(window < (1 << 30) ? window : 1 << 30);
+  p.window = (int)window;
   return launched(launch_kv4_attention(p, (int)D, dtype, pl, workspace, (hipStream_t)stream), who);
 }
 

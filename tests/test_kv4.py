@@ -417,6 +417,29 @@ def test_long_contexts_in_splits(dev, dtype):
 
 
 @pytest.mark.gpu
+def test_window_past_2_30_keys(dev):
+    """A table that repeats two pages: 2^30 + 65536 keys. Only the last 7 slots of the first page have large scores, and
+    a window of 2^30 + 7 keys begins with them; one of 2^30 does not reach them. exp(60) against 2^30 keys of score 0."""
+    kv4 = _kv4()
+    D, page, width = 64, 65536, 16385
+    cache = kv4.KV4Cache(2, page, 1, D, device=dev)  # zeros: keys of score 0, values 0
+    k = torch.zeros(page, 1, D, dtype=torch.bfloat16)
+    v = torch.zeros(page, 1, D, dtype=torch.bfloat16)
+    k[-7:] = 15.0 / 16
+    v[-7:, :, 0] = 15.0
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=dev)  # noqa: E731
+    kv4.kv4_append(cache, k.to(dev), v.to(dev), i32([1]), i32(0, page), i32(page))
+    table = torch.zeros(1, width, dtype=torch.int32, device=dev)
+    table[0, 0] = 1
+    q = torch.full((1, 1, D), 1.0, dtype=torch.bfloat16, device=dev)
+    for window, want in ((2 ** 30 + 7, 15.0), (2 ** 30, 0.0)):
+        out = kv4.kv4_attention(q, cache, table, i32(0, 1), i32(width * page), sm_scale=1.0, window=window)
+        # the 7 keys' share is 1 - 2^30 / (7 e^60) of the whole, and a row's error is within 3.5e-4 of the largest value
+        assert (out[0, 0, 0].float().cpu() - want).abs() <= 15 * (2.0 ** -9 + 3.5e-4)
+        assert out[0, 0, 1:].abs().max() <= 15 * 3.5e-4
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("scale", [1e-4, 30.0])
 def test_small_and_large_values(dev, dtype, scale):
