@@ -71,6 +71,14 @@ static int operands(const char* who, void* kc, void* vc, void* ks, void* vs, int
   return kOk;
 }
 
+// whether a (T, H, D) tensor of these strides has each element in a place of its own
+static bool apart(int64_t T, int64_t ld, int64_t H, int64_t hd, int64_t D) {
+  if (T <= 1) ld = H * (hd > D ? hd : D);
+  if (H <= 1) hd = T * (ld > D ? ld : D);
+  const bool rows_in = ld <= hd;  // the rows of a head are neighbours
+  return rows_in ? ld >= D && hd >= (T - 1) * ld + D : hd >= D && ld >= (H - 1) * hd + D;
+}
+
 static bool rows_ok(const void* p, int64_t ld, int64_t hd) { return p && aligned16(p) && ld % 8 == 0 && hd % 8 == 0; }
 
 extern "C" {
@@ -139,6 +147,8 @@ int w4a8_kv4_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_
   if (rc) return rc;
   if (!rows_ok(q, ldq, hq) || !rows_ok(out, ldo, ho))
     return fail(kErrInvalid, "%s: q and out rows must be 16-byte aligned, with strides that are multiples of 8 elements", who);
+  if (!apart(T, ldo, Hq, ho, D))
+    return fail(kErrInvalid, "%s: out's rows overlap (strides %lld and %lld)", who, (long long)ldo, (long long)ho);
   const Kv4Plan pl = kv4_plan(T, (int)B, (int)H, (int)(Hq / H), (int)D, max_q, max_kv);
   const int64_t need = kv4_workspace(T, (int)Hq, (int)D, pl.splits);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))

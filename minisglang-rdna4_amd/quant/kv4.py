@@ -191,7 +191,7 @@ def kv4_attention(
     num_qo_heads is a multiple of the cache's heads. sm_scale defaults to head_dim ** -0.5. causal: a
     token sees the keys up to its own position; window > 0: only the last ``window`` of those. A row
     that sees no key is 0 (lse -inf). out, where given, may be strided; rows outside cu_q keep what they
-    hold there, and are undefined in a fresh output.
+    hold there, and are undefined in a fresh output. Rows of out that overlap are refused.
 
     max_q and max_kv, the most new tokens and the greatest length of a sequence, are what the host
     plans the launch by (default: T rows, and the table's capacity). Too large a bound costs time, too

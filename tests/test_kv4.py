@@ -192,6 +192,25 @@ def test_calls_on_the_cpu_are_refused():
         kv4.kv4_attention(torch.zeros(1, 3, 128, dtype=torch.bfloat16), c, i32([0]).view(1, 1), i32(0, 1), i32(1))
 
 
+def test_abi_refuses_outputs_that_overlap():
+    """Host checks of the C entry point, with pointers that are never read: what passes them ends at the workspace."""
+    lib = pkg("_abi").load()
+    P = 1 << 20
+
+    def attend(T, Hq, ldo, ho, D=128):
+        rc = lib.w4a8_kv4_attention(P, 0, Hq * D, D, T, Hq, 1, D, P, P, P, P, 16, 16, P, 1 << 12, 1 << 12, P, P, 1, 1.0, 1, 0,
+                                    1, 1 << 16, P, ldo, ho, None, None, 0, None)
+        assert rc == 1
+        return lib.w4a8_last_error()
+
+    for T, Hq, ldo, ho in ((2, 4, 0, 128), (2, 4, 512, 0), (2, 4, 504, 128), (2, 4, 512, 120), (2, 4, 128, 248), (2, 1, 120, 128),
+                           (1, 2, 0, 120), (3, 2, -256, 128)):
+        assert b"overlap" in attend(T, Hq, ldo, ho), (T, Hq, ldo, ho)
+    for T, Hq, ldo, ho in ((2, 4, 512, 128), (2, 4, 128, 256), (2, 4, 1024, 256), (2, 4, 136, 512), (2, 1, 128, 0), (1, 4, 0, 128),
+                           (1, 1, 0, 0)):
+        assert b"workspace" in attend(T, Hq, ldo, ho), (T, Hq, ldo, ho)
+
+
 def test_abi_refuses_before_any_launch():
     """Host checks of the C entry points, with pointers that are never read."""
     lib = pkg("_abi").load()
@@ -604,6 +623,8 @@ def test_gpu_refusals(dev):
             kv4.kv4_attention(q, c, *args)
     with pytest.raises(ValueError, match="out must be"):
         kv4.kv4_attention(q, c, tab, cu, seq, out=torch.empty(2, 4, 64, dtype=torch.bfloat16, device=dev))
+    with pytest.raises(RuntimeError, match="overlap"):
+        kv4.kv4_attention(q, c, tab, cu, seq, out=torch.empty(1, 4, 128, dtype=torch.bfloat16, device=dev).expand(2, 4, 128))
     with pytest.raises(ValueError, match="window"):
         kv4.kv4_attention(q, c, tab, cu, seq, window=-1)
     with pytest.raises(TypeError, match="as the cache is"):
