@@ -30,6 +30,7 @@ static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 static int launched(int rc, const char* who) {
   if (rc == kOk) return kOk;
+  if (rc == kErrUnsupported) return fail(rc, "%s: past its index ranges", who);
   return fail(kErrHip, "%s: HIP launch failed (%s)", who, hipGetErrorString(hipGetLastError()));
 }
 
@@ -117,7 +118,7 @@ int w4a8_kv4_read(const void* k_codes, const void* v_codes, const void* k_scale,
 int64_t w4a8_kv4_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t B, int64_t max_q,
                                            int64_t max_kv) {
   if (T < 0 || B < 0 || H < 1 || Hq < H || Hq % H || max_q < 0 || max_kv < 0 || (D != 64 && D != 128 && D != 256) ||
-      T > 0x7fffffff || B > 65535 || Hq > 65535 || max_q > 0x7fffffff || max_kv > 0x7fffffff)
+      T > 0x7fffffff || B > 65535 || Hq > 32768 || max_q > 0x7fffffff || max_kv > 0x7fffffff)
     return -1;
   if (T == 0 || B == 0) return 0;
   return kv4_workspace(T, (int)Hq, (int)D, kv4_plan(T, (int)B, (int)H, (int)(Hq / H), (int)D, max_q, max_kv).splits);
@@ -132,8 +133,8 @@ int w4a8_kv4_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_
   const char* who = "w4a8_kv4_attention";
   int rc = shapes(who, dtype, T, H, D, pages, page_size, B, width);
   if (rc) return rc;
-  if (Hq < H || Hq % H || Hq > 65535)
-    return fail(kErrInvalid, "%s: %lld query heads for %lld key/value heads", who, (long long)Hq, (long long)H);
+  if (Hq < H || Hq % H || Hq > 32768)
+    return fail(kErrInvalid, "%s: %lld query heads (up to 32768) for %lld key/value heads", who, (long long)Hq, (long long)H);
   if (!(scale > 0.f && scale < 1e30f)) return fail(kErrInvalid, "%s: the softmax scale must be positive", who);
   if (T * Hq > 0x3fffffff)  // queries times heads are columns, indexed in 32 bits
     return fail(kErrUnsupported, "%s: past its index ranges (T=%lld, %lld query heads)", who, (long long)T, (long long)Hq);

@@ -565,8 +565,9 @@ kv4_join_kernel(const Kv4Attn p) {
 // tokens on 4096 37 / 134; one prompt of 2048 fills the card, 112 (unsplit) / 120 in two.
 Kv4Plan kv4_plan(int64_t T, int B, int H, int G, int D, int64_t max_q, int64_t max_kv) {
   Kv4Plan pl;
-  // a bound below the mean is wrong; the workspace would grow with it
+  // a bound below the mean or past all rows is wrong: the workspace or the grid would grow with it
   if (max_q < (T + B - 1) / B) max_q = (T + B - 1) / B;
+  if (max_q > T) max_q = T;
   const int64_t cols = max_q * G;
   pl.few = cols <= 16;
   // 32 columns a wave, or 16 where those of a workgroup cover a sequence's, and for 256 channels, whose 32 would
@@ -592,15 +593,14 @@ int64_t kv4_workspace(int64_t T, int Hq, int D, int splits) {
 
 template <int D, int DT>
 static int launch_dt(Kv4Attn& p, const Kv4Plan& pl, hipStream_t st) {
+  const int64_t rows = p.s.T * p.c.H * p.G;
+  if (pl.qgrid * pl.splits > kMaxGrid || (pl.splits > 1 && rows / 4 >= kMaxGrid)) return kErrUnsupported;
   const dim3 g((unsigned)(pl.qgrid * pl.splits), (unsigned)p.c.H, (unsigned)p.s.B), b(256);
   if (pl.few) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 4>), g, b, 0, st, p);
   else if (pl.nq == 1) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 1>), g, b, 0, st, p);
   else hipLaunchKernelGGL((kv4_attn_kernel<D, DT, D == 256 ? 1 : 2, 1>), g, b, 0, st, p);
   if (hipGetLastError() != hipSuccess) return kErrHip;
-  if (pl.splits > 1) {
-    const int64_t rows = p.s.T * p.c.H * p.G;
-    hipLaunchKernelGGL((kv4_join_kernel<D, DT>), dim3((unsigned)((rows + 3) / 4)), b, 0, st, p);
-  }
+  if (pl.splits > 1) hipLaunchKernelGGL((kv4_join_kernel<D, DT>), dim3((unsigned)((rows + 3) / 4)), b, 0, st, p);
   return hipGetLastError() == hipSuccess ? kOk : kErrHip;
 }
 

@@ -242,7 +242,9 @@ int launch_kv4_append(const void* k, int64_t ldk, int64_t hk, const void* v, int
                       const Kv4Cache& c, const Kv4Batch& s, hipStream_t st) {
   // one row per wave while that many waves (8192) fill the card no more than once
   const int rows = s.T * c.H <= 8192 ? 1 : 8;
-  const dim3 g((unsigned)(((s.T + rows - 1) / rows * c.H + 3) / 4));
+  const int64_t wgs = ((s.T + rows - 1) / rows * c.H + 3) / 4;
+  if (wgs > kMaxGrid) return kErrUnsupported;
+  const dim3 g((unsigned)wgs);
   auto kp = reinterpret_cast<const uint16_t*>(k), vp = reinterpret_cast<const uint16_t*>(v);
   if (dtype == kBF16) append<kBF16>(D, g, kp, ldk, hk, vp, ldv, hv, c, s, rows, st);
   else append<kF16>(D, g, kp, ldk, hk, vp, ldv, hv, c, s, rows, st);
@@ -258,7 +260,9 @@ static void read(int D, dim3 g, const Kv4Cache& c, const Kv4Batch& s, uint16_t* 
 
 int launch_kv4_read(const Kv4Cache& c, const Kv4Batch& s, int dtype, int D, void* k, void* v, hipStream_t st) {
   const int per = 4 * 512 / D;  // vectors per workgroup
-  const dim3 g((unsigned)((s.T * c.H + per - 1) / per));
+  const int64_t wgs = (s.T * c.H + per - 1) / per;
+  if (wgs > kMaxGrid) return kErrUnsupported;
+  const dim3 g((unsigned)wgs);
   auto kp = reinterpret_cast<uint16_t*>(k), vp = reinterpret_cast<uint16_t*>(v);
   if (dtype == kBF16) read<kBF16>(D, g, c, s, kp, vp, st);
   else read<kF16>(D, g, c, s, kp, vp, st);

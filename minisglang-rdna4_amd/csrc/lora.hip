@@ -333,6 +333,7 @@ int launch_lora(LoraArgs& p, int dtype, hipStream_t st) {
     p.chunk[i] = spans;
     if (i < p.slices) spans += (p.col[i + 1] - p.col[i] + p.span - 1) / p.span;
   }
+  if (blocks * groups * p.kc > kMaxGrid || spans * blocks > kMaxGrid) return kErrUnsupported;
   const dim3 gu((unsigned)(spans * blocks), 1, (unsigned)pl.slots);
   const unsigned lds = (unsigned)(16 * (p.rank + 4) * 4);
 #define W4A8_LORA_UP(DT_, F32_)                                                                       \

@@ -47,17 +47,16 @@ int w4a8_lora_add(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, c
   if (slices < 1 || slices > kLoraMaxSlices || !slice_cols)
     return fail(kErrUnsupported, "%s: 1 to %d slices, got %d", who, kLoraMaxSlices, slices);
   LoraArgs p = {};
-  int64_t n = 0, chunks = 0;
+  int64_t n = 0;
   for (int i = 0; i < slices; ++i) {
     if (slice_cols[i] <= 0 || slice_cols[i] % 16 || slice_cols[i] > 0x7fffffff)
       return fail(kErrInvalid, "%s: slice %d has %lld columns (multiples of 16)", who, i, (long long)slice_cols[i]);
     p.col[i] = n;
     n += slice_cols[i];
-    chunks += (slice_cols[i] + 255) / 256;
   }
   for (int i = slices; i <= kLoraMaxSlices; ++i) p.col[i] = n;
   if (M == 0) return kOk;
-  if ((M + 15) / 16 * chunks > 0x7fffffff || M > (1 << 26))
+  if (M > (1 << 26))
     return fail(kErrUnsupported, "%s: past its index ranges (M=%lld, N=%lld)", who, (long long)M, (long long)n);
   if (!x || !a || !b || !scaling || !adapters || !base || !out || !aligned16(x) || !aligned16(a) || !aligned16(b) ||
       !aligned16(base) || !aligned16(out))
@@ -79,7 +78,10 @@ int w4a8_lora_add(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, c
   p.out = static_cast<uint16_t*>(out);
   p.ldo = ldo;
   p.v = static_cast<float*>(workspace);
-  if (launch_lora(p, dtype, (hipStream_t)stream) != kOk)
+  const int rc = launch_lora(p, dtype, (hipStream_t)stream);
+  if (rc == kErrUnsupported)
+    return fail(rc, "%s: past its index ranges (M=%lld, N=%lld)", who, (long long)M, (long long)n);
+  if (rc != kOk)
     return fail(kErrHip, "%s: HIP launch failed (%s)", who, hipGetErrorString(hipGetLastError()));
   return kOk;
 }

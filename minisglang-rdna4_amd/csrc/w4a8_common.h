@@ -40,6 +40,8 @@ constexpr int kOk = 0;
 constexpr int kErrInvalid = 1;
 constexpr int kErrUnsupported = 2;
 constexpr int kErrHip = 3;
+// workgroups of 256 threads along a grid's axis: it has 32 bits of threads
+constexpr int64_t kMaxGrid = 0xffffff;
 
 enum DType { kBF16 = 0, kF16 = 1, kF32 = 2 };
 // kScaleE4M3: NVFP4's e4m3 block scales (group 16), times a per-output-channel f32 global that

@@ -211,6 +211,30 @@ def test_abi_refuses_outputs_that_overlap():
         assert b"workspace" in attend(T, Hq, ldo, ho), (T, Hq, ldo, ho)
 
 
+def test_grids_past_32_bits_are_refused():
+    """Sizes whose launch would not fit, refused by the host, and bounds of a call that do not size its grid."""
+    if torch.cuda.is_available():
+        pytest.skip("the pointers are not real")
+    lib = pkg("_abi").load()
+    P = 1 << 20
+    rows = (1 << 31) - 256
+    rc = lib.w4a8_kv4_append(P, 64, 64, P, 64, 64, 0, rows, 1, 64, P, P, P, P, 16, 16, P, 4, 4, P, P, 1, None)
+    assert rc == 2 and b"w4a8_kv4_append: past its index ranges" in lib.w4a8_last_error()
+    rc = lib.w4a8_kv4_read(P, P, P, P, 0, 16, 16, 1, 64, P, 4, 4, P, P, 1, rows, P, P, None)
+    assert rc == 2 and b"w4a8_kv4_read: past its index ranges" in lib.w4a8_last_error()
+    # 256 channels: 64 columns a workgroup
+    rows = (1 << 30) - 1
+    rc = lib.w4a8_kv4_attention(P, 0, 256, 256, rows, 1, 1, 256, P, P, P, P, 16, 16, P, 4, 4, P, P, 1, 1.0, 1, 0, rows, 64, P,
+                                256, 256, None, None, 0, None)
+    assert rc == 2 and b"past its index ranges" in lib.w4a8_last_error()
+    rc = lib.w4a8_kv4_attention(P, 0, 64 * 40000, 64, 1, 40000, 1, 64, P, P, P, P, 16, 16, P, 4, 4, P, P, 1, 1.0, 1, 0, 1, 64,
+                                P, 64 * 40000, 64, None, None, 0, None)
+    assert rc == 1 and b"up to 32768" in lib.w4a8_last_error()
+    f = lib.w4a8_kv4_attention_workspace_bytes
+    assert f(4, 40000, 1, 64, 1, 1, 64) == -1
+    assert f(4, 8, 8, 128, 1, (1 << 31) - 1, 1 << 17) == f(4, 8, 8, 128, 1, 4, 1 << 17) > 0
+
+
 def test_abi_refuses_before_any_launch():
     """Host checks of the C entry points, with pointers that are never read."""
     lib = pkg("_abi").load()

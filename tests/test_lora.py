@@ -92,6 +92,20 @@ def test_cpu_calls_are_refused():
         m.w4a8_linear_lora(x, None, None, None, 128, ad, ids[:3])
 
 
+def test_grids_past_32_bits_are_refused():
+    """2^22 blocks of rows by 8 slices: each has a workgroup of its own, and the launch would not fit."""
+    import ctypes
+
+    if torch.cuda.is_available():
+        pytest.skip("the pointers are not real")
+    lib = pkg("_abi").load()
+    P = 1 << 20
+    cols = (ctypes.c_int64 * 8)(*[16] * 8)
+    M = 1 << 26
+    rc = lib.w4a8_lora_add(P, 0, M, 8, 8, P, P, P, 2, 8, ctypes.addressof(cols), 8, P, P, 0, 128, P, 128, P, 1 << 50, None)
+    assert rc == 2 and b"w4a8_lora_add: past its index ranges" in lib.w4a8_last_error()
+
+
 def test_abi_refuses_before_any_launch():
     import ctypes
 
