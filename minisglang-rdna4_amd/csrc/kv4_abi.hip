@@ -135,7 +135,8 @@ int w4a8_kv4_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_
   if (rc) return rc;
   if (Hq < H || Hq % H || Hq > 32768)
     return fail(kErrInvalid, "%s: %lld query heads (up to 32768) for %lld key/value heads", who, (long long)Hq, (long long)H);
-  if (!(scale > 0.f && scale < 1e30f)) return fail(kErrInvalid, "%s: the softmax scale must be positive", who);
+  if (!(scale > 0.f && scale < 65536.f))  // times a large query's power of two it has to stay in f32
+    return fail(kErrInvalid, "%s: the softmax scale must be positive and below 65536", who);
   if (T * Hq > 0x3fffffff)  // queries times heads are columns, indexed in 32 bits
     return fail(kErrUnsupported, "%s: past its index ranges (T=%lld, %lld query heads)", who, (long long)T, (long long)Hq);
   if (window < 0 || window > 0x7fffffff || max_q < 0 || max_kv < 0 || max_q > 0x7fffffff || max_kv > 0x7fffffff)

@@ -19,7 +19,9 @@
 // lane holds (tokens 8 g + r in the first 16 rows' register r, 8 g + 4 + r in the second's), so p goes
 // from one product into the next in its lane, and nothing passes through LDS.
 // The running maximum is raised only when a score passes it by 8 (in powers of two): p stays below 2^8,
-// and most tiles need no exchange between lanes and no rescaling.
+// and most tiles need no exchange between lanes and no rescaling. M is x's rounded to f32, the same for every p of
+// the column and for its join with other waves, so the rounding drops out as long as it is within 1: to 2^24. From
+// there on (far_off) every tile passes the check, and the maximum is subtracted there, before the scale is applied.
 //
 // WKV = 4 (decode): the waves of a workgroup walk the same 16 columns over different tiles and join through
 // LDS. WKV = 1 (more than 16 columns): each wave has columns of its own; the waves read the same tiles at about
@@ -168,6 +170,11 @@ __device__ __forceinline__ int kv4_query(const Kv4Attn& p, int i0, int r0, int x
   return i0 + i;
 }
 
+// the maximum m itself where m times its factor is past what M holds to within 1, else 0
+__device__ __forceinline__ float far_off(float m, float sc) {
+  return fabsf(m) * sc >= 16777216.f && m != -__builtin_inff() ? m : 0.f;
+}
+
 template <int DT>
 __device__ __forceinline__ void unpack_query(const uint4& u, float (&f)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -308,8 +315,8 @@ kv4_attn_kernel(const Kv4Attn p) {
     }
 
     v4f o[NQ][DB], ws[NQ];                // ws: sum w (bf16 models), in every register
-    float thr[NQ];                        // scores up to here leave the maximum as it is: m and 8 powers of two
-    float m[NQ], mu[NQ], l[NQ], cc[NQ];   // mu: M, the maximum in powers of two (0 while no key was seen) plus e
+    float thr[NQ];                        // scores up to here leave the maximum as it is: m and 8 powers of two, or none
+    float m[NQ], mu[NQ], l[NQ], cc[NQ];   // mu: M, the maximum in powers of two (0 while no key was seen, or far_off) plus e
     float lim[NQ];                        // 2^(e + 6): steps up to here are in its range; 0: none was seen yet
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
@@ -400,16 +407,20 @@ kv4_attn_kernel(const Kv4Attn p) {
           const int nl = need ? min(max(max(le, old), 87), 227) : old;  // lim's exponent
           lim[j] = __uint_as_float((uint32_t)nl << 23);
           const float mn = need ? fmaxf(m[j], tp) : m[j];
-          const float mun = need ? (mn == -kInf ? 0.f : mn * sc[j]) + (float)(nl - 133) : mu[j];
-          const float f = m[j] == -kInf ? 1.f : __builtin_amdgcn_exp2f(mu[j] - mun);  // nothing summed yet: any
+          const float was = far_off(m[j], sc[j]), is = far_off(mn, sc[j]);
+          const float mun = need ? (mn == -kInf || is != 0.f ? 0.f : mn * sc[j]) + (float)(nl - 133) : mu[j];
+          // nothing summed yet: any
+          const float f = m[j] == -kInf ? 1.f : __builtin_amdgcn_exp2f(__builtin_fmaf(was - is, sc[j], mu[j] - mun));
           m[j] = mn;
           mu[j] = mun;
-          thr[j] = mn + 8.f / sc[j];
+          thr[j] = is != 0.f ? -kInf : mn + 8.f / sc[j];
           l[j] *= f;
           cc[j] *= f;
           ws[j] *= f;
 #pragma unroll
           for (int d = 0; d < DB; ++d) o[j][d] *= f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[j][i] -= is;
         }
       }
 #pragma unroll
@@ -455,11 +466,14 @@ kv4_attn_kernel(const Kv4Attn p) {
     for (int j = 0; j < NQ; ++j) {
       l[j] = col_sum(l[j]);
       cc[j] = col_sum(cc[j]) - (W == 1 ? 7.5f * ws[j][0] : 0.f);
-      if (m[j] == -kInf) mu[j] = -kInf;
+      // beside a far_off maximum e would be lost: it goes into the sums
+      const float is = far_off(m[j], sc[j]), fe = is != 0.f ? __builtin_amdgcn_exp2f(mu[j]) : 1.f;
+      mu[j] = m[j] == -kInf ? -kInf : is != 0.f ? is * sc[j] : mu[j];
+      l[j] *= fe;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[j][d][r] = __builtin_fmaf(o[j][d][r], 16777216.f, cc[j]);
+        for (int r = 0; r < 4; ++r) o[j][d][r] = fe * __builtin_fmaf(o[j][d][r], 16777216.f, cc[j]);
     }
     auto store = [&](int j, int r, const float (&v)[DB], float mx, float sum) {
       int head;

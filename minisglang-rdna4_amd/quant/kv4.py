@@ -188,7 +188,8 @@ def kv4_attention(
     among them: append first). (T, num_qo_heads, head_dim) in q's type; with return_lse also the natural
     logarithm of each softmax's sum, (T, num_qo_heads) f32.
 
-    num_qo_heads is a multiple of the cache's heads. sm_scale defaults to head_dim ** -0.5. causal: a
+    num_qo_heads is a multiple of the cache's heads. sm_scale defaults to head_dim ** -0.5; it is positive
+    and below 65536, and bf16 queries are below 2^96, cached values' steps below 2^100. causal: a
     token sees the keys up to its own position; window > 0: only the last ``window`` of those. A row
     that sees no key is 0 (lse -inf). out, where given, may be strided; rows outside cu_q keep what they
     hold there, and are undefined in a fresh output. Rows of out that overlap are refused.

@@ -491,6 +491,51 @@ def test_small_and_large_values(dev, dtype, scale):
     s.check(s.q(4), f"scale {scale}", max_q=30)
 
 
+def check_one_hot(s, q, causal, window, **kw):
+    """Scores so far apart that all but the largest have weights below 2^-100, or are equal to it: the output is the mean
+    of the values with the largest score."""
+    D, dtype = s.cache.head_dim, s.cache.dtype
+    kv = cache_values(s.cache)
+    out, lse = s.attend(q, causal=causal, window=window, return_lse=True, **kw)
+    ref, rl = ref_attention(q, kv, s.table, s.page, s.lens, s.news, kw.get("sm_scale", D ** -0.5), causal, window)
+    eps = 2.0 ** (-8 if dtype == torch.bfloat16 else -11)
+    vmax = s.v.float().abs().max().item()
+    err = (out.cpu().double() - ref).abs() - eps * ref.abs() - (3.5e-4 if dtype == torch.bfloat16 else 2e-4) * vmax
+    assert not torch.isnan(out).any() and err.max().item() <= 0, err.max().item()
+    # a score's roundings, 16 of 2^-24 of it as in Setup.check, and the f32 result's own
+    assert ((lse.cpu().double() - rl).abs() <= 2.0 ** -20 * rl.abs()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,power", [(t, p) for t in DTYPES for p in (20, 23, 24, 25, 30)] + [(torch.bfloat16, 60)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("new", [1, 40])
+def test_scores_far_from_zero(dev, dtype, power, sign, new):
+    """Keys that are integers 0 .. 15 in channel 0 and 15 in channel 1, or their negatives, and queries that are powers of
+    two there: scores are whole multiples of the score of a step, so the largest is shared by a sixteenth of the keys,
+    which are in all splits, with steps of V that grow along the sequence."""
+    kv4 = _kv4()
+    D, n = 64, 700
+    s = Setup(dev, dtype, D, 1, 16, [n], [new], seed=21)
+    g = torch.Generator().manual_seed(5)
+    k = torch.zeros(n, 1, D)
+    k[:, 0, 0] = torch.randint(0, 16, (n,), generator=g).float()
+    k[:, 0, 1] = 15.0
+    s.k = (sign * k).to(dtype)
+    s.v = (torch.randn(n, 1, D, generator=g) * torch.logspace(-3, 3, n, base=2.0).view(n, 1, 1)).to(dtype)
+    kv4.kv4_append(s.cache, s.k.to(dev), s.v.to(dev), s.d_table, s.cu_all.to(dev), s.d_seq)
+    q = torch.zeros(new, 2, D)
+    qp = 15 if power <= 30 else power - 15
+    q[:, 0, :2] = 2.0 ** qp
+    q[:, 1, :2] = 2.0 ** (qp - 1)
+    for kw in ({}, {"max_q": 1, "max_kv": 1 << 16}):
+        check_one_hot(s, q.to(dtype), True, 0, sm_scale=2.0 ** (power - qp), **kw)
+    if dtype == torch.bfloat16 and power == 60:
+        q = torch.zeros(new, 2, D)
+        q[:, :, :2] = 2.0 ** 90
+        check_one_hot(s, q.to(dtype), True, 0)
+
+
 @pytest.mark.gpu
 def test_unseen_tokens_do_not_reach_the_output(dev):
     """A NaN vector among the keys is seen by the rows behind it only; slots past the end, which hold NaN and
