@@ -29,10 +29,10 @@
 // too, and kv4_join_kernel joins the parts.
 //
 // Measured. Decode is bound by HBM: two sequences of 131072 tokens x 8 heads of 128 (280 MB) 64 us, 4.4 TB/s, with
-// cold caches, at 3 waves per SIMD (warm 57; at 4 waves, whose 128 registers spill, 70). Prompts by the vector unit: 8192 + 5690 + 3190 tokens,
-// 32 heads of 128 (898 GFLOP) 1.53 ms, 586 TFLOP/s: 330 vector instructions a tile and wave, 80 of them to widen
-// codes and 180 for the softmax of 32 columns, beside 34 MFMA of 16 cycles; 2 waves per SIMD (16 columns a wave, 3
-// waves: 1.69 ms).
+// cold caches, at 3 waves per SIMD (warm 57; at 4 waves, whose 128 registers spill, 70). Prompts by the vector unit:
+// 8192 + 5690 + 3190 tokens, 32 heads of 128 (898 GFLOP) 1.53 ms, 586 TFLOP/s: 330 vector instructions a tile and
+// wave, 80 of them to widen codes and 180 for the softmax of 32 columns, beside 34 MFMA of 16 cycles; 2 waves per
+// SIMD (16 columns a wave, 3 waves: 1.69 ms).
 #include "kv4.h"
 
 namespace w4a8 {
