@@ -145,10 +145,10 @@ __device__ __forceinline__ Span kv4_span(const Kv4Attn& p, int b) {
   s.first_pos = len - s.n;
   return s;
 }
-// the keys [from, upto) that query i of the span sees
+// the keys [from, upto) that query i of the span sees: a window past the table's end still has the missing token
 __device__ __forceinline__ int seen_from(const Kv4Attn& p, const Span& s, int i) {
   const int n = s.first_pos + i + 1;  // keys up to the query's own
-  return p.window && n > p.window ? min(n - p.window, s.len) : 0;
+  return p.window && n > p.window ? min(n - p.window, s.len - 1) : 0;
 }
 __device__ __forceinline__ int seen_upto(const Kv4Attn& p, const Span& s, int i) {
   return p.causal ? min(max(s.first_pos + i + 1, 0), s.len) : s.len;
