@@ -4,11 +4,15 @@
 // query c / G, query head h * G + c % G. A wave takes 16 NQ columns and walks tiles of 32 tokens, with
 // one pass over the cache and the running maximum and sum of the softmax in f32:
 //   S = c Q^T,   x = s S + m sum(q),   p = 2^(x scale - M),   O += (p s)^T c,   C += p m,   out = (O + C) / sum p.
-// Codes. A code in an fp16 number's lowest bits is the subnormal c 2^-24, four bits higher c 2^-20: a shift
+// Codes. A code in bits 2 .. 5 of an fp16 number is the subnormal c 2^-22, in bits 6 .. 9 c 2^-18: two shifts
 // and four ands turn the 8 codes of a word into an fp16 operand, with no offset and no rounding (the matrix
-// units keep subnormals). The other operand carries the 2^-4 of the higher codes, the sums the 2^24.
+// units keep subnormals). The other operand carries the 2^-4 of the higher codes, the sums the 2^22.
+// The matrix units line a subnormal's products up by the exponent of the least normal number, and cut what is then
+// below f32's last place of the largest: a code in the lowest bits, one shift less, loses 7 bits and more. Sums
+// over weights exp(1.5 N(0, 1)) then came out low by 22 units in the last place, and come out low by 2 (by 0.01 with
+// all codes in bits 6 .. 9, which takes four shifts), where outputs of long contexts are a hundredth of what is summed.
 // Queries enter in fp16 for either model type: a power of two per row puts their largest value at 2^14, so
-// values down to 2^-28 of it are exact.
+// values down to 2^-27 of it (bf16 models) or 2^-24 (fp16) are exact.
 // p s enters in fp16: for fp16 models as two terms (22 bits), for bf16 models as one, w, rounded by 2^-12
 // of itself. So that this error meets c - 7.5, and not the whole of c, bf16 models sum
 // O - 7.5 sum w + sum p (m + 7.5 s), sum w by one more product with a row of ones: the error is within 2^-12
@@ -44,11 +48,13 @@ __device__ __forceinline__ v4f mfma16(const v4w& a, const v4w& b, const v4f& c) 
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// The codes of a word as fp16 subnormals: register r holds codes r and r + 4, times 2^-24 for even r, 2^-20 for odd
+// The codes of a word as fp16 subnormals: register r holds codes r and r + 4, times 2^-22 for even r, 2^-18 for odd
 __device__ __forceinline__ v4w widen(uint32_t w) {
-  const uint32_t u = w >> 8;
-  return v4w{w & 0x000f000fu, w & 0x00f000f0u, u & 0x000f000fu, u & 0x00f000f0u};
+  const uint32_t u = w << 2, x = w >> 6;
+  return v4w{u & 0x003c003cu, u & 0x03c003c0u, x & 0x003c003cu, x & 0x03c003c0u};
 }
+constexpr int kUnit = 22;          // sums of codes are in 2^-kUnit
+constexpr float kOne = 4194304.f;  // 2^kUnit
 
 // the same value over the four lanes that hold a column (xor 16 and xor 32)
 __device__ __forceinline__ float col_max(float v) {
@@ -300,8 +306,8 @@ kv4_attn_kernel(const Kv4Attn p) {
       top = col_max(top);
       // 2^eq puts the largest value into [2^14, 2^15)
       const int eq = max(141 - (int)(__float_as_uint(top) >> 23), -100);
-      qs[j] = __builtin_ldexpf(col_sum(sum), eq - 24);
-      sc[j] = __builtin_ldexpf(p.scale, 24 - eq);
+      qs[j] = __builtin_ldexpf(col_sum(sum), eq - kUnit);
+      sc[j] = __builtin_ldexpf(p.scale, kUnit - eq);
 #pragma unroll
       for (int w = 0; w < KS; ++w) {
         float f[8];
@@ -461,7 +467,7 @@ kv4_attn_kernel(const Kv4Attn p) {
       tn = tnn;
     }
 
-    // O in the codes' units is 2^24 times the products' sum
+    // O in the codes' units is kOne times the products' sum
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
       l[j] = col_sum(l[j]);
@@ -473,7 +479,7 @@ kv4_attn_kernel(const Kv4Attn p) {
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[j][d][r] = fe * __builtin_fmaf(o[j][d][r], 16777216.f, cc[j]);
+        for (int r = 0; r < 4; ++r) o[j][d][r] = fe * __builtin_fmaf(o[j][d][r], kOne, cc[j]);
     }
     auto store = [&](int j, int r, const float (&v)[DB], float mx, float sum) {
       int head;
