@@ -13,11 +13,13 @@
 // all codes in bits 6 .. 9, which takes four shifts), where outputs of long contexts are a hundredth of what is summed.
 // Queries enter in fp16 for either model type: a power of two per row puts their largest value at 2^14, so
 // values down to 2^-27 of it (bf16 models) or 2^-24 (fp16) are exact.
-// p s enters in fp16: for fp16 models as two terms (22 bits), for bf16 models as one, w, rounded by 2^-12
-// of itself. So that this error meets c - 7.5, and not the whole of c, bf16 models sum
-// O - 7.5 sum w + sum p (m + 7.5 s), sum w by one more product with a row of ones: the error is within 2^-12
-// of half a V vector's range, an eighth of the output's own rounding. So that p s stays in fp16's range
-// whatever V's steps are, p carries 2^-e, 2^e about the largest step so far over 64: it moves with the running
+// p s enters in fp16, w: for fp16 models as two terms (22 bits), for bf16 models as one, rounded by at most 2^-11 of
+// itself. So that errors meet c - 7.5, and not the whole of c, what is summed is
+// O - 7.5 sum w + sum p (m + 7.5 s), sum w by one more product with a row of ones: bf16 models' error is within 2^-11
+// of half a V vector's range, an eighth of the output's own rounding. A wave subtracts 7.5 sum w from O every kFresh
+// tiles, since f32 sums of uncentred codes lose what the output is made of: one wave over 131072 tokens was off by
+// 2.7e-3 of the output's norm (D = 64, equal weights, fp16), where the rounding is 2.3e-4. So that p s stays in fp16's
+// range whatever V's steps are, p carries 2^-e, 2^e about the largest step so far over 64: it moves with the running
 // maximum, column by column, and drops out of the quotient.
 // The row of S that a lane of group g = lane / 16 holds is chosen to be the token whose V codes that
 // lane holds (tokens 8 g + r in the first 16 rows' register r, 8 g + 4 + r in the second's), so p goes
@@ -55,6 +57,7 @@ __device__ __forceinline__ v4w widen(uint32_t w) {
 }
 constexpr int kUnit = 22;          // sums of codes are in 2^-kUnit
 constexpr float kOne = 4194304.f;  // 2^kUnit
+constexpr int kFresh = 32;         // tiles that a wave sums before it takes the codes' mean out
 
 // the same value over the four lanes that hold a column (xor 16 and xor 32)
 __device__ __forceinline__ float col_max(float v) {
@@ -320,7 +323,7 @@ kv4_attn_kernel(const Kv4Attn p) {
       }
     }
 
-    v4f o[NQ][DB], ws[NQ];                // ws: sum w (bf16 models), in every register
+    v4f o[NQ][DB], ws[NQ];                // ws: sum w since O was last centred, in every register
     float thr[NQ];                        // scores up to here leave the maximum as it is: m and 8 powers of two, or none
     float m[NQ], mu[NQ], l[NQ], cc[NQ];   // mu: M, the maximum in powers of two (0 while no key was seen, or far_off) plus e
     float lim[NQ];                        // 2^(e + 6): steps up to here are in its range; 0: none was seen yet
@@ -334,6 +337,7 @@ kv4_attn_kernel(const Kv4Attn p) {
       for (int d = 0; d < DB; ++d) o[j][d] = v4f{0.f, 0.f, 0.f, 0.f};
     }
 
+    int fresh = kFresh;
     while (t < nt) {
       const int t0 = token(t);
       const int tnn = tn + step;
@@ -361,7 +365,7 @@ kv4_attn_kernel(const Kv4Attn p) {
 #pragma unroll
         for (int j = 0; j < NQ; ++j) y[j][i] = __builtin_fmaf(sk, s[j][i >> 2][i & 3], mk * qs[j]);
         sv[i] = lo16<DT>(vsw[i]);
-        mv[i] = W == 1 ? __builtin_fmaf(7.5f, sv[i], hi16<DT>(vsw[i])) : hi16<DT>(vsw[i]);
+        mv[i] = __builtin_fmaf(7.5f, sv[i], hi16<DT>(vsw[i]));
       }
       auto top8 = [](const float (&v)[8]) {
         return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
@@ -449,7 +453,9 @@ kv4_attn_kernel(const Kv4Attn p) {
             pl[j][r] = pack_f16(ps[r] - f16_to_f32((uint16_t)(ph[j][r] & 0xffffu)), ps[r + 4] - f16_to_f32((uint16_t)(ph[j][r] >> 16)));
         }
         // sum w: ones, sixteens against the higher codes' 1/16
-        if (W == 1) ws[j] = mfma16(v4w{0x3c003c00u, 0x4c004c00u, 0x3c003c00u, 0x4c004c00u}, ph[j], ws[j]);
+        const v4w ones = {0x3c003c00u, 0x4c004c00u, 0x3c003c00u, 0x4c004c00u};
+        ws[j] = mfma16(ones, ph[j], ws[j]);
+        if (W == 2) ws[j] = mfma16(ones, pl[j], ws[j]);
       }
       if (more) load_s(next);
 #pragma unroll
@@ -462,6 +468,15 @@ kv4_attn_kernel(const Kv4Attn p) {
         }
       }
       if (more) load_v(next);
+      if (--fresh == 0) {
+        fresh = kFresh;
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+#pragma unroll
+          for (int d = 0; d < DB; ++d) o[j][d] -= (7.5f / kOne) * ws[j];
+          ws[j] = v4f{0.f, 0.f, 0.f, 0.f};
+        }
+      }
       at = next;
       t = tn;
       tn = tnn;
@@ -471,7 +486,7 @@ kv4_attn_kernel(const Kv4Attn p) {
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
       l[j] = col_sum(l[j]);
-      cc[j] = col_sum(cc[j]) - (W == 1 ? 7.5f * ws[j][0] : 0.f);
+      cc[j] = col_sum(cc[j]) - 7.5f * ws[j][0];
       // beside a far_off maximum e would be lost: it goes into the sums
       const float is = far_off(m[j], sc[j]), fe = is != 0.f ? __builtin_amdgcn_exp2f(mu[j]) : 1.f;
       mu[j] = m[j] == -kInf ? -kInf : is != 0.f ? is * sc[j] : mu[j];

@@ -44,8 +44,9 @@ def _case(dev, dtype, n, D, G, T, scale, page=64):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,D", [(1024, 64), (16384, 128), (65536, 128), (131072, 64), (65536, 256)])
-# the tokens split over the card
-@pytest.mark.parametrize("G,T,kw", [(8, 1, {"max_q": 1})])
+# the tokens split over the card; over one workgroup's four waves; one wave for all of them (17 and 64 columns)
+@pytest.mark.parametrize("G,T,kw", [(8, 1, {"max_q": 1}), (8, 1, {"max_q": 1, "max_kv": 1}), (17, 1, {"max_q": 1, "max_kv": 1}),
+                                    (8, 16, {"max_kv": 1})])
 def test_error_does_not_grow_with_the_length(dev, dtype, n, D, G, T, kw):
     for scale in (0.0, 1.5):
         cache, table, cu, seq, q, ref = _case(dev, dtype, n, D, G, T, scale)
