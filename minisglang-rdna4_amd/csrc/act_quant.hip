@@ -415,7 +415,7 @@ static int launch_act_quant_tiled_short(const uint16_t* x, int dtype, int64_t M,
   const dim3 g((unsigned)(nblk < 65536 ? nblk : 65536)), b(256);
   hipLaunchKernelGGL(act_quant_tiled_short_kernel<CPL>, g, b, (size_t)(16 * K), stream, x, ldx, M, K, dtype, qt,
                      scales, seeds, seeds_ld, row_count);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 template <int CPL>
@@ -429,7 +429,7 @@ static int launch_act_quant_tiled_lds(const uint16_t* x, int dtype, int64_t M, i
   const int64_t nblk = (M + 15) / 16;
   const dim3 g((unsigned)(nblk < 8192 ? nblk : 8192)), b(1024);
   hipLaunchKernelGGL(kern, g, b, (size_t)(16 * K), stream, x, ldx, M, K, dtype, qt, scales, seeds, seeds_ld, row_count);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 // seeds null: the GEMM needs none (only symmetric int4 does)
@@ -452,12 +452,12 @@ int launch_act_quant_tiled(const void* x, int dtype, int64_t M, int64_t K, int64
                           : K <= 16384 ? act_quant_tiled_rows_kernel<2>
                           : K <= 24576 ? act_quant_tiled_rows_kernel<3> : act_quant_tiled_rows_kernel<4>;
     hipLaunchKernelGGL(kern, g, b, 0, stream, xp, ldx, M, K, dtype, qt, scales, row_count);
-    return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+    return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
   }
   const dim3 g((unsigned)(nblk < 8192 ? nblk : 8192)), b(1024);
   hipLaunchKernelGGL(act_quant_tiled_kernel, g, b, 0, stream, reinterpret_cast<const uint16_t*>(x), ldx, M, K, dtype,
                      qt, scales, seeds, seeds_ld, row_count);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 int launch_act_tile(const uint8_t* q, int64_t ldq, int64_t M, int64_t K, uint8_t* qt, float* seeds,
@@ -468,7 +468,7 @@ int launch_act_tile(const uint8_t* q, int64_t ldq, int64_t M, int64_t K, uint8_t
   const int64_t wgs = (units + 3) / 4;
   const dim3 g((unsigned)(wgs < 65536 ? wgs : 65536)), b(256);
   hipLaunchKernelGGL(act_tile_kernel, g, b, 0, stream, q, ldq, M, KT, qt, seeds, seeds_ld);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 int launch_act_quant(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* q,
@@ -485,7 +485,7 @@ int launch_act_quant(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx
     else if (cpw <= 4) W4A8_AQW(4);
     else W4A8_AQW(8);
 #undef W4A8_AQW
-    return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+    return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
   }
   const int64_t grid = M < 8192 ? M : 8192;
   const uint16_t* xp = reinterpret_cast<const uint16_t*>(x);
@@ -498,7 +498,7 @@ int launch_act_quant(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx
     case 16: hipLaunchKernelGGL(act_quant_kernel<16>, g, b, 0, stream, xp, ldx, M, K, dtype, q, ldq, scales, row_count); break;
     default: hipLaunchKernelGGL(act_quant_kernel<0>, g, b, 0, stream, xp, ldx, M, K, dtype, q, ldq, scales, row_count);
   }
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 }  // namespace w4a8

@@ -218,7 +218,7 @@ int launch_gemv(GemmArgs p, int64_t row_blocks, bool quant_src, hipStream_t stre
   WalkPlan wp;
   if (quant_src && plan_gemv_walk(p, row_blocks, wp)) {
     if (!launch_gemv_walk(p, wp, stream)) return kErrInvalid;
-    return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+    return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
   }
   const GemvPlan pl = plan_gemv(p, row_blocks, quant_src);
   if (quant_src && pl.amode != kAQuant) return kErrUnsupported;
@@ -230,7 +230,7 @@ int launch_gemv(GemmArgs p, int64_t row_blocks, bool quant_src, hipStream_t stre
   else if (pl.amode == kAStage) ok = launch_gemv_staged(p, grid, pl, stream);
   else ok = launch_gemv_global(p, grid, pl, stream);
   if (!ok) return kErrInvalid;
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 // K split (waves, tpw) the grouped GEMV runs for these arguments and row blocks; the fused gemm2 +

@@ -235,7 +235,7 @@ static int launch_prefill_cfg(const GemmArgs& p, int64_t row_tiles, hipStream_t 
     case 2: hipLaunchKernelGGL((gemm_prefill_kernel<WM, WN, RB, NSB, 2>), grid, block, 0, stream, p); break;
     default: hipLaunchKernelGGL((gemm_prefill_kernel<WM, WN, RB, NSB, 3>), grid, block, 0, stream, p); break;
   }
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 // bm_rows: rows per workgroup required by the caller (grouped: must divide the align block).

@@ -607,7 +607,7 @@ static int launch_dma_cfg_at(const GemmArgs& p, int64_t row_tiles, hipStream_t s
   const dim3 block(WM * WN * 64);
   auto kern = gemm_dma_kernel<WM, WN, RB, NSB, NST, MODE, AT>;
   hipLaunchKernelGGL(kern, grid, block, 0, stream, p);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 // int4; p.a_tiled takes the tiled-A instantiation (groups of 64 and 32 are row-major)

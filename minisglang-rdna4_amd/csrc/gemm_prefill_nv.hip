@@ -334,7 +334,7 @@ static int launch_nv_cfg(const GemmArgs& p, int64_t row_tiles, hipStream_t strea
   const int64_t colw = p.silu ? BN / 2 : BN;
   const dim3 grid((unsigned)((ncols + colw - 1) / colw), (unsigned)row_tiles);
   hipLaunchKernelGGL((gemm_nv_kernel<WM, WN, RB, NSB>), grid, dim3(WM * WN * 64), 0, stream, p);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 // NVFP4 (e2m1 codes, e4m3 block-16 scales, the f32 global in the zeros slot) with at least two K

@@ -292,7 +292,7 @@ int launch_prefill_wide(const GemmArgs& p, int64_t rows, hipStream_t stream) {
     hipLaunchKernelGGL((gemm_wide_kernel<2, 4, 8, 4, kPAsym>), grid, dim3(512), 0, stream, p);
   else
     hipLaunchKernelGGL((gemm_wide_kernel<2, 4, 8, 4, kPSym>), grid, dim3(512), 0, stream, p);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 }  // namespace w4a8

@@ -28,7 +28,7 @@ int launch_moe_route_gemm1(const GemmArgs& p, int64_t row_blocks, hipStream_t st
   pl.ch = kGemvChunk;
   const dim3 grid((unsigned)(p.N / kTileN / 2), 1, (unsigned)p.num_slots);
   if (!gemv_launch_fmt<kARoute, 2, kGemvChunk, kWinAfterA, true, true>(p, grid, stream, pl)) return kErrUnsupported;
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 }  // namespace w4a8

@@ -634,9 +634,9 @@ static int launch_dt(Kv4Attn& p, const Kv4Plan& pl, hipStream_t st) {
   if (pl.few) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 4>), g, b, 0, st, p);
   else if (pl.nq == 1) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 1>), g, b, 0, st, p);
   else hipLaunchKernelGGL((kv4_attn_kernel<D, DT, D == 256 ? 1 : 2, 1>), g, b, 0, st, p);
-  if (hipGetLastError() != hipSuccess) return kErrHip;
+  if (hipPeekAtLastError() != hipSuccess) return kErrHip;
   if (pl.splits > 1) hipLaunchKernelGGL((kv4_join_kernel<D, DT>), dim3((unsigned)((rows + 3) / 4)), b, 0, st, p);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 int launch_kv4_attention(Kv4Attn& p, int D, int dtype, const Kv4Plan& pl, void* ws, hipStream_t st) {

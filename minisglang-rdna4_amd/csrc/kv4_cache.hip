@@ -248,7 +248,7 @@ int launch_kv4_append(const void* k, int64_t ldk, int64_t hk, const void* v, int
   auto kp = reinterpret_cast<const uint16_t*>(k), vp = reinterpret_cast<const uint16_t*>(v);
   if (dtype == kBF16) append<kBF16>(D, g, kp, ldk, hk, vp, ldv, hv, c, s, rows, st);
   else append<kF16>(D, g, kp, ldk, hk, vp, ldv, hv, c, s, rows, st);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 template <int DT>
@@ -266,7 +266,7 @@ int launch_kv4_read(const Kv4Cache& c, const Kv4Batch& s, int dtype, int D, void
   auto kp = reinterpret_cast<uint16_t*>(k), vp = reinterpret_cast<uint16_t*>(v);
   if (dtype == kBF16) read<kBF16>(D, g, c, s, kp, vp, st);
   else read<kF16>(D, g, c, s, kp, vp, st);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 }  // namespace w4a8

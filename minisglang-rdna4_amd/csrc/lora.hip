@@ -347,7 +347,7 @@ int launch_lora(LoraArgs& p, int dtype, hipStream_t st) {
     if (pl.rb == 1) hipLaunchKernelGGL((lora_down_kernel<DT_, 1>), gd, bl, 0, st, p);                 \
     else if (pl.rb == 2) hipLaunchKernelGGL((lora_down_kernel<DT_, 2>), gd, bl, 0, st, p);            \
     else hipLaunchKernelGGL((lora_down_kernel<DT_, 4>), gd, bl, 0, st, p);                            \
-    if (hipGetLastError() != hipSuccess) return kErrHip;                                              \
+    if (hipPeekAtLastError() != hipSuccess) return kErrHip;                                           \
     if (p.base_f32) W4A8_LORA_UP(DT_, true);                                                          \
     else W4A8_LORA_UP(DT_, false);                                                                    \
   } while (0)
@@ -355,7 +355,7 @@ int launch_lora(LoraArgs& p, int dtype, hipStream_t st) {
   else W4A8_LORA(kF16);
 #undef W4A8_LORA
 #undef W4A8_LORA_UP
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 }  // namespace w4a8

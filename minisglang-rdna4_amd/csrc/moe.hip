@@ -573,7 +573,7 @@ int launch_moe_route(const void* logits, int dtype, int64_t T, int E, int top_k,
                      int32_t* ids, hipStream_t stream) {
   if (T <= 0) return kOk;
   with_per<RouteLaunch>(E, logits, dtype, T, E, top_k, renorm, tw, ids, stream);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 int launch_moe_align(const int32_t* ids, int64_t numel, int E, int bm, int64_t P, int32_t* sorted_ids,
@@ -587,7 +587,7 @@ int launch_moe_align(const int32_t* ids, int64_t numel, int E, int bm, int64_t P
     else
       hipLaunchKernelGGL((moe_align_multi_kernel<512, 512>), dim3((unsigned)((numel + 511) / 512)), dim3(512), 0,
                          stream, ids, numel, E, bm, P, sorted_ids, expert_ids, ntp, inv_pos);
-    return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+    return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
   }
   if (E <= 256)
     hipLaunchKernelGGL((moe_align_kernel<1024, 256>), dim3(1), dim3(1024), 0, stream, ids, numel, E, bm, P, sorted_ids,
@@ -595,7 +595,7 @@ int launch_moe_align(const int32_t* ids, int64_t numel, int E, int bm, int64_t P
   else
     hipLaunchKernelGGL((moe_align_kernel<512, 512>), dim3(1), dim3(512), 0, stream, ids, numel, E, bm, P, sorted_ids,
                        expert_ids, ntp, inv_pos);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 template <int PER> struct PrepLaunch {
@@ -650,7 +650,7 @@ int launch_moe_route_quant(const void* logits, int ldtype, int64_t T, int E, int
   const int cpw = (int)((K + 511) / 512);
   with_per<RouteQuantLaunch>(E, cpw, logits, ldtype, T, E, top_k, renorm, tw, ids,
                              reinterpret_cast<const uint16_t*>(x), xdtype, K, ldx, xq, ldq, xs, stream);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 bool moe_prep_fits(int64_t T, int top_k) { return T * top_k <= kPrepMaxSlots; }
@@ -666,7 +666,7 @@ int launch_moe_prep(const void* logits, int ldtype, int64_t T, int E, int top_k,
   const int cpt = c >= 1 && c <= 4 ? c : 0;
   with_per<PrepLaunch>(E, cpt, logits, ldtype, T, E, top_k, renorm, tw, ids, bm, P, sorted_ids, expert_ids, ntp,
                        inv_pos, x, xdtype, K, ldx, xq, ldq, xs, slots, stream);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 int launch_moe_combine(const void* y, int ydt, int64_t ldy, const int32_t* inv_pos, const float* tw, int64_t T,
@@ -676,7 +676,7 @@ int launch_moe_combine(const void* y, int ydt, int64_t ldy, const int32_t* inv_p
   if (ydt != kF32 && H % 8 == 0 && ldy % 8 == 0 && ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out)) & 15) == 0) {
     hipLaunchKernelGGL(moe_combine8_kernel, dim3((unsigned)((H / 8 + 255) / 256), gy), dim3(256), 0, stream,
                        reinterpret_cast<const uint16_t*>(y), ydt, ldy, inv_pos, tw, T, top_k, H, out, dtype);
-    return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+    return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
   }
   dim3 grid((unsigned)((H / 4 + 255) / 256), gy);
   if (ydt == kF32)
@@ -685,7 +685,7 @@ int launch_moe_combine(const void* y, int ydt, int64_t ldy, const int32_t* inv_p
   else
     hipLaunchKernelGGL(moe_combine_kernel<false>, grid, dim3(256), 0, stream, y, ydt, ldy, inv_pos, tw, T, top_k, H,
                        out, dtype);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 }  // namespace w4a8

@@ -55,7 +55,7 @@ int launch_gelu_tanh_mul(const void* y, int64_t ldy, int64_t rows, int64_t inter
   hipLaunchKernelGGL(gelu_tanh_mul_kernel, dim3((unsigned)grid), dim3(256), 0, stream,
                      reinterpret_cast<const uint16_t*>(y), ldy, rows, inter, dtype, reinterpret_cast<uint16_t*>(out),
                      ldo, row_count);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 }  // namespace w4a8

@@ -313,7 +313,7 @@ int launch_moe_gemm2_combine(const GemmArgs& p, int64_t row_blocks, const uint16
   else if (p.wfmt == kE2M1) g2c_launch<kModeNV, false>(g, T, lds, stream);
   else if (p.zeros == nullptr) g2c_launch<kModeI4, true>(g, T, lds, stream);
   else g2c_launch<kModeI4, false>(g, T, lds, stream);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 }  // namespace w4a8

@@ -201,7 +201,7 @@ int launch_rms_norm(const void* x, int64_t ldx, void* res, int64_t ldr, const vo
   else if (chunks <= 2) W4A8_NORM(1024, 2);
   else W4A8_NORM(1024, 4);
 #undef W4A8_NORM
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 }  // namespace w4a8

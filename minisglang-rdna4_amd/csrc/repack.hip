@@ -72,7 +72,7 @@ int launch_repack(const int32_t* w, int64_t N, int64_t K, int wfmt, void* out, h
   else
     hipLaunchKernelGGL(repack_e2m1_kernel, dim3((unsigned)blocks), dim3(threads), 0, stream, w, N, K,
                        KT, reinterpret_cast<uint4*>(out));
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 }  // namespace w4a8

@@ -198,7 +198,7 @@ int launch_act_split(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx
     hipLaunchKernelGGL(w4a16::act_split_kernel<2>, g, b, 0, stream, xp, ldx, M, K, dtype, q, ldq, scales);
   else
     hipLaunchKernelGGL(w4a16::act_split_kernel<3>, g, b, 0, stream, xp, ldx, M, K, dtype, q, ldq, scales);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 template <int T, int DT>
@@ -214,7 +214,7 @@ int launch_tsum(const float* y, int64_t N, int64_t M, int dtype, void* out, int6
   if (M <= 0) return kOk;
   if (dtype == kBF16) tsum_dt<2, kBF16>(y, N, M, out, ldo, silu, st);
   else tsum_dt<3, kF16>(y, N, M, out, ldo, silu, st);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 int64_t w4a16_moe_max_inter() { return w4a16::kMidMaxInter; }
@@ -233,7 +233,7 @@ int launch_moe_silu_split(const float* y, int64_t ldy, const int32_t* inv_pos, i
   else
     hipLaunchKernelGGL((w4a16::moe_silu_split_kernel<3, kF16>), g, b, lds, st, y, ldy, inv_pos, numel, top_k, I, q,
                        ldq, scales, hp, ldh);
-  return hipGetLastError() == hipSuccess ? kOk : kErrHip;
+  return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 }  // namespace w4a8

@@ -39,7 +39,7 @@ constexpr int kTileBytes = 1024;
 constexpr int kOk = 0;
 constexpr int kErrInvalid = 1;
 constexpr int kErrUnsupported = 2;
-constexpr int kErrHip = 3;
+constexpr int kErrHip = 3;  // from a launcher: the error is HIP's last one still, for the entry point to read and clear
 // workgroups of 256 threads along a grid's axis: it has 32 bits of threads
 constexpr int64_t kMaxGrid = 0xffffff;
 
