@@ -307,10 +307,11 @@ kv4_attn_kernel(const Kv4Attn p) {
         }
       }
       top = col_max(top);
-      // 2^eq puts the largest value into [2^14, 2^15)
-      const int eq = max(141 - (int)(__float_as_uint(top) >> 23), -100);
+      // 2^eq puts the largest value into [2^14, 2^15), where that is above 2^-106: below it, and for scales that small,
+      // scores are zero for any keys, and x's factor has to have a reciprocal and to leave -inf what it is
+      const int eq = min(max(141 - (int)(__float_as_uint(top) >> 23), -100), 120);
       qs[j] = __builtin_ldexpf(col_sum(sum), eq - kUnit);
-      sc[j] = __builtin_ldexpf(p.scale, kUnit - eq);
+      sc[j] = fmaxf(__builtin_ldexpf(p.scale, kUnit - eq), 0x1p-120f);
 #pragma unroll
       for (int w = 0; w < KS; ++w) {
         float f[8];

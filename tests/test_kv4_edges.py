@@ -35,3 +35,39 @@ def test_window_past_the_table_is_nan(dev, dtype, causal):
         assert torch.equal(torch.isnan(out).all(-1).all(-1).cpu(), missing), where
         assert torch.equal(torch.isnan(out).any(-1).any(-1).cpu(), missing), where
         assert torch.equal(torch.isnan(lse).all(-1).cpu(), missing) and torch.isfinite(lse.cpu()[~missing]).all(), where
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sm_scale", [1e-3, 1e-12, 1e-30])
+def test_small_queries_and_scales(dev, dtype, sm_scale):
+    """Queries of zeros (padding) and of the type's smallest numbers with scales far below 1: all scores are zero, or as
+    good as zero, and the output is the mean of the values that a row sees."""
+    s = Setup(dev, dtype, 64, 1, 16, [70, 300], [1, 66], seed=31)
+    fi = torch.finfo(dtype)
+    for q in (torch.zeros(67, 2, 64), torch.full((67, 2, 64), fi.smallest_normal), torch.full((67, 2, 64), fi.smallest_normal * fi.eps)):
+        for kw in ({}, {"max_q": 66}, {"max_q": 1, "max_kv": 300}):
+            s.check(q.to(dtype), f"queries of {q[0, 0, 0]}, {kw}", sm_scale=sm_scale, **kw)
+            s.check(q.to(dtype), f"queries of {q[0, 0, 0]}, window, {kw}", window=3, sm_scale=sm_scale, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sm_scale", [1e-3, 0.125])
+def test_slots_nobody_wrote_count_as_keys(dev, sm_scale):
+    """A fresh cache holds vectors of zeros with steps of zero: the output is 0, and a row's sum is its keys' number."""
+    kv4 = _kv4()
+    cache = kv4.KV4Cache(8, 16, 1, 64, device=dev)
+    table = torch.arange(7, dtype=torch.int32, device=dev).view(1, 7)
+    n, new = 100, 66
+    cu, seq = torch.tensor([0, new], dtype=torch.int32, device=dev), torch.tensor([n], dtype=torch.int32, device=dev)
+    seen = torch.arange(n - new + 1, n + 1).double()
+    for q in (torch.zeros(new, 1, 64, dtype=torch.bfloat16, device=dev), torch.ones(new, 1, 64, dtype=torch.bfloat16, device=dev)):
+        for window in (0, 1, 5):
+            for kw in ({}, {"max_q": 1}):
+                out, lse = kv4.kv4_attention(q, cache, table, cu, seq, sm_scale=sm_scale, window=window, return_lse=True, **kw)
+                want = torch.log(seen.clamp_max(window) if window else seen)
+                assert (out == 0).all()
+                # The sum is held as 2^46 of it, a power that follows from the steps: lse is log(2^46 n) - 46 log 2 in f32, terms
+                # below 37 and 32, the logarithm off by up to a last place (2^-23), the product by half of one, the
+                # difference of numbers below 5 by half of one again: 37 / 2^23 + 32 / 2^24 + 5 / 2^24 = 6.7e-6.
+                assert ((lse.flatten().cpu().double() - want).abs() <= 6.7e-6).all(), (window, kw)
