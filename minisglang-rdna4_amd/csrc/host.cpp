@@ -384,8 +384,8 @@ bool aligned16(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data
 
 // (T, heads, D) rows that the kernels take as they stand
 bool head_rows(const at::Tensor* t, at::ScalarType st, int64_t D) {
-  return t && t->dim() == 3 && t->scalar_type() == st && t->size(2) == D && t->stride(2) == 1 && t->stride(0) % 8 == 0 &&
-         t->stride(1) % 8 == 0 && aligned16(*t);
+  return t && t->dim() == 3 && t->scalar_type() == st && t->size(2) == D && t->stride(2) == 1 &&
+         (t->size(0) <= 1 || t->stride(0) % 8 == 0) && (t->size(1) <= 1 || t->stride(1) % 8 == 0) && aligned16(*t);
 }
 // (M, N) rows that the kernels take as they stand
 bool flat_rows(const at::Tensor* t, at::ScalarType st, int64_t M, int64_t N) {

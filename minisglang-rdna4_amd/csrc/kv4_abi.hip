@@ -80,7 +80,10 @@ static bool apart(int64_t T, int64_t ld, int64_t H, int64_t hd, int64_t D) {
   return rows_in ? ld >= D && hd >= (T - 1) * ld + D : hd >= D && ld >= (H - 1) * hd + D;
 }
 
-static bool rows_ok(const void* p, int64_t ld, int64_t hd) { return p && aligned16(p) && ld % 8 == 0 && hd % 8 == 0; }
+// (T, H, D) rows that 16-byte loads reach; a stride that leads nowhere may be anything
+static bool rows_ok(const void* p, int64_t T, int64_t ld, int64_t H, int64_t hd) {
+  return p && aligned16(p) && (T <= 1 || ld % 8 == 0) && (H <= 1 || hd % 8 == 0);
+}
 
 extern "C" {
 
@@ -95,7 +98,7 @@ int w4a8_kv4_append(const void* k, int64_t ldk, int64_t hk, const void* v, int64
   Kv4Batch s;
   rc = operands(who, k_codes, v_codes, k_scale, v_scale, pages, page_size, H, table, ldt, width, cu, seq_lens, B, T, c, s);
   if (rc) return rc;
-  if (!rows_ok(k, ldk, hk) || !rows_ok(v, ldv, hv))
+  if (!rows_ok(k, T, ldk, H, hk) || !rows_ok(v, T, ldv, H, hv))
     return fail(kErrInvalid, "%s: k and v rows must be 16-byte aligned, with strides that are multiples of 8 elements", who);
   return launched(launch_kv4_append(k, ldk, hk, v, ldv, hv, dtype, (int)D, c, s, (hipStream_t)stream), who);
 }
@@ -147,7 +150,7 @@ int w4a8_kv4_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_
   rc = operands(who, const_cast<void*>(k_codes), const_cast<void*>(v_codes), const_cast<void*>(k_scale),
                 const_cast<void*>(v_scale), pages, page_size, H, table, ldt, width, cu, seq_lens, B, T, p.c, p.s);
   if (rc) return rc;
-  if (!rows_ok(q, ldq, hq) || !rows_ok(out, ldo, ho))
+  if (!rows_ok(q, T, ldq, Hq, hq) || !rows_ok(out, T, ldo, Hq, ho))
     return fail(kErrInvalid, "%s: q and out rows must be 16-byte aligned, with strides that are multiples of 8 elements", who);
   if (!apart(T, ldo, Hq, ho, D))
     return fail(kErrInvalid, "%s: out's rows overlap (strides %lld and %lld)", who, (long long)ldo, (long long)ho);

@@ -108,6 +108,10 @@ def _batch(cache: KV4Cache, page_table: torch.Tensor, cu_q: torch.Tensor, seq_le
     return page_table.data_ptr(), ldt, width, cu_q.data_ptr(), seq_lens.data_ptr(), B
 
 
+def _rows_ok(t: torch.Tensor) -> bool:
+    return t.stride(2) == 1 and all(t.shape[i] <= 1 or t.stride(i) % 8 == 0 for i in (0, 1)) and t.data_ptr() % 16 == 0
+
+
 def _rows(t: torch.Tensor, cache: KV4Cache, heads: int | None, name: str, what: str) -> torch.Tensor:
     """(T, heads, head_dim) rows as the kernels take them: strided, each row of channels contiguous."""
     if t.dim() != 3 or t.dtype != cache.dtype or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
@@ -115,9 +119,8 @@ def _rows(t: torch.Tensor, cache: KV4Cache, heads: int | None, name: str, what: 
                         f"{cache.dtype} as the cache is, got {t.dtype} {tuple(t.shape)}")
     if t.device != cache.device:
         raise RuntimeError(f"{what}: {name} is on {t.device}, the cache on {cache.device}")
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
-        t = t.contiguous()
-    return t
+    # a copy, not contiguous(): a contiguous tensor may begin anywhere
+    return t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, cu_q: torch.Tensor,
@@ -220,8 +223,7 @@ def kv4_attention(
         raise ValueError(f"{what}: max_q={max_q}, max_kv={max_kv}")
     if out is None:
         out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
-    elif tuple(out.shape) != (T, Hq, D) or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1 \
-            or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
+    elif tuple(out.shape) != (T, Hq, D) or out.dtype != q.dtype or out.device != q.device or not _rows_ok(out):
         raise ValueError(f"{what}: out must be ({T}, {Hq}, {D}) {q.dtype} with 16-byte aligned rows, got {out.dtype} "
                          f"{tuple(out.shape)} {tuple(out.stride())}")
     if window:  # a block of queries sees no more than this

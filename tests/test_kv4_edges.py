@@ -71,3 +71,79 @@ def test_slots_nobody_wrote_count_as_keys(dev, sm_scale):
                 # below 37 and 32, the logarithm off by up to a last place (2^-23), the product by half of one, the
                 # difference of numbers below 5 by half of one again: 37 / 2^23 + 32 / 2^24 + 5 / 2^24 = 6.7e-6.
                 assert ((lse.flatten().cpu().double() - want).abs() <= 6.7e-6).all(), (window, kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_any_strides_and_alignment(dev, dtype):
+    """k, v and q whose rows the kernels do not take as they are: contiguous but not 16-byte aligned, and one row of a
+    wider buffer whose stride is no multiple of 8."""
+    kv4 = _kv4()
+    H, G, D, page, n = 2, 4, 64, 16, 21
+    want = Setup(dev, dtype, D, H, page, [n], [n], seed=41)
+    q = want.q(H * G)
+    ref = want.attend(q)
+
+    def shifted(t):
+        buf = torch.empty(t.numel() + 8, dtype=dtype, device=dev)
+        view = buf[1:1 + t.numel()].view(t.shape)
+        view.copy_(t)
+        assert view.is_contiguous() and view.data_ptr() % 16
+        return view
+
+    cu_all = torch.tensor([0, n], dtype=torch.int32, device=dev)
+
+    def same(cache):
+        for a, b in zip((cache.k, cache.v, cache.k_scale, cache.v_scale),
+                        (want.cache.k, want.cache.v, want.cache.k_scale, want.cache.v_scale)):
+            ids = want.table[0].long().to(dev)
+            tokens = 2 if a.dtype == torch.int32 else n  # whole blocks of V; the last one's other tokens hold anything
+            assert torch.equal(a[ids].transpose(1, 2).flatten(0, 1)[:tokens].contiguous().view(torch.uint8),
+                               b[ids].transpose(1, 2).flatten(0, 1)[:tokens].contiguous().view(torch.uint8))
+
+    cache = kv4.KV4Cache(want.cache.num_pages, page, H, D, dtype, dev)
+    kv4.kv4_append(cache, shifted(want.k), shifted(want.v), want.d_table, cu_all, want.d_seq)
+    same(cache)
+    assert torch.equal(kv4.kv4_attention(shifted(q), want.cache, want.d_table, want.d_cu, want.d_seq), ref)
+    # a decode step of one row at a time, out of a buffer of odd width
+    cache = kv4.KV4Cache(want.cache.num_pages, page, H, D, dtype, dev)
+    wide = torch.zeros(1, H * D + 4, dtype=dtype, device=dev)
+    qwide = torch.zeros(1, H * G * D + 4, dtype=dtype, device=dev)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    for i in range(n):
+        wide[:, :H * D].copy_(want.k[i].view(1, -1))
+        row = wide.as_strided((1, H, D), (H * D + 4, D, 1))
+        assert row.stride(0) % 8
+        v = want.v[i:i + 1].to(dev)
+        seq = torch.tensor([i + 1], dtype=torch.int32, device=dev)
+        kv4.kv4_append(cache, row, v, want.d_table, cu, seq)
+        qwide[:, :H * G * D].copy_(q[i].view(1, -1))
+        out = torch.full_like(qwide, 3.0)
+        view, qrow = (t.as_strided((1, H * G, D), (H * G * D + 4, D, 1)) for t in (out, qwide))
+        got = kv4.kv4_attention(qrow, cache, want.d_table, cu, seq, max_q=1, out=view)
+        assert got.data_ptr() == view.data_ptr() and (out[:, H * G * D:] == 3).all()
+        plain = kv4.kv4_attention(q[i:i + 1].to(dev), want.cache, want.d_table, cu, seq, max_q=1)
+        assert torch.equal(got, plain)
+    same(cache)
+    # one head: the stride between heads does not matter
+    one = Setup(dev, dtype, D, 1, page, [n], [n], seed=42)
+    qd = one.q(1).to(dev)
+    odd = torch.as_strided(qd, (n, 1, D), (D, 3, 1))
+    assert torch.equal(one.attend(odd), one.attend(qd))
+
+
+def test_one_row_of_any_stride_passes_the_abi():
+    """Host checks of the C entry points, with pointers that are never read: a stride between rows or heads that there is
+    only one of is not looked at; what passes them ends at the workspace."""
+    lib = pkg("_abi").load()
+    P = 1 << 20
+
+    def attend(T, Hq, ldq, hq, ldo, ho):
+        rc = lib.w4a8_kv4_attention(P, 0, ldq, hq, T, Hq, 1, 128, P, P, P, P, 16, 16, P, 1 << 12, 1 << 12, P, P, 1, 1.0, 1, 0, 1,
+                                    1 << 16, P, ldo, ho, None, None, 0, None)
+        assert rc == 1
+        return lib.w4a8_last_error()
+
+    assert b"workspace" in attend(1, 4, 516, 128, 516, 128) and b"workspace" in attend(4, 1, 128, 3, 128, 5)
+    assert b"multiples of 8" in attend(2, 4, 516, 128, 512, 128) and b"multiples of 8" in attend(1, 4, 512, 124, 512, 128)
+    assert b"multiples of 8" in attend(2, 4, 512, 128, 516, 128)
