@@ -75,10 +75,14 @@ def _check(x: torch.Tensor, lora: LoraAdapters, adapters: torch.Tensor, what: st
                            f"{adapters.device} and {lora.a.device}")
 
 
+def _rows_ok(t: torch.Tensor) -> bool:
+    return t.stride(1) == 1 and (t.shape[0] <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1])) and t.data_ptr() % 16 == 0
+
+
 def _add(base: torch.Tensor, x: torch.Tensor, lora: LoraAdapters, adapters: torch.Tensor, out: torch.Tensor, what: str):
     M, K = x.shape
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < K or x.data_ptr() % 16:
-        x = x.contiguous()
+    if not _rows_ok(x):
+        x = x.clone(memory_format=torch.contiguous_format)  # contiguous() leaves what is, wherever it begins
     adapters = adapters.contiguous()
     lib = _abi.load()
     ws_bytes = int(lib.w4a8_lora_workspace_bytes(M, K, lora.rank, len(lora.slices)))
@@ -91,10 +95,6 @@ def _add(base: torch.Tensor, x: torch.Tensor, lora: LoraAdapters, adapters: torc
             adapters.data_ptr(), base.data_ptr(), _abi.dtype_code(base.dtype), ld(base), out.data_ptr(), ld(out),
             ws.data_ptr(), ws_bytes, _abi.stream_of(x)), what)
     return out
-
-
-def _rows_ok(t: torch.Tensor) -> bool:
-    return t.stride(1) == 1 and t.stride(0) % 8 == 0 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) and t.data_ptr() % 16 == 0
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, lora: LoraAdapters, adapters: torch.Tensor,
