@@ -24,6 +24,17 @@ static int fail(int code, const char* fmt, ...) {
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// whether M rows of wa bytes, lda apart, may share bytes with M rows of wb bytes, ldb apart
+static bool collide(const void* a, int64_t lda, int64_t wa, const void* b, int64_t ldb, int64_t wb, int64_t M) {
+  const int64_t pa = (int64_t)reinterpret_cast<uintptr_t>(a), pb = (int64_t)reinterpret_cast<uintptr_t>(b);
+  if (pa + (M - 1) * lda + wa <= pb || pb + (M - 1) * ldb + wb <= pa) return false;
+  if (M > 1 && lda == ldb) {  // columns of one buffer
+    const int64_t d = ((pb - pa) % lda + lda) % lda;
+    return d < wa || d + wb > lda;
+  }
+  return true;
+}
+
 extern "C" {
 
 int64_t w4a8_lora_workspace_bytes(int64_t M, int64_t K, int64_t rank, int slices) {
@@ -64,6 +75,10 @@ int w4a8_lora_add(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, c
   if (ldx < K || ldx % 8 || ldo < n || ldo % 8 || ldb < n || ldb % 8)
     return fail(kErrInvalid, "%s: row strides must be multiples of 8 that hold a row (ldx=%lld ldb=%lld ldo=%lld)", who,
                 (long long)ldx, (long long)ldb, (long long)ldo);
+  // a row's workgroups read base where they write out, and nowhere else
+  const int64_t bs = base_dtype == kF32 ? 4 : 2;
+  if (!(base == out && bs == 2 && (M == 1 || ldb == ldo)) && collide(base, ldb * bs, n * bs, out, ldo * 2, n * 2, M))
+    return fail(kErrInvalid, "%s: out overlaps base without being base itself", who);
   const int64_t need = lora_workspace(M, K, rank * slices);
   if (!workspace || workspace_bytes < need || !aligned16(workspace))
     return fail(kErrInvalid, "%s: needs a 16-byte aligned workspace of %lld bytes, got %lld", who, (long long)need,

@@ -100,8 +100,8 @@ def _add(base: torch.Tensor, x: torch.Tensor, lora: LoraAdapters, adapters: torc
 def lora_add(y: torch.Tensor, x: torch.Tensor, lora: LoraAdapters, adapters: torch.Tensor,
              out: torch.Tensor | None = None) -> torch.Tensor:
     """y + scaling (x A^T) B^T per row, into y itself (returned) or into ``out``: y (M, N) is a projection's
-    output for x (M, K), both in the adapters' type, their rows strided or not. Rows without an adapter
-    keep y's values. The sum is in f32 and rounded once."""
+    output for x (M, K), both in the adapters' type, their rows strided or not. ``out`` shares no memory
+    with y, or is y. Rows without an adapter keep y's values. The sum is in f32 and rounded once."""
     what = "lora_add"
     if _host.load().lora_add(lora.a, lora.b, lora.scaling, lora.slices, adapters, y, x, y if out is None else out):
         engaged("w4a8_mi355x.lora_add")
