@@ -359,7 +359,7 @@ int64_t w4a8_kv4_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t H, int
  * multiple of H (query head h reads key/value head h / (Hq/H)). causal: row i, at position pos, sees keys up to pos
  * (else all of its sequence's); window > 0: only those after pos - window. A row that sees none is 0, its lse -inf.
  * scale: positive, below 65536. q's values below 2^96, the cached steps as w4a8_kv4_append writes them and V's below
- * 2^100 (a bf16 model's may be more). T * Hq < 2^30, Hq <= 32768.
+ * 2^100 (a bf16 model's may be more). T * Hq < 2^30, Hq <= 32768. out may be q itself; any other overlap is refused.
  * lse: (T, Hq) f32, the natural logarithm of the sum of exp(scale q k), or null. max_q and max_kv bound the new tokens
  * and the length of a sequence: they size the grid and the workspace, and a bound that is too low costs time only. */
 int w4a8_kv4_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_t T, int64_t Hq, int64_t H, int64_t D,

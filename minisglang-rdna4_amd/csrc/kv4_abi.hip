@@ -80,6 +80,32 @@ static bool apart(int64_t T, int64_t ld, int64_t H, int64_t hd, int64_t D) {
   return rows_in ? ld >= D && hd >= (T - 1) * ld + D : hd >= D && ld >= (H - 1) * hd + D;
 }
 
+// whether (T, H, D) tensors at a and b of 16-bit elements may share some, as far as their strides tell
+static bool collide(const void* a, int64_t lda, int64_t ha, const void* b, int64_t ldb, int64_t hb, int64_t T, int64_t H,
+                    int64_t D) {
+  // the longer stride outside, a row of the other inside
+  auto order = [&](int64_t ld, int64_t h, int64_t& outer, int64_t& n, int64_t& inner) {
+    const bool heads_in = H <= 1 || (T > 1 && ld >= h);
+    outer = heads_in ? ld : h;
+    n = heads_in ? T : H;
+    inner = heads_in ? (H > 1 ? (H - 1) * h : 0) + D : (T > 1 ? (T - 1) * ld : 0) + D;
+    if (n <= 1) outer = 0;
+  };
+  int64_t oa, na, ia, ob, nb, ib;
+  order(lda, ha, oa, na, ia);
+  order(ldb, hb, ob, nb, ib);
+  const int64_t pa = (int64_t)(reinterpret_cast<uintptr_t>(a) / 2), pb = (int64_t)(reinterpret_cast<uintptr_t>(b) / 2);
+  if (pa + (na - 1) * oa + ia <= pb || pb + (nb - 1) * ob + ib <= pa) return false;
+  auto apart_by = [&](int64_t stride, int64_t wa, int64_t wb) {
+    const int64_t d = ((pb - pa) % stride + stride) % stride;
+    return d >= wa && d + wb <= stride;
+  };
+  if (oa == ob && na == nb && oa > 0 && apart_by(oa, ia, ib)) return false;  // rows beside each other
+  // heads beside each other
+  if (ha == hb && ha > 0 && (T <= 1 || (lda == ldb && lda % ha == 0)) && apart_by(ha, D, D)) return false;
+  return true;
+}
+
 // (T, H, D) rows that 16-byte loads reach; a stride that leads nowhere may be anything
 static bool rows_ok(const void* p, int64_t T, int64_t ld, int64_t H, int64_t hd) {
   return p && aligned16(p) && (T <= 1 || ld % 8 == 0) && (H <= 1 || hd % 8 == 0);
@@ -159,6 +185,9 @@ int w4a8_kv4_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(kErrInvalid, "%s: needs a 16-byte aligned workspace of %lld bytes, got %lld", who, (long long)need,
                 (long long)workspace_bytes);
+  // a workgroup reads its queries where it writes their outputs, and nowhere else
+  if (!(q == out && (T <= 1 || ldq == ldo) && (Hq <= 1 || hq == ho)) && collide(q, ldq, hq, out, ldo, ho, T, Hq, D))
+    return fail(kErrInvalid, "%s: out overlaps q without being q itself", who);
   p.q = static_cast<const uint16_t*>(q);
   p.ldq = ldq; p.hq = hq;
   p.out = static_cast<uint16_t*>(out);

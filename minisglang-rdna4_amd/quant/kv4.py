@@ -195,7 +195,8 @@ def kv4_attention(
     and below 65536, and bf16 queries are below 2^96, cached values' steps below 2^100. causal: a
     token sees the keys up to its own position; window > 0: only the last ``window`` of those. A row
     that sees no key is 0 (lse -inf). out, where given, may be strided; rows outside cu_q keep what they
-    hold there, and are undefined in a fresh output. Rows of out that overlap are refused.
+    hold there, and are undefined in a fresh output. Rows of out that overlap are refused, and so is an out that
+    overlaps q without being q.
 
     max_q and max_kv, the most new tokens and the greatest length of a sequence, are what the host
     plans the launch by (default: T rows, and the table's capacity). Too large a bound costs time, too

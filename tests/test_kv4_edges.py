@@ -147,3 +147,50 @@ def test_one_row_of_any_stride_passes_the_abi():
     assert b"workspace" in attend(1, 4, 516, 128, 516, 128) and b"workspace" in attend(4, 1, 128, 3, 128, 5)
     assert b"multiples of 8" in attend(2, 4, 516, 128, 512, 128) and b"multiples of 8" in attend(1, 4, 512, 124, 512, 128)
     assert b"multiples of 8" in attend(2, 4, 512, 128, 516, 128)
+
+
+def test_abi_refuses_an_output_on_top_of_its_queries():
+    """Host checks of the C entry point: what passes them ends at the launch, for which there is no GPU."""
+    if torch.cuda.is_available():
+        pytest.skip("the pointers are not real")
+    lib = pkg("_abi").load()
+    P = 1 << 24
+
+    def attend(q, out, T=4, Hq=4, ld=512, h=128, ldo=None, ho=None):
+        rc = lib.w4a8_kv4_attention(P + 2 * q, 0, ld, h, T, Hq, 1, 128, P, P, P, P, 16, 16, P, 1 << 12, 1 << 12, P, P, 1, 1.0, 1, 0, 1,
+                                    64, P + 2 * out, ldo or ld, ho or h, None, P, 1 << 30, None)
+        return rc, lib.w4a8_last_error()
+
+    for kw in (dict(q=0, out=512), dict(q=512, out=0), dict(q=0, out=128), dict(q=0, out=8), dict(q=0, out=0, ldo=1024), dict(q=0, out=0, ho=256, ldo=1024),
+               dict(q=0, out=256, ld=1024, h=128), dict(q=0, out=64, ld=2048, h=256), dict(q=0, out=128, ld=128, h=512),
+               dict(q=0, out=8, T=1), dict(q=0, out=8, Hq=1), dict(q=0, out=0, ld=128, h=512, ldo=512, ho=128)):
+        rc, text = attend(**kw)
+        assert rc == 1 and b"overlaps q" in text, kw
+    for kw in (dict(q=0, out=0), dict(q=0, out=2048), dict(q=2048, out=0), dict(q=0, out=512, ld=1024), dict(q=512, out=0, ld=1024),
+               dict(q=0, out=128, ld=2048, h=256), dict(q=128, out=0, ld=1024, h=256), dict(q=0, out=512, ld=128, h=1024), dict(q=0, out=512, T=1),
+               dict(q=0, out=128, Hq=1, ld=256), dict(q=0, out=0, ld=128, h=512), dict(q=0, out=0, T=1, ldo=4096)):
+        rc, text = attend(**kw)
+        assert rc == 3 and b"launch failed" in text, kw
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_outputs_beside_and_on_top_of_q(dev, dtype):
+    """In place of the queries, and in other columns of their buffer: the bits of a fresh output. Shifted: refused."""
+    kv4 = _kv4()
+    for lens, news, kw in (([40, 333, 5], [1, 1, 1], {"max_q": 1}), ([40, 333], [33, 70], {}), ([3000], [1], {"max_q": 1}), ([3000], [300], {})):
+        s = Setup(dev, dtype, 128, 2, 16, lens, news, seed=51)
+        T = sum(news)
+        wide = torch.randn(T + 1, 32, 128, generator=torch.Generator().manual_seed(1)).to(dtype).to(dev)
+        args = s.cache, s.d_table, s.d_cu, s.d_seq
+        for cut in ((slice(0, 8), slice(8, 16)), (slice(0, 16, 2), slice(1, 16, 2))):
+            buf = wide.clone()
+            q = buf[:T, cut[0]]
+            want = kv4.kv4_attention(q, *args, **kw)
+            kv4.kv4_attention(q, *args, out=buf[:T, cut[1]], **kw)
+            assert torch.equal(buf[:T, cut[1]], want) and torch.equal(q, wide[:T, cut[0]]) and torch.equal(buf[:, 16:], wide[:, 16:])
+            assert kv4.kv4_attention(q, *args, out=q, **kw).data_ptr() == q.data_ptr() and torch.equal(q, want)
+        q = buf[:T, :8]
+        for out in (buf[:T, 4:12], buf[1:, :8]) if T > 1 else (buf[:T, 4:12],):
+            with pytest.raises(RuntimeError, match="overlaps q"):
+                kv4.kv4_attention(q, *args, out=out, **kw)
