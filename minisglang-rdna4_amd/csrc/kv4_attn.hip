@@ -148,9 +148,9 @@ __device__ __forceinline__ Span kv4_span(const Kv4Attn& p, int b) {
   kv4_rows(p.s, b, s.start, s.n);
   s.cols = s.n * p.G;
   const int64_t cap = (int64_t)p.s.width << p.c.shift;
-  const int len = p.s.lens[b];
+  const int len = max(p.s.lens[b], 0);  // -2^31 has no position n rows before it
   // one token past the table's end stands for all of them: its page is missing
-  s.len = len > cap ? (int)(cap + 1 < 0x7fffffff ? cap + 1 : 0x7fffffff) : len < 0 ? 0 : len;
+  s.len = len > cap ? (int)(cap + 1 < 0x7fffffff ? cap + 1 : 0x7fffffff) : len;
   s.first_pos = len - s.n;
   return s;
 }

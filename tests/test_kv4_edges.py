@@ -194,3 +194,23 @@ def test_outputs_beside_and_on_top_of_q(dev, dtype):
         for out in (buf[:T, 4:12], buf[1:, :8]) if T > 1 else (buf[:T, 4:12],):
             with pytest.raises(RuntimeError, match="overlaps q"):
                 kv4.kv4_attention(q, *args, out=out, **kw)
+
+
+@pytest.mark.gpu
+def test_lengths_below_zero_see_nothing(dev):
+    """Lengths of a padded batch that hold anything below zero: rows of 0, lse -inf, nothing appended."""
+    kv4 = _kv4()
+    s = Setup(dev, torch.bfloat16, 64, 1, 16, [40], [1], seed=61)
+    news = [3, 1, 40, 2]
+    seq = torch.tensor([-2 ** 31, -2 ** 31 + 2, -1, -2 ** 31 + 1], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 3, 4, 44, 46], dtype=torch.int32, device=dev)
+    table = s.d_table.expand(4, -1).contiguous()
+    q = torch.randn(sum(news), 2, 64, device=dev).bfloat16()
+    before = [t.clone() for t in (s.cache.k, s.cache.v)]
+    kv4.kv4_append(s.cache, q[:, :1], q[:, :1], table, cu, seq)
+    torch.cuda.synchronize()
+    assert torch.equal(before[0], s.cache.k) and torch.equal(before[1], s.cache.v)
+    for kw in (dict(window=2), dict(), dict(max_q=1, window=5), dict(max_q=1), dict(causal=False, window=1), dict(causal=False)):
+        out, lse = kv4.kv4_attention(q, s.cache, table, cu, seq, return_lse=True, **kw)
+        torch.cuda.synchronize()
+        assert (out == 0).all() and (lse == -math.inf).all(), kw
