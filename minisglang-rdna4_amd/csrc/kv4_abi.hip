@@ -45,8 +45,8 @@ static int shapes(const char* who, int dtype, int64_t T, int64_t H, int64_t D, i
   if (T < 0 || B < 0 || H < 1 || pages < 1 || width < 0)
     return fail(kErrInvalid, "%s: sizes T=%lld B=%lld H=%lld pages=%lld table width=%lld", who, (long long)T, (long long)B,
                 (long long)H, (long long)pages, (long long)width);
-  // blocks of 8 tokens, rows and a sequence's tokens are indexed in 32 bits
-  if (B > 65535 || H > 65535 || T > 0x7fffffff || T * H > 0x7fffff00 || width > 0x7fffffff / page_size ||
+  // blocks of 8 tokens, rows and a sequence's tokens, to the end of the tile that has the last, are indexed in 32 bits
+  if (B > 65535 || H > 65535 || T > 0x7fffffff || T * H > 0x7fffff00 || width > (0x7fffffff - 32) / page_size ||
       pages > ((int64_t)1 << 31) / (H * (page_size / 8)) - 1)
     return fail(kErrUnsupported, "%s: past its index ranges (T=%lld B=%lld H=%lld pages=%lld of %lld, width=%lld)", who,
                 (long long)T, (long long)B, (long long)H, (long long)pages, (long long)page_size, (long long)width);

@@ -150,7 +150,7 @@ __device__ __forceinline__ Span kv4_span(const Kv4Attn& p, int b) {
   const int64_t cap = (int64_t)p.s.width << p.c.shift;
   const int len = max(p.s.lens[b], 0);  // -2^31 has no position n rows before it
   // one token past the table's end stands for all of them: its page is missing
-  s.len = len > cap ? (int)(cap + 1 < 0x7fffffff ? cap + 1 : 0x7fffffff) : len;
+  s.len = len > cap ? (int)cap + 1 : len;
   s.first_pos = len - s.n;
   return s;
 }

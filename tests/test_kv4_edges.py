@@ -214,3 +214,23 @@ def test_lengths_below_zero_see_nothing(dev):
         out, lse = kv4.kv4_attention(q, s.cache, table, cu, seq, return_lse=True, **kw)
         torch.cuda.synchronize()
         assert (out == 0).all() and (lse == -math.inf).all(), kw
+
+
+def test_tables_that_reach_2_31_tokens_are_refused():
+    """A sequence's last tile has to end below 2^31 tokens."""
+    if torch.cuda.is_available():
+        pytest.skip("the pointers are not real")
+    lib = pkg("_abi").load()
+    P = 1 << 24
+
+    def attend(page, width):
+        rc = lib.w4a8_kv4_attention(P, 0, 128, 128, 1, 1, 1, 128, P, P, P, P, 16, page, P, width, width, P, P, 1, 1.0, 1, 0, 1, 64,
+                                    P + 4096, 128, 128, None, P, 1 << 30, None)
+        return rc, lib.w4a8_last_error()
+
+    for page in (16, 32, 65536):
+        most = (2 ** 31 - 1 - 32) // page
+        rc, text = attend(page, most + 1)
+        assert rc == 2 and b"past its index ranges" in text, (page, text)
+        rc, text = attend(page, most)
+        assert rc == 3 and b"launch failed" in text, (page, text)
