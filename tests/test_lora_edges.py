@@ -70,3 +70,105 @@ def test_outputs_beside_and_on_top_of_y(dev):
         with pytest.raises(RuntimeError, match="overlaps"):
             m.lora_add(buf[:M, :N], x, ad, ids, out=out)
     assert torch.equal(m.lora_add(buf[:M, :N], x, ad, ids, out=buf[:M, :N]), want)
+
+
+# ------------------------------------------------------------------------------------------------ calls of large sizes
+def delta_on(dev, x, a, b, s, slices, ids):
+    """test_lora.delta with the products of an adapter's rows at once, on the GPU."""
+    M, rank, L = x.shape[0], b.shape[2], b.shape[0]
+    d, mag = (torch.zeros(M, b.shape[1], dtype=torch.float64, device=dev) for _ in range(2))
+    ids = ids.to(dev)
+    for l in range(L):
+        rows = (ids == l).nonzero().squeeze(1)
+        v = x.to(dev)[rows].double() @ a[l].to(dev).double().t().contiguous()
+        col = 0
+        for i, w in enumerate(slices):
+            vi, bi = v[:, i * rank:(i + 1) * rank], b[l, col:col + w].to(dev).double().t().contiguous()
+            d[rows, col:col + w] = float(s[l]) * (vi @ bi)
+            mag[rows, col:col + w] = abs(float(s[l])) * (vi.abs() @ bi.abs())
+            col += w
+    return d, mag
+
+
+def close_on(got, want, mag, dtype, slack=0.0):
+    err = (got.double() - want).abs() - _eps(dtype) * want.abs() - 2.0 ** -14 * mag - (2.0 ** -25 if dtype == torch.float16 else 0.0) - slack
+    assert not torch.isnan(got).any() and err.max().item() <= 0, err.max().item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+# spans of 512 and of 2048 columns, the last of a slice and its last step cut anywhere; ranks in registers and from LDS
+@pytest.mark.parametrize("M,rank,slices", [(2048, 16, [8192, 272]), (2050, 40, [5136, 4112]), (8200, 8, [8208]), (2048, 72, [16, 8304])])
+def test_spans_of_many_columns(dev, dtype, M, rank, slices):
+    m = _lora()
+    K, L, N = 64, 5, sum(slices)
+    a, b, s = make(L, rank, K, slices, dtype, seed=M)
+    ad = m.LoraAdapters(*to(dev, a, b, s), slices)
+    g = torch.Generator().manual_seed(M)
+    x = torch.randn(M, K, generator=g).to(dtype)
+    y = torch.randn(M, N, generator=torch.Generator(device=dev).manual_seed(M), device=dev).to(dtype)
+    runs = (torch.arange(M) * 7 // M).int() - 1  # prompts; the first and the last have no adapter
+    mixed = torch.randint(-1, L, (M,), generator=g, dtype=torch.int32)
+    for ids in (runs, mixed):
+        d, mag = delta_on(dev, x, a, b, s, slices, ids)
+        out = m.lora_add(y, x.to(dev), ad, ids.to(dev), out=torch.full_like(y, 9.0))
+        close_on(out, y.double() + d, mag, dtype)
+        bare = ((ids < 0) | (ids >= L)).to(dev)
+        assert torch.equal(out[bare], y[bare])
+        assert torch.equal(m.lora_add(y.clone(), x.to(dev), ad, ids.to(dev)), out), "in place"
+        # an f32 base, as the merged projection's call has it
+        f32 = y.float() * 1.001
+        got = m._add(f32, x.to(dev), ad, ids.to(dev), torch.full_like(y, 9.0), "test")
+        close_on(got, f32.double() + d, mag, dtype)
+        assert torch.equal(got[bare], f32[bare].to(dtype))
+
+
+def _dense64(fmt, w, sc, z, group, xq, xs):
+    """x W^T in f64 from the fp8 codes and the packed weight."""
+    dev = xq.device
+    codes = ((w.to(dev).unsqueeze(-1) >> torch.arange(0, 32, 4, dtype=torch.int32, device=dev)) & 15).flatten(1)
+    if fmt in ("sym", "asym"):
+        zero = 8.0 if z is None else ((z.to(dev).unsqueeze(-1) >> torch.arange(0, 32, 4, dtype=torch.int32, device=dev)) & 15).flatten(1)
+        zero = zero if z is None else zero.double().repeat_interleave(group, 0).t()
+        val = (codes.double() - zero) * sc.to(dev).double().repeat_interleave(group, 0).t()
+    else:
+        e2m1 = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6, 0, -.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float64, device=dev)
+        step = torch.pow(2.0, sc.to(dev).double() - 127) if fmt == "mxfp4" else sc.to(dev).double()
+        val = e2m1[codes.long()] * step.repeat_interleave(group, 0).t()
+        if fmt == "nvfp4":
+            val = val * z.to(dev).view(torch.float32).double().unsqueeze(1)
+    xv = xq.view(torch.float8_e4m3fn).double() * xs.double().unsqueeze(1)
+    return xv @ val.t().contiguous()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt,M,slices", [("sym", 130, [2048, 512]), ("sym", 1100, [2048, 512]), ("asym", 130, [2048, 512]), ("asym", 1100, [8192, 8192]),
+                                          ("mxfp4", 130, [2048, 512]), ("mxfp4", 1100, [2048, 512]), ("nvfp4", 130, [2048, 512]),
+                                          ("nvfp4", 1100, [2048, 512])])
+def test_linear_lora_of_prompts(kernels, dev, dtype, fmt, M, slices):
+    """Sizes whose projection runs in the operand order of the GEMM, its f32 epilogue among them, against 64 bits from the
+    packed weights. The projection's own error: 1e-4 of its largest output (test_gpu_dense.py)."""
+    m = _lora()
+    K, rank, L, N = 512, 16, 4, sum(slices)
+    e2 = fmt in ("mxfp4", "nvfp4")
+    if fmt == "mxfp4":
+        (w, sc), z, group = synth.mxfp4_weight(N, K, seed=N), None, 32
+    elif fmt == "nvfp4":
+        w, sc, z = synth.nvfp4_weight(N, K, seed=N)
+        z, group = z.view(torch.int32), 16
+    else:
+        w, sc, z = synth.int4_weight(N, K, 128, seed=N, asym=fmt == "asym", scale_floor=1e-4)
+        group = 128
+    a, b, s = make(L, rank, K, slices, dtype, seed=M)
+    ad = m.LoraAdapters(*to(dev, a, b, s), slices)
+    x = synth.activations(M, K, seed=M, dtype=dtype)
+    ids = (torch.arange(M) * 5 // M).int() - 1
+    args = kernels.repack_w4(w.to(dev), e2), sc.to(dev), None if z is None else z.to(dev), group, ad, ids.to(dev)
+    out = m.w4a8_linear_lora(x.to(dev), *args, weight_is_e2m1=e2)
+    xq, xs = kernels.act_quant(x.to(dev))
+    base = _dense64(fmt, w, sc, z, group, xq, xs)
+    d, mag = delta_on(dev, x, a, b, s, slices, ids)
+    close_on(out, base + d, mag, dtype, 1e-4 * base.abs().max().item())
+    assert ((out.double() - (base + d).to(dtype).double()).norm() / (base + d).norm()).item() <= 5e-4
+    assert torch.equal(out, m.w4a8_linear_lora(x.to(dev), *args, weight_is_e2m1=e2, x_fp8=xq, act_scales=xs))
