@@ -376,7 +376,8 @@ int w4a8_kv4_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_
  * 8 up to 256 (adapters of lower rank are padded with zeros); slice_cols: host array of the slices' widths, multiples of
  * 16 that add up to N, at most 8. adapters (M,) int32 on the device, in any order; a row whose entry is outside
  * 0 .. L-1 has no adapter and is base rounded to the type. base: x's type, and then out may be base itself, or f32; any
- * other overlap of the two is refused. The sums are f32 and rounded once. Two launches. */
+ * other overlap of the two is refused. The sums are f32 and rounded once. An infinity in x a makes NaN of its row's slice,
+ * one in b NaN or an infinity of its column in the rows of that adapter. Two launches. */
 int64_t w4a8_lora_workspace_bytes(int64_t M, int64_t K, int64_t rank, int slices);
 int w4a8_lora_add(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* a, const void* b,
                   const float* scaling, int64_t L, int64_t rank, const int64_t* slice_cols, int slices,

@@ -237,7 +237,8 @@ lora_up_kernel(const LoraArgs p) {
     top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
     auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(top), __float_as_uint(top), false, false);
     top = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
-    // 2^-e with 2^e the power of two at or below the largest |v|; NaN and infinity pass through as they are
+    // 2^-e with 2^e the power of two at or below the largest |v|. A row with an infinity is not scaled, and the infinity
+    // becomes NaN: its second term is inf - inf
     const uint32_t ex = (__float_as_uint(top) >> 23) & 255u;
     const bool plain = ex > 1 && ex < 253;
     const float down = plain ? __uint_as_float((254u - ex) << 23) : 1.f;

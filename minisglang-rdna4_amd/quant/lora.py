@@ -101,7 +101,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora: LoraAdapters, adapters: tor
              out: torch.Tensor | None = None) -> torch.Tensor:
     """y + scaling (x A^T) B^T per row, into y itself (returned) or into ``out``: y (M, N) is a projection's
     output for x (M, K), both in the adapters' type, their rows strided or not. ``out`` shares no memory
-    with y, or is y. Rows without an adapter keep y's values. The sum is in f32 and rounded once."""
+    with y, or is y. Rows without an adapter keep y's values. The sum is in f32 and rounded once; an
+    infinity in x A^T makes NaN of that row's slice, and of nothing else."""
     what = "lora_add"
     if _host.load().lora_add(lora.a, lora.b, lora.scaling, lora.slices, adapters, y, x, y if out is None else out):
         engaged("w4a8_mi355x.lora_add")

@@ -172,3 +172,33 @@ def test_linear_lora_of_prompts(kernels, dev, dtype, fmt, M, slices):
     close_on(out, base + d, mag, dtype, 1e-4 * base.abs().max().item())
     assert ((out.double() - (base + d).to(dtype).double()).norm() / (base + d).norm()).item() <= 5e-4
     assert torch.equal(out, m.w4a8_linear_lora(x.to(dev), *args, weight_is_e2m1=e2, x_fp8=xq, act_scales=xs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [1, 40, 100])
+def test_an_infinity_in_x_a_is_nan_in_its_slice(dev, dtype, M):
+    """An infinite x A^T, from a weight or from x: NaN in all of that row's slice; the row's other slices and the other
+    rows keep every bit. One in B: its column alone is not finite."""
+    m = _lora()
+    K, rank, slices = 128, 16, [64, 48]
+    a, b, s = make(3, rank, K, slices, dtype, seed=M)
+    g = torch.Generator().manual_seed(M)
+    x, y = (torch.randn(M, K, generator=g) + 3).to(dtype), torch.randn(M, sum(slices), generator=g).to(dtype)
+    ids = ((torch.arange(M) + 1) % 4 - 1).int()  # row 0: adapter 0
+    run = lambda x, a, b: m.lora_add(y.to(dev), x.to(dev), m.LoraAdapters(*to(dev, a, b, s), slices), ids.to(dev)).cpu()  # noqa: E731
+    want = run(x, a, b)
+    a2, b2 = a.clone(), b.clone()
+    a2[0, rank + 2, 7] = float("inf")  # the second slice's
+    got = run(x, a2, b)
+    rows = ids == 0
+    assert torch.isnan(got[rows][:, 64:]).all() and torch.equal(got[rows][:, :64], want[rows][:, :64]) and torch.equal(got[~rows], want[~rows])
+    b2[0, 5, 3] = float("-inf")
+    got = run(x, a, b2)
+    keep = torch.ones(M, sum(slices), dtype=torch.bool)
+    keep[rows, 5] = False
+    assert not torch.isfinite(got[~keep]).any() and torch.equal(got[keep], want[keep])
+    x2 = x.clone()
+    x2[0, 9] = float("inf")
+    got = run(x2, a, b)
+    assert torch.isnan(got[0]).all() and torch.equal(got[1:], want[1:])
