@@ -150,8 +150,9 @@ def w4a8_linear_lora(
     # of its traffic (1777 x 2560 -> 19456 198 us where this takes 215, 2048 x 4096 -> 28672 305 and 365), and cost
     # 1.4 times the error of one rounding
     arm, _ = kernels._dense_arm(x, w_packed, group_size, kernel, weight_is_e2m1, x_fp8)
-    base, _ = kernels._dense(x, w_packed, scales, w_zeros, group_size, weight_is_e2m1, x_fp8, act_scales, False, arm,
-                             torch.float32)
+    with torch.cuda.device(x.device):  # _dense launches on the current one
+        base, _ = kernels._dense(x, w_packed, scales, w_zeros, group_size, weight_is_e2m1, x_fp8, act_scales, False, arm,
+                                 torch.float32)
     out = torch.empty((x.shape[0], lora.out_features), dtype=x.dtype, device=x.device)
     _add(base, x, lora, adapters, out, what)
     engaged(_LEDGER[bool(weight_is_e2m1)])

@@ -53,6 +53,39 @@ def test_abi_refuses_an_output_on_top_of_its_base():
         assert b"workspace" in call(**kw), kw
 
 
+def test_the_projection_runs_on_its_tensors_device(monkeypatch):
+    """On another device than the current one the extension leaves the call to the Python path, whose launches are all made
+    with the tensors' device as the current one."""
+    m = _lora()
+    a, b, s = make(2, 8, 64, [32], torch.bfloat16)
+    current, seen = ["another"], []
+
+    class Device:
+        def __init__(self, d):
+            self.d = d
+
+        def __enter__(self):
+            current.append(self.d)
+
+        def __exit__(self, *exc):
+            current.pop()
+
+    class Lib:
+        w4a8_lora_workspace_bytes = staticmethod(lambda *a: 64)
+        w4a8_lora_add = staticmethod(lambda *a: seen.append(("add", current[-1])) or 0)
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(m, "_check", lambda *a: None)
+    monkeypatch.setattr(m.kernels, "_n_of", lambda w: 32)
+    monkeypatch.setattr(m.kernels, "_dense_arm", lambda *a: (1, "decode_gemv"))
+    monkeypatch.setattr(m.kernels, "_dense", lambda *a: (seen.append(("linear", current[-1])) or torch.zeros(4, 32), False))
+    monkeypatch.setattr(m._abi, "load", lambda: Lib)
+    monkeypatch.setattr(m._abi, "stream_of", lambda t: 0)
+    x = torch.zeros(4, 64).bfloat16()
+    m.w4a8_linear_lora(x, None, None, None, 128, m.LoraAdapters(a, b, s), torch.zeros(4, dtype=torch.int32))
+    assert seen == [("linear", x.device), ("add", x.device)] and current == ["another"]
+
+
 @pytest.mark.gpu
 def test_outputs_beside_and_on_top_of_y(dev):
     m = _lora()
