@@ -53,6 +53,27 @@ def test_abi_refuses_an_output_on_top_of_its_base():
         assert b"workspace" in call(**kw), kw
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_calls_without_rows(kernels, dev, dtype):
+    """A step in which nobody has a token."""
+    m = _lora()
+    K, N = 256, 64
+    w, sc, _ = synth.int4_weight(N, K, 128, seed=1, asym=False)
+    a, b, s = make(2, 8, K, [N], dtype)
+    ad = m.LoraAdapters(*to(dev, a, b, s))
+    x, ids = torch.zeros(0, K, dtype=dtype, device=dev), torch.zeros(0, dtype=torch.int32, device=dev)
+    out = m.w4a8_linear_lora(x, kernels.repack_w4(w.to(dev)), sc.to(dev), None, 128, ad, ids)
+    assert out.shape == (0, N) and out.dtype == dtype
+    assert m.lora_add(out, x, ad, ids) is out
+    att, kv4 = pkg("layers.attention"), pkg("quant.kv4")
+    layer = att.KV4Attention(4, kv4.KV4Cache(2, 16, 2, 64, dtype, dev))
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    for B in (0, 2):
+        batch = att.KV4Batch(torch.zeros(B, 1, dtype=torch.int32, device=dev), i32(*[0] * (B + 1)), i32(*[0] * B), 0, 0)
+        assert layer.forward_qkv(torch.zeros(0, 8 * 64, dtype=dtype, device=dev), batch).shape == (0, 4 * 64)
+
+
 def test_the_projection_runs_on_its_tensors_device(monkeypatch):
     """On another device than the current one the extension leaves the call to the Python path, whose launches are all made
     with the tensors' device as the current one."""
