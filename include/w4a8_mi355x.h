@@ -328,7 +328,7 @@ int w4a16_moe_silu_split(const float* y, int64_t ldy, const int32_t* inv_pos, in
  * model's type (bf16 or fp16), and stands for s * code + m:
  *   m = min x, s = max((max x - min x) / 15, 2^-14 max |x|) rounded to the type and at least its smallest positive
  *   value (2^-24 for fp16, 2^-126 for bf16), code = clamp(rint((x - m) / s), 0, 15), in f32.
- * A vector with an infinity or a NaN in it is stored as s = m = NaN.
+ * A vector with an infinity or a NaN in it, or with max x - min x past f32's range, is stored as s = m = NaN.
  * The cache's arrays, contiguous, for pages of page_size tokens (a power of two, 16 to 65536):
  *   k_codes (pages, H, page_size, D/2) bytes, code d in nibble d % 8 of the row's 32-bit word d / 8;
  *   v_codes (pages, H, page_size/8, D) 32-bit words, nibble j the code of token 8 i + j;

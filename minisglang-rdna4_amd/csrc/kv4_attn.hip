@@ -35,10 +35,11 @@
 // too, and kv4_join_kernel joins the parts.
 //
 // Measured. Decode is bound by HBM: two sequences of 131072 tokens x 8 heads of 128 (280 MB) 64 us, 4.4 TB/s, with
-// cold caches, at 3 waves per SIMD (warm 57; at 4 waves, whose 128 registers spill, 70). Prompts by the vector unit:
-// 8192 + 5690 + 3190 tokens, 32 heads of 128 (898 GFLOP) 1.53 ms, 586 TFLOP/s: 330 vector instructions a tile and
-// wave, 80 of them to widen codes and 180 for the softmax of 32 columns, beside 34 MFMA of 16 cycles; 2 waves per
-// SIMD (16 columns a wave, 3 waves: 1.69 ms).
+// cold caches, at 3 waves per SIMD (warm 59; at 4 waves, whose 128 registers spill, 87). Prompts by the vector unit:
+// 8192 + 5690 + 3190 tokens, 32 heads of 128 (898 GFLOP) 1.56 ms, 574 TFLOP/s: 354 vector instructions a tile and
+// wave, 96 of them to widen codes and 180 for the softmax of 32 columns, beside 34 MFMA of 16 cycles; 2 waves per
+// SIMD (16 columns a wave, 3 waves: 1.66 ms). Of that, codes in bits 2 and up instead of 0 and up take 2%, and so does
+// centring O every 32 tiles (every 8: 3%); fp16 models' sum w takes a tenth of their 150 us for chunks at 64 channels.
 #include "kv4.h"
 
 namespace w4a8 {
@@ -594,11 +595,15 @@ kv4_join_kernel(const Kv4Attn p) {
 // Splits of the tokens. Decode (3 workgroups of 4 waves per CU, 768 on the card): one round of the card, and up to
 // four per sequence and head where that many more workgroups even out sequences of different lengths; a split has
 // 8 tiles, two for each wave, and the first 8 are not worth the join's launch. us, with the splits that
-// this gives / without: 64 sequences of up to 8192 tokens x 8 heads 73 / 81, 16 of 4000 21 / 37, one of 8000
-// 13 / 61, two of 131072 57 / 1060; 48 of 500 10 (unsplit) / 14 in two.
+// this gives / without: 64 sequences of up to 8192 tokens x 8 heads 76 / 84, 16 of 4000 22 / 39, one of 8000
+// 14 / 62, two of 131072 59 / 1050; 48 of 500 12 (unsplit) / 15 in two. No more than 16 splits, or one per 64 tiles,
+// up to the 64 that kv4_join_kernel has lanes for: the join's time grows with them, which short contexts do not earn
+// back. us, at most 16 / this / at most 64, one sequence on 8 heads: 8192 tokens 13.7 / 13.7 / 15.0, 32768
+// 27.6 / 28.0 / 24.3, 131072 78 / 39.7 / 39.5; on one head 8192 13.4 / 13.1 / 14.0, 32768 25.1 / 25.2 / 20.3, 131072
+// 72 / 32 / 32.
 // More columns (2 workgroups of 32-column waves per CU, 512; 16-column waves 1024): as many rounds, up to four
-// splits below one round. us: 512 new tokens on 8192 127 / 265, 7 chunks of 257 on up to 6001 137 / 194, 16 x 8 new
-// tokens on 4096 37 / 134; one prompt of 2048 fills the card, 112 (unsplit) / 120 in two.
+// splits below one round. us: 512 new tokens on 8192 141 / 352, 7 chunks of 257 on up to 6001 155 / 205, 16 x 8 new
+// tokens on 4096 38 / 122; one prompt of 2048 fills the card, 121 (unsplit) / 130 in two.
 Kv4Plan kv4_plan(int64_t T, int B, int H, int G, int D, int64_t max_q, int64_t max_kv) {
   Kv4Plan pl;
   // a bound below the mean or past all rows is wrong: the workspace or the grid would grow with it
@@ -618,7 +623,7 @@ Kv4Plan kv4_plan(int64_t T, int B, int H, int G, int D, int64_t max_q, int64_t m
   int64_t s = round / pairs;
   if (pl.few || pairs < round) s = most(s, least(4, 2048 / pairs));
   s = least(s, pl.few ? tiles / 8 - 1 : tiles / 8);
-  s = least(s, least(64, most(16, tiles / 64)));  // kv4_join_kernel has a lane per split
+  s = least(s, least(64, most(16, tiles / 64)));
   pl.splits = (int)most(s, 1);
   return pl;
 }
