@@ -234,3 +234,34 @@ def test_tables_that_reach_2_31_tokens_are_refused():
         assert rc == 2 and b"past its index ranges" in text, (page, text)
         rc, text = attend(page, most)
         assert rc == 3 and b"launch failed" in text, (page, text)
+
+
+@pytest.mark.gpu
+def test_pages_past_4_gib(dev):
+    """A cache whose codes pass 4 GiB, its first, middle and last pages in use: every bit of a small cache's results."""
+    kv4 = _kv4()
+    D, page, lens, news = 64, 16, [150, 33, 16], [20, 33, 1]
+    s = Setup(dev, torch.bfloat16, D, 1, page, lens, news, seed=71)
+    pages = (1 << 32) // (page * D // 2) + 50
+    big = kv4.KV4Cache(pages, page, 1, D, device=dev)
+    assert big.k.numel() > 1 << 32
+    used = sum(-(-n // page) for n in lens)
+    g = torch.Generator().manual_seed(3)
+    ids = torch.cat([torch.arange(5), pages // 2 + torch.arange(4), torch.arange(pages - 11, pages)])
+    ids = ids[torch.randperm(len(ids), generator=g)][:used].int()
+    table, at = torch.full_like(s.table, -1), 0
+    for b, n in enumerate(lens):
+        c = -(-n // page)
+        table[b, :c] = ids[at:at + c]
+        at += c
+    args = table.to(dev), s.cu_all.to(dev), s.d_seq
+    kv4.kv4_append(big, s.k.to(dev), s.v.to(dev), *args)
+    for got, want in zip(kv4.kv4_read(big, *args, sum(lens)), kv4.kv4_read(s.cache, s.d_table, *args[1:], sum(lens))):
+        assert torch.equal(got, want)
+    q = s.q(4)
+    for kw in ({}, {"max_q": 1}, {"window": 9}):
+        assert torch.equal(kv4.kv4_attention(q.to(dev), big, table.to(dev), s.d_cu, s.d_seq, **kw), s.attend(q, **kw))
+    # nothing beside the pages in use was written
+    for t in (big.k, big.v, big.k_scale, big.v_scale):
+        t.index_fill_(0, ids.long().to(dev), 0)
+        assert t.view(-1).view(torch.int64).max() == 0 and t.view(-1).view(torch.int64).min() == 0

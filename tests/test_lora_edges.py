@@ -256,3 +256,27 @@ def test_an_infinity_in_x_a_is_nan_in_its_slice(dev, dtype, M):
     x2[0, 9] = float("inf")
     got = run(x2, a, b)
     assert torch.isnan(got[0]).all() and torch.equal(got[1:], want[1:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("inplace", [True, False])
+def test_outputs_past_4_gib(dev, inplace):
+    """Rows past 2^32 bytes of y and of a strided out: the bits that the same rows give in a call of their own."""
+    m = _lora()
+    dtype, K, slices, rank, M = torch.bfloat16, 64, [16384, 16384 + 16], 16, 65600
+    N = sum(slices)
+    a, b, s = make(3, rank, K, slices, dtype)
+    ad = m.LoraAdapters(*to(dev, a, b, s), slices)
+    g = torch.Generator(device=dev).manual_seed(4)
+    x = torch.randn(M, K, generator=g, device=dev).to(dtype)
+    y = torch.empty(M, N, dtype=dtype, device=dev).normal_(generator=g)
+    ids = (torch.arange(M, device=dev) * 5 // M).int() - 1
+    assert y.numel() * 2 > 1 << 32
+    pick = [slice(0, 2048), slice(M // 2, M // 2 + 2048), slice(M - 2048, M)]
+    before = [y[p].clone() for p in pick]
+    out = y if inplace else torch.empty(M, N + 48, dtype=dtype, device=dev)[:, 16:N + 16]
+    m.lora_add(y, x, ad, ids, out=out)
+    for p, t in zip(pick, before):
+        # more than 64 rows and as many parts of K: the same sums
+        assert torch.equal(out[p], m.lora_add(t, x[p].contiguous(), ad, ids[p].contiguous(), out=torch.empty_like(t)))
+        assert inplace or torch.equal(y[p], t)
