@@ -5,9 +5,8 @@
 //   m = min x, s = max((max x - min x) / 15, 2^-14 max |x|) rounded to the type and at least its smallest
 //   positive value (2^-24 for fp16, 2^-126 for bf16), c = clamp(rint((x - m) / s), 0, 15), in f32.
 // m is exact, and c is the nearest code for the step as it is stored. The floor on s keeps m / s, which
-// nothing divides by zero, within 2^14. A vector that holds an infinity or a NaN, or whose max x - min x passes f32's
-// range, has s = m = NaN, c = 0:
-// whoever attends to it gets NaN, and nobody else.
+// nothing divides by zero, within 2^14. A vector that holds an infinity or a NaN, or whose max x - min x
+// passes f32's range, has s = m = NaN, c = 0: whoever attends to it gets NaN, and nobody else.
 //
 // Memory, for pages of `page` tokens (a power of two from 16): everything is in blocks of 8 tokens of
 // one head, block ((p * H + h) * page + t) / 8 of slot t in page p,
