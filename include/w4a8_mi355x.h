@@ -369,6 +369,64 @@ int w4a8_kv4_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_
                        int64_t max_kv, void* out, int64_t ldo, int64_t ho, float* lse, void* workspace,
                        int64_t workspace_bytes, void* stream);
 
+/* A tree of drafted tokens. parents (T): of each new token the index, among its sequence's new tokens, of the one that it
+ * follows, or -1: it follows the cached context. A parent stands before its children; an entry that does not is -1.
+ * bits (T, words): bit j of row i is 1 for the new tokens j that token i follows, itself included; window > 0: only the
+ * last so many of them. Nodes from 32 * words on (up to 128 words) have no bit. positions (T): seq_lens[b] - n + depth. */
+int w4a8_kv4_tree(const int32_t* parents, int64_t T, const int32_t* cu, const int32_t* seq_lens, int64_t B, int64_t words,
+                  int64_t window, uint32_t* bits, int32_t* positions, void* stream);
+
+/* w4a8_kv4_attention where row i sees, of its sequence's new tokens, those whose bit is set in its row of bits (T, words; ldb
+ * words between rows; bits past the new tokens count for nothing), and all cached tokens before the new ones; window > 0: of
+ * those only the ones after positions[i] - window. Any bits are allowed; a row that sees nothing is 0, its lse -inf. */
+int w4a8_kv4_tree_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_t T, int64_t Hq, int64_t H, int64_t D,
+                            const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, int64_t pages,
+                            int64_t page_size, const int32_t* table, int64_t ldt, int64_t width, const int32_t* cu,
+                            const int32_t* seq_lens, int64_t B, float scale, int64_t window, int64_t max_q, int64_t max_kv,
+                            const uint32_t* bits, int64_t ldb, int64_t words, const int32_t* positions, void* out,
+                            int64_t ldo, int64_t ho, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Copies page src[i] to page dst[i], i < n, in each of several caches of one shape: arrays is a host array of their four
+ * arrays each (k_codes, v_codes, k_scale, v_scale), no cache twice. src and dst are read on the device; a pair with an entry
+ * outside 0 .. pages-1, or with both the same, copies nothing. The destinations are distinct and none is a source of another
+ * pair: such a page would hold parts of either. One launch per 64 caches. */
+int w4a8_kv4_copy_pages(const void* const* arrays, int64_t caches, int64_t pages, int64_t page_size, int64_t H, int64_t D,
+                        const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+
+/* Puts accepted tokens behind the context, in each of several caches of one shape (as above): of sequence b's n new tokens,
+ * slot j < kept[b] gets what token keep[b * ldk + j] holds (ascending, so that keep[.][j] >= j; an entry below j or not below n
+ * leaves slot j as it is, and so does a page that does not exist). kept is taken between 0 and the smaller of n and most.
+ * new_lens (B), where given, receives seq_lens[b] - n + kept; it is not seq_lens. The 8 tokens of a block are one sequence's,
+ * as for w4a8_kv4_append. One launch per 64 caches. */
+int w4a8_kv4_keep(const void* const* arrays, int64_t caches, int64_t pages, int64_t page_size, int64_t H, int64_t D,
+                  const int32_t* table, int64_t ldt, int64_t width, const int32_t* cu, const int32_t* seq_lens, int64_t B,
+                  const int32_t* keep, int64_t ldk, int64_t most, const int32_t* kept, int32_t* new_lens, void* stream);
+
+/* Attention over whole prompts, packed, in 16 bits: every key is a row of this call. q, out (T, Hq, D) and k, v (T, H, D)
+ * with strides (multiples of 8 elements; ldk and ldv at least D and below 2^23), D 64, 128 or 256, bf16 or fp16; rows
+ * cu[b] .. cu[b+1]-1 (cu (B + 1, ascending), read on the device) are sequence b's, query head h reads key/value head
+ * h / (Hq/H). causal: row i sees the sequence's rows up to itself (else all); window > 0: only those after i - window.
+ * scale: positive, below 65536. A value of v that is not finite makes its channel not finite in the rows that see it, and
+ * leaves the others alone. Rows outside cu[0] .. cu[B]-1 are left as they are. out may be q itself; any other overlap with
+ * q, k or v is refused. lse: (T, Hq) f32, the natural logarithm of the sum of exp(scale q k), or null. max_q bounds a
+ * sequence's rows: it sizes the grid, and a bound that is too low costs time only. T * Hq < 2^30, B up to 65535. */
+int w4a8_prompt_attention(const void* q, int64_t ldq, int64_t hq, const void* k, int64_t ldk, int64_t hk, const void* v,
+                          int64_t ldv, int64_t hv, int dtype, int64_t T, int64_t Hq, int64_t H, int64_t D,
+                          const int32_t* cu, int64_t B, float scale, int causal, int64_t window, int64_t max_q, void* out,
+                          int64_t ldo, int64_t ho, float* lse, void* stream);
+
+/* ---- Rotary positions. The first R channels of a head (16 to D, a multiple of 16) are R/2 pairs, channels i and i + R/2, or
+ * 2i and 2i + 1 (adjacent); pair i is turned by t = positions[axis[i], token] * f_i:
+ *   a' = scale (a cos t - b sin t),  b' = scale (a sin t + b cos t),
+ * in f32, rounded once; channels behind R stay. turns[i]: f_i / (2 pi) modulo 1 in units of 2^-64, so that any position's
+ * angle is exact to 2^-32 of a turn. positions (axes, T), ldp entries between axes, 32 or 64 bits, signed; axis (R/2) with
+ * entries below axes, or null for one axis. q (T, Hq, D) and k (T, Hk, D; Hk may be 0) with strides that are multiples of 8
+ * elements; D a multiple of 8 up to 1024. q_out and k_out may be q and k themselves; any other overlap is refused. */
+int w4a8_rotary(const void* q, int64_t ldq, int64_t hq, int64_t Hq, const void* k, int64_t ldk, int64_t hk, int64_t Hk,
+                int dtype, int64_t T, int64_t D, int64_t R, int adjacent, const void* positions, int positions_64,
+                int64_t axes, int64_t ldp, const uint64_t* turns, const int32_t* axis, float scale, void* q_out,
+                int64_t ldqo, int64_t hqo, void* k_out, int64_t ldko, int64_t hko, void* stream);
+
 /* ---- Low-rank adapters of many requests beside a shared projection. No counterpart in the reference.
  *   out[m, n] = base[m, n] + scaling[l] * sum_r (sum_k x[m, k] a[l, s * rank + r, k]) b[l, n, r],  l = adapters[m],
  * s the slice that column n is in: projections merged in one weight (q, k and v; gate and up) keep a low-rank pair each.

@@ -91,6 +91,20 @@ SIGNATURES = {
     "w4a8_kv4_attention": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _vp,
                                     _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, ctypes.c_float, _c_int,
                                     _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp]),
+    "w4a8_prompt_attention": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_int, _c_i64, _c_i64,
+                                       _c_i64, _c_i64, _vp, _c_i64, ctypes.c_float, _c_int, _c_i64, _c_i64, _vp, _c_i64,
+                                       _c_i64, _vp, _vp]),
+    "w4a8_rotary": (_c_int, [_vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_int, _c_i64, _c_i64, _c_i64, _c_int,
+                             _vp, _c_int, _c_i64, _c_i64, _vp, _vp, ctypes.c_float, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
+                             _vp]),
+    "w4a8_kv4_tree": (_c_int, [_vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp]),
+    "w4a8_kv4_tree_attention": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _vp,
+                                         _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, ctypes.c_float, _c_i64,
+                                         _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64,
+                                         _vp]),
+    "w4a8_kv4_copy_pages": (_c_int, [_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp]),
+    "w4a8_kv4_keep": (_c_int, [_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp, _c_i64,
+                               _c_i64, _vp, _vp, _vp]),
 }
 
 _lock = threading.Lock()

@@ -1,6 +1,6 @@
 // The operators' host path for plain calls, as a CPython extension: checks of shapes and types,
 // outputs and workspaces from torch's caching allocator, and the C ABI call, without the interpreter
-// in between. quant/kernels.py, quant/kv4.py, quant/lora.py and layers/norm.py try it first; anything
+// in between. quant/kernels.py, quant/kv4.py, quant/lora.py, layers/norm.py, layers/attention.py and layers/rotary.py try it first; anything
 // it does not take as it stands (op-layout weights, strided or CPU tensors, tensor subclasses, invalid
 // arguments) returns None before anything is allocated or launched, and the Python path serves or
 // refuses it as it always did.
@@ -23,6 +23,7 @@
 
 #include <algorithm>
 #include <exception>
+#include <vector>
 
 #include "../../include/w4a8_mi355x.h"
 
@@ -58,6 +59,12 @@ struct Abi {
   decltype(&w4a8_kv4_attention) kv4_attention;
   decltype(&w4a8_lora_workspace_bytes) lora_ws;
   decltype(&w4a8_lora_add) lora_add;
+  decltype(&w4a8_kv4_tree) kv4_tree;
+  decltype(&w4a8_kv4_tree_attention) kv4_tree_attention;
+  decltype(&w4a8_kv4_copy_pages) kv4_copy_pages;
+  decltype(&w4a8_kv4_keep) kv4_keep;
+  decltype(&w4a8_prompt_attention) prompt_attention;
+  decltype(&w4a8_rotary) rotary;
 };
 Abi abi;
 bool bound = false;
@@ -470,6 +477,63 @@ PyObject* kv4_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// attention over the cache: q = a[7], max_q = a[8], max_kv = a[9], scale = a[10], then causal (null: a tree, with its
+// mask and positions), window, out and lse
+PyObject* attend(PyObject* const* a, PyObject* pcausal, PyObject* pwindow, PyObject* pout, PyObject* plse, PyObject* pmask,
+                 PyObject* ppos) {
+  Kv4 c;
+  if (!kv4(a, c)) Py_RETURN_NONE;
+  const at::Tensor *q = strided(a[7]), *o = pout == Py_None ? nullptr : strided(pout), *mask = nullptr, *pos = nullptr;
+  if (!head_rows(q, c.ks->scalar_type(), c.D) || (pout != Py_None && !head_rows(o, q->scalar_type(), c.D)))
+    Py_RETURN_NONE;
+  const int64_t T = q->size(0), Hq = q->size(1);
+  if (pmask) {
+    mask = plain(pmask);
+    pos = plain(ppos);
+    if (!mask || !pos || mask->scalar_type() != at::kInt || pos->scalar_type() != at::kInt || mask->dim() != 2 ||
+        pos->dim() != 1 || mask->size(0) != T || pos->size(0) != T || mask->size(1) < 1 || mask->size(1) > 128)
+      Py_RETURN_NONE;
+  }
+  if ((o && (o->size(0) != T || o->size(1) != Hq)) ||
+      !same_device(*q, o, c.k, c.v, c.ks, c.vs, c.table, c.cu, c.lens, mask, pos) || Hq < c.H || Hq % c.H)
+    Py_RETURN_NONE;
+  const int64_t cap = c.width * c.page;
+  int64_t max_q = T, max_kv = cap;
+  if ((a[8] != Py_None && !PyLong_Check(a[8])) || (a[9] != Py_None && !PyLong_Check(a[9])) || !PyLong_Check(pwindow))
+    Py_RETURN_NONE;
+  if (a[8] != Py_None) max_q = std::min<int64_t>(PyLong_AsLongLong(a[8]), T);
+  if (a[9] != Py_None) max_kv = std::min<int64_t>(PyLong_AsLongLong(a[9]), cap);
+  const double scale = PyFloat_AsDouble(a[10]);
+  const int64_t window = PyLong_AsLongLong(pwindow);
+  const bool causal = !pcausal || PyObject_IsTrue(pcausal) == 1, want_lse = PyObject_IsTrue(plse) == 1;
+  if (PyErr_Occurred()) return nullptr;
+  if (window < 0 || max_q < 0 || max_kv < 0) Py_RETURN_NONE;
+  if (window) max_kv = std::min(max_kv, window + max_q);
+  const int64_t wsb = abi.kv4_attention_ws(T, Hq, c.H, c.D, c.B, max_q, max_kv);
+  at::Tensor out = o ? *o : empty(*q, {T, Hq, c.D}, q->scalar_type()), lse, ws;
+  if (want_lse) lse = empty(*q, {T, Hq}, at::kFloat);
+  if (wsb > 0) ws = empty(*q, {wsb}, at::kByte);
+  void* st = stream_of(*q);
+  float* lp = want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
+  void* wp = ws.defined() ? ws.data_ptr() : nullptr;
+  const int rc = unlocked([&] {
+    if (mask)
+      return abi.kv4_tree_attention(q->data_ptr(), c.dt, q->stride(0), q->stride(1), T, Hq, c.H, c.D, c.k->data_ptr(),
+                                    c.v->data_ptr(), c.ks->data_ptr(), c.vs->data_ptr(), c.pages, c.page, i32(c.table), c.ldt,
+                                    c.width, i32(c.cu), i32(c.lens), c.B, (float)scale, window, max_q, max_kv,
+                                    reinterpret_cast<const uint32_t*>(i32(mask)), mask->size(1), mask->size(1), i32(pos),
+                                    out.data_ptr(), out.stride(0), out.stride(1), lp, wp, wsb > 0 ? wsb : 0, st);
+    return abi.kv4_attention(q->data_ptr(), c.dt, q->stride(0), q->stride(1), T, Hq, c.H, c.D, c.k->data_ptr(),
+                             c.v->data_ptr(), c.ks->data_ptr(), c.vs->data_ptr(), c.pages, c.page, i32(c.table), c.ldt,
+                             c.width, i32(c.cu), i32(c.lens), c.B, (float)scale, causal, window, max_q, max_kv,
+                             out.data_ptr(), out.stride(0), out.stride(1), lp, wp, wsb > 0 ? wsb : 0, st);
+  });
+  if (rc) return failed(rc, "kv4_attention");
+  PyObject* po = o ? Py_NewRef(pout) : THPVariable_Wrap(std::move(out));
+  PyObject* pl = want_lse ? THPVariable_Wrap(std::move(lse)) : Py_NewRef(Py_None);
+  return Py_BuildValue("(NN)", po, pl);
+}
+
 // kv4_attention(cache and batch, q, max_q or None, max_kv or None, scale, causal, window, out or None, lse)
 // -> (out, lse or None) or None
 PyObject* kv4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -477,45 +541,193 @@ PyObject* kv4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     PyErr_SetString(PyExc_TypeError, "kv4_attention: 15 arguments, after bind()");
     return nullptr;
   }
+  return guarded([&]() -> PyObject* { return attend(a, a[11], a[12], a[13], a[14], nullptr, nullptr); });
+}
+
+// kv4_tree_attention(cache and batch, q, max_q or None, max_kv or None, scale, window, out or None, lse, mask, positions)
+// -> (out, lse or None) or None
+PyObject* kv4_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 16 || !bound) {
+    PyErr_SetString(PyExc_TypeError, "kv4_tree_attention: 16 arguments, after bind()");
+    return nullptr;
+  }
+  return guarded([&]() -> PyObject* { return attend(a, nullptr, a[11], a[12], a[13], a[14], a[15]); });
+}
+
+bool ints(const at::Tensor* t, int64_t dim) { return t && t->scalar_type() == at::kInt && t->dim() == dim; }
+
+// kv4_tree(parents, cu, lens, max_q, window) -> (mask, positions) or None
+PyObject* kv4_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 5 || !bound) {
+    PyErr_SetString(PyExc_TypeError, "kv4_tree: 5 arguments, after bind()");
+    return nullptr;
+  }
   return guarded([&]() -> PyObject* {
-    Kv4 c;
-    if (!kv4(a, c)) Py_RETURN_NONE;
-    const at::Tensor *q = strided(a[7]), *o = a[13] == Py_None ? nullptr : strided(a[13]);
-    if (!head_rows(q, c.ks->scalar_type(), c.D) || (a[13] != Py_None && !head_rows(o, q->scalar_type(), c.D)))
-      Py_RETURN_NONE;
-    const int64_t T = q->size(0), Hq = q->size(1);
-    if ((o && (o->size(0) != T || o->size(1) != Hq)) || !same_device(*q, o, c.k, c.v, c.ks, c.vs, c.table, c.cu, c.lens) ||
-        Hq < c.H || Hq % c.H)
-      Py_RETURN_NONE;
-    const int64_t cap = c.width * c.page;
-    int64_t max_q = T, max_kv = cap;
-    if ((a[8] != Py_None && !PyLong_Check(a[8])) || (a[9] != Py_None && !PyLong_Check(a[9])) || !PyLong_Check(a[12]))
-      Py_RETURN_NONE;
-    if (a[8] != Py_None) max_q = std::min<int64_t>(PyLong_AsLongLong(a[8]), T);
-    if (a[9] != Py_None) max_kv = std::min<int64_t>(PyLong_AsLongLong(a[9]), cap);
-    const double scale = PyFloat_AsDouble(a[10]);
-    const int64_t window = PyLong_AsLongLong(a[12]);
-    const bool causal = PyObject_IsTrue(a[11]) == 1, want_lse = PyObject_IsTrue(a[14]) == 1;
+    const at::Tensor *parents = plain(a[0]), *cu = plain(a[1]), *lens = plain(a[2]);
+    if (!ints(parents, 1) || !ints(cu, 1) || !ints(lens, 1) || !PyLong_Check(a[3]) || !PyLong_Check(a[4])) Py_RETURN_NONE;
+    const int64_t max_q = PyLong_AsLongLong(a[3]), window = PyLong_AsLongLong(a[4]);
     if (PyErr_Occurred()) return nullptr;
-    if (window < 0 || max_q < 0 || max_kv < 0) Py_RETURN_NONE;
-    if (window) max_kv = std::min(max_kv, window + max_q);
-    const int64_t wsb = abi.kv4_attention_ws(T, Hq, c.H, c.D, c.B, max_q, max_kv);
-    at::Tensor out = o ? *o : empty(*q, {T, Hq, c.D}, q->scalar_type()), lse, ws;
+    const int64_t T = parents->size(0), B = lens->size(0), words = (max_q + 31) / 32;
+    if (max_q < 1 || words > 128 || window < 0 || cu->size(0) != B + 1 || !same_device(*parents, cu, lens)) Py_RETURN_NONE;
+    at::Tensor mask = empty(*parents, {T, words}, at::kInt), pos = empty(*parents, {T}, at::kInt);
+    void* st = stream_of(*parents);
+    const int rc = unlocked([&] {
+      return abi.kv4_tree(i32(parents), T, i32(cu), i32(lens), B, words, window, static_cast<uint32_t*>(mask.data_ptr()),
+                          static_cast<int32_t*>(pos.data_ptr()), st);
+    });
+    if (rc) return failed(rc, "kv4_tree");
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(mask)), THPVariable_Wrap(std::move(pos)));
+  });
+}
+
+// caches of one shape, as a tuple of four tensors each: their pointers, and the first one's tensors in `c`
+bool caches(PyObject* o, std::vector<const void*>& arrays, const at::Tensor* (&c)[4]) {
+  if (!PyTuple_CheckExact(o)) return false;
+  const Py_ssize_t n = PyTuple_GET_SIZE(o);
+  if (n < 4 || n % 4) return false;
+  arrays.reserve(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const at::Tensor* t = plain(PyTuple_GET_ITEM(o, i));
+    if (!t || t->dim() != 4) return false;
+    if (i < 4) c[i] = t;
+    if (t->scalar_type() != c[i % 4]->scalar_type() || t->sizes() != c[i % 4]->sizes() || !same_device(*c[0], t)) return false;
+    if (i % 4 == 0)
+      for (Py_ssize_t j = 0; j < i; j += 4)
+        if (arrays[j] == t->data_ptr()) return false;
+    arrays.push_back(t->data_ptr());
+  }
+  return true;
+}
+
+// kv4_copy_pages(caches' tensors, src, dst) -> True or None
+PyObject* kv4_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 3 || !bound) {
+    PyErr_SetString(PyExc_TypeError, "kv4_copy_pages: 3 arguments, after bind()");
+    return nullptr;
+  }
+  return guarded([&]() -> PyObject* {
+    std::vector<const void*> arrays;
+    const at::Tensor* c[4];
+    const at::Tensor *src = plain(a[1]), *dst = plain(a[2]);
+    if (!ints(src, 1) || !ints(dst, 1) || src->size(0) != dst->size(0) || !caches(a[0], arrays, c) ||
+        !same_device(*c[0], src, dst))
+      Py_RETURN_NONE;
+    void* st = stream_of(*src);
+    const int rc = unlocked([&] {
+      return abi.kv4_copy_pages(arrays.data(), (int64_t)arrays.size() / 4, c[0]->size(0), c[0]->size(2), c[0]->size(1),
+                                c[0]->size(3) * 2, i32(src), i32(dst), src->size(0), st);
+    });
+    if (rc) return failed(rc, "kv4_copy_pages");
+    Py_RETURN_TRUE;
+  });
+}
+
+// kv4_keep(caches' tensors, page_table, cu, lens, keep, kept) -> new lengths or None
+PyObject* kv4_keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 6 || !bound) {
+    PyErr_SetString(PyExc_TypeError, "kv4_keep: 6 arguments, after bind()");
+    return nullptr;
+  }
+  return guarded([&]() -> PyObject* {
+    std::vector<const void*> arrays;
+    const at::Tensor* c[4];
+    const at::Tensor *keep = plain(a[4]), *kept = plain(a[5]);
+    if (!ints(keep, 2) || !ints(kept, 1) || !caches(a[0], arrays, c)) Py_RETURN_NONE;
+    PyObject* const first[7] = {PyTuple_GET_ITEM(a[0], 0), PyTuple_GET_ITEM(a[0], 1), PyTuple_GET_ITEM(a[0], 2),
+                                PyTuple_GET_ITEM(a[0], 3), a[1], a[2], a[3]};
+    Kv4 s;
+    if (!kv4(first, s) || keep->size(0) != s.B || kept->size(0) != s.B ||
+        !same_device(*c[0], s.table, s.cu, s.lens, keep, kept))
+      Py_RETURN_NONE;
+    at::Tensor now = empty(*kept, {s.B}, at::kInt);
+    void* st = stream_of(*kept);
+    const int rc = unlocked([&] {
+      return abi.kv4_keep(arrays.data(), (int64_t)arrays.size() / 4, s.pages, s.page, s.H, s.D, i32(s.table), s.ldt, s.width,
+                          i32(s.cu), i32(s.lens), s.B, i32(keep), keep->size(1), keep->size(1), i32(kept),
+                          static_cast<int32_t*>(now.data_ptr()), st);
+    });
+    if (rc) return failed(rc, "kv4_keep");
+    return THPVariable_Wrap(std::move(now));
+  });
+}
+
+// prompt_attention(q, k, v, cu, max_q or None, scale, causal, window, out or None, lse) -> (out, lse or None) or None
+PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 10 || !bound) {
+    PyErr_SetString(PyExc_TypeError, "prompt_attention: 10 arguments, after bind()");
+    return nullptr;
+  }
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *q = strided(a[0]), *k = strided(a[1]), *v = strided(a[2]), *cu = plain(a[3]);
+    const at::Tensor* o = a[8] == Py_None ? nullptr : strided(a[8]);
+    if (!q || !ints(cu, 1) || cu->size(0) < 1 || q->dim() != 3 || act_dtype(*q) < 0) Py_RETURN_NONE;
+    const int64_t T = q->size(0), Hq = q->size(1), D = q->size(2);
+    const auto t = q->scalar_type();
+    if ((D != 64 && D != 128 && D != 256) || !head_rows(q, t, D) || !head_rows(k, t, D) || !head_rows(v, t, D) ||
+        (a[8] != Py_None && !head_rows(o, t, D)))
+      Py_RETURN_NONE;
+    const int64_t H = k->size(1);
+    for (const at::Tensor* r : {k, v})
+      if (r->size(0) != T || r->size(1) != H || (T > 1 && (r->stride(0) < D || r->stride(0) >= 1 << 23))) Py_RETURN_NONE;
+    if (H < 1 || Hq < H || Hq % H || (o && (o->size(0) != T || o->size(1) != Hq)) || !same_device(*q, k, v, cu, o))
+      Py_RETURN_NONE;
+    if ((a[4] != Py_None && !PyLong_Check(a[4])) || !PyLong_Check(a[7])) Py_RETURN_NONE;
+    const int64_t max_q = a[4] == Py_None ? T : std::min<int64_t>(PyLong_AsLongLong(a[4]), T);
+    const double scale = PyFloat_AsDouble(a[5]);
+    const int64_t window = PyLong_AsLongLong(a[7]);
+    const bool causal = PyObject_IsTrue(a[6]) == 1, want_lse = PyObject_IsTrue(a[9]) == 1;
+    if (PyErr_Occurred()) return nullptr;
+    if (window < 0 || max_q < 0) Py_RETURN_NONE;
+    at::Tensor out = o ? *o : empty(*q, {T, Hq, D}, t), lse;
     if (want_lse) lse = empty(*q, {T, Hq}, at::kFloat);
-    if (wsb > 0) ws = empty(*q, {wsb}, at::kByte);
     void* st = stream_of(*q);
     const int rc = unlocked([&] {
-      return abi.kv4_attention(q->data_ptr(), c.dt, q->stride(0), q->stride(1), T, Hq, c.H, c.D, c.k->data_ptr(),
-                               c.v->data_ptr(), c.ks->data_ptr(), c.vs->data_ptr(), c.pages, c.page, i32(c.table), c.ldt,
-                               c.width, i32(c.cu), i32(c.lens), c.B, (float)scale, causal, window, max_q, max_kv,
-                               out.data_ptr(), out.stride(0), out.stride(1),
-                               want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr,
-                               ws.defined() ? ws.data_ptr() : nullptr, wsb > 0 ? wsb : 0, st);
+      return abi.prompt_attention(q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), k->stride(0), k->stride(1),
+                                  v->data_ptr(), v->stride(0), v->stride(1), act_dtype(*q), T, Hq, H, D, i32(cu),
+                                  cu->size(0) - 1, (float)scale, causal, window, max_q, out.data_ptr(), out.stride(0),
+                                  out.stride(1), want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, st);
     });
-    if (rc) return failed(rc, "kv4_attention");
-    PyObject* po = o ? Py_NewRef(a[13]) : THPVariable_Wrap(std::move(out));
+    if (rc) return failed(rc, "prompt_attention");
+    PyObject* po = o ? Py_NewRef(a[8]) : THPVariable_Wrap(std::move(out));
     PyObject* pl = want_lse ? THPVariable_Wrap(std::move(lse)) : Py_NewRef(Py_None);
     return Py_BuildValue("(NN)", po, pl);
+  });
+}
+
+// rotary(turns, axis, axes, head_dim, rotary_dim, adjacent, scale, q, k, positions, in place) -> (q, k) or None
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 11 || !bound) {
+    PyErr_SetString(PyExc_TypeError, "rotary: 11 arguments, after bind()");
+    return nullptr;
+  }
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *turns = plain(a[0]), *axis = plain(a[1]), *q = strided(a[7]), *k = strided(a[8]), *pos = plain(a[9]);
+    if (!turns || !axis || !q || !k || !pos) Py_RETURN_NONE;
+    const int64_t axes = PyLong_AsLongLong(a[2]), D = PyLong_AsLongLong(a[3]), R = PyLong_AsLongLong(a[4]);
+    const bool adjacent = PyObject_IsTrue(a[5]) == 1, inplace = PyObject_IsTrue(a[10]) == 1;
+    const double scale = PyFloat_AsDouble(a[6]);
+    if (PyErr_Occurred()) return nullptr;
+    const auto t = q->scalar_type();
+    if (act_dtype(*q) < 0 || !head_rows(q, t, D) || !head_rows(k, t, D)) Py_RETURN_NONE;
+    const int64_t T = q->size(0), Hq = q->size(1), Hk = k->size(1);
+    const bool wide = pos->scalar_type() == at::kLong;
+    if (k->size(0) != T || Hq < 1 || Hk < 1 || (!wide && pos->scalar_type() != at::kInt) || turns->numel() != R / 2 ||
+        axis->numel() != R / 2 || !same_device(*q, k, pos, turns, axis))
+      Py_RETURN_NONE;
+    if (!(pos->dim() == 2 && pos->size(0) == axes && pos->size(1) == T) && !(pos->dim() == 1 && axes == 1 && pos->size(0) == T))
+      Py_RETURN_NONE;
+    at::Tensor qo = inplace ? *q : empty(*q, {T, Hq, D}, t), ko = inplace ? *k : empty(*k, {T, Hk, D}, t);
+    void* st = stream_of(*q);
+    const int rc = unlocked([&] {
+      return abi.rotary(q->data_ptr(), q->stride(0), q->stride(1), Hq, k->data_ptr(), k->stride(0), k->stride(1), Hk,
+                        act_dtype(*q), T, D, R, adjacent, pos->data_ptr(), wide, axes, T,
+                        static_cast<const uint64_t*>(turns->data_ptr()), i32(axis), (float)scale, qo.data_ptr(), qo.stride(0),
+                        qo.stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), st);
+    });
+    if (rc) return failed(rc, "Rotary");
+    PyObject* pq = inplace ? Py_NewRef(a[7]) : THPVariable_Wrap(std::move(qo));
+    PyObject* pk = inplace ? Py_NewRef(a[8]) : THPVariable_Wrap(std::move(ko));
+    return Py_BuildValue("(NN)", pq, pk);
   });
 }
 
@@ -647,6 +859,13 @@ PyMethodDef methods[] = {
     {"kv4_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_append)), METH_FASTCALL, nullptr},
     {"kv4_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_read)), METH_FASTCALL, nullptr},
     {"kv4_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_attention)), METH_FASTCALL, nullptr},
+    {"kv4_tree", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_tree)), METH_FASTCALL, nullptr},
+    {"kv4_tree_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_tree_attention)), METH_FASTCALL,
+     nullptr},
+    {"kv4_copy_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_copy_pages)), METH_FASTCALL, nullptr},
+    {"kv4_keep", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_keep)), METH_FASTCALL, nullptr},
+    {"prompt_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prompt_attention)), METH_FASTCALL, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary)), METH_FASTCALL, nullptr},
     {"lora_add", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(lora_add)), METH_FASTCALL, nullptr},
     {"linear_lora", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_lora)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -59,6 +59,24 @@ struct Kv4Attn {
   int splits;       // of the tokens, over the grid
   float* po;        // (splits, T, Hq, D) partial outputs
   float* pml;       // (splits, T, Hq, 2) their maximum and sum
+  // a tree of drafted tokens, or null: bit j of row i is whether it sees its sequence's new token j, and pos[i] is its
+  // position, which the window counts from
+  const uint32_t* bits;
+  int64_t ldb;      // words between rows
+  int words;        // words of a row
+  const int32_t* pos;
+};
+
+// Several layers' caches of one shape, for one launch
+constexpr int kKv4Caches = 64;
+struct Kv4Arrays {
+  uint8_t* k;
+  uint8_t* v;
+  uint32_t* ks;
+  uint32_t* vs;
+};
+struct Kv4Caches {
+  Kv4Arrays c[kKv4Caches];
 };
 
 // How a call is cut. few: 16 columns and the waves of a workgroup over the tokens; else nq * 16 columns per

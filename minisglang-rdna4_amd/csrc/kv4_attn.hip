@@ -144,14 +144,15 @@ struct Span {
   int64_t start;
   int n, cols, len, first_pos;  // new tokens, columns, length, position of the first new token
 };
+template <bool TREE>
 __device__ __forceinline__ Span kv4_span(const Kv4Attn& p, int b) {
   Span s;
   kv4_rows(p.s, b, s.start, s.n);
   s.cols = s.n * p.G;
   const int64_t cap = (int64_t)p.s.width << p.c.shift;
   const int len = max(p.s.lens[b], 0);  // -2^31 has no position n rows before it
-  // one token past the table's end stands for all of them: its page is missing
-  s.len = len > cap ? (int)cap + 1 : len;
+  // one token past the table's end stands for all of them: its page is missing (of a tree each node has its own)
+  s.len = len > cap ? (int)min((int64_t)len, cap + (TREE ? s.n + 1 : 1)) : len;
   s.first_pos = len - s.n;
   return s;
 }
@@ -178,6 +179,31 @@ __device__ __forceinline__ int kv4_query(const Kv4Attn& p, int i0, int r0, int x
   const int c = r0 + x, i = (int)__umulhi((uint32_t)c << 1, p.gmul);
   head = c - i * p.G;
   return i0 + i;
+}
+
+// Of a tree: the first cached key that query i sees, and its 8 bits of the tokens at .. at + 7, counted from the
+// first new one
+__device__ __forceinline__ int tree_from(const Kv4Attn& p, const Span& s, int i) {
+  if (!p.window) return 0;
+  const int64_t lo = (int64_t)p.pos[s.start + i] - p.window + 1;
+  return lo < 0 ? 0 : lo > 0x7fffffff ? 0x7fffffff : (int)lo;
+}
+__device__ __forceinline__ uint32_t tree_bits(const Kv4Attn& p, const Span& s, int i, int at) {
+  if (at <= -8 || at >= s.n) return 0;
+  const uint32_t* row = p.bits + (s.start + i) * p.ldb;
+  const int w = at >> 5;
+  const uint64_t lo = w >= 0 && w < p.words ? row[w] : 0, hi = w + 1 < p.words ? row[w + 1] : 0;
+  const uint32_t b = (uint32_t)((lo | (hi << 32)) >> (at & 31)) & 0xffu;
+  return s.n - at < 8 ? b & ((1u << (s.n - at)) - 1) : b;
+}
+// over the wave
+__device__ __forceinline__ int wave_min_i(int v) {
+  v = min(v, dpp_i<kDppXor1>(v));
+  v = min(v, dpp_i<kDppXor2>(v));
+  v = min(v, dpp_i<kDppHalfMirror>(v));
+  v = min(v, dpp_i<kDppRowMirror>(v));
+  return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 
 // the maximum m itself where m times its factor is past what M holds to within 1, else 0
@@ -227,8 +253,8 @@ __device__ __forceinline__ void kv4_store(const Kv4Attn& p, int split, int64_t r
 }
 
 // D: channels; DT: the model's type; NQ: blocks of 16 columns per wave; WKV: waves of a workgroup that share
-// their columns
-template <int D, int DT, int NQ, int WKV>
+// their columns; TREE: new tokens are seen as the bits tell, and not up to the query's own
+template <int D, int DT, int NQ, int WKV, bool TREE>
 __global__ void __launch_bounds__(256, D == 256 || (NQ == 2 && D == 128) ? 2 : 3)
 kv4_attn_kernel(const Kv4Attn p) {
   static_assert(WKV == 1 || (WKV == 4 && NQ == 1), "side by side, or one block of columns");
@@ -240,7 +266,7 @@ kv4_attn_kernel(const Kv4Attn p) {
   const int g = lane >> 4, col = lane & 15;
   const int h = blockIdx.y, b = blockIdx.z;
   const int split = blockIdx.x % p.splits;
-  const Span sp = kv4_span(p, b);
+  const Span sp = kv4_span<TREE>(p, b);
   const Table table = (Table)(uintptr_t)(p.s.table + b * p.s.ldt);
   __shared__ float red_o[WKV == 1 ? 1 : 4 * 16 * D];
   __shared__ float red_ml[WKV == 1 ? 1 : 4 * 16 * 2];
@@ -250,7 +276,28 @@ kv4_attn_kernel(const Kv4Attn p) {
   for (int qi = blockIdx.x / p.splits; qi < qtiles; qi += gq) {
     // the last columns have the most keys: first
     const int c0 = (qtiles - 1 - qi) * kCols + (WKV == 1 ? wave * 16 * NQ : 0);
-    const Keys ks = kv4_keys(p, sp, c0, min(c0 + 16 * NQ, sp.cols));
+    Keys ks = kv4_keys(p, sp, c0, min(c0 + 16 * NQ, sp.cols));
+    // this lane's queries: columns 16 j + col
+    const int i0 = c0 / p.G, r0 = c0 - i0 * p.G;
+    int tree_lo[NQ];
+    if constexpr (TREE) {
+      // the cached keys come before the new ones; which of those a query sees, its bits tell
+      const int first = min(max(sp.first_pos, 0), sp.len);
+      int lo = first, lo_all = 0;
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        int head;
+        const int i = kv4_query(p, i0, r0, 16 * j + col, head);
+        const bool on = c0 + 16 * j + col < sp.cols;
+        tree_lo[j] = on ? tree_from(p, sp, i) : first;
+        lo = min(lo, tree_lo[j]);
+        lo_all = max(lo_all, on ? tree_lo[j] : 0);
+      }
+      ks.lo = wave_min_i(lo);
+      ks.lo_all = -wave_min_i(-lo_all);
+      ks.hi = c0 < sp.cols ? sp.len : ks.lo;
+      ks.hi_all = first;
+    }
     const int t_first = ks.lo >> 5, nt = ks.lo < ks.hi ? ((ks.hi + 31) >> 5) - t_first : 0;
     auto token = [&](int t) { return (t_first + t) * 32; };
     // Each part of the next tile is loaded into the registers of this one's as soon as they are free.
@@ -274,8 +321,6 @@ kv4_attn_kernel(const Kv4Attn p) {
     if (t < nt) first = look_up(p, table, token(t), ks.hi);
     if (tn < nt) nat = look_up(p, table, token(tn), ks.hi);
 
-    // this lane's queries: columns 16 j + col
-    const int i0 = c0 / p.G, r0 = c0 - i0 * p.G;
     uint4 qr[NQ][KS];
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
@@ -380,12 +425,20 @@ kv4_attn_kernel(const Kv4Attn p) {
         // is NaN in the score of whoever sees it, and 0 here.
         const bool ha = at.has_a, hb = at.has_b, missing = !(g < 2 ? ha : hb);
         int klo[NQ], khi[NQ];  // the column's keys, from this lane's first token
+        uint32_t tree[NQ];
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
           int head;
           const int i = kv4_query(p, i0, r0, 16 * j + col, head);
-          khi[j] = (c0 + 16 * j + col < sp.cols ? seen_upto(p, sp, i) : 0) - (t0 + 8 * g);
-          klo[j] = seen_from(p, sp, i) - (t0 + 8 * g);
+          const bool on = c0 + 16 * j + col < sp.cols;
+          if constexpr (TREE) {
+            klo[j] = tree_lo[j] - (t0 + 8 * g);
+            khi[j] = (on ? ks.hi_all : 0) - (t0 + 8 * g);
+            tree[j] = on ? tree_bits(p, sp, i, t0 + 8 * g - sp.first_pos) : 0;
+          } else {
+            khi[j] = (on ? seen_upto(p, sp, i) : 0) - (t0 + 8 * g);
+            klo[j] = seen_from(p, sp, i) - (t0 + 8 * g);
+          }
           ts[j] = 0.f;
         }
 #pragma unroll
@@ -395,7 +448,7 @@ kv4_attn_kernel(const Kv4Attn p) {
           mv[i] = bad ? 0.f : mv[i];
 #pragma unroll
           for (int j = 0; j < NQ; ++j) {
-            const bool see = i >= klo[j] && i < khi[j];
+            const bool see = (i >= klo[j] && i < khi[j]) || (TREE && (tree[j] >> i & 1));
             y[j][i] = see ? (bad ? __builtin_nanf("") : y[j][i]) : -kInf;
             ts[j] = see ? fmaxf(ts[j], sv[i]) : ts[j];
           }
@@ -632,26 +685,30 @@ int64_t kv4_workspace(int64_t T, int Hq, int D, int splits) {
   return splits <= 1 ? 0 : (int64_t)splits * T * Hq * (D + 2) * 4;
 }
 
-template <int D, int DT>
+template <int D, int DT, bool TREE>
 static int launch_dt(Kv4Attn& p, const Kv4Plan& pl, hipStream_t st) {
   const int64_t rows = p.s.T * p.c.H * p.G;
   if (pl.qgrid * pl.splits > kMaxGrid || (pl.splits > 1 && rows / 4 >= kMaxGrid)) return kErrUnsupported;
   const dim3 g((unsigned)(pl.qgrid * pl.splits), (unsigned)p.c.H, (unsigned)p.s.B), b(256);
-  if (pl.few) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 4>), g, b, 0, st, p);
-  else if (pl.nq == 1) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 1>), g, b, 0, st, p);
-  else hipLaunchKernelGGL((kv4_attn_kernel<D, DT, D == 256 ? 1 : 2, 1>), g, b, 0, st, p);
+  if (pl.few) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 4, TREE>), g, b, 0, st, p);
+  else if (pl.nq == 1) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 1, TREE>), g, b, 0, st, p);
+  else hipLaunchKernelGGL((kv4_attn_kernel<D, DT, D == 256 ? 1 : 2, 1, TREE>), g, b, 0, st, p);
   if (hipPeekAtLastError() != hipSuccess) return kErrHip;
   if (pl.splits > 1) hipLaunchKernelGGL((kv4_join_kernel<D, DT>), dim3((unsigned)((rows + 3) / 4)), b, 0, st, p);
   return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
+}
+
+template <int DT, bool TREE>
+static int launch_d(Kv4Attn& p, int D, const Kv4Plan& pl, hipStream_t st) {
+  return D == 64 ? launch_dt<64, DT, TREE>(p, pl, st) : D == 128 ? launch_dt<128, DT, TREE>(p, pl, st) : launch_dt<256, DT, TREE>(p, pl, st);
 }
 
 int launch_kv4_attention(Kv4Attn& p, int D, int dtype, const Kv4Plan& pl, void* ws, hipStream_t st) {
   p.splits = pl.splits;
   p.po = reinterpret_cast<float*>(ws);
   p.pml = p.po + (int64_t)pl.splits * p.s.T * p.c.H * p.G * D;
-  if (dtype == kBF16)
-    return D == 64 ? launch_dt<64, kBF16>(p, pl, st) : D == 128 ? launch_dt<128, kBF16>(p, pl, st) : launch_dt<256, kBF16>(p, pl, st);
-  return D == 64 ? launch_dt<64, kF16>(p, pl, st) : D == 128 ? launch_dt<128, kF16>(p, pl, st) : launch_dt<256, kF16>(p, pl, st);
+  if (dtype == kBF16) return p.bits ? launch_d<kBF16, true>(p, D, pl, st) : launch_d<kBF16, false>(p, D, pl, st);
+  return p.bits ? launch_d<kF16, true>(p, D, pl, st) : launch_d<kF16, false>(p, D, pl, st);
 }
 
 }  // namespace w4a8

@@ -11,10 +11,17 @@ Sequences are described as attention backends describe a ragged batch: ``page_ta
 device: a captured call replays with new ones. Decode passes one row per sequence, ``cu_q`` 0, 1, 2, ...
 A padded sequence has length 0 (its rows are 0 in the output) or no rows.
 
+Drafted tokens (speculative decoding) are appended like any others; ``kv4_tree`` turns their parents into what
+``kv4_attention(tree=)`` masks by, and ``kv4_keep`` puts the accepted ones behind the context. A sequence is forked by
+sharing its full pages and copying the last one (``kv4_copy_pages``); freeing a page takes nothing.
+
 Every function runs on the current stream of its tensors' device and allocates with torch; nothing
 synchronises.
 """
 from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Sequence
 
 import torch
 
@@ -23,6 +30,7 @@ from .._hip_engage import engaged
 
 _DTYPES = (torch.bfloat16, torch.float16)
 _HEAD_DIMS = (64, 128, 256)
+_TREE_WORDS = 128
 
 
 class KV4Cache:
@@ -108,6 +116,13 @@ def _batch(cache: KV4Cache, page_table: torch.Tensor, cu_q: torch.Tensor, seq_le
     return page_table.data_ptr(), ldt, width, cu_q.data_ptr(), seq_lens.data_ptr(), B
 
 
+def _tensors(caches) -> tuple:
+    """The caches' tensors as the host path takes them, four of each."""
+    if isinstance(caches, KV4Cache):
+        return caches.k, caches.v, caches.k_scale, caches.v_scale
+    return tuple(t for c in caches for t in (c.k, c.v, c.k_scale, c.v_scale))
+
+
 def _rows_ok(t: torch.Tensor) -> bool:
     return t.stride(2) == 1 and all(t.shape[i] <= 1 or t.stride(i) % 8 == 0 for i in (0, 1)) and t.data_ptr() % 16 == 0
 
@@ -172,6 +187,129 @@ def kv4_read(cache: KV4Cache, page_table: torch.Tensor, cu_q: torch.Tensor, seq_
     return k, v
 
 
+class KV4Tree(NamedTuple):
+    """What the new tokens of a call see of each other: ``mask`` (T, words) int32, bit j % 32 of word j / 32 for the
+    sequence's new token j, and ``positions`` (T,) int32, as rotary embeddings and windows count them. ``kv4_tree`` makes
+    it from parents; any other bits may stand there."""
+
+    mask: torch.Tensor
+    positions: torch.Tensor
+
+
+def kv4_tree(parents: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor, *, max_q: int, window: int = 0) -> KV4Tree:
+    """The tree of drafted tokens whose parents these are: (T,) int32, each the index among its sequence's new tokens of
+    the one that it follows, or -1 for the context's last token; a parent stands before its children, and what does not
+    is taken as -1. A token sees its ancestors and itself, window > 0: the last ``window`` of them.
+
+    max_q: the most new tokens of a sequence, up to 4096; a token from there on is seen by none. Rows outside cu_q are not
+    written. One launch."""
+    what = "kv4_tree"
+    r = _host.load().kv4_tree(parents, cu_q, seq_lens, max_q, window)
+    if r is not None:
+        engaged("w4a8_mi355x.kv4_tree")
+        return KV4Tree(*r)
+    for name, t in (("parents", parents), ("cu_q", cu_q), ("seq_lens", seq_lens)):
+        if t.dtype != torch.int32 or t.dim() != 1:
+            raise TypeError(f"{what}: {name} must be a 1-D int32 tensor, got {t.dtype} {tuple(t.shape)}")
+        if not t.is_cuda or t.device != parents.device:
+            raise RuntimeError(f"{what}: parents, cu_q and seq_lens must be on one GPU, got {name} on {t.device}")
+    B, T = seq_lens.shape[0], parents.shape[0]
+    if cu_q.shape[0] != B + 1:
+        raise ValueError(f"{what}: for {B} sequences cu_q must have {B + 1} entries, got {tuple(cu_q.shape)}")
+    if not 1 <= max_q <= 32 * _TREE_WORDS or window < 0:
+        raise ValueError(f"{what}: max_q={max_q} (1 to {32 * _TREE_WORDS}), window={window}")
+    parents, cu_q, seq_lens = (t.contiguous() for t in (parents, cu_q, seq_lens))
+    words = (int(max_q) + 31) // 32
+    mask = torch.empty((T, words), dtype=torch.int32, device=parents.device)
+    pos = torch.empty((T,), dtype=torch.int32, device=parents.device)
+    with torch.cuda.device(parents.device):
+        _abi.check(_abi.load().w4a8_kv4_tree(parents.data_ptr(), T, cu_q.data_ptr(), seq_lens.data_ptr(), B, words, int(window),
+                                             mask.data_ptr(), pos.data_ptr(), _abi.stream_of(parents)), what)
+    engaged("w4a8_mi355x.kv4_tree")
+    return KV4Tree(mask, pos)
+
+
+def _layers(caches: KV4Cache | Sequence[KV4Cache], what: str) -> Sequence[KV4Cache]:
+    caches = (caches,) if isinstance(caches, KV4Cache) else tuple(caches)
+    if not caches:
+        raise ValueError(f"{what}: no cache")
+    c = caches[0]
+    if c.device.type != "cuda":
+        raise RuntimeError(f"{what}: the cache must be on the GPU")
+    for o in caches[1:]:
+        if (o.k.shape, o.dtype, o.device) != (c.k.shape, c.dtype, c.device):
+            raise ValueError(f"{what}: the caches must be alike, got {tuple(c.k.shape)} {c.dtype} on {c.device} and "
+                             f"{tuple(o.k.shape)} {o.dtype} on {o.device}")
+    if len({o.k.data_ptr() for o in caches}) != len(caches):
+        raise ValueError(f"{what}: a cache is given twice")
+    return caches
+
+
+def _arrays(caches: Sequence[KV4Cache]):
+    return (ctypes.c_void_p * (4 * len(caches)))(*(p for c in caches for p in c._ptrs()))
+
+
+def kv4_copy_pages(caches: KV4Cache | Sequence[KV4Cache], src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Copy page src[i] to page dst[i] in each of the caches (layers of one shape), src and dst (n,) int32 on the device:
+    the partial last page of a sequence that is forked, or pages that move to make a cache compact. One launch per 64 caches.
+
+    The destinations are distinct and none of them is another pair's source: such a page would hold parts of either. A
+    pair with a page that does not exist, or with twice the same, copies nothing."""
+    what = "kv4_copy_pages"
+    if _host.load().kv4_copy_pages(_tensors(caches), src, dst):
+        engaged("w4a8_mi355x.kv4_copy_pages")
+        return
+    caches = _layers(caches, what)
+    c = caches[0]
+    for name, t in (("src", src), ("dst", dst)):
+        if t.dtype != torch.int32 or t.dim() != 1:
+            raise TypeError(f"{what}: {name} must be a 1-D int32 tensor, got {t.dtype} {tuple(t.shape)}")
+        if t.device != c.device:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, the caches on {c.device}")
+    if src.shape != dst.shape:
+        raise ValueError(f"{what}: {src.shape[0]} sources, {dst.shape[0]} destinations")
+    src, dst = src.contiguous(), dst.contiguous()
+    arrays = _arrays(caches)
+    with torch.cuda.device(c.device):
+        _abi.check(_abi.load().w4a8_kv4_copy_pages(
+            ctypes.addressof(arrays), len(caches), c.num_pages, c.page_size, c.num_kv_heads, c.head_dim, src.data_ptr(),
+            dst.data_ptr(), src.shape[0], _abi.stream_of(src)), what)
+    engaged("w4a8_mi355x.kv4_copy_pages")
+
+
+def kv4_keep(caches: KV4Cache | Sequence[KV4Cache], page_table: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor,
+             keep: torch.Tensor, kept: torch.Tensor) -> torch.Tensor:
+    """Put the accepted ones of the new tokens behind the context, in each of the caches (layers of one shape), and return
+    the sequences' lengths with them alone, (B,) int32. ``keep`` (B, width) int32: of sequence b's new tokens, in ascending
+    order, the indices of its ``kept[b]`` accepted ones ((B,) int32, between 0 and what is there). page_table, cu_q and
+    seq_lens are those that the tokens were appended with.
+
+    An entry below its own place, or not of a new token, leaves its slot as it is. Slots behind the new length keep what
+    they hold, and the next tokens are appended over them. One launch per 64 caches."""
+    what = "kv4_keep"
+    r = _host.load().kv4_keep(_tensors(caches), page_table, cu_q, seq_lens, keep, kept)
+    if r is not None:
+        engaged("w4a8_mi355x.kv4_keep")
+        return r
+    caches = _layers(caches, what)
+    c = caches[0]
+    table, ldt, width, cu, lens, B = _batch(c, page_table, cu_q, seq_lens, what)
+    for name, t, dim in (("keep", keep, 2), ("kept", kept, 1)):
+        if t.dtype != torch.int32 or t.dim() != dim or t.shape[0] != B:
+            raise TypeError(f"{what}: {name} must be a {dim}-D int32 tensor of {B} rows, got {t.dtype} {tuple(t.shape)}")
+        if t.device != c.device:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, the caches on {c.device}")
+    keep, kept = keep.contiguous(), kept.contiguous()
+    now = torch.empty((B,), dtype=torch.int32, device=c.device)
+    arrays = _arrays(caches)
+    with torch.cuda.device(c.device):
+        _abi.check(_abi.load().w4a8_kv4_keep(
+            ctypes.addressof(arrays), len(caches), c.num_pages, c.page_size, c.num_kv_heads, c.head_dim, table, ldt, width, cu,
+            lens, B, keep.data_ptr(), keep.shape[1], keep.shape[1], kept.data_ptr(), now.data_ptr(), _abi.stream_of(now)), what)
+    engaged("w4a8_mi355x.kv4_keep")
+    return now
+
+
 def kv4_attention(
     q: torch.Tensor,  # (T, num_qo_heads, head_dim), any strides between rows
     cache: KV4Cache,
@@ -186,6 +324,7 @@ def kv4_attention(
     window: int = 0,
     out: torch.Tensor | None = None,
     return_lse: bool = False,
+    tree: KV4Tree | None = None,
 ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """Attention of the new tokens over their sequences' cached keys and values (the new tokens' own
     among them: append first). (T, num_qo_heads, head_dim) in q's type; with return_lse also the natural
@@ -198,6 +337,10 @@ def kv4_attention(
     hold there, and are undefined in a fresh output. Rows of out that overlap are refused, and so is an out that
     overlaps q without being q.
 
+    tree: the new tokens are drafted ones; a token sees the cached context before them and, of them, those that its
+    row of ``tree.mask`` names (``causal`` says nothing then). window > 0 counts from ``tree.positions``, among cached
+    tokens: of the new ones the mask alone decides.
+
     max_q and max_kv, the most new tokens and the greatest length of a sequence, are what the host
     plans the launch by (default: T rows, and the table's capacity). Too large a bound costs time, too
     low a one as well; neither changes which keys are read. One launch, and a second that joins the
@@ -205,8 +348,12 @@ def kv4_attention(
     what = "kv4_attention"
     if sm_scale is None:
         sm_scale = cache.head_dim ** -0.5
-    r = _host.load().kv4_attention(cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, cu_q, seq_lens, q, max_q,
-                                   max_kv, sm_scale, causal, window, out, return_lse)
+    if tree is None:
+        r = _host.load().kv4_attention(cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, cu_q, seq_lens, q, max_q,
+                                       max_kv, sm_scale, causal, window, out, return_lse)
+    else:
+        r = _host.load().kv4_tree_attention(cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, cu_q, seq_lens, q,
+                                            max_q, max_kv, sm_scale, window, out, return_lse, tree.mask, tree.positions)
     if r is not None:
         engaged("w4a8_mi355x.kv4_attention")
         return r if return_lse else r[0]
@@ -217,6 +364,16 @@ def kv4_attention(
     table, ldt, width, cu, lens, B = _batch(cache, page_table, cu_q, seq_lens, what)
     if window < 0:
         raise ValueError(f"{what}: window={window}")
+    mask = None
+    if tree is not None:
+        mask, pos = tree
+        if mask.dtype != torch.int32 or mask.dim() != 2 or mask.shape[0] != T or not 1 <= mask.shape[1] <= _TREE_WORDS \
+                or pos.dtype != torch.int32 or tuple(pos.shape) != (T,):
+            raise TypeError(f"{what}: tree must be ({T}, 1 to {_TREE_WORDS}) int32 words and ({T},) int32 positions, got "
+                            f"{mask.dtype} {tuple(mask.shape)} and {pos.dtype} {tuple(pos.shape)}")
+        if mask.device != cache.device or pos.device != cache.device:
+            raise RuntimeError(f"{what}: tree is on {mask.device} and {pos.device}, the cache on {cache.device}")
+        mask, pos = mask.contiguous(), pos.contiguous()
     cap = width * cache.page_size
     max_q = T if max_q is None else min(int(max_q), T)
     max_kv = cap if max_kv is None else min(int(max_kv), cap)
@@ -233,12 +390,15 @@ def kv4_attention(
     lib = _abi.load()
     ws_bytes = int(lib.w4a8_kv4_attention_workspace_bytes(T, Hq, cache.num_kv_heads, D, B, max_q, max_kv))
     ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes > 0 else None
+    before = (q.data_ptr(), _abi.dtype_code(q.dtype), q.stride(0), q.stride(1), T, Hq, cache.num_kv_heads, D, *cache._ptrs(),
+              cache.num_pages, cache.page_size, table, ldt, width, cu, lens, B, float(sm_scale))
+    after = (out.data_ptr(), out.stride(0), out.stride(1), _abi.ptr(lse), _abi.ptr(ws), max(ws_bytes, 0), _abi.stream_of(q))
     with torch.cuda.device(cache.device):
-        _abi.check(lib.w4a8_kv4_attention(
-            q.data_ptr(), _abi.dtype_code(q.dtype), q.stride(0), q.stride(1), T, Hq, cache.num_kv_heads, D, *cache._ptrs(),
-            cache.num_pages, cache.page_size, table, ldt, width, cu, lens, B,
-            float(sm_scale), int(bool(causal)), int(window), max_q, max_kv,
-            out.data_ptr(), out.stride(0), out.stride(1), _abi.ptr(lse), _abi.ptr(ws), max(ws_bytes, 0),
-            _abi.stream_of(q)), what)
+        if mask is None:
+            rc = lib.w4a8_kv4_attention(*before, int(bool(causal)), int(window), max_q, max_kv, *after)
+        else:
+            rc = lib.w4a8_kv4_tree_attention(*before, int(window), max_q, max_kv, mask.data_ptr(), mask.shape[1], mask.shape[1],
+                                             pos.data_ptr(), *after)
+        _abi.check(rc, what)
     engaged("w4a8_mi355x.kv4_attention")
     return (out, lse) if return_lse else out

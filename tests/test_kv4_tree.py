@@ -1,0 +1,294 @@
+"""Trees of drafted tokens over the 4-bit cache (quant/kv4.py kv4_tree, kv4_attention(tree=)): refusals on the CPU, and on
+the GPU bits and positions against a walk up the tree, and attention against 64 bits over the cached values, with the
+tolerances that attention over the cache is tested with."""
+import math
+import random
+
+import pytest
+import torch
+
+from conftest import pkg
+from test_kv4 import Setup, cache_values
+
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+def _kv4():
+    return pkg("quant.kv4")
+
+
+def lines(parents):
+    """Each node's ancestors and itself, the root first."""
+    out = []
+    for i, p in enumerate(parents):
+        out.append((out[p] if 0 <= p < i else []) + [i])
+    return out
+
+
+def random_tree(n, rng, near=6):
+    return [-1 if i == 0 or rng.random() < 0.15 else rng.randrange(max(0, i - near), i) for i in range(n)]
+
+
+def pack(see, words):
+    """(rows, words) int32 of lists of seen tokens."""
+    out = []
+    for s in see:
+        bits = sum(1 << j for j in s if j < 32 * words)
+        part = [(bits >> (32 * w)) & 0xffffffff for w in range(words)]
+        out.append([w - (1 << 32) if w >> 31 else w for w in part])
+    return torch.tensor(out, dtype=torch.int32).view(len(see), words)
+
+
+def ref(q, kv, table, page, lens, news, see, positions, scale, window=0):
+    """see: per row the new tokens that it sees. out and lse in f64, NaN where a page is missing."""
+    k, v = kv
+    H = k.shape[1]
+    T, Hq, D = q.shape
+    G = Hq // H
+    out = torch.zeros(T, Hq, D, dtype=torch.float64)
+    lse = torch.full((T, Hq), -math.inf, dtype=torch.float64)
+    row = 0
+    for b, (n, new) in enumerate(zip(lens, news)):
+        for i in range(new):
+            r = row + i
+            lo = max(0, positions[r] - window + 1) if window else 0
+            keys = list(range(lo, max(n - new, 0))) + [n - new + j for j in see[r] if j < new and n - new + j >= 0]
+            if not keys:
+                continue
+            pos = torch.tensor(keys)
+            missing = pos // page >= table.shape[1]
+            pages = table[b, (pos // page).clamp_max(table.shape[1] - 1)].long()
+            missing |= (pages < 0) | (pages >= k.shape[0])
+            if missing.any():
+                out[r], lse[r] = math.nan, math.nan
+                continue
+            kk = k[pages, :, pos % page].repeat_interleave(G, 1).transpose(0, 1)  # (Hq, keys, D)
+            vv = v[pages, :, pos % page].repeat_interleave(G, 1).transpose(0, 1)
+            x = (kk * q[r].double().unsqueeze(1)).sum(-1) * scale
+            out[r] = (torch.softmax(x, 1).unsqueeze(-1) * vv).sum(1)
+            lse[r] = torch.logsumexp(x, 1)
+        row += new
+    return out, lse
+
+
+def check(s, q, tree, see, window=0, lse_of_nan=True, **kw):
+    out, lse = s.attend(q, tree=tree, window=window, return_lse=True, **kw)
+    D = s.cache.head_dim
+    scale = kw.get("sm_scale", D ** -0.5)
+    want, rl = ref(q, cache_values(s.cache), s.table, s.page, s.lens, s.news, see, tree.positions.tolist(), scale, window)
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(out.cpu()), nan)
+    eps = 2.0 ** (-8 if q.dtype == torch.bfloat16 else -11)
+    vmax = s.v.float().abs().max().item()
+    err = (out.cpu().double() - want).abs() - eps * want.abs() - (3.5e-4 if q.dtype == torch.bfloat16 else 2e-4) * vmax - 2.0 ** -25
+    assert err[~nan].numel() == 0 or err[~nan].max().item() <= 0, f"off by {err[~nan].max().item():.3e} past the tolerance"
+    lf = torch.isfinite(rl)
+    if not lse_of_nan:  # a row that sees a value that is NaN: its lse is not specified
+        lf &= ~nan.any(-1)
+    assert torch.equal(torch.isfinite(lse.cpu()) & lf, lf) and (not lse_of_nan or torch.equal(torch.isfinite(lse.cpu()), lf))
+    most = 2 * s.k.double().abs().max().item() * q.double().abs().sum(-1).max().item() * scale
+    assert not lf.any() or (lse.cpu().double() - rl)[lf].abs().max().item() < 2e-4 + 2.0 ** -21 * most
+    return out
+
+
+# ------------------------------------------------------------------------------------------------
+# CPU
+# ------------------------------------------------------------------------------------------------
+def test_refusals():
+    kv4 = _kv4()
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(RuntimeError, match="one GPU"):
+        kv4.kv4_tree(i32(-1, 0), i32(0, 2), i32(5), max_q=2)
+    with pytest.raises(TypeError, match="parents"):
+        kv4.kv4_tree(i32(-1, 0).long(), i32(0, 2), i32(5), max_q=2)
+    c = kv4.KV4Cache(4, 32, 2, 128, device="cpu")
+    x = torch.zeros(2, 2, 128, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        kv4.kv4_attention(x, c, i32([0]).view(1, 1), i32(0, 2), i32(5), tree=kv4.KV4Tree(i32([1], [3]), i32(3, 4)))
+
+
+def test_abi_refusals():
+    if torch.cuda.is_available():
+        pytest.skip("the pointers are not real")
+    lib = pkg("_abi").load()
+    P = 1 << 20
+    for a, code in (((P, 4, P, P, 1, 0, 0, P, P), 1), ((P, 4, P, P, 1, 129, 0, P, P), 1), ((P, 4, P, P, 1, 1, -1, P, P), 1),
+                    ((P, -1, P, P, 1, 1, 0, P, P), 1), ((None, 4, P, P, 1, 1, 0, P, P), 1), ((P, 4, P, P, 1, 1, 0, P, None), 1),
+                    ((P, 1 << 31, P, P, 1, 1, 0, P, P), 2), ((P, 0, P, P, 1, 1, 0, P, P), 0), ((P, 4, P, P, 0, 1, 0, P, P), 0)):
+        assert lib.w4a8_kv4_tree(*a, None) == code, a
+
+    def attend(bits=P, ldb=1, words=1, pos=P, window=0, width=4, T=2):
+        rc = lib.w4a8_kv4_tree_attention(P, 0, 512, 128, T, 4, 1, 128, P, P, P, P, 16, 16, P, width, width, P, P, 1, 1.0, window, 2, 64, bits,
+                                         ldb, words, pos, P, 256, 64, None, None, 0, None)
+        return rc, lib.w4a8_last_error().decode()
+
+    for kw in (dict(bits=None), dict(words=0), dict(words=129, ldb=129), dict(ldb=1, words=2), dict(window=4, pos=None)):
+        rc, msg = attend(**kw)
+        assert rc == 1 and "bits" in msg, (kw, rc, msg)
+    rc, msg = attend(width=(1 << 27) - 4)
+    assert rc == 2 and "index ranges" in msg
+    assert attend()[1].startswith("w4a8_kv4_tree_attention: out's rows overlap")
+
+
+# ------------------------------------------------------------------------------------------------
+# GPU
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [0, 1, 3])
+def test_bits_and_positions(dev, window):
+    rng = random.Random(window)
+    news = [1, 0, 33, 64, 5, 150, 700]
+    trees = [random_tree(n, rng) for n in news]
+    trees[3] = list(range(-1, 63))   # a chain
+    trees[4] = [3, -7, 2, 0, 4]      # entries that do not stand before their node
+    lens = [n + rng.randrange(0, 50) for n in news]
+    cu = [3 + sum(news[:i]) for i in range(len(news) + 1)]
+    parents = torch.full((cu[-1] + 4,), 77, dtype=torch.int32)
+    parents[3:cu[-1]] = torch.tensor([p for t in trees for p in t], dtype=torch.int32)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=dev)  # noqa: E731
+    for max_q in (700, 1024, 90):
+        tree = _kv4().kv4_tree(parents.to(dev), i32(cu), i32(lens), max_q=max_q, window=window)
+        assert tree.mask.shape == (len(parents), -(-max_q // 32))
+        at = 3
+        for t, n in zip(trees, lens):
+            line = lines(t)
+            see = [x[-window:] if window else x for x in line]
+            assert torch.equal(tree.mask[at:at + len(t)].cpu(), pack(see, tree.mask.shape[1]))
+            assert tree.positions[at:at + len(t)].tolist() == [n - len(t) + len(x) - 1 for x in line]
+            at += len(t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,H,G,page", [(128, 2, 4, 16), (64, 1, 3, 32), (256, 1, 2, 16), (128, 1, 8, 64), (64, 2, 1, 16)])
+@pytest.mark.parametrize("lens,news", [([40, 9, 200], [7, 9, 3]), ([500, 0, 1, 90], [33, 0, 1, 70]), ([1100], [13]), ([2000, 77], [64, 2])])
+def test_trees(dev, dtype, D, H, G, page, lens, news):
+    s = Setup(dev, dtype, D, H, page, lens, news, seed=D + G)
+    q = s.q(H * G, scale=1.5)
+    rng = random.Random(sum(news))
+    trees = [random_tree(n, rng) for n in news]
+    parents = torch.tensor([p for t in trees for p in t], dtype=torch.int32, device=dev)
+    for window, kw in ((0, dict(max_q=max(news), max_kv=max(lens))), (5, {}), (64, dict(max_q=max(news))), (0, dict(max_q=1, sm_scale=0.3))):
+        tree = _kv4().kv4_tree(parents, s.d_cu, s.d_seq, max_q=max(news), window=window)
+        see = [x[-window:] if window else x for t in trees for x in lines(t)]
+        check(s, q, tree, see, window, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_chain_is_causal_attention(dev, dtype):
+    """The same bits, where every drafted token follows the one before it."""
+    for D, G, lens, news in ((128, 4, [300, 40, 9000], [20, 40, 4]), (64, 3, [64, 100], [1, 3])):
+        s = Setup(dev, dtype, D, 2, 16, lens, news, seed=1)
+        q = s.q(2 * G)
+        parents = torch.tensor([i - 1 for n in news for i in range(n)], dtype=torch.int32, device=dev)
+        for window in (0, 17):
+            tree = _kv4().kv4_tree(parents, s.d_cu, s.d_seq, max_q=max(news), window=window)
+            for kw in ({}, dict(max_q=max(news), max_kv=max(lens))):
+                a, al = s.attend(q, tree=tree, window=window, return_lse=True, **kw)
+                b, bl = s.attend(q, window=window, return_lse=True, **kw)
+                assert torch.equal(a, b) and torch.equal(al, bl)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("news", [[3, 2], [40, 100]])
+def test_any_mask(dev, dtype, news):
+    """Rows that see nothing, everything, only others, bits past the tokens, and too few words."""
+    lens = [60, 100]
+    s = Setup(dev, dtype, 64, 2, 16, lens, news, seed=4)
+    q = s.q(4)
+    T = sum(news)
+    rng = random.Random(5)
+    see = [sorted(rng.sample(range(n), rng.randrange(0, n + 1))) for n in news for _ in range(n)]
+    see[0], see[1] = [], list(range(news[0]))
+    positions = [n - w + rng.randrange(0, w) for n, w in zip(lens, news) for _ in range(w)]
+    for words in (1, 4, 7):
+        mask = pack(see, words)
+        if words > 4:
+            mask[:, -1] = -1  # tokens 192 .. 223: there are none
+        seen = [[j for j in x if j < 32 * words] for x in see]
+        tree = _kv4().KV4Tree(mask.to(dev), torch.tensor(positions, dtype=torch.int32, device=dev))
+        for window in (0, 30, 1):
+            check(s, q, tree, seen, window)
+    # no context at all: what sees nothing is 0
+    s = Setup(dev, dtype, 64, 2, 16, news, news, seed=4)
+    tree = _kv4().KV4Tree(pack(see, 4).to(dev), torch.zeros(T, dtype=torch.int32, device=dev))
+    out = check(s, q, tree, see)
+    assert not out[0].any()
+    # a window from a position far behind: none of the context
+    tree = _kv4().KV4Tree(pack(see, 4).to(dev), torch.full((T,), 2 ** 31 - 1, dtype=torch.int32, device=dev))
+    check(s, q, tree, see, 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("news", [[5, 3], [64, 40]])
+def test_missing_pages_and_unseen_values(dev, dtype, news):
+    """Tokens on pages that do not exist, or past the table: NaN in who sees them and in nobody else; so are tokens whose
+    vectors are not finite."""
+    lens = [70, 90]
+    s = Setup(dev, dtype, 128, 1, 16, lens, news, seed=2)
+    q = s.q(4)
+    rng = random.Random(1)
+    trees = [random_tree(n, rng) for n in news]
+    see = [x for t in trees for x in lines(t)]
+    parents = torch.tensor([p for t in trees for p in t], dtype=torch.int32, device=dev)
+    tree = _kv4().kv4_tree(parents, s.d_cu, s.d_seq, max_q=max(news))
+    s.table[0, (lens[0] - 1) // 16] = -1     # the last tokens of the first sequence
+    s.d_table = s.table.to(dev)
+    check(s, q, tree, see)
+    # lengths past the table: the last nodes have no place
+    s.table = s.table[:, :5].contiguous()
+    s.d_table = s.table.to(dev)
+    check(s, q, tree, see)
+    wide = torch.full((2, 5), 2 ** 30, dtype=torch.int32)
+    s.table = wide
+    s.d_table = wide.to(dev)
+    check(s, q, tree, see)
+    # a node that holds NaN
+    s = Setup(dev, dtype, 128, 1, 16, lens, news, seed=2)
+    at = lens[1] - news[1] + 1
+    page, slot = s.table[1, at // 16].item(), at % 16
+    s.cache.v_scale[page, :, slot] = math.nan
+    tree = _kv4().kv4_tree(parents, s.d_cu, s.d_seq, max_q=max(news))
+    out = check(s, q, tree, see, lse_of_nan=False)
+    sees = torch.tensor([r >= news[0] and 1 in see[r] for r in range(sum(news))])
+    assert torch.equal(torch.isnan(out.cpu()).flatten(1).all(1), sees)
+
+
+@pytest.mark.gpu
+def test_out_rows_streams_and_refusals(dev):
+    kv4 = _kv4()
+    s = Setup(dev, torch.bfloat16, 128, 2, 16, [100, 50], [6, 4], seed=3)
+    q = s.q(8)
+    parents = torch.tensor([-1, 0, 0, 1, 1, 2, -1, -1, 0, 1], dtype=torch.int32, device=dev)
+    tree = kv4.kv4_tree(parents, s.d_cu, s.d_seq, max_q=6)
+    want = s.attend(q, tree=tree)
+    pad = torch.cat([torch.zeros_like(q[:2]), q, torch.zeros_like(q[:3])]).to(dev)
+    mask = torch.cat([torch.full((2, 1), -1, dtype=torch.int32, device=dev), tree.mask, torch.full((3, 1), -1, dtype=torch.int32, device=dev)])
+    pos = torch.cat([torch.zeros(2, dtype=torch.int32, device=dev), tree.positions, torch.zeros(3, dtype=torch.int32, device=dev)])
+    out = torch.full_like(pad, 9.0)
+    kv4.kv4_attention(pad, s.cache, s.d_table, s.d_cu + 2, s.d_seq, tree=kv4.KV4Tree(mask, pos), out=out)
+    assert torch.equal(out[2:12], want) and (out[:2] == 9).all() and (out[12:] == 9).all()
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(other):
+        t2 = kv4.kv4_tree(parents, s.d_cu, s.d_seq, max_q=6)
+        got = s.attend(q, tree=t2)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    m, p = tree
+    for bad, e in (((m[:9], p), TypeError), ((m.long(), p), TypeError), ((m, p[:9]), TypeError), ((m.cpu(), p), RuntimeError),
+                   ((m[:, :0], p), TypeError), ((m.expand(10, 1).repeat(1, 129), p), TypeError)):
+        with pytest.raises(e):
+            s.attend(q, tree=kv4.KV4Tree(*bad))
+    strided = m.repeat(1, 3)[:, ::3]
+    assert torch.equal(s.attend(q, tree=kv4.KV4Tree(strided, p)), want)
+    for kw, e in ((dict(max_q=0), ValueError), (dict(max_q=4097), ValueError), (dict(max_q=6, window=-1), ValueError)):
+        with pytest.raises(e):
+            kv4.kv4_tree(parents, s.d_cu, s.d_seq, **kw)
+    with pytest.raises(ValueError, match="cu_q"):
+        kv4.kv4_tree(parents, s.d_cu[:2], s.d_seq, max_q=6)
+    none = kv4.kv4_tree(parents[:0], s.d_cu * 0, s.d_seq, max_q=6)
+    assert none.mask.shape == (0, 1) and none.positions.shape == (0,)
