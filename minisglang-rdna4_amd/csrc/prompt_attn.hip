@@ -2,18 +2,33 @@
 //
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(scale log2(e) q k_j - M),  j over the keys that the row sees.
 //
-// The queries that share a key/value head are columns: column c of a sequence is its query c / G, head h G + c % G, so
-// 256 columns are 256 / G neighbouring queries, which see almost the same keys. A wave has 32 columns; per 32 keys
+// The queries that share a key/value head are columns: column c of a sequence is its query c / G, head h G + c % G, so the
+// 128 columns of a workgroup are 128 / G neighbouring queries, which see almost the same keys. A wave has 32 columns; per
+// 32 keys
 //   S = K Q^T (32x32x16, keys are rows),  P = exp of S,  O += V^T P (channels are rows).
 // A lane's 16 values of S are one column's, and P's operand wants 8 keys of one column in a lane: any 8, as long as V's
 // operand has the same. So P stays in its registers; V's operand comes from LDS by transposed reads.
-// K and V tiles of 64 keys go from memory straight into LDS (LDS-DMA), the next one while this one is worked on. A
-// DMA lane's 16 bytes land side by side; which 16 bytes those are is free. They are put so that 4 rows times 64 bytes
-// lie together, and groups of 4 rows 16 bytes off a multiple of 256: both kinds of read then meet every bank once, at
-// addresses that are one register and a constant.
+// K and V tiles go from memory straight into LDS (LDS-DMA), the next one while this one is worked on. A DMA lane's 16
+// bytes land side by side; which 16 bytes those are is free. They are put so that 4 rows times 64 bytes lie together, and
+// groups of 4 rows 16 bytes off a multiple of 256: both kinds of read then meet every bank once, at addresses that are one
+// register and a constant.
 // The running maximum is raised only when a score passes it by 8 (in powers of two): p stays below 2^8, and most tiles
-// need neither an exchange between lanes nor a rescaling of O. Sums and O are f32; p is rounded to the type for its
-// product (by at most 2^-8 of itself for bf16, 2^-11 for fp16; sum p is of the unrounded ones), as v is.
+// need neither an exchange between lanes nor a rescaling of O. Sums and O are f32. p is rounded to the type for its product
+// (by at most 2^-8 of itself for bf16, 2^-11 for fp16), as v is, and the sum that divides is of the rounded ones: the
+// rounding then weighs values a little differently, and equal values keep their bits.
+//
+// Measured: 8192 + 5690 + 3190 tokens, 32 heads on 8 of 128 channels (898 GFLOP), 1.02 ms, 882 TFLOP/s, bf16; heads of 64
+// 754, of 256 857. Bound by power: the matrix units are busy for half of the cycles at 1.75 GHz, and the same cycles take
+// 0.79 ms at 2.2 GHz where all values are 0; products alone, from registers, reach 1.7 PFLOP/s on such values. No
+// exponentials at all would save 6% of the time, no reads of K from LDS 5%, no copies of K and V into LDS 12%.
+// First version 774: S, exponentials and products one after another, 8 waves a workgroup (two workgroups of 4 waves on a CU
+// do not wait for each other: 23 prompts of up to 1999 tokens, heads of 64, 281 -> 234 us). Other steps: blocks of 32 keys
+// whose S is computed while the block before passes through its exponentials (1161 -> 1055 us, heads of 64 762 -> 653), what
+// is not finite dealt with before the products and not beside them, whose outputs then stay in their registers (-> 1016, 193
+// us). Tried: tiles of 32 keys for all (three waves per SIMD spill, two are no faster, heads of 64 slower: 660 TFLOP/s); 64
+// columns a wave (heads of 64 the same; of 128 take the registers of a SIMD, and half the time goes into moving them).
+#include <type_traits>
+
 #include "prompt_attn.h"
 
 namespace w4a8 {
@@ -28,7 +43,6 @@ typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef short v4s __attribute__((__vector_size__(8)));
 
-constexpr int kTile = 64;  // keys
 
 template <int DT>
 __device__ __forceinline__ v16f mfma32(const v4w& a, const v4w& b, const v16f& c) {
@@ -42,6 +56,19 @@ template <int DT>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
   if constexpr (DT == kBF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2b));
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2h));
+}
+
+// both halves of a packed pair onto an f32 sum
+template <int DT>
+__device__ __forceinline__ float add_pair(uint32_t w, float c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  if constexpr (DT == kBF16)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, w), __builtin_bit_cast(v2b, 0x3f803f80u), c, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), __builtin_bit_cast(v2h, 0x3c003c00u), c, false);
+#else
+  return c;
+#endif
 }
 
 // over the two lanes that hold a column (xor 32)
@@ -62,6 +89,8 @@ __device__ __forceinline__ float far_off(float m, float sc) {
 // Where the 16 bytes `chunk` (8 channels) of row `r` lie in a tile of D channels, for the DMA and both kinds of read
 template <int D>
 struct Place {
+  // keys. 256 channels: 8 waves share a tile (copies into LDS weigh most there: 4 waves 517 TFLOP/s, 8 waves 768)
+  static constexpr int kTile = D == 256 ? 32 : 64;
   // rows of 64 channels come 8 to a DMA; the second 4 of them swap neighbouring chunks
   static constexpr int kGroup = D == 64 ? 1024 + 32 : 8 * D + 16;  // bytes from one group of rows to the next
   static constexpr int kRows = D == 64 ? 8 : 4;                    // rows of a group
@@ -97,13 +126,18 @@ __device__ __forceinline__ v2w lds_read_tr(const unsigned char* p) {
 
 // D: channels; DT: the type; NW: waves
 template <int D, int DT, int NW>
-__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2)
+__global__ void __launch_bounds__(64 * NW, D == 64 ? 3 : 2)
 prompt_attn_kernel(const PromptAttn p) {
   using P = Place<D>;
+  constexpr int kTile = P::kTile;
   constexpr int KS = D / 16, CT = D / 32;       // steps of S, tiles of 32 channels
   constexpr int kDma = P::kDmas / NW;           // DMAs of a wave and tile
-  static_assert(P::kDmas % NW == 0, "every wave has the same");
+  static_assert(P::kDmas % NW == 0 && (D < 256 || kDma % 2 == 0), "every wave has the same, of whole rows");
   constexpr int kCols = 32 * NW;
+  // Whether S of the next 32 keys is computed while these pass through their exponentials. Heads of 256 channels have no
+  // registers for it, and twice the products per exponential.
+  constexpr bool kAhead = D < 256;
+  constexpr int kLead = kAhead ? 32 : 0;
   constexpr float kInf = __builtin_inff();
   constexpr uint32_t kExp = DT == kBF16 ? 0x7f807f80u : 0x7c007c00u;  // exponents of two values
   constexpr uint32_t kOnes = DT == kBF16 ? 0x3f80u : 0x3c00u;
@@ -111,6 +145,7 @@ prompt_attn_kernel(const PromptAttn p) {
   __shared__ __align__(16) unsigned char k1[P::kBytes];
   __shared__ __align__(16) unsigned char v0[P::kBytes];
   __shared__ __align__(16) unsigned char v1[P::kBytes];
+  __shared__ int flags[NW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
   const int h = blockIdx.x % p.H, b = blockIdx.y;
@@ -128,13 +163,20 @@ prompt_attn_kernel(const PromptAttn p) {
   const int i16 = lane & 15;
   const int v_lane = P::at(half * 4 + (i16 >> 2), ((lane >> 4) & 1) * 2 + ((i16 & 3) >> 1)) + (i16 & 1) * 8;
 
-  auto fetch = [&](const uint16_t* base, int64_t ld, int t, unsigned char* dst) {
-    const int rows = min(kTile, n - t * kTile);  // rows past the end are zeros in LDS
-    const BufRsrc r = make_rsrc(base + (int64_t)t * kTile * ld, (uint32_t)(((rows - 1) * (int)ld + D) * 2));
+  // a lane's offset in its wave's first DMA of a tile; the wave's others are of the next rows, or for 256 channels of the
+  // rows' other half
+  const int x0 = wave * kDma;
+  const uint32_t k_off = (uint32_t)(P::dma_row(x0, lane) * (int)p.ldk * 2 + P::dma_chunk(x0, lane) * 16);
+  const uint32_t v_off = (uint32_t)(P::dma_row(x0, lane) * (int)p.ldv * 2 + P::dma_chunk(x0, lane) * 16);
+  auto fetch = [&](const uint16_t* base, int64_t ld, uint32_t off, int row0, unsigned char* dst) {
+    const int rows = min(kTile, n - row0);  // rows past the end are zeros in LDS
+    if (rows <= 0) return;
+    const BufRsrc r = make_rsrc(base + (int64_t)row0 * ld, (uint32_t)(((rows - 1) * (int)ld + D) * 2));
+    asm volatile("" : "+v"(off));  // offsets of all DMAs, kept over the loop, would take registers
 #pragma unroll
     for (int u = 0; u < kDma; ++u) {
-      const int x = wave * kDma + u;
-      lds_dma16(r, dst + P::dma_at(x), (uint32_t)(P::dma_row(x, lane) * (int)ld * 2 + P::dma_chunk(x, lane) * 16), 0);
+      const uint32_t step = D == 256 ? (uint32_t)(u >> 1) * 8 * (uint32_t)ld + (u & 1) * 256 : (uint32_t)u * (2 * P::kRows) * (uint32_t)ld;
+      lds_dma16(r, dst + P::dma_at(x0 + u), off + step, 0);
     }
   };
   auto landed = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
@@ -147,6 +189,7 @@ prompt_attn_kernel(const PromptAttn p) {
     auto upto = [&](int i) { return p.causal ? i + 1 : n; };
     const int iw0 = w0 / p.G, iw1 = (min(w0 + kCols, cols) - 1) / p.G;
     const int t_first = from(iw0) / kTile, t_end = (upto(iw1) + kTile - 1) / kTile;
+    const int wg_lo = from(iw1), wg_hi = upto(iw0);  // what all of the workgroup's columns see
     // of the wave: what some, and what all of its columns see
     const bool any = c0 < cols;
     const int i0 = c0 / p.G, i1 = any ? (min(c0 + 32, cols) - 1) / p.G : i0;
@@ -157,138 +200,181 @@ prompt_attn_kernel(const PromptAttn p) {
     const bool on = c0 + col < cols;
     const int klo = from(query), khi = on ? upto(query) : 0;
 
-    fetch(kbase, p.ldk, t_first, k0);
-    fetch(vbase, p.ldv, t_first, v0);
+    // So that an iteration uses up a tile of each, K's tiles lie kLead keys behind V's.
+    if (kAhead) fetch(kbase, p.ldk, k_off, t_first * kTile, k1);
+    fetch(kbase, p.ldk, k_off, t_first * kTile + kLead, k0);
+    fetch(vbase, p.ldv, v_off, t_first * kTile, v0);
     v4w qf[KS];
     {
       const uint16_t* qp = p.q + (start + (on ? query : 0)) * p.ldq + (on ? head : h * p.G) * p.hq + half * 8;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
+      for (int w = 0; w < KS; ++w) {
         const v4w z = {0, 0, 0, 0};
-        qf[s] = on ? *reinterpret_cast<const v4w*>(qp + 16 * s) : z;
+        qf[w] = on ? *reinterpret_cast<const v4w*>(qp + 16 * w) : z;
       }
     }
-    v16f o[CT];
+    v16f o[CT], s0, s1 = v16f{};
+    uint32_t marks[CT];  // channels that saw what is not finite, a bit each
 #pragma unroll
-    for (int c = 0; c < CT; ++c) o[c] = v16f{};
+    for (int c = 0; c < CT; ++c) {
+      o[c] = v16f{};
+      marks[c] = 0;
+    }
     float m = -kInf, thr = -kInf, mu = 0.f, l = 0.f;
+    auto scores = [&](const unsigned char* kc, int kb) {
+      v16f r = v16f{};
+#pragma unroll
+      for (int w = 0; w < KS; ++w) r = mfma32<DT>(lds_read(kc + k_lane + P::at(32 * kb, 2 * w)), qf[w], r);
+      return r;
+    };
     landed();
+    if (kAhead) {
+      s0 = scores(k1, 0);
+      landed();
+    }
 
-    auto tile = [&](int t, const unsigned char* kc, const unsigned char* vc, unsigned char* kn, unsigned char* vn) {
+    // Edge tiles, that not all of the workgroup's columns see whole, may hold infinities or NaN that some do not see, and
+    // 0 times those is not 0. Where a tile has any, they leave it, and who sees them has its channels marked.
+    auto seen = [](int r, int rlo, int rhi) {  // key r of the lane's 16, by its column [rlo, rhi)
+      const int at = (r >> 2) * 8 + (r & 3);
+      return at >= rlo && at < rhi;
+    };
+    auto gone = [](uint32_t w) {  // the halves that are not finite
+      const uint32_t x = ~w & kExp;
+      return ((x & 0xffffu) == 0 ? 0xffffu : 0u) | ((x >> 16) == 0 ? 0xffff0000u : 0u);
+    };
+    auto clean = [&](int t, unsigned char* vc) {
+      uint32_t some = 0;
+#pragma unroll
+      for (int u = 0; u < kDma; ++u) {
+        const v4w w = lds_read(vc + P::dma_at(wave * kDma + u) + lane * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) some |= gone(w[e]);
+      }
+      if (lane == 0) flags[wave] = 0;
+      if (some) flags[wave] = 1;
+      __syncthreads();
+      int f = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) f |= flags[w];
+      if (!f) return;
+#pragma unroll 1
+      for (int k = 0; k < kTile; k += 32) {
+        const int rlo = klo - t * kTile - k - 4 * half, rhi = khi - t * kTile - k - 4 * half;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          v16f hit = v16f{};
+#pragma unroll
+          for (int s2 = 0; s2 < 2; ++s2) {
+            v4w is, who;
+            const unsigned char* vp = vc + v_lane + P::at(16 * s2, 4 * c) + (k ? P::at(32, 0) : 0);
+            const v2w a = lds_read_tr(vp), d = lds_read_tr(vp + P::at(8, 0));
+            const v4w v = {a.x, a.y, d.x, d.y};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              is[e] = gone(v[e]) & (kOnes | (kOnes << 16));
+              who[e] = (seen(8 * s2 + 2 * e, rlo, rhi) ? kOnes : 0u) | (seen(8 * s2 + 2 * e + 1, rlo, rhi) ? kOnes << 16 : 0u);
+            }
+            hit = mfma32<DT>(is, who, hit);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) marks[c] |= hit[r] > 0.f ? 1u << r : 0u;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < kDma; ++u) {
+        unsigned char* at = vc + P::dma_at(wave * kDma + u) + lane * 16;
+        v4w w = lds_read(at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] &= ~gone(w[e]);
+        *reinterpret_cast<v4w*>(at) = w;
+      }
+      __syncthreads();
+    };
+
+    // the 32 keys from key0: values in block kb of vc. Ahead: S in s, and S of the next 32 keys, in block kb of kc, into
+    // sn; else their keys are there.
+    auto block = [&](int key0, auto kb_, const unsigned char* kc, const unsigned char* vc, v16f& s, v16f& sn) {
+      constexpr int kb = decltype(kb_)::value;
+      if (key0 >= key_hi) return;
+      v4w ka[KS];
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int w = 0; w < KS; ++w) ka[w] = lds_read(kc + k_lane + P::at(32 * kb, 2 * w));
+      } else {
+        s = scores(kc, kb);
+      }
+      if (key0 < all_lo || key0 + 32 > all_hi) {
+        const int rlo = klo - key0 - 4 * half, rhi = khi - key0 - 4 * half;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = seen(r, rlo, rhi) ? s[r] : -kInf;
+      }
+      float top = -kInf;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+      if (__ballot(top > thr)) {
+        const float tp = pair_max(top);
+        // a column that has no need keeps its bits, whatever its neighbours do
+        const bool need = tp > thr;
+        const float mn = need ? fmaxf(m, tp) : m;
+        const float was = far_off(m, p.scale), is = far_off(mn, p.scale);
+        const float mun = need ? (mn == -kInf || is != 0.f ? 0.f : mn * p.scale) : mu;
+        const float f = m == -kInf ? 1.f : __builtin_amdgcn_exp2f(__builtin_fmaf(was - is, p.scale, mu - mun));
+        m = mn;
+        mu = mun;
+        thr = is != 0.f ? -kInf : mn + 8.f / p.scale;
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) o[c] *= f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] -= is;
+      }
+      auto v_operand = [&](int c, int s2) {
+        const v2w a = lds_read_tr(vc + v_lane + P::at(32 * kb + 16 * s2, 4 * c));
+        const v2w d = lds_read_tr(vc + v_lane + P::at(32 * kb + 16 * s2 + 8, 4 * c));
+        return v4w{a.x, a.y, d.x, d.y};
+      };
+      v4w va[CT];
+      if constexpr (kAhead)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) va[c] = v_operand(c, 0);
+      if constexpr (kAhead) {
+        sn = v16f{};
+#pragma unroll
+        for (int w = 0; w < KS; ++w) sn = mfma32<DT>(ka[w], qf[w], sn);  // behind the last keys: of what was there
+      }
+      v4w pf[2];
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.scale, -mu));
+        const float c = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.scale, -mu));
+        const uint32_t w = pack16<DT>(a, c);
+        pf[r >> 3][(r & 7) >> 1] = w;
+        l = add_pair<DT>(w, l);
+      }
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int c = 0; c < CT; ++c) o[c] = mfma32<DT>(va[c], pf[0], o[c]);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) va[c] = v_operand(c, 1);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) o[c] = mfma32<DT>(va[c], pf[1], o[c]);
+      } else {
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+          for (int c = 0; c < CT; ++c) o[c] = mfma32<DT>(v_operand(c, s2), pf[s2], o[c]);
+      }
+    };
+    auto tile = [&](int t, const unsigned char* kc, unsigned char* vc, unsigned char* kn, unsigned char* vn) {
       if (t + 1 < t_end) {
-        fetch(kbase, p.ldk, t + 1, kn);
-        fetch(vbase, p.ldv, t + 1, vn);
+        fetch(vbase, p.ldv, v_off, (t + 1) * kTile, vn);
+        fetch(kbase, p.ldk, k_off, (t + 1) * kTile + kLead, kn);
       }
-      const int key0 = t * kTile;
-      if (key0 < key_hi && key0 + kTile > key_lo) {
-        v16f s[2];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          s[kb] = v16f{};
-#pragma unroll
-          for (int w = 0; w < KS; ++w)
-            s[kb] = mfma32<DT>(lds_read(kc + k_lane + P::at(32 * kb, 2 * w)), qf[w], s[kb]);
-        }
-        const bool full = key0 >= all_lo && key0 + kTile <= all_hi;
-        bool bad = false;  // an infinity or a NaN in V that some column may not see
-        // key r of the lane's in block kb, seen by its column [rlo, rhi)
-        auto seen = [](int kb, int r, int rlo, int rhi) {
-          const int at = kb * 32 + (r >> 2) * 8 + (r & 3);
-          return at >= rlo && at < rhi;
-        };
-        if (!full) {
-          typedef unsigned short v2us __attribute__((ext_vector_type(2)));
-          v2us least = {0xffff, 0xffff};
-          for (int i = 0; i < P::kDmas; ++i) {
-            const v4w u = lds_read(vc + P::dma_at(i) + lane * 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              least = __builtin_elementwise_min(least, __builtin_bit_cast(v2us, ~u[e] & kExp));
-          }
-          const int rlo = klo - key0 - 4 * half, rhi = khi - key0 - 4 * half;
-          bad = __ballot(least[0] == 0 || least[1] == 0) != 0;
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[kb][r] = seen(kb, r, rlo, rhi) ? s[kb][r] : -kInf;
-        }
-        float top = -kInf;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
-        if (__ballot(top > thr)) {
-          const float tp = pair_max(top);
-          // a column that has no need keeps its bits, whatever its neighbours do
-          const bool need = tp > thr;
-          const float mn = need ? fmaxf(m, tp) : m;
-          const float was = far_off(m, p.scale), is = far_off(mn, p.scale);
-          const float mun = need ? (mn == -kInf || is != 0.f ? 0.f : mn * p.scale) : mu;
-          const float f = m == -kInf ? 1.f : __builtin_amdgcn_exp2f(__builtin_fmaf(was - is, p.scale, mu - mun));
-          m = mn;
-          mu = mun;
-          thr = is != 0.f ? -kInf : mn + 8.f / p.scale;
-          l *= f;
-#pragma unroll
-          for (int c = 0; c < CT; ++c) o[c] *= f;
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[kb][r] -= is;
-        }
-        v4w pf[2][2];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; r += 2) {
-            const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], p.scale, -mu));
-            const float c = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r + 1], p.scale, -mu));
-            l += a;
-            l += c;
-            pf[kb][r >> 3][(r & 7) >> 1] = pack16<DT>(a, c);
-          }
-        auto v_operand = [&](int c, int kb, int s2) {
-          const v2w a = lds_read_tr(vc + v_lane + P::at(32 * kb + 16 * s2, 4 * c));
-          const v2w d = lds_read_tr(vc + v_lane + P::at(32 * kb + 16 * s2 + 8, 4 * c));
-          return v4w{a.x, a.y, d.x, d.y};
-        };
-        if (!bad) {
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-              for (int c = 0; c < CT; ++c) o[c] = mfma32<DT>(v_operand(c, kb, s2), pf[kb][s2], o[c]);
-        } else {
-          // 0 times what is not finite is not 0: such values leave the product, and a product of where they are with
-          // who sees them makes NaN of those channels
-          int rlo = klo - key0 - 4 * half, rhi = khi - key0 - 4 * half;
-          asm volatile("" : "+v"(rlo), "+v"(rhi));  // worked out again: 64 masks would not fit the scalar registers
-#pragma unroll
-          for (int c = 0; c < CT; ++c) {
-            v16f hit = v16f{};
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-              for (int s2 = 0; s2 < 2; ++s2) {
-                v4w a = v_operand(c, kb, s2), is, who;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const uint32_t x = ~a[e] & kExp;
-                  const uint32_t gone = ((x & 0xffffu) == 0 ? 0xffffu : 0u) | ((x >> 16) == 0 ? 0xffff0000u : 0u);
-                  a[e] &= ~gone;
-                  is[e] = gone & (kOnes | (kOnes << 16));
-                  who[e] = (seen(kb, 8 * s2 + 2 * e, rlo, rhi) ? kOnes : 0u) |
-                           (seen(kb, 8 * s2 + 2 * e + 1, rlo, rhi) ? kOnes << 16 : 0u);
-                }
-                o[c] = mfma32<DT>(a, pf[kb][s2], o[c]);
-                hit = mfma32<DT>(is, who, hit);
-              }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[c][r] = hit[r] > 0.f ? __builtin_nanf("") : o[c][r];
-          }
-        }
-      }
+      if (t * kTile < wg_lo || (t + 1) * kTile > wg_hi) clean(t, vc);
+      block(t * kTile, std::integral_constant<int, 0>{}, kc, vc, s0, s1);
+      if constexpr (kTile == 64) block(t * kTile + 32, std::integral_constant<int, 1>{}, kc, vc, s1, s0);
       landed();
     };
     for (int t = t_first; t < t_end; t += 2) {
@@ -304,6 +390,8 @@ prompt_attn_kernel(const PromptAttn p) {
       for (int c = 0; c < CT; ++c)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
+#pragma unroll
+          for (int e = r; e < r + 4; ++e) o[c][e] = marks[c] >> e & 1 ? __builtin_nanf("") : o[c][e];
           const v2w u = {pack16<DT>(o[c][r] * inv, o[c][r + 1] * inv), pack16<DT>(o[c][r + 2] * inv, o[c][r + 3] * inv)};
           *reinterpret_cast<v2w*>(op + c * 32 + 2 * r) = u;
         }
@@ -318,7 +406,7 @@ prompt_attn_kernel(const PromptAttn p) {
 
 template <int D, int DT>
 static int launch_dt(const PromptAttn& p, int64_t max_q, hipStream_t st) {
-  constexpr int NW = D == 256 ? 4 : 8;
+  constexpr int NW = D == 256 ? 8 : 4;
   const int64_t tiles = (max_q * p.G + 32 * NW - 1) / (32 * NW);
   if (tiles * p.H > kMaxGrid / 2) return kErrUnsupported;
   const dim3 g((unsigned)(tiles * p.H), (unsigned)p.B);

@@ -180,6 +180,29 @@ def test_scores_of_any_size(dev, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("below", [13.5, 15.25, 18.0, 23.0])
+def test_many_small_weights(dev, dtype, below):
+    """One key before thousands that weigh 2^-below of it each, subnormal in fp16: together they weigh what they should, in
+    the products and in the sum. In fp16 a weight below 2^-14 is off by up to 2^-25, of what n such weights are among 1."""
+    n, D = 3001, 64
+    q, k, v = (t.clone() for t in make(n, 1, 1, D, dtype, dev, seed=6))
+    q.zero_()
+    k.zero_()
+    q[:, 0, 0] = 1
+    k[1:, 0, 0] = -below * math.log(2)
+    k[1:, 0, 1] = -below * math.log(2) - k[1:, 0, 0].float()  # what the type rounds away
+    q[:, 0, 1] = 1
+    v[1:] = v[1:].abs()
+    out, lse = _att().prompt_attention(q, k, v, _i32(dev, 0, n), sm_scale=1.0, return_lse=True)
+    want = ref(q, k, v, [0, n], 1.0)
+    sub = n * 2.0 ** -25 if dtype == torch.float16 else 0.0
+    most = v.float().abs().max().item()
+    compare(out, None, (want[0], want[1] + 2 * sub * most * 2.0 ** 11, want[2], want[3]), dtype, D, n)
+    assert ((lse.cpu().double() - want[2]).abs() <= sub + (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11) + n * 2.0 ** -26).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("at", [0, 5, 63, 64, 100])
 @pytest.mark.parametrize("D", [64, 128, 256])
