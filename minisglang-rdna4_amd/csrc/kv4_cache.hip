@@ -189,45 +189,79 @@ kv4_append_kernel(const uint16_t* __restrict__ k, int64_t ldk, int64_t hk, const
 
 // Rows of the cache as values in the model's type: s c + m with one rounding to f32 (the product is
 // exact) and one to the type. A row without a place in the cache (before the sequence's first token,
-// on a page that does not exist) is NaN. A vector per D / 8 lanes, heads of a row side by side.
+// on a page that does not exist) is NaN. A vector per D / 8 lanes; a wave has 8 rows, which as a rule are one block's and share
+// its words of V, and `per` heads of them: row -> sequence -> page, dependent reads, are looked up once for all of those.
+// 131072 rows of 8 heads of 128 (142 MB in, 537 out) 137 us, 5.0 TB/s; 232 with a lookup for every 4 vectors.
 template <int D, int DT>
 __global__ void __launch_bounds__(256)
-kv4_read_kernel(Kv4Cache c, Kv4Batch s, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
-  constexpr int L = D / 8, VP = 64 / L;
+kv4_read_kernel(Kv4Cache c, Kv4Batch s, int per, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
+  constexpr int L = D / 8, VP = 64 / L, PASS = 8 / VP;  // lanes per vector, vectors per wave, passes for 8 rows
   const int lane = threadIdx.x & 63;
-  const uint32_t id0 = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * VP;
-  if (id0 >= s.T * c.H) return;
-  const int b0 = kv4_sequence(s, id0 / (uint32_t)c.H, lane);
-  const uint32_t id = id0 + lane / L;
-  const int64_t i = id / (uint32_t)c.H;
-  const int h = (int)(id % (uint32_t)c.H), ch = (lane & (L - 1)) * 8;
-  Place pl;
-  if (i >= s.T || !kv4_place(s, b0, i, pl)) return;
-  const int page = kv4_page(c, s, pl.b, pl.pos);
-  uint32_t ks = DT == kF16 ? 0x7e007e00u : 0x7fc07fc0u, vs = ks, kc = 0, vc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  const int j = (int)(pl.pos & 7);
-  if (page >= 0) {
-    const int64_t blk = kv4_block(c, page, h, (int)(pl.pos & ~(int64_t)7));
-    const uint4* vd = reinterpret_cast<const uint4*>(c.v + blk * (4 * D) + ch * 4);
-    kc = *reinterpret_cast<const uint32_t*>(c.k + blk * (4 * D) + j * (D / 2) + ch / 2);
-    const uint4 a = vd[0], b = vd[1];
-    vc[0] = a.x; vc[1] = a.y; vc[2] = a.z; vc[3] = a.w;
-    vc[4] = b.x; vc[5] = b.y; vc[6] = b.z; vc[7] = b.w;
-    ks = c.ks[blk * 8 + j];
-    vs = c.vs[blk * 8 + j];
+  const uint32_t id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t parts = ((uint32_t)c.H + per - 1) / per, group = id / parts;
+  const int h0 = (int)(id - group * parts) * per, h1 = min(h0 + per, c.H);
+  const int64_t i0 = (int64_t)group * 8;
+  if (i0 >= s.T) return;
+  const int b0 = kv4_sequence(s, i0, lane), ch = (lane & (L - 1)) * 8;
+  // a lane looks one of the 8 rows up: its block of head 0, or -1 without a page, -2 without a sequence
+  int64_t look = -2;
+  int slot = 0;
+  {
+    const int64_t i = i0 + (lane & 7);
+    Place pl;
+    if (i < s.T && kv4_place(s, b0, i, pl)) {
+      const int page = kv4_page(c, s, pl.b, pl.pos);
+      slot = (int)(pl.pos & 7);
+      look = page >= 0 ? kv4_block(c, page, 0, (int)(pl.pos & ~(int64_t)7)) : -1;
+    }
   }
-  auto value = [&](uint32_t code, uint32_t sm) {
-    return (uint32_t)to_dtype(__builtin_fmaf((float)code, from_dtype((uint16_t)(sm & 0xffffu), DT),
-                                             from_dtype((uint16_t)(sm >> 16), DT)), DT);
-  };
-  uint32_t kw[4], vw[4];
+  int64_t blk[PASS], at[PASS];  // of the lane's vectors; their places among the outputs
+  int j[PASS];
 #pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    kw[e / 2] = value((kc >> (4 * e)) & 15u, ks) | (value((kc >> (4 * e + 4)) & 15u, ks) << 16);
-    vw[e / 2] = value((vc[e] >> (4 * j)) & 15u, vs) | (value((vc[e + 1] >> (4 * j)) & 15u, vs) << 16);
+  for (int p = 0; p < PASS; ++p) {
+    const int r = p * VP + lane / L;
+    blk[p] = __shfl(look, r);
+    j[p] = __shfl(slot, r);
+    at[p] = (i0 + r) * c.H * D + ch;
   }
-  *reinterpret_cast<uint4*>(k + (int64_t)id * D + ch) = make_uint4(kw[0], kw[1], kw[2], kw[3]);
-  *reinterpret_cast<uint4*>(v + (int64_t)id * D + ch) = make_uint4(vw[0], vw[1], vw[2], vw[3]);
+  const int step = 1 << (c.shift - 3);  // blocks from one head to the next
+  for (int h = h0; h < h1; ++h) {
+    uint32_t ks[PASS], vs[PASS], kc[PASS];
+    v4u vc[PASS][2];
+#pragma unroll
+    for (int p = 0; p < PASS; ++p) {
+      const int64_t b = (blk[p] < 0 ? 0 : blk[p]) + (int64_t)h * step;  // block 0 is there; its values are not used
+      kc[p] = *reinterpret_cast<const uint32_t*>(c.k + b * (4 * D) + j[p] * (D / 2) + ch / 2);
+      const v4u* vd = reinterpret_cast<const v4u*>(c.v + b * (4 * D) + ch * 4);
+      vc[p][0] = vd[0];
+      vc[p][1] = vd[1];
+      ks[p] = c.ks[b * 8 + j[p]];
+      vs[p] = c.vs[b * 8 + j[p]];
+    }
+#pragma unroll
+    for (int p = 0; p < PASS; ++p) {
+      const uint32_t nan = DT == kF16 ? 0x7e007e00u : 0x7fc07fc0u;
+      if (blk[p] < 0) {
+        ks[p] = vs[p] = nan;
+      }
+      const float sk = from_dtype((uint16_t)(ks[p] & 0xffffu), DT), mk = from_dtype((uint16_t)(ks[p] >> 16), DT);
+      const float sv = from_dtype((uint16_t)(vs[p] & 0xffffu), DT), mv = from_dtype((uint16_t)(vs[p] >> 16), DT);
+      v4u kw, vw;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        auto two = [](uint32_t a, uint32_t b, float st, float least) {
+          return (uint32_t)to_dtype(__builtin_fmaf((float)a, st, least), DT) |
+                 ((uint32_t)to_dtype(__builtin_fmaf((float)b, st, least), DT) << 16);
+        };
+        kw[e / 2] = two((kc[p] >> (4 * e)) & 15u, (kc[p] >> (4 * e + 4)) & 15u, sk, mk);
+        vw[e / 2] = two((vc[p][e / 4][e % 4] >> (4 * j[p])) & 15u, (vc[p][e / 4][e % 4 + 1] >> (4 * j[p])) & 15u, sv, mv);
+      }
+      if (blk[p] != -2) {
+        *reinterpret_cast<v4u*>(k + at[p] + h * D) = kw;
+        *reinterpret_cast<v4u*>(v + at[p] + h * D) = vw;
+      }
+    }
+  }
 }
 
 template <int DT>
@@ -252,20 +286,22 @@ int launch_kv4_append(const void* k, int64_t ldk, int64_t hk, const void* v, int
 }
 
 template <int DT>
-static void read(int D, dim3 g, const Kv4Cache& c, const Kv4Batch& s, uint16_t* k, uint16_t* v, hipStream_t st) {
-  if (D == 64) hipLaunchKernelGGL((kv4_read_kernel<64, DT>), g, dim3(256), 0, st, c, s, k, v);
-  else if (D == 128) hipLaunchKernelGGL((kv4_read_kernel<128, DT>), g, dim3(256), 0, st, c, s, k, v);
-  else hipLaunchKernelGGL((kv4_read_kernel<256, DT>), g, dim3(256), 0, st, c, s, k, v);
+static void read(int D, dim3 g, const Kv4Cache& c, const Kv4Batch& s, int per, uint16_t* k, uint16_t* v, hipStream_t st) {
+  if (D == 64) hipLaunchKernelGGL((kv4_read_kernel<64, DT>), g, dim3(256), 0, st, c, s, per, k, v);
+  else if (D == 128) hipLaunchKernelGGL((kv4_read_kernel<128, DT>), g, dim3(256), 0, st, c, s, per, k, v);
+  else hipLaunchKernelGGL((kv4_read_kernel<256, DT>), g, dim3(256), 0, st, c, s, per, k, v);
 }
 
 int launch_kv4_read(const Kv4Cache& c, const Kv4Batch& s, int dtype, int D, void* k, void* v, hipStream_t st) {
-  const int per = 4 * 512 / D;  // vectors per workgroup
-  const int64_t wgs = (s.T * c.H + per - 1) / per;
+  // as many heads a wave as leave two waves for each place on the card (8192)
+  const int64_t groups = (s.T + 7) / 8, most = groups * c.H / 16384;
+  const int per = (int)(most < 1 ? 1 : most > c.H ? c.H : most);
+  const int64_t wgs = (groups * ((c.H + per - 1) / per) + 3) / 4;
   if (wgs > kMaxGrid) return kErrUnsupported;
   const dim3 g((unsigned)wgs);
   auto kp = reinterpret_cast<uint16_t*>(k), vp = reinterpret_cast<uint16_t*>(v);
-  if (dtype == kBF16) read<kBF16>(D, g, c, s, kp, vp, st);
-  else read<kF16>(D, g, c, s, kp, vp, st);
+  if (dtype == kBF16) read<kBF16>(D, g, c, s, per, kp, vp, st);
+  else read<kF16>(D, g, c, s, per, kp, vp, st);
   return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 

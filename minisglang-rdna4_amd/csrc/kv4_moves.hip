@@ -5,60 +5,62 @@
 
 namespace w4a8 {
 
-// ---- pages: a workgroup copies 32 KB of one pair's page, 4 loads of 16 bytes a lane in flight. The page's four arrays
-// are taken as one row of vectors: K codes, V codes, K scales, V scales.
-constexpr int kCopyPart = 2048;  // vectors of a workgroup
+// ---- pages: a workgroup copies 1024 vectors of 16 bytes of one pair's page, 4 a lane and all in flight, of its K codes, its
+// V codes, or its scales (K's, then V's). Nothing branches before the loads, so that what they wait for is read at once:
+// the pair, the cache's pointers. 64 pairs of 17 KB in 4 layers 6 us (18.8 with 2048 vectors a workgroup over all four arrays
+// in a row, whose places were worked out one after another).
+constexpr int kCopyPart = 1024;  // vectors of a workgroup
 
 __global__ void __launch_bounds__(256)
-kv4_copy_kernel(const Kv4Caches cs, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int64_t pages, int parts,
-                int64_t codes, int64_t scales) {
-  const uint32_t pair = blockIdx.x / (uint32_t)parts, part = blockIdx.x - pair * (uint32_t)parts;
-  const int64_t s = src[pair], d = dst[pair];
-  if (s < 0 || s >= pages || d < 0 || d >= pages || s == d) return;
-  const Kv4Arrays& c = cs.c[blockIdx.y];
-  const int64_t total = 2 * (codes + scales);
-  const int64_t lo = (int64_t)part * kCopyPart, hi = lo + kCopyPart < total ? lo + kCopyPart : total;
-  auto at = [&](int64_t i, uint4*& base, int64_t& n) {  // vector i's array, and the page's vectors there; its place in them
-    if (i < codes) { base = reinterpret_cast<uint4*>(c.k); n = codes; return i; }
-    i -= codes;
-    if (i < codes) { base = reinterpret_cast<uint4*>(c.v); n = codes; return i; }
-    i -= codes;
-    if (i < scales) { base = reinterpret_cast<uint4*>(c.ks); n = scales; return i; }
-    base = reinterpret_cast<uint4*>(c.vs);
-    n = scales;
-    return i - scales;
-  };
-  for (int64_t i0 = lo + threadIdx.x; i0 < hi; i0 += 1024) {
-    uint4 x[4];
-    uint4* to[4];
+kv4_copy_kernel(const Kv4Caches cs, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int pages, int parts,
+                uint32_t codes, uint32_t scales) {
+  const int pair = blockIdx.x, part = blockIdx.y;
+  const Kv4Arrays c = cs.c[blockIdx.z];
+  const int s = src[pair], d = dst[pair];
+  const bool on = s >= 0 && s < pages && d >= 0 && d < pages && s != d;
+  const int64_t from = on ? s : 0, to = on ? d : 0;
+  const bool of_k = part < parts, of_v = !of_k && part < 2 * parts;
+  const uint32_t i0 = (uint32_t)(of_k ? part : of_v ? part - parts : part - 2 * parts) * kCopyPart + threadIdx.x;
+  v4u x[4];
+  if (of_k || of_v) {
+    v4u* base = reinterpret_cast<v4u*>(of_k ? c.k : c.v);
+    const v4u* in = base + from * codes;
+    v4u* out = base + to * codes;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t i = i0 + 256 * u;
-      uint4* base;
-      int64_t n;
-      const int64_t j = at(i < hi ? i : i0, base, n);
-      x[u] = base[s * n + j];
-      to[u] = base + d * n + j;
-    }
+    for (int u = 0; u < 4; ++u) x[u] = in[min(i0 + 256 * u, codes - 1)];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (i0 + 256 * u < hi) *to[u] = x[u];
+      if (on && i0 + 256 * u < codes) out[i0 + 256 * u] = x[u];
+  } else {
+    v4u *ks = reinterpret_cast<v4u*>(c.ks), *vs = reinterpret_cast<v4u*>(c.vs);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t i = min(i0 + 256 * u, 2 * scales - 1);
+      x[u] = i < scales ? ks[from * scales + i] : vs[from * scales + i - scales];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t i = i0 + 256 * u;
+      if (on && i < scales) ks[to * scales + i] = x[u];
+      if (on && i >= scales && i < 2 * scales) vs[to * scales + i - scales] = x[u];
+    }
   }
 }
 
 int launch_kv4_copy(const Kv4Caches& cs, int caches, const int32_t* src, const int32_t* dst, int64_t n, int64_t pages,
                     int64_t codes, int64_t scales, hipStream_t st) {
-  const int64_t parts = (2 * (codes + scales) + kCopyPart - 1) / kCopyPart;
-  if (n * parts > kMaxGrid) return kErrUnsupported;
-  hipLaunchKernelGGL(kv4_copy_kernel, dim3((unsigned)(n * parts), (unsigned)caches), dim3(256), 0, st, cs, src, dst, pages,
-                     (int)parts, codes, scales);
+  const int64_t parts = (codes + kCopyPart - 1) / kCopyPart, all = 2 * parts + (2 * scales + kCopyPart - 1) / kCopyPart;
+  if (n > kMaxGrid || all > 65535) return kErrUnsupported;
+  hipLaunchKernelGGL(kv4_copy_kernel, dim3((unsigned)n, (unsigned)all, (unsigned)caches), dim3(256), 0, st, cs, src, dst,
+                     (int)pages, (int)parts, (uint32_t)codes, (uint32_t)scales);
   return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
 // ---- accepted tokens. Slot j behind the context gets what slot keep[j] >= j holds. A workgroup has one sequence, head
-// and layer and takes the 8 slots of one block at a time, in order: all 8 are read before the first is written, and
-// what is read lies behind what is written, so no block reads what an earlier one has written. A thread has one
-// channel of V (words of 8 tokens, a nibble of each moves), and words of the tokens' K.
+// and layer. It looks 64 slots up at once, a lane each (the list's first entries are read beside the lengths), and takes the 8
+// slots of one block at a time, in order: all 8 are read before the first is written, and what is read lies behind what is
+// written, so no block reads what an earlier one has written. A thread has one channel of V (words of 8 tokens, a nibble
+// of each moves), and words of the tokens' K. Bound by a chain of dependent reads, lengths -> page -> codes.
 template <int D>
 __global__ void __launch_bounds__(D < 128 ? 128 : D)
 kv4_keep_kernel(const Kv4Caches cs, Kv4Cache c, Kv4Batch s, const int32_t* __restrict__ keep, int64_t ldk, int width,
@@ -66,79 +68,83 @@ kv4_keep_kernel(const Kv4Caches cs, Kv4Cache c, Kv4Batch s, const int32_t* __res
   constexpr int kThreads = D < 128 ? 128 : D;
   constexpr int KW = D / 8;                       // words of a token's K codes
   constexpr int PASS = (8 * KW + kThreads - 1) / kThreads;
+  __shared__ int lst[64], s_where[64];
+  __shared__ int64_t s_from[64], s_to[8];
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const Kv4Arrays& a = cs.c[blockIdx.z];
+  const Kv4Arrays a = cs.c[blockIdx.z];
+  const int32_t* list = keep + b * ldk;
   int64_t start;
   int n;
+  if (tid < 64 && tid < width) lst[tid] = list[tid];
   kv4_rows(s, b, start, n);
   const int64_t base = (int64_t)s.lens[b] - n;  // the first new token
   const int m = min(max(kept[b], 0), min(n, width));
   if (now && h == 0 && blockIdx.z == 0 && tid == 0) now[b] = (int32_t)(base + m);
-  const int32_t* list = keep + b * ldk;
-  // slot j's source, or -1: it stays as it is
-  auto source = [&](int j) -> int64_t {
-    if (j < 0 || j >= m) return -1;
-    const int i = list[j];
-    return i > j && i < n ? base + i : -1;
-  };
-  // block and place in it of a position, or -1
+  // block of a position, or -1
   auto block = [&](int64_t pos) -> int64_t {
     const int page = kv4_page(c, s, b, pos);
     return page < 0 ? -1 : kv4_block(c, page, h, (int)(pos & ~(int64_t)7));
   };
-  for (int64_t p0 = base & ~(int64_t)7; p0 < base + m; p0 += 8) {
-    const int64_t to = p0 < 0 ? -1 : block(p0);
-    if (to < 0) continue;
-    int64_t from[8];
-    int where[8];
-    bool some = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int64_t src = source((int)(p0 + e - base));
-      from[e] = src < 0 ? -1 : block(src);
-      where[e] = (int)(src & 7);
-      some = some || from[e] >= 0;
+  for (int64_t p64 = base & ~(int64_t)7; p64 < base + m; p64 += 64) {
+    __syncthreads();
+    if (tid < 64) {
+      const int64_t p = p64 + tid;
+      const int j = (int)(p - base);
+      int i = -1;
+      if (j >= 0 && j < m) i = j < 64 ? lst[j] : list[j];
+      const bool moves = j >= 0 && i > j && i < n;
+      s_from[tid] = moves ? block(base + i) : -1;
+      s_where[tid] = (int)((base + i) & 7);
+      if ((tid & 7) == 0) s_to[tid >> 3] = j + 8 > 0 && j < m ? block(p) : -1;
     }
-    if (!some) continue;
-    uint32_t kw[PASS], ksm = 0, vsm = 0, word = 0, vw[8];
-    const bool channel = tid < D;
+    __syncthreads();
+    for (int e0 = 0; e0 < 64 && p64 + e0 < base + m; e0 += 8) {
+      const int64_t to = s_to[e0 >> 3];
+      if (to < 0) continue;
+      int64_t from[8];
+      int where[8];
+      bool some = false;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      vw[e] = channel && from[e] >= 0 ? reinterpret_cast<const uint32_t*>(a.v)[from[e] * D + tid] : 0u;
-    if (channel) word = reinterpret_cast<const uint32_t*>(a.v)[to * D + tid];
-    auto pick = [&](int e, int64_t& f, int& w) {  // from[e] and where[e], e a lane's own
-      f = -1;
-      w = 0;
+      for (int e = 0; e < 8; ++e) {
+        from[e] = s_from[e0 + e];
+        where[e] = s_where[e0 + e];
+        some = some || from[e] >= 0;
+      }
+      if (!some) continue;
+      uint32_t kw[PASS], ksm = 0, vsm = 0, word = 0, vw[8];
+      int64_t kf[PASS], sf = -1;
+      const bool channel = tid < D;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i == e) { f = from[i]; w = where[i]; }
-    };
-    int64_t kf[PASS], sf = -1;
-    int kx[PASS], sx = 0;
+      for (int e = 0; e < 8; ++e)
+        vw[e] = channel && from[e] >= 0 ? reinterpret_cast<const uint32_t*>(a.v)[from[e] * D + tid] : 0u;
+      if (channel) word = reinterpret_cast<const uint32_t*>(a.v)[to * D + tid];
 #pragma unroll
-    for (int u = 0; u < PASS; ++u) {
-      const int id = tid + u * kThreads;
-      pick(id / KW, kf[u], kx[u]);
-      kw[u] = kf[u] >= 0 ? reinterpret_cast<const uint32_t*>(a.k)[(kf[u] * 8 + kx[u]) * KW + id % KW] : 0u;
-    }
-    if (tid < 8) pick(tid, sf, sx);
-    if (sf >= 0) {
-      ksm = a.ks[sf * 8 + sx];
-      vsm = a.vs[sf * 8 + sx];
-    }
-    __syncthreads();  // all is read, and arrived
+      for (int u = 0; u < PASS; ++u) {
+        const int id = tid + u * kThreads, e = (id / KW) & 7;
+        kf[u] = id < 8 * KW ? s_from[e0 + e] : -1;
+        kw[u] = kf[u] >= 0 ? reinterpret_cast<const uint32_t*>(a.k)[(kf[u] * 8 + s_where[e0 + e]) * KW + id % KW] : 0u;
+      }
+      if (tid < 8) {
+        sf = s_from[e0 + tid];
+        if (sf >= 0) {
+          ksm = a.ks[sf * 8 + s_where[e0 + tid]];
+          vsm = a.vs[sf * 8 + s_where[e0 + tid]];
+        }
+      }
+      __syncthreads();  // all is read, and arrived
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (from[e] >= 0) word = (word & ~(15u << (4 * e))) | (((vw[e] >> (4 * where[e])) & 15u) << (4 * e));
-    if (channel) reinterpret_cast<uint32_t*>(a.v)[to * D + tid] = word;
+      for (int e = 0; e < 8; ++e)
+        if (from[e] >= 0) word = (word & ~(15u << (4 * e))) | (((vw[e] >> (4 * where[e])) & 15u) << (4 * e));
+      if (channel) reinterpret_cast<uint32_t*>(a.v)[to * D + tid] = word;
 #pragma unroll
-    for (int u = 0; u < PASS; ++u) {
-      const int id = tid + u * kThreads;
-      if (kf[u] >= 0) reinterpret_cast<uint32_t*>(a.k)[(to * 8 + id / KW) * KW + id % KW] = kw[u];
-    }
-    if (sf >= 0) {
-      a.ks[to * 8 + tid] = ksm;
-      a.vs[to * 8 + tid] = vsm;
+      for (int u = 0; u < PASS; ++u) {
+        const int id = tid + u * kThreads;
+        if (kf[u] >= 0) reinterpret_cast<uint32_t*>(a.k)[(to * 8 + id / KW) * KW + id % KW] = kw[u];
+      }
+      if (sf >= 0) {
+        a.ks[to * 8 + tid] = ksm;
+        a.vs[to * 8 + tid] = vsm;
+      }
     }
   }
 }
