@@ -189,25 +189,25 @@ kv4_append_kernel(const uint16_t* __restrict__ k, int64_t ldk, int64_t hk, const
 
 // Rows of the cache as values in the model's type: s c + m with one rounding to f32 (the product is
 // exact) and one to the type. A row without a place in the cache (before the sequence's first token,
-// on a page that does not exist) is NaN. A vector per D / 8 lanes; a wave has 8 rows, which as a rule are one block's and share
-// its words of V, and `per` heads of them: row -> sequence -> page, dependent reads, are looked up once for all of those.
+// on a page that does not exist) is NaN. A vector per D / 8 lanes; a wave has 8 rows (ROWS), which as a rule are one block's and
+// share its words of V, and `per` heads of them: row -> sequence -> page, dependent reads, are looked up once for all of those.
 // 131072 rows of 8 heads of 128 (142 MB in, 537 out) 137 us, 5.0 TB/s; 232 with a lookup for every 4 vectors.
-template <int D, int DT>
+template <int D, int DT, int ROWS>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(Kv4Cache c, Kv4Batch s, int per, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
-  constexpr int L = D / 8, VP = 64 / L, PASS = 8 / VP;  // lanes per vector, vectors per wave, passes for 8 rows
+  constexpr int L = D / 8, VP = 64 / L, PASS = ROWS / VP;  // lanes per vector, vectors per wave, passes for its rows
   const int lane = threadIdx.x & 63;
   const uint32_t id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t parts = ((uint32_t)c.H + per - 1) / per, group = id / parts;
   const int h0 = (int)(id - group * parts) * per, h1 = min(h0 + per, c.H);
-  const int64_t i0 = (int64_t)group * 8;
+  const int64_t i0 = (int64_t)group * ROWS;
   if (i0 >= s.T) return;
   const int b0 = kv4_sequence(s, i0, lane), ch = (lane & (L - 1)) * 8;
-  // a lane looks one of the 8 rows up: its block of head 0, or -1 without a page, -2 without a sequence
+  // a lane looks one of the rows up: its block of head 0, or -1 without a page, -2 without a sequence
   int64_t look = -2;
   int slot = 0;
   {
-    const int64_t i = i0 + (lane & 7);
+    const int64_t i = i0 + (lane & (ROWS - 1));
     Place pl;
     if (i < s.T && kv4_place(s, b0, i, pl)) {
       const int page = kv4_page(c, s, pl.b, pl.pos);
@@ -285,24 +285,29 @@ int launch_kv4_append(const void* k, int64_t ldk, int64_t hk, const void* v, int
   return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
-template <int DT>
-static void read(int D, dim3 g, const Kv4Cache& c, const Kv4Batch& s, int per, uint16_t* k, uint16_t* v, hipStream_t st) {
-  if (D == 64) hipLaunchKernelGGL((kv4_read_kernel<64, DT>), g, dim3(256), 0, st, c, s, per, k, v);
-  else if (D == 128) hipLaunchKernelGGL((kv4_read_kernel<128, DT>), g, dim3(256), 0, st, c, s, per, k, v);
-  else hipLaunchKernelGGL((kv4_read_kernel<256, DT>), g, dim3(256), 0, st, c, s, per, k, v);
-}
-
-int launch_kv4_read(const Kv4Cache& c, const Kv4Batch& s, int dtype, int D, void* k, void* v, hipStream_t st) {
+template <int D, int DT>
+static int read(const Kv4Cache& c, const Kv4Batch& s, uint16_t* k, uint16_t* v, hipStream_t st) {
+  constexpr int VP = 512 / D;
+  // few rows (a decode step's, each of another sequence): as many as a wave holds side by side, and a head. us, 64 rows of 8
+  // heads: 3.3, 4.8 with 8 rows a wave
+  const bool few = s.T * c.H <= 8192;
+  const int rows = few ? VP : 8;
   // as many heads a wave as leave two waves for each place on the card (8192)
-  const int64_t groups = (s.T + 7) / 8, most = groups * c.H / 16384;
+  const int64_t groups = (s.T + rows - 1) / rows, most = groups * c.H / 16384;
   const int per = (int)(most < 1 ? 1 : most > c.H ? c.H : most);
   const int64_t wgs = (groups * ((c.H + per - 1) / per) + 3) / 4;
   if (wgs > kMaxGrid) return kErrUnsupported;
-  const dim3 g((unsigned)wgs);
-  auto kp = reinterpret_cast<uint16_t*>(k), vp = reinterpret_cast<uint16_t*>(v);
-  if (dtype == kBF16) read<kBF16>(D, g, c, s, per, kp, vp, st);
-  else read<kF16>(D, g, c, s, per, kp, vp, st);
+  const dim3 g((unsigned)wgs), b(256);
+  if (few) hipLaunchKernelGGL((kv4_read_kernel<D, DT, VP>), g, b, 0, st, c, s, per, k, v);
+  else hipLaunchKernelGGL((kv4_read_kernel<D, DT, 8>), g, b, 0, st, c, s, per, k, v);
   return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
+}
+
+int launch_kv4_read(const Kv4Cache& c, const Kv4Batch& s, int dtype, int D, void* k, void* v, hipStream_t st) {
+  auto kp = reinterpret_cast<uint16_t*>(k), vp = reinterpret_cast<uint16_t*>(v);
+  if (dtype == kBF16)
+    return D == 64 ? read<64, kBF16>(c, s, kp, vp, st) : D == 128 ? read<128, kBF16>(c, s, kp, vp, st) : read<256, kBF16>(c, s, kp, vp, st);
+  return D == 64 ? read<64, kF16>(c, s, kp, vp, st) : D == 128 ? read<128, kF16>(c, s, kp, vp, st) : read<256, kF16>(c, s, kp, vp, st);
 }
 
 }  // namespace w4a8
