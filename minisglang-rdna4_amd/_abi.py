@@ -98,6 +98,7 @@ SIGNATURES = {
                              _vp, _c_int, _c_i64, _c_i64, _vp, _vp, ctypes.c_float, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
                              _vp]),
     "w4a8_kv4_tree": (_c_int, [_vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp]),
+    "w4a8_kv4_tree_attention_workspace_bytes": (_c_i64, [_c_i64] * 8),
     "w4a8_kv4_tree_attention": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _vp,
                                          _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, ctypes.c_float, _c_i64,
                                          _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64,

@@ -25,8 +25,9 @@ _ENTRY_POINTS = (
     "w4a8_moe_route_align", "w4a8_moe_gemm_workspace_bytes", "w4a8_moe_gemm", "w4a8_moe_gemm2_combine_supported",
     "w4a8_moe_gemm2_combine", "w4a8_moe_gemm_quant_workspace_bytes", "w4a8_moe_gemm_quant", "w4a8_moe_combine",
     "w4a8_kv4_append", "w4a8_kv4_read", "w4a8_kv4_attention_workspace_bytes", "w4a8_kv4_attention",
-    "w4a8_lora_workspace_bytes", "w4a8_lora_add", "w4a8_kv4_tree", "w4a8_kv4_tree_attention", "w4a8_kv4_copy_pages",
-    "w4a8_kv4_keep", "w4a8_prompt_attention", "w4a8_rotary",
+    "w4a8_lora_workspace_bytes", "w4a8_lora_add", "w4a8_kv4_tree",
+    "w4a8_kv4_tree_attention_workspace_bytes", "w4a8_kv4_tree_attention", "w4a8_kv4_copy_pages", "w4a8_kv4_keep",
+    "w4a8_prompt_attention", "w4a8_rotary",
 )
 
 _lock = threading.Lock()

@@ -60,6 +60,7 @@ struct Abi {
   decltype(&w4a8_lora_workspace_bytes) lora_ws;
   decltype(&w4a8_lora_add) lora_add;
   decltype(&w4a8_kv4_tree) kv4_tree;
+  decltype(&w4a8_kv4_tree_attention_workspace_bytes) kv4_tree_attention_ws;
   decltype(&w4a8_kv4_tree_attention) kv4_tree_attention;
   decltype(&w4a8_kv4_copy_pages) kv4_copy_pages;
   decltype(&w4a8_kv4_keep) kv4_keep;
@@ -509,7 +510,8 @@ PyObject* attend(PyObject* const* a, PyObject* pcausal, PyObject* pwindow, PyObj
   if (PyErr_Occurred()) return nullptr;
   if (window < 0 || max_q < 0 || max_kv < 0) Py_RETURN_NONE;
   if (window) max_kv = std::min(max_kv, window + max_q);
-  const int64_t wsb = abi.kv4_attention_ws(T, Hq, c.H, c.D, c.B, max_q, max_kv);
+  const int64_t wsb = mask ? abi.kv4_tree_attention_ws(T, Hq, c.H, c.D, c.B, window, max_q, max_kv)
+                           : abi.kv4_attention_ws(T, Hq, c.H, c.D, c.B, max_q, max_kv);
   at::Tensor out = o ? *o : empty(*q, {T, Hq, c.D}, q->scalar_type()), lse, ws;
   if (want_lse) lse = empty(*q, {T, Hq}, at::kFloat);
   if (wsb > 0) ws = empty(*q, {wsb}, at::kByte);

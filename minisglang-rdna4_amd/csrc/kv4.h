@@ -86,6 +86,7 @@ struct Kv4Plan {
   int nq;
   int splits;      // of the tokens, over the grid
   int64_t qgrid;   // tiles of columns per sequence and head
+  bool wide;       // kv4_tree_attn_kernel, 256 columns a tile
 };
 
 // rows [start, start + n) of sequence b, kept inside the call's rows whatever cu holds
@@ -109,4 +110,36 @@ __device__ __forceinline__ int kv4_page(const Kv4Cache& c, const Kv4Batch& s, in
   return page >= 0 && page < c.pages ? page : -1;
 }
 
+// A sequence of the call: its rows and its length. Columns are its queries in order, G heads each.
+struct Span {
+  int64_t start;
+  int n, cols, len, first_pos;  // new tokens, columns, length, position of the first new token
+};
+template <bool TREE>
+__device__ __forceinline__ Span kv4_span(const Kv4Attn& p, int b) {
+  Span s;
+  kv4_rows(p.s, b, s.start, s.n);
+  s.cols = s.n * p.G;
+  const int64_t cap = (int64_t)p.s.width << p.c.shift;
+  const int len = max(p.s.lens[b], 0);  // -2^31 has no position n rows before it
+  // one token past the table's end stands for all of them: its page is missing (of a tree each node has its own)
+  s.len = len > cap ? (int)min((int64_t)len, cap + (TREE ? s.n + 1 : 1)) : len;
+  s.first_pos = len - s.n;
+  return s;
+}
+// Of a tree: the first cached key that query i sees, and its 8 bits of the tokens at .. at + 7, counted from the
+// first new one
+__device__ __forceinline__ int tree_from(const Kv4Attn& p, const Span& s, int i) {
+  if (!p.window) return 0;
+  const int64_t lo = (int64_t)p.pos[s.start + i] - p.window + 1;
+  return lo < 0 ? 0 : lo > 0x7fffffff ? 0x7fffffff : (int)lo;
+}
+__device__ __forceinline__ uint32_t tree_bits(const Kv4Attn& p, const Span& s, int i, int at) {
+  if (at <= -8 || at >= s.n) return 0;
+  const uint32_t* row = p.bits + (s.start + i) * p.ldb;
+  const int w = at >> 5;
+  const uint64_t lo = w >= 0 && w < p.words ? row[w] : 0, hi = w + 1 < p.words ? row[w + 1] : 0;
+  const uint32_t b = (uint32_t)((lo | (hi << 32)) >> (at & 31)) & 0xffu;
+  return s.n - at < 8 ? b & ((1u << (s.n - at)) - 1) : b;
+}
 }  // namespace w4a8

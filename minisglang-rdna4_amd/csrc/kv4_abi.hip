@@ -8,6 +8,7 @@ int launch_kv4_append(const void* k, int64_t ldk, int64_t hk, const void* v, int
                       const Kv4Cache& c, const Kv4Batch& s, hipStream_t st);
 int launch_kv4_read(const Kv4Cache& c, const Kv4Batch& s, int dtype, int D, void* k, void* v, hipStream_t st);
 Kv4Plan kv4_plan(int64_t T, int B, int H, int G, int D, int64_t max_q, int64_t max_kv);
+Kv4Plan kv4_tree_plan(int64_t T, int B, int H, int G, int D, int64_t window, int64_t max_q, int64_t max_kv);
 int64_t kv4_workspace(int64_t T, int Hq, int D, int splits);
 int launch_kv4_attention(Kv4Attn& p, int D, int dtype, const Kv4Plan& pl, void* ws, hipStream_t st);
 int launch_kv4_copy(const Kv4Caches& cs, int caches, const int32_t* src, const int32_t* dst, int64_t n, int64_t pages,
@@ -85,7 +86,8 @@ static int attend(const char* who, const void* q, int dtype, int64_t ldq, int64_
     return fail(kErrInvalid, "%s: q and out rows must be 16-byte aligned, with strides that are multiples of 8 elements", who);
   if (!apart(T, ldo, Hq, ho, D))
     return fail(kErrInvalid, "%s: out's rows overlap (strides %lld and %lld)", who, (long long)ldo, (long long)ho);
-  const Kv4Plan pl = kv4_plan(T, (int)B, (int)H, (int)(Hq / H), (int)D, max_q, max_kv);
+  const Kv4Plan pl = bits ? kv4_tree_plan(T, (int)B, (int)H, (int)(Hq / H), (int)D, window, max_q, max_kv)
+                          : kv4_plan(T, (int)B, (int)H, (int)(Hq / H), (int)D, max_q, max_kv);
   const int64_t need = kv4_workspace(T, (int)Hq, (int)D, pl.splits);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(kErrInvalid, "%s: needs a 16-byte aligned workspace of %lld bytes, got %lld", who, (long long)need,
@@ -195,6 +197,13 @@ int w4a8_kv4_tree(const int32_t* parents, int64_t T, const int32_t* cu, const in
   Kv4Batch s = {};
   s.cu = cu; s.lens = seq_lens; s.B = (int)B; s.T = T;
   return launched(launch_kv4_tree(parents, s, (int)words, (int)window, bits, positions, (hipStream_t)stream), who);
+}
+
+int64_t w4a8_kv4_tree_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t B, int64_t window,
+                                                int64_t max_q, int64_t max_kv) {
+  if (w4a8_kv4_attention_workspace_bytes(T, Hq, H, D, B, max_q, max_kv) < 0 || window < 0) return -1;
+  if (T == 0 || B == 0) return 0;
+  return kv4_workspace(T, (int)Hq, (int)D, kv4_tree_plan(T, (int)B, (int)H, (int)(Hq / H), (int)D, window, max_q, max_kv).splits);
 }
 
 int w4a8_kv4_tree_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_t T, int64_t Hq, int64_t H, int64_t D,

@@ -44,6 +44,8 @@
 
 namespace w4a8 {
 
+int launch_kv4_tree_attn(const Kv4Attn& p, int D, int dtype, int64_t qgrid, hipStream_t st);
+
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef uint32_t v4w __attribute__((ext_vector_type(4)));
 
@@ -139,23 +141,6 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2h));
 }
 
-// A sequence of the call: its rows and its length. Columns are its queries in order, G heads each.
-struct Span {
-  int64_t start;
-  int n, cols, len, first_pos;  // new tokens, columns, length, position of the first new token
-};
-template <bool TREE>
-__device__ __forceinline__ Span kv4_span(const Kv4Attn& p, int b) {
-  Span s;
-  kv4_rows(p.s, b, s.start, s.n);
-  s.cols = s.n * p.G;
-  const int64_t cap = (int64_t)p.s.width << p.c.shift;
-  const int len = max(p.s.lens[b], 0);  // -2^31 has no position n rows before it
-  // one token past the table's end stands for all of them: its page is missing (of a tree each node has its own)
-  s.len = len > cap ? (int)min((int64_t)len, cap + (TREE ? s.n + 1 : 1)) : len;
-  s.first_pos = len - s.n;
-  return s;
-}
 // the keys [from, upto) that query i of the span sees: a window past the table's end still has the missing token
 __device__ __forceinline__ int seen_from(const Kv4Attn& p, const Span& s, int i) {
   const int n = s.first_pos + i + 1;  // keys up to the query's own
@@ -181,21 +166,6 @@ __device__ __forceinline__ int kv4_query(const Kv4Attn& p, int i0, int r0, int x
   return i0 + i;
 }
 
-// Of a tree: the first cached key that query i sees, and its 8 bits of the tokens at .. at + 7, counted from the
-// first new one
-__device__ __forceinline__ int tree_from(const Kv4Attn& p, const Span& s, int i) {
-  if (!p.window) return 0;
-  const int64_t lo = (int64_t)p.pos[s.start + i] - p.window + 1;
-  return lo < 0 ? 0 : lo > 0x7fffffff ? 0x7fffffff : (int)lo;
-}
-__device__ __forceinline__ uint32_t tree_bits(const Kv4Attn& p, const Span& s, int i, int at) {
-  if (at <= -8 || at >= s.n) return 0;
-  const uint32_t* row = p.bits + (s.start + i) * p.ldb;
-  const int w = at >> 5;
-  const uint64_t lo = w >= 0 && w < p.words ? row[w] : 0, hi = w + 1 < p.words ? row[w + 1] : 0;
-  const uint32_t b = (uint32_t)((lo | (hi << 32)) >> (at & 31)) & 0xffu;
-  return s.n - at < 8 ? b & ((1u << (s.n - at)) - 1) : b;
-}
 // over the wave
 __device__ __forceinline__ int wave_min_i(int v) {
   v = min(v, dpp_i<kDppXor1>(v));
@@ -658,7 +628,7 @@ kv4_join_kernel(const Kv4Attn p) {
 // splits below one round. us: 512 new tokens on 8192 141 / 352, 7 chunks of 257 on up to 6001 155 / 205, 16 x 8 new
 // tokens on 4096 38 / 122; one prompt of 2048 fills the card, 121 (unsplit) / 130 in two.
 Kv4Plan kv4_plan(int64_t T, int B, int H, int G, int D, int64_t max_q, int64_t max_kv) {
-  Kv4Plan pl;
+  Kv4Plan pl = {};
   // a bound below the mean or past all rows is wrong: the workspace or the grid would grow with it
   if (max_q < (T + B - 1) / B) max_q = (T + B - 1) / B;
   if (max_q > T) max_q = T;
@@ -681,6 +651,24 @@ Kv4Plan kv4_plan(int64_t T, int B, int H, int G, int D, int64_t max_q, int64_t m
   return pl;
 }
 
+// A tree's: more than 128 columns without a window, and a context that is worth its tables, go to kv4_tree_attn_kernel, one
+// workgroup of 8 waves per CU, with as many splits as rounds of the card ask for (as above).
+Kv4Plan kv4_tree_plan(int64_t T, int B, int H, int G, int D, int64_t window, int64_t max_q, int64_t max_kv) {
+  Kv4Plan pl = kv4_plan(T, B, H, G, D, max_q, max_kv);
+  if (max_q < (T + B - 1) / B) max_q = (T + B - 1) / B;
+  const int64_t cols = (max_q < T ? max_q : T) * G;
+  if (window || D > 128 || cols <= 128 || max_kv < 512) return pl;
+  auto most = [](int64_t a, int64_t b) { return a > b ? a : b; };
+  auto least = [](int64_t a, int64_t b) { return a < b ? a : b; };
+  pl.wide = true;
+  pl.qgrid = (cols + 255) / 256;
+  const int64_t pairs = pl.qgrid * H * B, tiles = (max_kv + 63) / 64, round = 256;
+  int64_t s = round / pairs;
+  if (pairs < round) s = most(s, least(4, 1024 / pairs));
+  pl.splits = (int)most(least(least(s, tiles / 4), 64), 1);
+  return pl;
+}
+
 int64_t kv4_workspace(int64_t T, int Hq, int D, int splits) {
   return splits <= 1 ? 0 : (int64_t)splits * T * Hq * (D + 2) * 4;
 }
@@ -690,7 +678,10 @@ static int launch_dt(Kv4Attn& p, const Kv4Plan& pl, hipStream_t st) {
   const int64_t rows = p.s.T * p.c.H * p.G;
   if (pl.qgrid * pl.splits > kMaxGrid || (pl.splits > 1 && rows / 4 >= kMaxGrid)) return kErrUnsupported;
   const dim3 g((unsigned)(pl.qgrid * pl.splits), (unsigned)p.c.H, (unsigned)p.s.B), b(256);
-  if (pl.few) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 4, TREE>), g, b, 0, st, p);
+  if (pl.wide) {
+    const int rc = launch_kv4_tree_attn(p, D, DT, pl.qgrid, st);
+    if (rc) return rc;
+  } else if (pl.few) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 4, TREE>), g, b, 0, st, p);
   else if (pl.nq == 1) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 1, TREE>), g, b, 0, st, p);
   else hipLaunchKernelGGL((kv4_attn_kernel<D, DT, D == 256 ? 1 : 2, 1, TREE>), g, b, 0, st, p);
   if (hipPeekAtLastError() != hipSuccess) return kErrHip;

@@ -339,7 +339,8 @@ def kv4_attention(
 
     tree: the new tokens are drafted ones; a token sees the cached context before them and, of them, those that its
     row of ``tree.mask`` names (``causal`` says nothing then). window > 0 counts from ``tree.positions``, among cached
-    tokens: of the new ones the mask alone decides.
+    tokens: of the new ones the mask alone decides. With more than 128 queries that share a key (max_q times the heads of a
+    group) and no window, bf16 models' values below 2^-29 of their sequence's largest count as 0.
 
     max_q and max_kv, the most new tokens and the greatest length of a sequence, are what the host
     plans the launch by (default: T rows, and the table's capacity). Too large a bound costs time, too
@@ -388,7 +389,10 @@ def kv4_attention(
         max_kv = min(max_kv, window + max_q)
     lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     lib = _abi.load()
-    ws_bytes = int(lib.w4a8_kv4_attention_workspace_bytes(T, Hq, cache.num_kv_heads, D, B, max_q, max_kv))
+    if mask is None:
+        ws_bytes = int(lib.w4a8_kv4_attention_workspace_bytes(T, Hq, cache.num_kv_heads, D, B, max_q, max_kv))
+    else:
+        ws_bytes = int(lib.w4a8_kv4_tree_attention_workspace_bytes(T, Hq, cache.num_kv_heads, D, B, window, max_q, max_kv))
     ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes > 0 else None
     before = (q.data_ptr(), _abi.dtype_code(q.dtype), q.stride(0), q.stride(1), T, Hq, cache.num_kv_heads, D, *cache._ptrs(),
               cache.num_pages, cache.page_size, table, ldt, width, cu, lens, B, float(sm_scale))
