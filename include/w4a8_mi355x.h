@@ -383,7 +383,7 @@ int64_t w4a8_kv4_tree_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t H
 /* w4a8_kv4_attention where row i sees, of its sequence's new tokens, those whose bit is set in its row of bits (T, words; ldb
  * words between rows; bits past the new tokens count for nothing), and all cached tokens before the new ones; window > 0: of
  * those only the ones after positions[i] - window. Any bits are allowed; a row that sees nothing is 0, its lse -inf.
- * max_q * Hq / H above 128 without a window: bf16 values below 2^-29 of their sequence's largest count as 0. */
+ * max_q * Hq / H above 64 without a window: bf16 values below 2^-29 of their sequence's largest count as 0. */
 int w4a8_kv4_tree_attention(const void* q, int dtype, int64_t ldq, int64_t hq, int64_t T, int64_t Hq, int64_t H, int64_t D,
                             const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, int64_t pages,
                             int64_t page_size, const int32_t* table, int64_t ldt, int64_t width, const int32_t* cu,

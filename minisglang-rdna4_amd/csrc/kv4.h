@@ -86,7 +86,7 @@ struct Kv4Plan {
   int nq;
   int splits;      // of the tokens, over the grid
   int64_t qgrid;   // tiles of columns per sequence and head
-  bool wide;       // kv4_tree_attn_kernel, 256 columns a tile
+  int wide;        // waves of kv4_tree_attn_kernel, 32 columns each, or 0
 };
 
 // rows [start, start + n) of sequence b, kept inside the call's rows whatever cu holds
@@ -126,6 +126,20 @@ __device__ __forceinline__ Span kv4_span(const Kv4Attn& p, int b) {
   s.len = len > cap ? (int)min((int64_t)len, cap + (TREE ? s.n + 1 : 1)) : len;
   s.first_pos = len - s.n;
   return s;
+}
+// The sequence of the launch's z-th workgroups: the longest first, up to 64 sequences, so that short ones fill the launch's
+// end (more sequences even themselves out). The whole wave calls. us, in this order / as they come: 48 sequences of up to
+// 26 drafted tokens on up to 8192 193 / 269.
+__device__ __forceinline__ int kv4_longest(const Kv4Batch& s, int z) {
+  if (s.B > 64 || s.B == 1) return z;
+  const int lane = threadIdx.x & 63;
+  const int mine = lane < s.B ? s.lens[lane] : 0;
+  int before = 0;  // sequences that come before the lane's
+  for (int j = 0; j < s.B; ++j) {
+    const int other = __builtin_amdgcn_readlane(mine, j);
+    before += other > mine || (other == mine && j < lane);
+  }
+  return __builtin_ctzll(__ballot(before == z && lane < s.B));
 }
 // Of a tree: the first cached key that query i sees, and its 8 bits of the tokens at .. at + 7, counted from the
 // first new one

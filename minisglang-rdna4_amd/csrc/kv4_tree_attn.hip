@@ -1,15 +1,16 @@
-// Attention of many drafted tokens, more than 128 columns of them, over the 4-bit cache (layout: kv4.h). All of a sequence's
+// Attention of many drafted tokens, more than 64 columns of them, over the 4-bit cache (layout: kv4.h). All of a sequence's
 // drafted tokens see the same context and all of it, so all but the last tiles have no masks, and what a tile's keys share
 // need not be kept apart by column. (Fewer columns, and windows, are kv4_attn_kernel's.)
 //
-// The queries that share a key/value head are columns (column c: query c / G, head h G + c % G), 32 a wave, and the waves of a
-// workgroup share tiles of 64 tokens that are widened to fp16 once, in LDS:
-//   S = K' Q^T,  y = S + b sum(q),  p = 2^(y scale - M),  O += V'^T p   (32x32x16 products; tokens, then channels are rows).
+// The queries that share a key/value head are columns (column c: query c / G, head h G + c % G), 32 a wave, and the 4 or 8
+// waves of a workgroup share tiles of 64 tokens that are widened to fp16 once, in LDS:
+//   S = b sum(q) + K' Q^T,  p = 2^(S scale - M),  O += V'^T p   (32x32x16 products; tokens, then channels are rows).
 // K' = s (c - 7.5) as s/2 (2 c - 15), b = m + 7.5 s. bf16 models: s comes as s 2^-e, e one for the tile, so that it fits fp16: 8 bits
 // times the code's 4 lose one bit at most, 2^-11 of what is left once the middle of the vector's range is taken out; fp16
-// models, whose scores ought to be better than that, have K' = 2 c - 15, exactly, and y = s/2 S + b sum(q). V' = s c + m, rounded once to fp16 (2^-11), bf16
-// models' times 2^-e with e the largest so far; p is rounded to fp16, and its sum is of the rounded ones. Powers of two
-// change no bits, unless values of a bf16 model's context and drafts are more than 2^29 apart: the small ones are then lost.
+// models, whose scores ought to be better than that, have K' = 2 c - 15, exactly, b = 2 m / s + 15, and S times s/2 afterwards.
+// V' = s c + m, rounded once to fp16 (2^-11), bf16 models' times 2^-e with e the largest so far; p is rounded to fp16, and its
+// sum is of the rounded ones. Powers of two change no bits, unless values of a bf16 model's context and drafts are more than
+// 2^29 apart: the small ones are then lost.
 // Queries enter in fp16 with a power of two per row, as in kv4_attn_kernel.
 //
 // Codes become fp16 by an or into the lowest bits of 1024 and a packed subtraction. A word of K codes is 8 channels of a
@@ -17,7 +18,14 @@
 // nibbles 0, 4, 1, 5, 2, 6, 3, 7. Q's channels, and which token each row of S is, follow that order, and p goes from one product
 // into the next in its lane.
 // Codes of the next tile and scales of the one after the next are loaded while a tile is worked on, and widened behind it.
-// The scales are unpacked by two of the waves, by turns, a token a lane, into tables.
+// The scales are unpacked by two of the waves, by turns, a token a lane, into tables. What is read from LDS is read a product
+// or more ahead, exponentials run behind the products of the 16 tokens before them, and the next tile's widening behind the
+// last products: in the compiler's own order each product waited for its operands (us, in this order / in that one: 193 /
+// 207 for the first case below, 191 / 206 for the second).
+// us: 48 users' 26 tokens and less on up to 8192 (8 heads of 4 queries) 193, with kv4_attn_kernel 216; two users' 60 tokens
+// on 65536 and less, fp16, 191 / 279, 650 TFLOP/s. 4 waves for up to 128 columns: the second in two workgroups of those 211.
+// No unit is full: of a CU's time vector instructions take 54 %, matrix products 34 %, LDS 40 %; two waves a SIMD, which
+// the accumulators leave room for, do not cover each other's latencies.
 #include "kv4.h"
 #include "tile32.h"
 
@@ -65,7 +73,7 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
   __shared__ __align__(16) ScaleTable tab[3];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
-  const int h = blockIdx.y, b = blockIdx.z;
+  const int h = blockIdx.y, b = kv4_longest(p.s, blockIdx.z);
   const int splits = p.splits, split = blockIdx.x % splits;
   const Span sp = kv4_span<true>(p, b);
   if (sp.cols == 0) return;
@@ -86,6 +94,13 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
   auto unit_of = [&](int k, int u) {
     return block_of(__builtin_amdgcn_readlane((k >> 4) == group ? pages : ahead, (k & 15) * 4 + u), k, u);
   };
+  // K's words in the order of Place, 16 bytes of a row at a time
+  auto row_of = [](int at) {
+    return D == 64 ? ((at >> 6) & 1) * 8 + ((at >> 5) & 1) * 4 + ((at >> 2) & 3) : (at >> 6) * 4 + ((at >> 2) & 3);
+  };
+  auto chunk_of = [](int at) {
+    return D == 64 ? ((at >> 4) & 1) * 4 + ((at & 3) ^ ((at >> 5) & 1)) : ((at >> 4) & 3) * 4 + (at & 3);
+  };
   uint32_t kw[U], vw[U];
   const Masks ms = masks();
   auto load_codes = [&](int k) {
@@ -94,36 +109,45 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
       const int unit = (i * NT + wave * 64) / (2 * D), at = (i * NT + (int)threadIdx.x) & (2 * D - 1);
       const int x = unit_of(k, unit);
       const uint64_t base = (uint64_t)(x < 0 ? 0 : x) * (4 * D);  // block 0 is there; its values are not used
-      // lanes in the order of Place, 16 bytes of a row at a time
-      const int row = D == 64 ? ((at >> 6) & 1) * 8 + ((at >> 5) & 1) * 4 + ((at >> 2) & 3) : (at >> 6) * 4 + ((at >> 2) & 3);
-      const int chunk = D == 64 ? ((at >> 4) & 1) * 4 + ((at & 3) ^ ((at >> 5) & 1)) : ((at >> 4) & 3) * 4 + (at & 3);
-      kw[i] = *reinterpret_cast<const uint32_t*>(p.c.k + base + (row * (D / 8) + chunk) * 4);
+      kw[i] = *reinterpret_cast<const uint32_t*>(p.c.k + base + (row_of(at) * (D / 8) + chunk_of(at)) * 4);
       vw[i] = *reinterpret_cast<const uint32_t*>(p.c.v + base + at * 4);
     }
   };
-  auto widen = [&](const ScaleTable& tb, unsigned char* kd, unsigned char* vd) {
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int unit = (i * NT + wave * 64) / (2 * D), at = (i * NT + (int)threadIdx.x) & (2 * D - 1);
-      const int row = D == 64 ? ((at >> 6) & 1) * 8 + ((at >> 5) & 1) * 4 + ((at >> 2) & 3) : (at >> 6) * 4 + ((at >> 2) & 3);
-      const int chunk = D == 64 ? ((at >> 4) & 1) * 4 + ((at & 3) ^ ((at >> 5) & 1)) : ((at >> 4) & 3) * 4 + (at & 3);
-      v4w x;
-      const v2h ks = __builtin_bit_cast(v2h, kFold ? tb.ks[unit * 16 + row] : 0u);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const v2h c = centred(kw[i], j, ms);
-        x[j] = __builtin_bit_cast(uint32_t, kFold ? c * ks : c);
-      }
-      *reinterpret_cast<v4w*>(kd + P::at(unit * 16 + row, chunk)) = x;
+  // piece j of 2 U of the next tile: a word of K, or one of V
+  struct Steps {
+    v4w s, m;
+  };
+  auto steps_of = [&](const ScaleTable& tb, int j) {
+    const int i = j >> 1, unit = (i * NT + wave * 64) / (2 * D), at = (i * NT + (int)threadIdx.x) & (2 * D - 1);
+    Steps r = {};
+    if (j & 1) {
       const int blk = unit * 2 + at / D;
-      const v4w sv = *reinterpret_cast<const v4w*>(&tb.v[blk][0]), mv = *reinterpret_cast<const v4w*>(&tb.v[blk][4]);
+      r.s = *reinterpret_cast<const v4w*>(&tb.v[blk][0]);
+      r.m = *reinterpret_cast<const v4w*>(&tb.v[blk][4]);
+    } else if (kFold) {
+      r.s[0] = tb.ks[unit * 16 + row_of(at)];
+    }
+    return r;
+  };
+  auto widen = [&](const Steps& sm, int j, unsigned char* kd, unsigned char* vd) {
+    const int i = j >> 1, unit = (i * NT + wave * 64) / (2 * D), at = (i * NT + (int)threadIdx.x) & (2 * D - 1);
+    v4w x;
+    if (j & 1) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t s2 = sv[j], m2 = mv[j];
-        x[j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(codes_of(vw[i], j, ms), __builtin_bit_cast(v2h, s2),
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t s2 = sm.s[e], m2 = sm.m[e];
+        x[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(codes_of(vw[i], e, ms), __builtin_bit_cast(v2h, s2),
                                                                       __builtin_bit_cast(v2h, m2)));
       }
       *reinterpret_cast<v4w*>(vd + unit * (32 * D) + at * 16) = x;
+    } else {
+      const uint32_t s2 = sm.s[0];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const v2h c = centred(kw[i], e, ms);
+        x[e] = __builtin_bit_cast(uint32_t, kFold ? c * __builtin_bit_cast(v2h, s2) : c);
+      }
+      *reinterpret_cast<v4w*>(kd + P::at(unit * 16 + row_of(at), chunk_of(at))) = x;
     }
   };
   // two of the waves, others in the next tile: a token's scales, of K and of V
@@ -159,8 +183,14 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
         tb.ks[lane] = x | (x << 16);
       }
       const int r = (lane >> 5) * 32 + ((lane >> 3) & 1) * 16 + ((lane >> 4) & 1) * 8 + (nib < 4 ? 2 * nib : 2 * nib - 7);
-      tb.b[r] = !in ? 0.f : bad ? __builtin_nanf("") : __builtin_ldexpf(c0, -e);
-      if (!kFold) tb.s[r] = 0.5f * s;
+      if (kFold) {
+        tb.b[r] = !in ? 0.f : bad ? __builtin_nanf("") : __builtin_ldexpf(c0, -e);
+      } else {
+        // a vector of equal values has no step, and codes of 0: any small one does
+        const float s2 = fmaxf(0.5f * s, fmaxf(fabsf(m0) * 0x1p-30f, 0x1p-60f));
+        tb.b[r] = !in ? 0.f : bad ? __builtin_nanf("") : m0 / s2 + 15.f;
+        tb.s[r] = s2;
+      }
       if (lane == 0) tb.ek = e;
     } else {
       const bool use = in && !bad;
@@ -188,6 +218,10 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
     const int c = qi * kCols + wave * 32 + col;
     const bool on = c < sp.cols;
     const int i = on ? c / p.G : 0, head = h * p.G + (on ? c - i * p.G : 0);
+    const uint16_t* qp = p.q + (sp.start + i) * p.ldq + head * p.hq + half * 8;
+    uint4 qr[KS];
+#pragma unroll
+    for (int w = 0; w < KS; ++w) qr[w] = on ? *reinterpret_cast<const uint4*>(qp + 16 * w) : make_uint4(0, 0, 0, 0);
     group = 0;
     pages = look_up(0);
     ahead = look_up(1);
@@ -199,10 +233,6 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
     v4w qf[KS];
     float qs, sc;
     {
-      const uint16_t* qp = p.q + (sp.start + i) * p.ldq + head * p.hq + half * 8;
-      uint4 qr[KS];
-#pragma unroll
-      for (int w = 0; w < KS; ++w) qr[w] = on ? *reinterpret_cast<const uint4*>(qp + 16 * w) : make_uint4(0, 0, 0, 0);
       float sum = 0.f, top = 0.f;
 #pragma unroll
       for (int w = 0; w < KS; ++w) {
@@ -232,14 +262,36 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
     for (int d = 0; d < CT; ++d) o[d] = v16f{};
     float m = -kInf, thr = -kInf, mu = 0.f, l = 0.f;  // m: the maximum as a score over scale, times the query's power of two
     int ev = -100;
+    // S starts as b sum(q)
+    v16f s[2];
+    auto start = [&](const ScaleTable& tb) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const float* tbl = &tb.b[kb * 32 + half * 16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kb][r] = tbl[r] * qs;
+      }
+    };
+    auto v_operand = [&](const unsigned char* vc, int f, int d) { return lds_read(vc + v_lane + (2 * f * D + 32 * d) * 16); };
+    auto in_order = [] { __builtin_amdgcn_sched_barrier(0); };  // the compiler would have each read of LDS wait where it is used
     __syncthreads();
     unpack_scales(1, tab[1], tab[0]);
     load_scales(2);
-    if (count) widen(tab[0], kt[0], vt[0]);
+#pragma unroll
+    for (int j = 0; j < 2 * U; ++j) widen(steps_of(tab[0], j), j, kt[0], vt[0]);
+    start(tab[0]);
     __syncthreads();
 
     for (int k = 0; k < count; ++k) {
-      if (k + 1 < count) load_codes(k + 1);
+      const ScaleTable& tb = tab[k % 3];
+      const unsigned char* kc = kt[k & 1];
+      const unsigned char* vc = vt[k & 1];
+      const int t0 = (split + k * splits) * kStep;
+      v4w ka[KS], va[CT];
+#pragma unroll
+      for (int w = 0; w < KS; ++w) ka[w] = lds_read(kc + k_lane + P::at(0, 2 * w));
+      in_order();
+      load_codes(k + 1);  // behind the last tile: of block 0, for nobody
       unpack_scales(k + 2, tab[(k + 2) % 3], tab[(k + 1) % 3]);
       load_scales(k + 3);
       if (((k + 2) & 15) == 0) {  // the next iteration's codes are the next group's first
@@ -247,10 +299,6 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
         ahead = look_up(++group + 1);
       }
 
-      const ScaleTable& tb = tab[k % 3];
-      const unsigned char* kc = kt[k & 1];
-      const unsigned char* vc = vt[k & 1];
-      const int t0 = (split + k * splits) * kStep;
       float fe = 1.f;
       if (kFold) {
         const int now = __builtin_amdgcn_readfirstlane(tb.ev);
@@ -263,64 +311,102 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
         fe = __builtin_ldexpf(1.f, __builtin_amdgcn_readfirstlane(tb.ek));
       }
       const float sct = sc * fe;
+      in_order();
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        if (t0 + 32 * kb >= sp.len) break;
-        v16f s = v16f{};
+      for (int w = 0; w < KS; ++w) {
+        s[0] = mfma32<kF16>(ka[w], qf[w], s[0]);
+        ka[w] = lds_read(kc + k_lane + P::at(32, 2 * w));
+        in_order();
+      }
 #pragma unroll
-        for (int w = 0; w < KS; ++w) s = mfma32<kF16>(lds_read(kc + k_lane + P::at(32 * kb, 2 * w)), qf[w], s);
-        const float* tbl = &tb.b[kb * 32 + half * 16];
-        const float* tsl = &tb.s[kb * 32 + half * 16];
+      for (int w = 0; w < KS; ++w) {
+        s[1] = mfma32<kF16>(ka[w], qf[w], s[1]);
+        if (w < CT) va[w] = v_operand(vc, 0, w);
+        in_order();
+      }
+      if (!kFold) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[r] = kFold ? __builtin_fmaf(tbl[r], qs, s[r]) : __builtin_fmaf(tsl[r], s[r], tbl[r] * qs);
-        if (t0 + 32 * kb + 32 > first) {
+        for (int kb = 0; kb < 2; ++kb) {
+          const float* tsl = &tb.s[kb * 32 + half * 16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kb][r] *= tsl[r];
+        }
+      }
+      if (t0 + kStep > first) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int s2 = 0; s2 < 2; ++s2) {
             const int at = t0 + 32 * kb + 16 * s2 + 8 * half, old = first - at;  // tokens of the context among the 8
             const uint32_t see = (on ? tree_bits(p, sp, i, at - sp.first_pos) : 0u) | (old <= 0 ? 0u : old >= 8 ? 255u : (1u << old) - 1);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[8 * s2 + e] = see >> ((e >> 1) + 4 * (e & 1)) & 1 ? s[8 * s2 + e] : -kInf;
+            for (int e = 0; e < 8; ++e) s[kb][8 * s2 + e] = see >> ((e >> 1) + 4 * (e & 1)) & 1 ? s[kb][8 * s2 + e] : -kInf;
+          }
+      }
+      float top = -kInf;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
+      top *= fe;
+      if (__ballot(top > thr)) {
+        const float tp = pair_max(top);
+        // a column that has no need keeps its bits, whatever its neighbours do
+        const bool need = tp > thr;
+        const float mn = need ? fmaxf(m, tp) : m;
+        const float was = far_off(m, sc), is = far_off(mn, sc);
+        const float mun = need ? (mn == -kInf || is != 0.f ? 0.f : mn * sc) : mu;
+        const float f = m == -kInf ? 1.f : __builtin_amdgcn_exp2f(__builtin_fmaf(was - is, sc, mu - mun));
+        m = mn;
+        mu = mun;
+        thr = is != 0.f ? -kInf : mn + 8.f / sc;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < CT; ++d) o[d] *= f;
+        const float back = is / fe;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[0][r] -= back;
+          s[1][r] -= back;
+        }
+      }
+      // Exponentials run behind products of the ones before them, and the next tile is widened behind the last ones.
+      v4w pf[4];
+      auto two = [&](int x) {  // p of values 2 x and 2 x + 1 of the 32
+        const v16f& sv = s[x >> 3];
+        const int e = (2 * x) & 15;
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], sct, -mu));
+        const float z = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e + 1], sct, -mu));
+        const uint32_t w = pack16<kF16>(a, z);
+        pf[x >> 2][x & 3] = w;
+        l = add_pair<kF16>(w, l);
+      };
+#pragma unroll
+      for (int x = 0; x < 4; ++x) two(x);
+      const ScaleTable& tn = tab[(k + 1) % 3];
+      Steps sm[2];
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int d = 0; d < CT; ++d) {
+          in_order();
+          o[d] = mfma32<kF16>(va[d], pf[f], o[d]);
+          if (f < 3) {
+            va[d] = v_operand(vc, f + 1, d);
+#pragma unroll
+            for (int x = 0; x < 4 / CT; ++x) two(4 * f + 4 + d * (4 / CT) + x);
+          }
+          if (f == 2 && d < 2) sm[d] = steps_of(tn, d);
+          if (f == 3 && d < 2 * U) {
+            widen(sm[d & 1], d, kt[(k + 1) & 1], vt[(k + 1) & 1]);
+            if (d + 2 < 2 * U) sm[d & 1] = steps_of(tn, d + 2);
           }
         }
-        float top = -kInf;
+      in_order();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
-        top *= fe;
-        if (__ballot(top > thr)) {
-          const float tp = pair_max(top);
-          // a column that has no need keeps its bits, whatever its neighbours do
-          const bool need = tp > thr;
-          const float mn = need ? fmaxf(m, tp) : m;
-          const float was = far_off(m, sc), is = far_off(mn, sc);
-          const float mun = need ? (mn == -kInf || is != 0.f ? 0.f : mn * sc) : mu;
-          const float f = m == -kInf ? 1.f : __builtin_amdgcn_exp2f(__builtin_fmaf(was - is, sc, mu - mun));
-          m = mn;
-          mu = mun;
-          thr = is != 0.f ? -kInf : mn + 8.f / sc;
-          l *= f;
-#pragma unroll
-          for (int d = 0; d < CT; ++d) o[d] *= f;
-          const float back = is / fe;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] -= back;
-        }
-        v4w pf[2];
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sct, -mu));
-          const float z = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], sct, -mu));
-          const uint32_t w = pack16<kF16>(a, z);
-          pf[r >> 3][(r & 7) >> 1] = w;
-          l = add_pair<kF16>(w, l);
-        }
-#pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-          for (int d = 0; d < CT; ++d)
-            o[d] = mfma32<kF16>(lds_read(vc + v_lane + ((4 * kb + 2 * s2) * D + 32 * d) * 16), pf[s2], o[d]);
+      for (int j = CT; j < 2 * U; ++j) {
+        widen(sm[j & 1], j, kt[(k + 1) & 1], vt[(k + 1) & 1]);
+        if (j + 2 < 2 * U) sm[j & 1] = steps_of(tn, j + 2);
       }
-      if (k + 1 < count) widen(tab[(k + 1) % 3], kt[(k + 1) & 1], vt[(k + 1) & 1]);
+      start(tn);
       __syncthreads();
     }
 
@@ -358,17 +444,18 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
 }
 
 template <int D, int DT>
-static int launch_dt(const Kv4Attn& p, int64_t qgrid, hipStream_t st) {
-  if (qgrid * p.splits > kMaxGrid / 2) return kErrUnsupported;
-  const dim3 g((unsigned)(qgrid * p.splits), (unsigned)p.c.H, (unsigned)p.s.B);
-  hipLaunchKernelGGL((kv4_tree_attn_kernel<D, DT, 8>), g, dim3(512), 0, st, p);
+static int launch_dt(const Kv4Attn& p, const Kv4Plan& pl, hipStream_t st) {
+  if (pl.qgrid * p.splits > kMaxGrid / 2) return kErrUnsupported;
+  const dim3 g((unsigned)(pl.qgrid * p.splits), (unsigned)p.c.H, (unsigned)p.s.B);
+  if (pl.wide == 4) hipLaunchKernelGGL((kv4_tree_attn_kernel<D, DT, 4>), g, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((kv4_tree_attn_kernel<D, DT, 8>), g, dim3(512), 0, st, p);
   return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 
-// qgrid: tiles of 256 columns per sequence and head
-int launch_kv4_tree_attn(const Kv4Attn& p, int D, int dtype, int64_t qgrid, hipStream_t st) {
-  if (dtype == kBF16) return D == 64 ? launch_dt<64, kBF16>(p, qgrid, st) : launch_dt<128, kBF16>(p, qgrid, st);
-  return D == 64 ? launch_dt<64, kF16>(p, qgrid, st) : launch_dt<128, kF16>(p, qgrid, st);
+// pl: that of a tree (kv4_tree_plan), its workgroups of 4 or 8 waves
+int launch_kv4_tree_attn(const Kv4Attn& p, int D, int dtype, const Kv4Plan& pl, hipStream_t st) {
+  if (dtype == kBF16) return D == 64 ? launch_dt<64, kBF16>(p, pl, st) : launch_dt<128, kBF16>(p, pl, st);
+  return D == 64 ? launch_dt<64, kF16>(p, pl, st) : launch_dt<128, kF16>(p, pl, st);
 }
 
 }  // namespace w4a8

@@ -339,7 +339,7 @@ def kv4_attention(
 
     tree: the new tokens are drafted ones; a token sees the cached context before them and, of them, those that its
     row of ``tree.mask`` names (``causal`` says nothing then). window > 0 counts from ``tree.positions``, among cached
-    tokens: of the new ones the mask alone decides. With more than 128 queries that share a key (max_q times the heads of a
+    tokens: of the new ones the mask alone decides. With more than 64 queries that share a key (max_q times the heads of a
     group) and no window, bf16 models' values below 2^-29 of their sequence's largest count as 0.
 
     max_q and max_kv, the most new tokens and the greatest length of a sequence, are what the host
