@@ -22,8 +22,8 @@
 // or more ahead, exponentials run behind the products of the 16 tokens before them, and the next tile's widening behind the
 // last products: in the compiler's own order each product waited for its operands (us, in this order / in that one: 193 /
 // 207 for the first case below, 191 / 206 for the second).
-// us: 48 users' 26 tokens and less on up to 8192 (8 heads of 4 queries) 193, with kv4_attn_kernel 216; two users' 60 tokens
-// on 65536 and less, fp16, 191 / 279, 650 TFLOP/s. 4 waves for up to 128 columns: the second in two workgroups of those 211.
+// us: 48 users' 26 tokens and less on up to 8192 (8 heads of 4 queries) 192, with kv4_attn_kernel 216; two users' 60 tokens
+// on 65536 and less, fp16, 185 (waves without columns wait, else 191) / 279, 670 TFLOP/s. 4 waves for up to 128 columns: the second in two workgroups of those 211.
 // No unit is full: of a CU's time vector instructions take 54 %, matrix products 34 %, LDS 40 %; two waves a SIMD, which
 // the accumulators leave room for, do not cover each other's latencies.
 #include "kv4.h"
@@ -282,6 +282,24 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
     start(tab[0]);
     __syncthreads();
 
+    auto fetch = [&](int k) {  // of the tiles after k
+      load_codes(k + 1);  // behind the last tile: of block 0, for nobody
+      unpack_scales(k + 2, tab[(k + 2) % 3], tab[(k + 1) % 3]);
+      load_scales(k + 3);
+      if (((k + 2) & 15) == 0) {  // the next iteration's codes are the next group's first
+        pages = ahead;
+        ahead = look_up(++group + 1);
+      }
+    };
+    if (qi * kCols + wave * 32 >= sp.cols) {  // no columns: only the wave's part of the tiles
+      for (int k = 0; k < count; ++k) {
+        fetch(k);
+#pragma unroll
+        for (int j = 0; j < 2 * U; ++j) widen(steps_of(tab[(k + 1) % 3], j), j, kt[(k + 1) & 1], vt[(k + 1) & 1]);
+        __syncthreads();
+      }
+      continue;
+    }
     for (int k = 0; k < count; ++k) {
       const ScaleTable& tb = tab[k % 3];
       const unsigned char* kc = kt[k & 1];
@@ -291,13 +309,7 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
 #pragma unroll
       for (int w = 0; w < KS; ++w) ka[w] = lds_read(kc + k_lane + P::at(0, 2 * w));
       in_order();
-      load_codes(k + 1);  // behind the last tile: of block 0, for nobody
-      unpack_scales(k + 2, tab[(k + 2) % 3], tab[(k + 1) % 3]);
-      load_scales(k + 3);
-      if (((k + 2) & 15) == 0) {  // the next iteration's codes are the next group's first
-        pages = ahead;
-        ahead = look_up(++group + 1);
-      }
+      fetch(k);
 
       float fe = 1.f;
       if (kFold) {
