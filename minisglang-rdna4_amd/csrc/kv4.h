@@ -49,6 +49,7 @@ struct Kv4Attn {
   uint16_t* out;
   int64_t ldo, ho;
   float* lse;       // (T, Hq) or null
+  float lse_more;   // what kv4_join_kernel adds to it
   Kv4Cache c;
   Kv4Batch s;
   int G;            // query heads per key/value head
@@ -81,6 +82,9 @@ struct Kv4Caches {
 
 // How a call is cut. few: 16 columns and the waves of a workgroup over the tokens; else nq * 16 columns per
 // wave, the waves side by side.
+// kv4_tree_attn_kernel's parts are 2^-15 of the sums, which then stay in f32 where the values do
+constexpr float kWidePart = 0x1p-15f, kWideLse = 15.f * 0.69314718055994531f;
+
 struct Kv4Plan {
   bool few;
   int nq;

@@ -612,7 +612,7 @@ kv4_join_kernel(const Kv4Attn p) {
   uint16_t* op = p.out + row * p.ldo + head * p.ho + lane * E;
 #pragma unroll
   for (int e = 0; e < E; ++e) op[e] = to_dtype(o[e] * inv, DT);
-  if (p.lse && lane == 0) p.lse[id] = l == 0.f ? -__builtin_inff() : mn * 0.69314718055994531f + logf(l);
+  if (p.lse && lane == 0) p.lse[id] = l == 0.f ? -__builtin_inff() : mn * 0.69314718055994531f + logf(l) + p.lse_more;
 }
 
 // Splits of the tokens. Decode (3 workgroups of 4 waves per CU, 768 on the card): one round of the card, and up to
@@ -686,6 +686,7 @@ static int launch_dt(Kv4Attn& p, const Kv4Plan& pl, hipStream_t st) {
   if (pl.qgrid * pl.splits > kMaxGrid || (pl.splits > 1 && rows / 4 >= kMaxGrid)) return kErrUnsupported;
   const dim3 g((unsigned)(pl.qgrid * pl.splits), (unsigned)p.c.H, (unsigned)p.s.B), b(256);
   if (pl.wide) {
+    p.lse_more = kWideLse;
     const int rc = launch_kv4_tree_attn(p, D, DT, pl, st);
     if (rc) return rc;
   } else if (pl.few) hipLaunchKernelGGL((kv4_attn_kernel<D, DT, 1, 4, TREE>), g, b, 0, st, p);

@@ -8,8 +8,9 @@
 // K' = s (c - 7.5) as s/2 (2 c - 15), b = m + 7.5 s. bf16 models: s comes as s 2^-e, e one for the tile, so that it fits fp16: 8 bits
 // times the code's 4 lose one bit at most, 2^-11 of what is left once the middle of the vector's range is taken out; fp16
 // models, whose scores ought to be better than that, have K' = 2 c - 15, exactly, b = 2 m / s + 15, and S times s/2 afterwards.
-// V' = s c + m, rounded once to fp16 (2^-11), bf16 models' times 2^-e with e the largest so far; p is rounded to fp16, and its
-// sum is of the rounded ones. Powers of two change no bits, unless values of a bf16 model's context and drafts are more than
+// V' = s c + m, rounded once to fp16 (2^-11), times 2^-e with e the largest so far; p is rounded to fp16, and its sum is of the
+// rounded ones: 2^7 and more for the largest score, so that what is lost below fp16's least, 2^-32 of that a token, is nothing
+// over any context. Powers of two change no bits, unless values of a bf16 model's context and drafts are more than
 // 2^29 apart: the small ones are then lost.
 // Queries enter in fp16 with a power of two per row, as in kv4_attn_kernel.
 //
@@ -23,7 +24,8 @@
 // last products: in the compiler's own order each product waited for its operands (us, in this order / in that one: 193 /
 // 207 for the first case below, 191 / 206 for the second).
 // us: 48 users' 26 tokens and less on up to 8192 (8 heads of 4 queries) 192, with kv4_attn_kernel 216; two users' 60 tokens
-// on 65536 and less, fp16, 185 (waves without columns wait, else 191) / 279, 670 TFLOP/s. 4 waves for up to 128 columns: the second in two workgroups of those 211.
+// on 65536 and less, fp16, 185 (waves without columns wait, else 191) / 279, 670 TFLOP/s; in twice as many workgroups of
+// 4 waves 211.
 // No unit is full: of a CU's time vector instructions take 54 %, matrix products 34 %, LDS 40 %; two waves a SIMD, which
 // the accumulators leave room for, do not cover each other's latencies.
 #include "kv4.h"
@@ -67,6 +69,8 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
   constexpr int KS = D / 16, CT = D / 32, kCols = 32 * NW, NT = 64 * NW;
   constexpr int U = 8 * D / NT;     // words of K, and of V, of a thread and tile
   constexpr bool kFold = DT == kBF16;
+  constexpr int kLeastEv = DT == kBF16 ? -100 : 0;  // fp16 models: only what s c + m takes past fp16's end needs an e
+  constexpr float kMost = 7.f;  // p is 2^7 and up to 2^15 (what may come before M follows) for the largest score
   constexpr float kInf = __builtin_inff();
   __shared__ __align__(16) unsigned char kt[2][P::kBytes];
   __shared__ __align__(16) unsigned char vt[2][kStep * D * 2];
@@ -195,13 +199,8 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
     } else {
       const bool use = in && !bad;
       const float s = use ? s1 : 0.f, m = use ? m1 : 0.f;
-      int ev_run = k == 0 ? -100 : last.ev;
-      if (kFold) {
-        const float most = wave_max(fmaxf(fabsf(m), fabsf(__builtin_fmaf(15.f, s, m))));
-        ev_run = max(ev_run, min((int)(__float_as_uint(most) >> 23) - 141, 120));
-      } else {
-        ev_run = 0;
-      }
+      const float most = wave_max(fmaxf(fabsf(m), fabsf(__builtin_fmaf(15.f, s, m))));
+      const int ev_run = max(k == 0 ? kLeastEv : last.ev, min((int)(__float_as_uint(most) >> 23) - 141, 120));
       uint16_t* v = reinterpret_cast<uint16_t*>(&tb.v[lane >> 3][0]) + (nib & 3) * 2 + (nib >> 2);
       v[0] = f32_to_f16(__builtin_ldexpf(s, -ev_run));
       v[8] = f32_to_f16(__builtin_ldexpf(m, -ev_run));
@@ -261,7 +260,7 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
 #pragma unroll
     for (int d = 0; d < CT; ++d) o[d] = v16f{};
     float m = -kInf, thr = -kInf, mu = 0.f, l = 0.f;  // m: the maximum as a score over scale, times the query's power of two
-    int ev = -100;
+    int ev = kLeastEv;
     // S starts as b sum(q)
     v16f s[2];
     auto start = [&](const ScaleTable& tb) {
@@ -311,17 +310,14 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
       in_order();
       fetch(k);
 
-      float fe = 1.f;
-      if (kFold) {
-        const int now = __builtin_amdgcn_readfirstlane(tb.ev);
-        if (now != ev) {
-          const float f = __builtin_ldexpf(1.f, ev - now);
+      const int now = __builtin_amdgcn_readfirstlane(tb.ev);
+      if (now != ev) {
+        const float f = __builtin_ldexpf(1.f, ev - now);
 #pragma unroll
-          for (int d = 0; d < CT; ++d) o[d] *= f;
-          ev = now;
-        }
-        fe = __builtin_ldexpf(1.f, __builtin_amdgcn_readfirstlane(tb.ek));
+        for (int d = 0; d < CT; ++d) o[d] *= f;
+        ev = now;
       }
+      const float fe = kFold ? __builtin_ldexpf(1.f, __builtin_amdgcn_readfirstlane(tb.ek)) : 1.f;
       const float sct = sc * fe;
       in_order();
 #pragma unroll
@@ -365,7 +361,7 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
         const bool need = tp > thr;
         const float mn = need ? fmaxf(m, tp) : m;
         const float was = far_off(m, sc), is = far_off(mn, sc);
-        const float mun = need ? (mn == -kInf || is != 0.f ? 0.f : mn * sc) : mu;
+        const float mun = need ? (mn == -kInf || is != 0.f ? 0.f : __builtin_fmaf(mn, sc, -kMost)) : mu;
         const float f = m == -kInf ? 1.f : __builtin_amdgcn_exp2f(__builtin_fmaf(was - is, sc, mu - mun));
         m = mn;
         mu = mun;
@@ -425,19 +421,20 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
     l = pair_sum(l);
     if (on) {
       const int Hq = p.c.H * p.G;
-      const float back = kFold ? __builtin_ldexpf(1.f, ev) : 1.f, is = far_off(m, sc);
+      const float back = __builtin_ldexpf(1.f, ev), is = far_off(m, sc);
       const float most = m == -kInf ? -kInf : is != 0.f ? is * sc : mu;
       if (splits > 1) {
         const int64_t at = ((int64_t)split * p.s.T + sp.start + i) * Hq + head;
         float* op = p.po + at * D + half * 4;
+        const float part = back * kWidePart;
 #pragma unroll
         for (int d = 0; d < CT; ++d)
 #pragma unroll
           for (int r = 0; r < 16; r += 4)
-            *reinterpret_cast<v4f*>(op + d * 32 + 2 * r) = v4f{o[d][r] * back, o[d][r + 1] * back, o[d][r + 2] * back, o[d][r + 3] * back};
+            *reinterpret_cast<v4f*>(op + d * 32 + 2 * r) = v4f{o[d][r] * part, o[d][r + 1] * part, o[d][r + 2] * part, o[d][r + 3] * part};
         if (half == 0) {
           p.pml[at * 2] = most;
-          p.pml[at * 2 + 1] = l;
+          p.pml[at * 2 + 1] = l * kWidePart;
         }
       } else {
         const float inv = l == 0.f ? 0.f : back / l;  // no key seen: 0

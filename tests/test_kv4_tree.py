@@ -357,3 +357,71 @@ def test_out_rows_streams_and_refusals(dev):
         kv4.kv4_tree(parents, s.d_cu[:2], s.d_seq, max_q=6)
     none = kv4.kv4_tree(parents[:0], s.d_cu * 0, s.d_seq, max_q=6)
     assert none.mask.shape == (0, 1) and none.positions.shape == (0,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_kv", [512, 2000])
+def test_wide_trees_at_the_ends_of_fp16(dev, max_kv):
+    """fp16 vectors from the least to the greatest number, whose steps and least values give 65536, and many small weights
+    beside a great one."""
+    lens, news = [2000], [40]
+    s = Setup(dev, torch.float16, 128, 1, 64, lens, news, seed=3)
+    s.v[100::7, 0, 0], s.v[100::7, 0, 5] = 65504, -65504
+    s.k[:], s.k[::16, 0, 0] = 0, 0.25
+    s.k[50, 0, 0] = 16
+    _kv4().kv4_append(s.cache, s.k.to(dev), s.v.to(dev), s.d_table, s.cu_all.to(dev), s.d_seq)
+    q = torch.zeros(40, 4, 128, dtype=torch.float16)
+    q[:, :2, 0] = 11  # one score is 17.6 above the others; the other heads weigh all the same
+    tree = _kv4().kv4_tree(torch.full((40,), -1, dtype=torch.int32, device=dev), s.d_cu, s.d_seq, max_q=40)
+    see = [[i] for i in range(40)]
+    out, lse = s.attend(q, tree=tree, max_q=40, max_kv=max_kv, sm_scale=0.1, return_lse=True)
+    want, rl, A, _ = ref(q, cache_values(s.cache), s.table, s.page, lens, news, see, tree.positions.tolist(), 0.1, bounds=True)
+    assert torch.isfinite(want).all() and (want.abs() > 2.0 ** -6 * 65504).any()
+    assert ((out.cpu().double() - want).abs() <= 2.0 ** -11 * (2.5 * A + 2 * want.abs()) + 2.0 ** -24).all()
+    assert (lse.cpu().double() - rl).abs().max().item() < 2e-4 + 2.0 ** -11
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_wide_trees_in_place_and_padded(dev, dtype):
+    """The output in q's place; a sequence with one token, one with none and one that is all new beside a long one; rows
+    behind the last sequence; a captured launch replayed over other lengths; the same rows whatever lies beside them."""
+    lens, news = [1200, 33, 0, 70, 900], [60, 1, 0, 70, 33]
+    s = Setup(dev, dtype, 128, 2, 32, lens, news, seed=8)
+    rng = random.Random(8)
+    trees = [random_tree(n, rng) for n in news]
+    see = [x for t in trees for x in lines(t)]
+    parents = torch.tensor([p for t in trees for p in t], dtype=torch.int32, device=dev)
+    tree = _kv4().kv4_tree(parents, s.d_cu, s.d_seq, max_q=70)
+    q = s.q(8)
+    a = check(s, q, tree, see, max_q=70, max_kv=1200)
+    T = sum(news)
+    mine = torch.full((T + 5, 8, 128), 7.0, dtype=dtype, device=dev)
+    mine[:T] = q.to(dev)
+    big = _kv4().KV4Tree(torch.cat([tree.mask, tree.mask[:5]]), torch.cat([tree.positions, tree.positions[:5]]))
+    kw = dict(max_q=70, max_kv=1200, tree=big)
+    _kv4().kv4_attention(mine, s.cache, s.d_table, s.d_cu, s.d_seq, out=mine, **kw)
+    assert torch.equal(mine[:T], a) and (mine[T:] == 7).all()
+    # replays over other contexts of the same tokens
+    q2, seq, out = q.to(dev), s.d_seq.clone(), torch.empty_like(q, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        s_kw = dict(max_q=70, max_kv=1200, tree=tree, out=out)
+        _kv4().kv4_attention(q2, s.cache, s.d_table, s.d_cu, seq, **s_kw)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _kv4().kv4_attention(q2, s.cache, s.d_table, s.d_cu, seq, **s_kw)
+    for less in (0, 100, 7, 0):
+        seq.copy_(torch.tensor([lens[0] - less] + lens[1:], dtype=torch.int32))
+        out.fill_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = out.clone()
+        torch.empty(1 << 20, device=dev).normal_()
+        _kv4().kv4_attention(q2, s.cache, s.d_table, s.d_cu, seq, **s_kw)
+        assert torch.equal(replayed, out)
+        assert torch.equal(replayed[60:], a[60:])
+    assert torch.equal(out, a)
