@@ -8,8 +8,10 @@
 // K' = s (c - 7.5) as s/2 (2 c - 15), b = m + 7.5 s. bf16 models: s comes as s 2^-e, e one for the tile, so that it fits fp16: 8 bits
 // times the code's 4 lose one bit at most, 2^-11 of what is left once the middle of the vector's range is taken out; fp16
 // models, whose scores ought to be better than that, have K' = 2 c - 15, exactly, b = 2 m / s + 15, and S times s/2 afterwards.
-// V' = s c + m, rounded once to fp16 (2^-11), times 2^-e with e the largest so far; p is rounded to fp16, and its sum is of the
-// rounded ones: 2^7 and more for the largest score, so that what is lost below fp16's least, 2^-32 of that a token, is nothing
+// V' = s c + m, rounded once to fp16 (2^-11), times 2^-e with e the largest so far; fp16 models have the codes, exactly, p s
+// rounded instead (times 2^-e, e of the largest step so far) and sum p (m + 7.5 s) beside the product, its middles in fp16: their output would show the
+// rounding of V' (norm of the error over the output's 3.5e-4, so 2.6e-4, of which rounding the output is 2.1e-4).
+// p is rounded to fp16, and its sum is of the rounded ones: 2^7 and more for the largest score, so that what is lost below fp16's least, 2^-32 of that a token, is nothing
 // over any context. Powers of two change no bits, unless values of a bf16 model's context and drafts are more than
 // 2^29 apart: the small ones are then lost.
 // Queries enter in fp16 with a power of two per row, as in kv4_attn_kernel.
@@ -21,13 +23,12 @@
 // Codes of the next tile and scales of the one after the next are loaded while a tile is worked on, and widened behind it.
 // The scales are unpacked by two of the waves, by turns, a token a lane, into tables. What is read from LDS is read a product
 // or more ahead, exponentials run behind the products of the 16 tokens before them, and the next tile's widening behind the
-// last products: in the compiler's own order each product waited for its operands (us, in this order / in that one: 193 /
-// 207 for the first case below, 191 / 206 for the second).
-// us: 48 users' 26 tokens and less on up to 8192 (8 heads of 4 queries) 192, with kv4_attn_kernel 216; two users' 60 tokens
-// on 65536 and less, fp16, 185 (waves without columns wait, else 191) / 279, 670 TFLOP/s; in twice as many workgroups of
-// 4 waves 211.
-// No unit is full: of a CU's time vector instructions take 54 %, matrix products 34 %, LDS 40 %; two waves a SIMD, which
-// the accumulators leave room for, do not cover each other's latencies.
+// last products: in the compiler's own order each product waited for its operands (14 us more in either case below).
+// us: 48 users' 26 tokens and less on up to 8192 (8 heads of 4 queries, bf16) 191, with kv4_attn_kernel 216; two users' 60
+// tokens on 65536 and less, fp16, 202 (with V' rounded as bf16 models have it 187) / 279, 620 TFLOP/s. Waves without columns
+// only widen: 6 us of the second. No unit is full: of a CU's time vector instructions take 54 %, matrix products 34 %, LDS
+// 40 %; two waves a SIMD, which the accumulators leave room for, do not cover each other's latencies. Tried: the waves of a
+// SIMD half a tile apart, so that one has products while the other has exponentials (no faster).
 #include "kv4.h"
 #include "tile32.h"
 
@@ -35,11 +36,15 @@ namespace w4a8 {
 
 constexpr int kStep = 64;  // tokens of a tile
 
-struct alignas(16) ScaleTable {
+typedef float v8f __attribute__((ext_vector_type(8)));
+
+struct alignas(32) ScaleTable {
   float b[kStep];        // in the order of S's rows: [32 tokens][half][16 registers]
   float s[kStep];        // fp16 models: half of K's steps in that order
   uint32_t ks[kStep];    // bf16 models: half of K's step, twice, by token
-  uint32_t v[8][8];      // V's steps of tokens j and j + 4 of the block (j < 4), and their least values
+  uint32_t v[8][8];      // bf16 models: V's steps of tokens j and j + 4 of the block (j < 4), and their least values
+  float sv[kStep];       // fp16 models: V's steps, in the order of S's rows,
+  uint16_t bv[kStep];    // and the middles m + 7.5 s, in fp16
   int ek, ev;
 };
 
@@ -69,12 +74,12 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
   constexpr int KS = D / 16, CT = D / 32, kCols = 32 * NW, NT = 64 * NW;
   constexpr int U = 8 * D / NT;     // words of K, and of V, of a thread and tile
   constexpr bool kFold = DT == kBF16;
-  constexpr int kLeastEv = DT == kBF16 ? -100 : 0;  // fp16 models: only what s c + m takes past fp16's end needs an e
+  constexpr int kLeastEv = -100;
   constexpr float kMost = 7.f;  // p is 2^7 and up to 2^15 (what may come before M follows) for the largest score
   constexpr float kInf = __builtin_inff();
   __shared__ __align__(16) unsigned char kt[2][P::kBytes];
   __shared__ __align__(16) unsigned char vt[2][kStep * D * 2];
-  __shared__ __align__(16) ScaleTable tab[3];
+  __shared__ __align__(32) ScaleTable tab[3];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
   const int h = blockIdx.y, b = kv4_longest(p.s, blockIdx.z);
@@ -125,6 +130,7 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
     const int i = j >> 1, unit = (i * NT + wave * 64) / (2 * D), at = (i * NT + (int)threadIdx.x) & (2 * D - 1);
     Steps r = {};
     if (j & 1) {
+      if (!kFold) return r;
       const int blk = unit * 2 + at / D;
       r.s = *reinterpret_cast<const v4w*>(&tb.v[blk][0]);
       r.m = *reinterpret_cast<const v4w*>(&tb.v[blk][4]);
@@ -140,7 +146,8 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t s2 = sm.s[e], m2 = sm.m[e];
-        x[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(codes_of(vw[i], e, ms), __builtin_bit_cast(v2h, s2),
+        if (!kFold) x[e] = __builtin_bit_cast(uint32_t, centred(vw[i], e, ms));
+        else x[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(codes_of(vw[i], e, ms), __builtin_bit_cast(v2h, s2),
                                                                       __builtin_bit_cast(v2h, m2)));
       }
       *reinterpret_cast<v4w*>(vd + unit * (32 * D) + at * 16) = x;
@@ -176,6 +183,7 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
     const float c0 = __builtin_fmaf(7.5f, s0, m0);
     const bool bad = bad_v || !__builtin_isfinite(s0) || !__builtin_isfinite(c0);
     const int nib = lane & 7;
+    const int r = (lane >> 5) * 32 + ((lane >> 3) & 1) * 16 + ((lane >> 4) & 1) * 8 + (nib < 4 ? 2 * nib : 2 * nib - 7);
     if (turn(k) == 0) {
       const float s = in && !bad ? s0 : 0.f;
       int e = 0;
@@ -186,7 +194,6 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
         const uint32_t x = (uint32_t)f32_to_f16(__builtin_ldexpf(s, -e - 1));
         tb.ks[lane] = x | (x << 16);
       }
-      const int r = (lane >> 5) * 32 + ((lane >> 3) & 1) * 16 + ((lane >> 4) & 1) * 8 + (nib < 4 ? 2 * nib : 2 * nib - 7);
       if (kFold) {
         tb.b[r] = !in ? 0.f : bad ? __builtin_nanf("") : __builtin_ldexpf(c0, -e);
       } else {
@@ -199,11 +206,17 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
     } else {
       const bool use = in && !bad;
       const float s = use ? s1 : 0.f, m = use ? m1 : 0.f;
-      const float most = wave_max(fmaxf(fabsf(m), fabsf(__builtin_fmaf(15.f, s, m))));
-      const int ev_run = max(k == 0 ? kLeastEv : last.ev, min((int)(__float_as_uint(most) >> 23) - 141, 120));
-      uint16_t* v = reinterpret_cast<uint16_t*>(&tb.v[lane >> 3][0]) + (nib & 3) * 2 + (nib >> 2);
-      v[0] = f32_to_f16(__builtin_ldexpf(s, -ev_run));
-      v[8] = f32_to_f16(__builtin_ldexpf(m, -ev_run));
+      // bf16 models: the largest value into [2^14, 2^15); fp16 models: the largest step into [1/2, 1)
+      const float most = wave_max(kFold ? fmaxf(fabsf(m), fabsf(__builtin_fmaf(15.f, s, m))) : s);
+      const int ev_run = max(k == 0 ? kLeastEv : last.ev, min((int)(__float_as_uint(most) >> 23) - (kFold ? 141 : 126), 120));
+      if (kFold) {
+        uint16_t* v = reinterpret_cast<uint16_t*>(&tb.v[lane >> 3][0]) + (nib & 3) * 2 + (nib >> 2);
+        v[0] = f32_to_f16(__builtin_ldexpf(s, -ev_run));
+        v[8] = f32_to_f16(__builtin_ldexpf(m, -ev_run));
+      } else {
+        tb.sv[r] = __builtin_ldexpf(s, -ev_run);
+        tb.bv[r] = f32_to_f16(__builtin_fmaf(7.5f, s, m));
+      }
       if (lane == 0) tb.ev = ev_run;
     }
   };
@@ -259,8 +272,10 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
     v16f o[CT];
 #pragma unroll
     for (int d = 0; d < CT; ++d) o[d] = v16f{};
+    float bo = 0.f;  // fp16 models: sum of p (m + 7.5 s)
     float m = -kInf, thr = -kInf, mu = 0.f, l = 0.f;  // m: the maximum as a score over scale, times the query's power of two
     int ev = kLeastEv;
+    auto in_order = [] { __builtin_amdgcn_sched_barrier(0); };  // the compiler would have each read of LDS wait where it is used
     // S starts as b sum(q)
     v16f s[2];
     auto start = [&](const ScaleTable& tb) {
@@ -268,11 +283,22 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
       for (int kb = 0; kb < 2; ++kb) {
         const float* tbl = &tb.b[kb * 32 + half * 16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[kb][r] = tbl[r] * qs;
+        for (int r = 0; r < 16; ++r) s[kb][r] = tbl[r];
       }
+      in_order();
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) s[kb] *= qs;
+    };
+    // of 8 of a lane's 32 values of S
+    struct Weights {
+      v8f s;
+      v4w b;
+    };
+    auto weights = [&](const ScaleTable& tb, int g) {
+      const int at = (g >> 1) * 32 + half * 16 + (g & 1) * 8;
+      return Weights{*reinterpret_cast<const v8f*>(&tb.sv[at]), *reinterpret_cast<const v4w*>(&tb.bv[at])};
     };
     auto v_operand = [&](const unsigned char* vc, int f, int d) { return lds_read(vc + v_lane + (2 * f * D + 32 * d) * 16); };
-    auto in_order = [] { __builtin_amdgcn_sched_barrier(0); };  // the compiler would have each read of LDS wait where it is used
     __syncthreads();
     unpack_scales(1, tab[1], tab[0]);
     load_scales(2);
@@ -305,6 +331,7 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
       const unsigned char* vc = vt[k & 1];
       const int t0 = (split + k * splits) * kStep;
       v4w ka[KS], va[CT];
+      Weights ws[2];
 #pragma unroll
       for (int w = 0; w < KS; ++w) ka[w] = lds_read(kc + k_lane + P::at(0, 2 * w));
       in_order();
@@ -330,6 +357,7 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
       for (int w = 0; w < KS; ++w) {
         s[1] = mfma32<kF16>(ka[w], qf[w], s[1]);
         if (w < CT) va[w] = v_operand(vc, 0, w);
+        if (!kFold && w >= KS - 2) ws[w & 1] = weights(tb, w & 1);
         in_order();
       }
       if (!kFold) {
@@ -367,6 +395,7 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
         mu = mun;
         thr = is != 0.f ? -kInf : mn + 8.f / sc;
         l *= f;
+        bo *= f;
 #pragma unroll
         for (int d = 0; d < CT; ++d) o[d] *= f;
         const float back = is / fe;
@@ -384,8 +413,10 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
         const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], sct, -mu));
         const float z = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e + 1], sct, -mu));
         const uint32_t w = pack16<kF16>(a, z);
-        pf[x >> 2][x & 3] = w;
         l = add_pair<kF16>(w, l);
+        const Weights& ww = ws[(x >> 2) & 1];
+        if (!kFold) bo = add_pair_of(w, ww.b[x & 3], bo);
+        pf[x >> 2][x & 3] = kFold ? w : pack16<kF16>(a * ww.s[(2 * x) & 7], z * ww.s[(2 * x + 1) & 7]);
       };
 #pragma unroll
       for (int x = 0; x < 4; ++x) two(x);
@@ -402,6 +433,7 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
 #pragma unroll
             for (int x = 0; x < 4 / CT; ++x) two(4 * f + 4 + d * (4 / CT) + x);
           }
+          if (!kFold && f < 2 && d == 0) ws[f] = weights(tb, f + 2);
           if (f == 2 && d < 2) sm[d] = steps_of(tn, d);
           if (f == 3 && d < 2 * U) {
             widen(sm[d & 1], d, kt[(k + 1) & 1], vt[(k + 1) & 1]);
@@ -419,32 +451,35 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
     }
 
     l = pair_sum(l);
+    bo = pair_sum(bo);
     if (on) {
       const int Hq = p.c.H * p.G;
-      const float back = __builtin_ldexpf(1.f, ev), is = far_off(m, sc);
+      const float back = __builtin_ldexpf(1.f, kFold ? ev : ev - 1), is = far_off(m, sc);
       const float most = m == -kInf ? -kInf : is != 0.f ? is * sc : mu;
       if (splits > 1) {
         const int64_t at = ((int64_t)split * p.s.T + sp.start + i) * Hq + head;
         float* op = p.po + at * D + half * 4;
-        const float part = back * kWidePart;
+        const float part = back * kWidePart, more = bo * kWidePart;
 #pragma unroll
         for (int d = 0; d < CT; ++d)
 #pragma unroll
           for (int r = 0; r < 16; r += 4)
-            *reinterpret_cast<v4f*>(op + d * 32 + 2 * r) = v4f{o[d][r] * part, o[d][r + 1] * part, o[d][r + 2] * part, o[d][r + 3] * part};
+            *reinterpret_cast<v4f*>(op + d * 32 + 2 * r) = v4f{__builtin_fmaf(o[d][r], part, more), __builtin_fmaf(o[d][r + 1], part, more),
+                                                              __builtin_fmaf(o[d][r + 2], part, more), __builtin_fmaf(o[d][r + 3], part, more)};
         if (half == 0) {
           p.pml[at * 2] = most;
           p.pml[at * 2 + 1] = l * kWidePart;
         }
       } else {
-        const float inv = l == 0.f ? 0.f : back / l;  // no key seen: 0
+        const float inv = l == 0.f ? 0.f : back / l, more = l == 0.f ? 0.f : bo / l;  // no key seen: 0
         uint16_t* op = p.out + (sp.start + i) * p.ldo + head * p.ho + half * 4;
 #pragma unroll
         for (int d = 0; d < CT; ++d)
 #pragma unroll
           for (int r = 0; r < 16; r += 4)
             *reinterpret_cast<v2w*>(op + d * 32 + 2 * r) =
-                v2w{pack16<DT>(o[d][r] * inv, o[d][r + 1] * inv), pack16<DT>(o[d][r + 2] * inv, o[d][r + 3] * inv)};
+                v2w{pack16<DT>(__builtin_fmaf(o[d][r], inv, more), __builtin_fmaf(o[d][r + 1], inv, more)),
+                    pack16<DT>(__builtin_fmaf(o[d][r + 2], inv, more), __builtin_fmaf(o[d][r + 3], inv, more))};
         if (p.lse && half == 0)
           p.lse[(sp.start + i) * Hq + head] = l == 0.f ? -kInf : most * 0.69314718055994531f + logf(l);
       }

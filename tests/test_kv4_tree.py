@@ -3,7 +3,10 @@ the GPU bits and positions against a walk up the tree, and attention against 64 
 
 Tolerances. Up to 64 columns (queries times heads that share a key), and with a window, the ones that attention over the
 cache is tested with. More columns: with A = sum p |v| / sum p, the output o is off by
-  - V' = s c + m rounded to fp16, 2^-11 A; p rounded to fp16, and its sum, 2^-11 (A + |o|);
+  - p rounded to fp16, and its sum, 2^-11 (A + |o|);
+  - bf16 models: V' = s c + m rounded to fp16, 2^-11 A;
+  - fp16 models instead: p s rounded to fp16, 2^-11 of sum p |v - mid| / sum p, mid the middle of the value's range;
+    mid and the p that it is summed with, both rounded to fp16: 2^-11 2 sum p |mid| / sum p;
   - bf16 models: s (c - 7.5), 8 bits by 4, rounded to fp16's 11, 2^-11 of it: a score is off by d = 2^-11 scale sum |q| |k - mid|,
     mid the middle of the key's range, p by d of itself and o by d (A + |o|);
   - 2^-25 of the largest cached value's power of two where V' is subnormal, and f32's sums and exponentials, 2^-12 A here,
@@ -52,7 +55,7 @@ def ref(q, kv, table, page, lens, news, see, positions, scale, window=0, bounds=
     H = k.shape[1]
     T, Hq, D = q.shape
     G = Hq // H
-    out, A = torch.zeros(T, Hq, D, dtype=torch.float64), torch.zeros(T, Hq, D, dtype=torch.float64)
+    out, A, C = (torch.zeros(T, Hq, D, dtype=torch.float64) for _ in range(3))
     lse, d = torch.full((T, Hq), -math.inf, dtype=torch.float64), torch.zeros(T, Hq, 1, dtype=torch.float64)
     row = 0
     for b, (n, new) in enumerate(zip(lens, news)):
@@ -74,18 +77,20 @@ def ref(q, kv, table, page, lens, news, see, positions, scale, window=0, bounds=
             x = (kk * q[r].double().unsqueeze(1)).sum(-1) * scale
             pr = torch.softmax(x, 1).unsqueeze(-1)
             out[r], A[r] = (pr * vv).sum(1), (pr * vv.abs()).sum(1)
+            half = (vv.amax(-1, keepdim=True) + vv.amin(-1, keepdim=True)) / 2
+            C[r] = (pr * ((vv - half).abs() + 2 * half.abs())).sum(1)
             lse[r] = torch.logsumexp(x, 1)
             mid = (kk.amax(-1, keepdim=True) + kk.amin(-1, keepdim=True)) / 2
             d[r, :, 0] = ((kk - mid).abs() * q[r].double().abs().unsqueeze(1)).sum(-1).amax(1) * scale * 2.0 ** -11
         row += new
-    return (out, lse, A, d) if bounds else (out, lse)
+    return (out, lse, A, C, d) if bounds else (out, lse)
 
 
 def check(s, q, tree, see, window=0, lse_of_nan=True, **kw):
     out, lse = s.attend(q, tree=tree, window=window, return_lse=True, **kw)
     D = s.cache.head_dim
     scale = kw.get("sm_scale", D ** -0.5)
-    want, rl, A, d = ref(q, cache_values(s.cache), s.table, s.page, s.lens, s.news, see, tree.positions.tolist(), scale, window, True)
+    want, rl, A, C, d = ref(q, cache_values(s.cache), s.table, s.page, s.lens, s.news, see, tree.positions.tolist(), scale, window, True)
     nan = torch.isnan(want)
     assert torch.equal(torch.isnan(out.cpu()), nan)
     eps = 2.0 ** (-8 if q.dtype == torch.bfloat16 else -11)
@@ -95,7 +100,8 @@ def check(s, q, tree, see, window=0, lse_of_nan=True, **kw):
     wide = not window and D <= 128 and rows * (q.shape[1] // s.cache.num_kv_heads) > 64
     if wide:
         d = d if q.dtype == torch.bfloat16 else torch.zeros_like(d)
-        rest = torch.maximum(rest, 2.0 ** -11 * (2.5 * A + want.abs()) + d * (A + want.abs()) + 2.0 ** -25 * max(vmax, 2.0 ** -24))
+        rounded = 2 * A if q.dtype == torch.bfloat16 else C
+        rest = torch.maximum(rest, 2.0 ** -11 * (rounded + 0.5 * A + want.abs()) + d * (A + want.abs()) + 2.0 ** -25 * max(vmax, 2.0 ** -24))
     err = (out.cpu().double() - want).abs() - eps * want.abs() - rest - 2.0 ** -25
     assert err[~nan].numel() == 0 or err[~nan].max().item() <= 0, f"off by {err[~nan].max().item():.3e} past the tolerance"
     lf = torch.isfinite(rl)
@@ -375,9 +381,14 @@ def test_wide_trees_at_the_ends_of_fp16(dev, max_kv):
     tree = _kv4().kv4_tree(torch.full((40,), -1, dtype=torch.int32, device=dev), s.d_cu, s.d_seq, max_q=40)
     see = [[i] for i in range(40)]
     out, lse = s.attend(q, tree=tree, max_q=40, max_kv=max_kv, sm_scale=0.1, return_lse=True)
-    want, rl, A, _ = ref(q, cache_values(s.cache), s.table, s.page, lens, news, see, tree.positions.tolist(), 0.1, bounds=True)
+    want, rl, A, C, _ = ref(q, cache_values(s.cache), s.table, s.page, lens, news, see, tree.positions.tolist(), 0.1, bounds=True)
     assert torch.isfinite(want).all() and (want.abs() > 2.0 ** -6 * 65504).any()
-    assert ((out.cpu().double() - want).abs() <= 2.0 ** -11 * (2.5 * A + 2 * want.abs()) + 2.0 ** -24).all()
+    # a weight below fp16's normal numbers is off by 2^-25 at most, where the largest, and so their sum, is 2^7 at least
+    at = torch.arange(lens[0])
+    v = cache_values(s.cache)[1][s.table[0, at // 64].long(), 0, at % 64]
+    mid = (v.amax(-1, keepdim=True) + v.amin(-1, keepdim=True)) / 2
+    least = 2.0 ** -32 * ((v - mid).abs() + mid.abs()).sum(0)
+    assert ((out.cpu().double() - want).abs() <= 2.0 ** -11 * (C + 0.5 * A + 2 * want.abs()) + least + 2.0 ** -24).all()
     assert (lse.cpu().double() - rl).abs().max().item() < 2e-4 + 2.0 ** -11
 
 
