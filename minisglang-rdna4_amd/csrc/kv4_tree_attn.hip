@@ -8,12 +8,12 @@
 // K' = s (c - 7.5) as s/2 (2 c - 15), b = m + 7.5 s. bf16 models: s comes as s 2^-e, e one for the tile, so that it fits fp16: 8 bits
 // times the code's 4 lose one bit at most, 2^-11 of what is left once the middle of the vector's range is taken out; fp16
 // models, whose scores ought to be better than that, have K' = 2 c - 15, exactly, b = 2 m / s + 15, and S times s/2 afterwards.
-// V' = s c + m, rounded once to fp16 (2^-11), times 2^-e with e the largest so far; fp16 models have the codes, exactly, p s
-// rounded instead (times 2^-e, e of the largest step so far) and sum p (m + 7.5 s) beside the product, its middles in fp16: their output would show the
-// rounding of V' (norm of the error over the output's 3.5e-4, so 2.6e-4, of which rounding the output is 2.1e-4).
-// p is rounded to fp16, and its sum is of the rounded ones: 2^7 and more for the largest score, so that what is lost below fp16's least, 2^-32 of that a token, is nothing
-// over any context. Powers of two change no bits, unless values of a bf16 model's context and drafts are more than
-// 2^29 apart: the small ones are then lost.
+// V' = s c + m, rounded once to fp16 (2^-11), times 2^-e with e the largest so far. fp16 models have the codes, exactly, p s
+// rounded instead (times 2^-e, e of the largest step so far) and sum p (m + 7.5 s) beside the product, its middles in fp16: their
+// output would show the rounding of V' (norm of the error over the output's 3.5e-4, so 3.0e-4; rounding the output 2.1e-4).
+// p is rounded to fp16, and its sum is of the rounded ones: 2^7 and more for the largest score, so that what is lost below
+// fp16's least, 2^-32 of that a token, is nothing over any context. Powers of two change no bits, unless values of a bf16
+// model's context and drafts are more than 2^29 apart: the small ones are then lost.
 // Queries enter in fp16 with a power of two per row, as in kv4_attn_kernel.
 //
 // Codes become fp16 by an or into the lowest bits of 1024 and a packed subtraction. A word of K codes is 8 channels of a
@@ -25,7 +25,7 @@
 // or more ahead, exponentials run behind the products of the 16 tokens before them, and the next tile's widening behind the
 // last products: in the compiler's own order each product waited for its operands (14 us more in either case below).
 // us: 48 users' 26 tokens and less on up to 8192 (8 heads of 4 queries, bf16) 191, with kv4_attn_kernel 216; two users' 60
-// tokens on 65536 and less, fp16, 202 (with V' rounded as bf16 models have it 187) / 279, 620 TFLOP/s. Waves without columns
+// tokens on 65536 and less, fp16, 205 (with V' rounded as bf16 models have it 187) / 279, 610 TFLOP/s. Waves without columns
 // only widen: 6 us of the second. No unit is full: of a CU's time vector instructions take 54 %, matrix products 34 %, LDS
 // 40 %; two waves a SIMD, which the accumulators leave room for, do not cover each other's latencies. Tried: the waves of a
 // SIMD half a tile apart, so that one has products while the other has exponentials (no faster).
@@ -415,7 +415,12 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
         const uint32_t w = pack16<kF16>(a, z);
         l = add_pair<kF16>(w, l);
         const Weights& ww = ws[(x >> 2) & 1];
-        if (!kFold) bo = add_pair_of(w, ww.b[x & 3], bo);
+        if (!kFold) {
+          const uint32_t mid = ww.b[x & 3];
+          const v2h h = __builtin_bit_cast(v2h, mid);
+          bo = __builtin_fmaf(a, (float)h.x, bo);
+          bo = __builtin_fmaf(z, (float)h.y, bo);
+        }
         pf[x >> 2][x & 3] = kFold ? w : pack16<kF16>(a * ww.s[(2 * x) & 7], z * ww.s[(2 * x + 1) & 7]);
       };
 #pragma unroll

@@ -43,15 +43,6 @@ __device__ __forceinline__ float add_pair(uint32_t w, float c) {
 #endif
 }
 
-// and of two products of fp16 pairs
-__device__ __forceinline__ float add_pair_of(uint32_t w, uint32_t v, float c) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), __builtin_bit_cast(v2h, v), c, false);
-#else
-  return c;
-#endif
-}
-
 // over the two lanes that hold a column (xor 32)
 __device__ __forceinline__ float pair_max(float v) {
   auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);

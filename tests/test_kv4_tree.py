@@ -6,7 +6,7 @@ cache is tested with. More columns: with A = sum p |v| / sum p, the output o is 
   - p rounded to fp16, and its sum, 2^-11 (A + |o|);
   - bf16 models: V' = s c + m rounded to fp16, 2^-11 A;
   - fp16 models instead: p s rounded to fp16, 2^-11 of sum p |v - mid| / sum p, mid the middle of the value's range;
-    mid and the p that it is summed with, both rounded to fp16: 2^-11 2 sum p |mid| / sum p;
+    mid rounded to fp16, and summed with p as it is but divided by the rounded ones' sum: 2^-11 2 sum p |mid| / sum p;
   - bf16 models: s (c - 7.5), 8 bits by 4, rounded to fp16's 11, 2^-11 of it: a score is off by d = 2^-11 scale sum |q| |k - mid|,
     mid the middle of the key's range, p by d of itself and o by d (A + |o|);
   - 2^-25 of the largest cached value's power of two where V' is subnormal, and f32's sums and exponentials, 2^-12 A here,
@@ -436,3 +436,26 @@ def test_wide_trees_in_place_and_padded(dev, dtype):
         assert torch.equal(replayed, out)
         assert torch.equal(replayed[60:], a[60:])
     assert torch.equal(out, a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,D", [(1024, 64), (16384, 128), (131072, 64), (131072, 128)])
+@pytest.mark.parametrize("T,kw", [(16, {}), (16, {"max_kv": 512}), (40, {"max_kv": 512})])
+def test_wide_trees_error_does_not_grow_with_the_length(dev, dtype, n, D, T, kw):
+    """As test_kv4_accuracy has it, a norm over the output's, of 8 T columns that all see everything. Beside the output's one
+    rounding, fp16's 2^-11 is 2^-11 / sqrt(3) = 2.8e-4 in the square's mean. bf16 models: of p, of V' and, in a score, of
+    K' (sqrt(D) terms of |q| 1.5 and |k| 1 at a scale of D^-1/2: 4.2e-4 of p), together 5.8e-4. fp16 models: of p s (c - 7.5),
+    whose square's mean is below 1.1 times a value's variance, 3e-4; of the range's middle and of the sum that divides it,
+    twice of less than a third of a value, 1.3e-4; sums 1.5e-4 (test_kv4_accuracy): 3.6e-4."""
+    from test_kv4_accuracy import _case
+    for scale in (0.0, 1.5):
+        cache, table, cu, seq, q, want = _case(dev, dtype, n, D, 8, T, scale)
+        tree = _kv4().KV4Tree(torch.full((T, 2), -1, dtype=torch.int32, device=dev), torch.zeros(T, dtype=torch.int32, device=dev))
+        out = _kv4().kv4_attention(q, cache, table, cu, seq, tree=tree, **kw).double()
+        norm = want.norm().item()
+        rounding = ((want.to(dtype).double() - want).norm() / norm).item()
+        err = ((out - want).norm() / norm).item()
+        extra = 5.8e-4 if dtype == torch.bfloat16 else 3.6e-4
+        print(f"{dtype} n={n} D={D} T={T} {kw} q={scale}: {err:.3e} rounding {rounding:.3e}", flush=True)
+        assert err <= math.hypot(rounding, extra), f"{err:.3e}, of which the rounding is {rounding:.3e} (queries of {scale})"
