@@ -191,7 +191,7 @@ kv4_append_kernel(const uint16_t* __restrict__ k, int64_t ldk, int64_t hk, const
 // exact) and one to the type. A row without a place in the cache (before the sequence's first token,
 // on a page that does not exist) is NaN. A vector per D / 8 lanes; a wave has 8 rows (ROWS), which as a rule are one block's and
 // share its words of V, and `per` heads of them: row -> sequence -> page, dependent reads, are looked up once for all of those.
-// 131072 rows of 8 heads of 128 (142 MB in, 537 out) 137 us, 5.0 TB/s; 232 with a lookup for every 4 vectors.
+// 131072 rows of 8 heads of 128 (142 MB in, 537 out) 143 us, 4.75 TB/s; 232 with a lookup for every 4 vectors.
 template <int D, int DT, int ROWS>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(Kv4Cache c, Kv4Batch s, int per, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {

@@ -7,7 +7,7 @@ namespace w4a8 {
 
 // ---- pages: a workgroup copies 1024 vectors of 16 bytes of one pair's page, 4 a lane and all in flight, of its K codes, its
 // V codes, or its scales (K's, then V's). Nothing branches before the loads, so that what they wait for is read at once:
-// the pair, the cache's pointers. 64 pairs of 17 KB in 4 layers 6 us (18.8 with 2048 vectors a workgroup over all four arrays
+// the pair, the cache's pointers. 64 pairs of 17 KB in 4 layers 4.4 us (18.8 with 2048 vectors a workgroup over all four arrays
 // in a row, whose places were worked out one after another).
 constexpr int kCopyPart = 1024;  // vectors of a workgroup
 
