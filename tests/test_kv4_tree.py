@@ -459,3 +459,29 @@ def test_wide_trees_error_does_not_grow_with_the_length(dev, dtype, n, D, T, kw)
         extra = 5.8e-4 if dtype == torch.bfloat16 else 3.6e-4
         print(f"{dtype} n={n} D={D} T={T} {kw} q={scale}: {err:.3e} rounding {rounding:.3e}", flush=True)
         assert err <= math.hypot(rounding, extra), f"{err:.3e}, of which the rounding is {rounding:.3e} (queries of {scale})"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,H,G,page,B", [(128, 2, 5, 16, 70), (64, 1, 7, 2048, 64), (128, 1, 32, 128, 3)])
+def test_wide_trees_many_sequences_and_strides(dev, dtype, D, H, G, page, B):
+    """More sequences than are put in order, and as many; heads that divide nothing; pages shorter and longer than tiles; q and
+    out as columns of wider rows."""
+    rng = random.Random(B)
+    news = [rng.choice((0, 1, 5, 14, 20)) for _ in range(B)]
+    lens = [n + rng.choice((0, 0, 3, 60, 64, 200, 700)) for n in news]
+    s = Setup(dev, dtype, D, H, page, lens, news, seed=B)
+    trees = [random_tree(n, rng) for n in news]
+    see = [x for t in trees for x in lines(t)]
+    parents = torch.tensor([p for t in trees for p in t], dtype=torch.int32, device=dev)
+    tree = _kv4().kv4_tree(parents, s.d_cu, s.d_seq, max_q=20)
+    q = s.q(H * G)
+    out = check(s, q, tree, see, max_q=20, max_kv=max(520, max(lens)))
+    T = sum(news)
+    wide = torch.zeros(T, (H * G + 3) * D + 16, dtype=dtype, device=dev)
+    mine = wide[:, 8:8 + H * G * D].view(T, H * G, D)
+    mine.copy_(q)
+    to = torch.full((T, 2 * H * G, D + 8), 5.0, dtype=dtype, device=dev)
+    _kv4().kv4_attention(mine, s.cache, s.d_table, s.d_cu, s.d_seq, tree=tree, max_q=20, max_kv=max(520, max(lens)), out=to[:, ::2, :D])
+    assert torch.equal(to[:, ::2, :D], out)
+    assert (to[:, 1::2] == 5).all() and (to[:, :, D:] == 5).all()
