@@ -485,3 +485,23 @@ def test_wide_trees_many_sequences_and_strides(dev, dtype, D, H, G, page, B):
     _kv4().kv4_attention(mine, s.cache, s.d_table, s.d_cu, s.d_seq, tree=tree, max_q=20, max_kv=max(520, max(lens)), out=to[:, ::2, :D])
     assert torch.equal(to[:, ::2, :D], out)
     assert (to[:, 1::2] == 5).all() and (to[:, :, D:] == 5).all()
+
+
+@pytest.mark.gpu
+def test_wide_trees_past_4_gib(dev):
+    """The same bits from pages whose codes lie past 32 bits."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GiB")
+    lens, news = [700, 90], [40, 33]
+    s = Setup(dev, torch.bfloat16, 128, 8, 64, lens, news, seed=6)
+    tree = _kv4().kv4_tree(torch.tensor([i - 1 for n in news for i in range(n)], dtype=torch.int32, device=dev), s.d_cu, s.d_seq, max_q=40)
+    q = s.q(32)
+    want = s.attend(q, tree=tree, max_q=40, max_kv=700)
+    pages, bytes_ = 140000, 8 * 64 * 64
+    far = _kv4().KV4Cache(pages, 64, 8, 128, torch.bfloat16, dev)
+    table = pages - 1 - s.table
+    assert int(table[:, :2].min()) * bytes_ > 1 << 32
+    table = table.int().to(dev)
+    _kv4().kv4_append(far, s.k.to(dev), s.v.to(dev), table, s.cu_all.to(dev), s.d_seq)
+    got = _kv4().kv4_attention(q.to(dev), far, table, s.d_cu, s.d_seq, tree=tree, max_q=40, max_kv=700)
+    assert torch.equal(got, want)
