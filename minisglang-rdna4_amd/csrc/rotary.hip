@@ -7,7 +7,7 @@
 // eighth, whose sine and cosine are Taylor's polynomials (to x^9 and x^10: the next terms are below 2e-9 and 2e-10).
 //
 // A thread has one token and one unit of 8 pairs, 16 bytes each of a and b, works its 8 angles out once, and turns that
-// unit in `per` heads. Bound by memory for prompts (8191 tokens of 40 heads of 128, 168 MB in and out: 36.5 us, 4.6 TB/s), by the
+// unit in `per` heads. Bound by memory for prompts (8191 tokens of 40 heads of 128, 168 MB in and out: 40 us, 4.2 TB/s), by the
 // launch for decode (3.5 us).
 #include "rotary.h"
 
@@ -34,14 +34,29 @@ __device__ __forceinline__ void sincos_turn(uint32_t turn, float& s, float& c) {
 }
 
 template <int DT>
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+__device__ __forceinline__ v4u pack8(const float (&f)[8]) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = (uint32_t)to_dtype(f[2 * i], DT) | ((uint32_t)to_dtype(f[2 * i + 1], DT) << 16);
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return v4u{w[0], w[1], w[2], w[3]};
 }
 
-template <int DT, bool ADJ>
+// NT: past the caches
+template <bool NT>
+__device__ __forceinline__ v4u read(const uint16_t* p) {
+  const v4u* at = reinterpret_cast<const v4u*>(p);
+  return NT ? __builtin_nontemporal_load(at) : *at;
+}
+template <bool NT>
+__device__ __forceinline__ void write(uint16_t* p, v4u x) {
+  v4u* at = reinterpret_cast<v4u*>(p);
+  if (NT) __builtin_nontemporal_store(x, at);
+  else *at = x;
+}
+
+constexpr int kHeads = 4;  // of a thread, at most
+
+template <int DT, bool ADJ, bool NT>
 __global__ void __launch_bounds__(256)
 rotary_kernel(const Rotary p) {
   const int groups = (p.heads + p.per - 1) / p.per;  // of heads
@@ -70,6 +85,16 @@ rotary_kernel(const Rotary p) {
     }
     return;
   }
+  const int ca = ADJ ? unit * 16 : unit * 8, cb = ADJ ? ca + 8 : p.R / 2 + ca;
+  v4u a[kHeads], b[kHeads];
+#pragma unroll
+  for (int u = 0; u < kHeads; ++u) {  // before the angles, which take a chain of reads too
+    const uint16_t* in;
+    uint16_t* out;
+    at(min(h0 + u, h1 - 1), in, out);
+    a[u] = read<NT>(in + ca);
+    b[u] = read<NT>(in + cb);
+  }
   float sn[8], cs[8];
   auto position = [&](int axis) -> uint64_t {
     const int64_t i = axis * p.ldp + t;
@@ -84,43 +109,42 @@ rotary_kernel(const Rotary p) {
     sn[e] *= p.scale;
     cs[e] *= p.scale;
   }
-  const int ca = ADJ ? unit * 16 : unit * 8, cb = ADJ ? ca + 8 : p.R / 2 + ca;
-  constexpr int U = 4;  // heads in flight
-  for (int h = h0; h < h1; h += U) {
-    uint4 a[U], b[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint16_t* in;
-      uint16_t* out;
-      at(min(h + u, h1 - 1), in, out);
-      a[u] = *reinterpret_cast<const uint4*>(in + ca);
-      b[u] = *reinterpret_cast<const uint4*>(in + cb);
-    }
+  for (int u = 0; u < kHeads; ++u) {
+    if (h0 + u >= h1) break;
+    float x[8], y[8], v[8], w[8];
+    unpack8(make_uint4(a[u].x, a[u].y, a[u].z, a[u].w), DT, x);
+    unpack8(make_uint4(b[u].x, b[u].y, b[u].z, b[u].w), DT, y);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (h + u >= h1) break;
-      float x[8], y[8], v[8], w[8];
-      unpack8(a[u], DT, x);
-      unpack8(b[u], DT, y);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (ADJ) {
-          float* src = e < 4 ? x : y;
-          float* dst = e < 4 ? v : w;
-          const int j = 2 * (e & 3);
-          dst[j] = __builtin_fmaf(src[j], cs[e], -(src[j + 1] * sn[e]));
-          dst[j + 1] = __builtin_fmaf(src[j], sn[e], src[j + 1] * cs[e]);
-        } else {
-          v[e] = __builtin_fmaf(x[e], cs[e], -(y[e] * sn[e]));
-          w[e] = __builtin_fmaf(x[e], sn[e], y[e] * cs[e]);
-        }
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (ADJ) {
+        float* src = e < 4 ? x : y;
+        float* dst = e < 4 ? v : w;
+        const int j = 2 * (e & 3);
+        dst[j] = __builtin_fmaf(src[j], cs[e], -(src[j + 1] * sn[e]));
+        dst[j + 1] = __builtin_fmaf(src[j], sn[e], src[j + 1] * cs[e]);
+      } else {
+        v[e] = __builtin_fmaf(x[e], cs[e], -(y[e] * sn[e]));
+        w[e] = __builtin_fmaf(x[e], sn[e], y[e] * cs[e]);
       }
-      const uint16_t* in;
-      uint16_t* out;
-      at(h + u, in, out);
-      *reinterpret_cast<uint4*>(out + ca) = pack8<DT>(v);
-      *reinterpret_cast<uint4*>(out + cb) = pack8<DT>(w);
     }
+    const uint16_t* in;
+    uint16_t* out;
+    at(h0 + u, in, out);
+    write<NT>(out + ca, pack8<DT>(v));
+    write<NT>(out + cb, pack8<DT>(w));
+  }
+}
+
+template <bool NT>
+static void launch(const Rotary& p, int dtype, dim3 g, hipStream_t st) {
+  const dim3 b(256);
+  if (dtype == kBF16) {
+    if (p.adjacent) hipLaunchKernelGGL((rotary_kernel<kBF16, true, NT>), g, b, 0, st, p);
+    else hipLaunchKernelGGL((rotary_kernel<kBF16, false, NT>), g, b, 0, st, p);
+  } else {
+    if (p.adjacent) hipLaunchKernelGGL((rotary_kernel<kF16, true, NT>), g, b, 0, st, p);
+    else hipLaunchKernelGGL((rotary_kernel<kF16, false, NT>), g, b, 0, st, p);
   }
 }
 
@@ -128,19 +152,14 @@ int launch_rotary(Rotary& p, int D, int dtype, hipStream_t st) {
   p.heads = p.q.heads + p.k.heads;
   const bool rest = p.R < D && (p.q.in != p.q.out || (p.k.heads && p.k.in != p.k.out));  // in place they stay
   p.units = p.R / 16 + (rest ? (D - p.R) / 8 : 0);
-  // more heads a thread while the card stays full (8 waves per SIMD: 524288 threads)
+  // more heads a thread while the card stays full (8 waves per SIMD: 524288 threads); 8 in flight 45 us
   const int64_t rows = p.T * p.heads * p.units;
-  p.per = (int)(rows / 524288 < 1 ? 1 : rows / 524288 > 8 ? 8 : rows / 524288);
+  p.per = (int)(rows / 524288 < 1 ? 1 : rows / 524288 > kHeads ? kHeads : rows / 524288);
   const int64_t threads = p.T * ((p.heads + p.per - 1) / p.per) * p.units, wgs = (threads + 255) / 256;
   if (wgs > kMaxGrid) return kErrUnsupported;
-  const dim3 g((unsigned)wgs), b(256);
-  if (dtype == kBF16) {
-    if (p.adjacent) hipLaunchKernelGGL((rotary_kernel<kBF16, true>), g, b, 0, st, p);
-    else hipLaunchKernelGGL((rotary_kernel<kBF16, false>), g, b, 0, st, p);
-  } else {
-    if (p.adjacent) hipLaunchKernelGGL((rotary_kernel<kF16, true>), g, b, 0, st, p);
-    else hipLaunchKernelGGL((rotary_kernel<kF16, false>), g, b, 0, st, p);
-  }
+  // what the L2s do not hold, 32 MB, does not pass through them. us, 168 MB in and out, other rows each time: 39.9 / 48.5
+  if (p.T * p.heads * D * 4 > (32 << 20)) launch<true>(p, dtype, dim3((unsigned)wgs), st);
+  else launch<false>(p, dtype, dim3((unsigned)wgs), st);
   return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 

@@ -234,3 +234,24 @@ def test_rows_past_4_gib(dev):
     r.forward_inplace(q, k, pos)
     a, b = r.forward(x[:, :2], x[:, 2:], pos[-4:])
     assert torch.equal(q[-4:], a) and torch.equal(k[-4:], b) and not q[:-4].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("adjacent,rotary_dim", [(False, 128), (True, 128), (False, 64)])
+def test_many_rows_as_few(dev, dtype, adjacent, rotary_dim):
+    """More rows than the caches hold, that take the way past them: the bits of the same rows a few at a time, in place too."""
+    T, Hq, H, D = 1801, 37, 5, 128
+    assert T * (Hq + H) * D * 4 > 32 << 20
+    g = torch.Generator(device=dev).manual_seed(1)
+    qkv = torch.randn(T, (Hq + 2 * H) * D, generator=g, device=dev).to(dtype)
+    q, k, v = (t.view(T, -1, D) for t in qkv.split([Hq * D, H * D, H * D], dim=1))
+    pos = torch.randint(0, 1 << 20, (T,), generator=g, device=dev)
+    rot = pkg("layers.rotary").Rotary(D, rotary_dim=rotary_dim, adjacent=adjacent, scale=1.25, device=dev)
+    want = [rot.forward(q[i:i + 100], k[i:i + 100], pos[i:i + 100]) for i in range(0, T, 100)]
+    want = tuple(torch.cat(t) for t in zip(*want))
+    got = rot.forward(q, k, pos)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    before = v.clone()
+    rot.forward_inplace(q, k, pos)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, before)
