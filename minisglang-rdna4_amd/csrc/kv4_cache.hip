@@ -191,8 +191,8 @@ kv4_append_kernel(const uint16_t* __restrict__ k, int64_t ldk, int64_t hk, const
 // exact) and one to the type. A row without a place in the cache (before the sequence's first token,
 // on a page that does not exist) is NaN. A vector per D / 8 lanes; a wave has 8 rows (ROWS), which as a rule are one block's and
 // share its words of V, and `per` heads of them: row -> sequence -> page, dependent reads, are looked up once for all of those.
-// 131072 rows of 8 heads of 128 (142 MB in, 537 out) 143 us, 4.75 TB/s; 232 with a lookup for every 4 vectors.
-template <int D, int DT, int ROWS>
+// 131072 rows of 8 heads of 128 (142 MB in, 537 out) 141 us, 4.8 TB/s; 232 with a lookup for every 4 vectors.
+template <int D, int DT, int ROWS, bool NT>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(Kv4Cache c, Kv4Batch s, int per, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
   constexpr int L = D / 8, VP = 64 / L, PASS = ROWS / VP;  // lanes per vector, vectors per wave, passes for its rows
@@ -257,8 +257,8 @@ kv4_read_kernel(Kv4Cache c, Kv4Batch s, int per, uint16_t* __restrict__ k, uint1
         vw[e / 2] = two((vc[p][e / 4][e % 4] >> (4 * j[p])) & 15u, (vc[p][e / 4][e % 4 + 1] >> (4 * j[p])) & 15u, sv, mv);
       }
       if (blk[p] != -2) {
-        *reinterpret_cast<v4u*>(k + at[p] + h * D) = kw;
-        *reinterpret_cast<v4u*>(v + at[p] + h * D) = vw;
+        stream_write<NT>(k + at[p] + h * D, kw);
+        stream_write<NT>(v + at[p] + h * D, vw);
       }
     }
   }
@@ -298,8 +298,9 @@ static int read(const Kv4Cache& c, const Kv4Batch& s, uint16_t* k, uint16_t* v, 
   const int64_t wgs = (groups * ((c.H + per - 1) / per) + 3) / 4;
   if (wgs > kMaxGrid) return kErrUnsupported;
   const dim3 g((unsigned)wgs), b(256);
-  if (few) hipLaunchKernelGGL((kv4_read_kernel<D, DT, VP>), g, b, 0, st, c, s, per, k, v);
-  else hipLaunchKernelGGL((kv4_read_kernel<D, DT, 8>), g, b, 0, st, c, s, per, k, v);
+  if (few) hipLaunchKernelGGL((kv4_read_kernel<D, DT, VP, false>), g, b, 0, st, c, s, per, k, v);
+  else if (s.T * c.H * D * 4 > kL2Bytes) hipLaunchKernelGGL((kv4_read_kernel<D, DT, 8, true>), g, b, 0, st, c, s, per, k, v);
+  else hipLaunchKernelGGL((kv4_read_kernel<D, DT, 8, false>), g, b, 0, st, c, s, per, k, v);
   return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 

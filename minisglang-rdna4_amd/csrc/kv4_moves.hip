@@ -11,6 +11,7 @@ namespace w4a8 {
 // in a row, whose places were worked out one after another).
 constexpr int kCopyPart = 1024;  // vectors of a workgroup
 
+template <bool NT>
 __global__ void __launch_bounds__(256)
 kv4_copy_kernel(const Kv4Caches cs, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int pages, int parts,
                 uint32_t codes, uint32_t scales) {
@@ -30,7 +31,7 @@ kv4_copy_kernel(const Kv4Caches cs, const int32_t* __restrict__ src, const int32
     for (int u = 0; u < 4; ++u) x[u] = in[min(i0 + 256 * u, codes - 1)];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (on && i0 + 256 * u < codes) out[i0 + 256 * u] = x[u];
+      if (on && i0 + 256 * u < codes) stream_write<NT>(out + i0 + 256 * u, x[u]);
   } else {
     v4u *ks = reinterpret_cast<v4u*>(c.ks), *vs = reinterpret_cast<v4u*>(c.vs);
 #pragma unroll
@@ -51,8 +52,12 @@ int launch_kv4_copy(const Kv4Caches& cs, int caches, const int32_t* src, const i
                     int64_t codes, int64_t scales, hipStream_t st) {
   const int64_t parts = (codes + kCopyPart - 1) / kCopyPart, all = 2 * parts + (2 * scales + kCopyPart - 1) / kCopyPart;
   if (n > kMaxGrid || all > 65535) return kErrUnsupported;
-  hipLaunchKernelGGL(kv4_copy_kernel, dim3((unsigned)n, (unsigned)all, (unsigned)caches), dim3(256), 0, st, cs, src, dst,
-                     (int)pages, (int)parts, (uint32_t)codes, (uint32_t)scales);
+  const dim3 g((unsigned)n, (unsigned)all, (unsigned)caches), b(256);
+  // us, 143 MB copied and then read back as 537 MB, both kernels' writes past the caches / one's / none: 190 / 200 / 200
+  if (n * caches * (codes + scales) * 64 > kL2Bytes)
+    hipLaunchKernelGGL((kv4_copy_kernel<true>), g, b, 0, st, cs, src, dst, (int)pages, (int)parts, (uint32_t)codes, (uint32_t)scales);
+  else
+    hipLaunchKernelGGL((kv4_copy_kernel<false>), g, b, 0, st, cs, src, dst, (int)pages, (int)parts, (uint32_t)codes, (uint32_t)scales);
   return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }
 

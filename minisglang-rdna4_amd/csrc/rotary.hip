@@ -41,19 +41,6 @@ __device__ __forceinline__ v4u pack8(const float (&f)[8]) {
   return v4u{w[0], w[1], w[2], w[3]};
 }
 
-// NT: past the caches
-template <bool NT>
-__device__ __forceinline__ v4u read(const uint16_t* p) {
-  const v4u* at = reinterpret_cast<const v4u*>(p);
-  return NT ? __builtin_nontemporal_load(at) : *at;
-}
-template <bool NT>
-__device__ __forceinline__ void write(uint16_t* p, v4u x) {
-  v4u* at = reinterpret_cast<v4u*>(p);
-  if (NT) __builtin_nontemporal_store(x, at);
-  else *at = x;
-}
-
 constexpr int kHeads = 4;  // of a thread, at most
 
 template <int DT, bool ADJ, bool NT>
@@ -92,8 +79,8 @@ rotary_kernel(const Rotary p) {
     const uint16_t* in;
     uint16_t* out;
     at(min(h0 + u, h1 - 1), in, out);
-    a[u] = read<NT>(in + ca);
-    b[u] = read<NT>(in + cb);
+    a[u] = stream_read<NT>(in + ca);
+    b[u] = stream_read<NT>(in + cb);
   }
   float sn[8], cs[8];
   auto position = [&](int axis) -> uint64_t {
@@ -131,8 +118,8 @@ rotary_kernel(const Rotary p) {
     const uint16_t* in;
     uint16_t* out;
     at(h0 + u, in, out);
-    write<NT>(out + ca, pack8<DT>(v));
-    write<NT>(out + cb, pack8<DT>(w));
+    stream_write<NT>(out + ca, pack8<DT>(v));
+    stream_write<NT>(out + cb, pack8<DT>(w));
   }
 }
 
@@ -157,8 +144,8 @@ int launch_rotary(Rotary& p, int D, int dtype, hipStream_t st) {
   p.per = (int)(rows / 524288 < 1 ? 1 : rows / 524288 > kHeads ? kHeads : rows / 524288);
   const int64_t threads = p.T * ((p.heads + p.per - 1) / p.per) * p.units, wgs = (threads + 255) / 256;
   if (wgs > kMaxGrid) return kErrUnsupported;
-  // what the L2s do not hold, 32 MB, does not pass through them. us, 168 MB in and out, other rows each time: 39.9 / 48.5
-  if (p.T * p.heads * D * 4 > (32 << 20)) launch<true>(p, dtype, dim3((unsigned)wgs), st);
+  // us, 168 MB in and out, other rows each time, past the caches / through them: 39.9 / 48.5
+  if (p.T * p.heads * D * 4 > kL2Bytes) launch<true>(p, dtype, dim3((unsigned)wgs), st);
   else launch<false>(p, dtype, dim3((unsigned)wgs), st);
   return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }

@@ -135,6 +135,21 @@ __device__ __forceinline__ float from_dtype(uint16_t h, int dtype) {
 // offset, and a scalar offset that the compiler computes with SALU. Loads whose per-lane offset is past
 // `bytes` return 0; the scalar offset is not part of that check.
 typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+
+// 16 bytes of what is read or written once; NT: past the caches, for calls with more of it than the 8 L2s hold
+constexpr int64_t kL2Bytes = 32 << 20;
+template <bool NT>
+__device__ __forceinline__ v4u stream_read(const void* p) {
+  const v4u* at = reinterpret_cast<const v4u*>(p);
+  return NT ? __builtin_nontemporal_load(at) : *at;
+}
+template <bool NT>
+__device__ __forceinline__ void stream_write(void* p, v4u x) {
+  v4u* at = reinterpret_cast<v4u*>(p);
+  if (NT) __builtin_nontemporal_store(x, at);
+  else *at = x;
+}
+
 typedef __amdgpu_buffer_rsrc_t BufRsrc;
 
 __device__ __forceinline__ BufRsrc make_rsrc(const void* base, uint32_t bytes) {
