@@ -345,7 +345,9 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
         ev = now;
       }
       const float fe = kFold ? __builtin_ldexpf(1.f, __builtin_amdgcn_readfirstlane(tb.ek)) : 1.f;
-      const float sct = sc * fe;
+      // f32 holds either factor, but not each product of them. Below 2^-120, where scores of the tile are as good as zero, it
+      // has to leave -inf what it is, as sc has; past f32's end it has to leave a score of 0 at that.
+      const float sct = kFold ? __builtin_amdgcn_fmed3f(sc * fe, 0x1p-120f, 0x1.fffffep+127f) : sc;
       in_order();
 #pragma unroll
       for (int w = 0; w < KS; ++w) {

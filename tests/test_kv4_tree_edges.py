@@ -1,0 +1,69 @@
+"""Trees of drafted tokens over the 4-bit cache at the edges of what a call may hold: queries, keys and steps whose powers of
+two leave f32's range, maxima that one tile's units cannot hold, sequences longer than their table under a window, values at
+fp16's ends. References and tolerances are test_kv4_tree's."""
+import math
+import random
+
+import pytest
+import torch
+
+from test_kv4_tree import DTYPES, Setup, _kv4, cache_values, check, lines, pack, random_tree, ref
+
+
+def again(s):
+    """The cache of s's keys and values as they are now."""
+    _kv4().kv4_append(s.cache, s.k.to(s.dev), s.v.to(s.dev), s.d_table, s.cu_all.to(s.dev), s.d_seq)
+
+
+def mask_tree(see, positions, dev, words=4):
+    return _kv4().KV4Tree(pack(see, words).to(dev), torch.tensor(positions, dtype=torch.int32, device=dev))
+
+
+# ------------------------------------------------------------------------------------------------
+# GPU: more than 64 columns
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,G", [(128, 4), (64, 2)])
+def test_small_queries_over_small_keys(dev, dtype, D, G):
+    """Queries and keys of zeros (a warm-up) and of the smallest numbers: all scores are zero, or as good as zero, and the
+    output is the mean of the values that a row sees, masked ones not among them."""
+    rng = random.Random(D)
+    lens, news = [700, 90], [40, 33]
+    trees = [random_tree(n, rng) for n in news]
+    see = [x for t in trees for x in lines(t)]
+    parents = torch.tensor([p for t in trees for p in t], dtype=torch.int32, device=dev)
+    least = torch.finfo(dtype).smallest_normal
+    s = Setup(dev, dtype, D, 1, 64, lens, news, seed=7)
+    tree = _kv4().kv4_tree(parents, s.d_cu, s.d_seq, max_q=40)
+    keys, q = s.k, s.q(G)
+    for k in (0.0, least, 2.0 ** -10, 1.0):
+        s.k = (keys.float() * k).to(dtype)
+        again(s)
+        for x in (0.0, least, 2.0 ** -10):
+            for sm in (D ** -0.5, 1e-30):
+                out = check(s, (q.float() * x).to(dtype), tree, see, max_q=40, max_kv=700, sm_scale=sm)
+                assert torch.isfinite(out.float()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,G", [(128, 4), (64, 2)])
+def test_large_queries_beside_large_keys(dev, D, G):
+    """Queries near 2^96 in a channel that the keys have as 0, keys near 2^99 in the others: every score is 0, without a
+    rounding. The steps are a power of two, so that c - 7.5 times one has 4 bits. The output is the mean, off by p's, its sum's
+    and V's roundings to fp16 (2^-11 each of A, of A and of the output) and f32's sums (2^-12 A)."""
+    rng = random.Random(D)
+    lens, news = [700, 90], [40, 33]
+    see = [x for n in news for x in lines(random_tree(n, rng))]
+    s = Setup(dev, torch.bfloat16, D, 1, 64, lens, news, seed=9)
+    s.k = (torch.randint(0, 16, s.k.shape, generator=torch.Generator().manual_seed(1)) * 2.0 ** 95).to(torch.bfloat16)
+    s.k[:, :, 0], s.k[:, :, 1] = 0, 15 * 2.0 ** 95
+    again(s)
+    q = torch.zeros(sum(news), G, D, dtype=torch.bfloat16)
+    q[:, :, 0] = 2.0 ** 95
+    q[::3, :, 0] = -(2.0 ** 93)
+    tree = mask_tree(see, [0] * len(see), dev, 2)
+    out, lse = s.attend(q, tree=tree, max_q=40, max_kv=700, return_lse=True)
+    want, rl, A, _, _ = ref(q, cache_values(s.cache), s.table, s.page, lens, news, see, [0] * len(see), D ** -0.5, bounds=True)
+    assert ((out.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -11 * (2.5 * A + want.abs()) + 2.0 ** -25).all()
+    assert (lse.cpu().double() - rl).abs().max().item() < 2e-4 + 2.0 ** -11
