@@ -400,7 +400,8 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
         bo *= f;
 #pragma unroll
         for (int d = 0; d < CT; ++d) o[d] *= f;
-        const float back = is / fe;
+        // kept finite: where the tile's unit is far below the maximum, a masked score's -inf and -inf / fe would be NaN
+        const float back = kFold ? __builtin_amdgcn_fmed3f(is / fe, -0x1.fffffep+127f, 0x1.fffffep+127f) : is;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[0][r] -= back;

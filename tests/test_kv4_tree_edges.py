@@ -67,3 +67,22 @@ def test_large_queries_beside_large_keys(dev, D, G):
     want, rl, A, _, _ = ref(q, cache_values(s.cache), s.table, s.page, lens, news, see, [0] * len(see), D ** -0.5, bounds=True)
     assert ((out.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -11 * (2.5 * A + want.abs()) + 2.0 ** -25).all()
     assert (lse.cpu().double() - rl).abs().max().item() < 2e-4 + 2.0 ** -11
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_a_far_maximum_beside_keys_of_zeros(dev, dtype, sign):
+    """Scores of 2^24 and more (in size) over the context, drafted tokens with keys of zeros that some rows do not see: those rows
+    are the mean of the context, the others the one end of the softmax."""
+    lens, news = [544, 500], [32, 20]
+    s = Setup(dev, dtype, 128, 1, 64, lens, news, seed=11)
+    for b, (n, new) in enumerate(zip(lens, news)):
+        at = sum(lens[:b])
+        s.k[at:at + n - new] = 2.0 ** 20 if dtype == torch.bfloat16 else 2.0 ** 15
+        s.k[at + n - new:at + n] = 0
+    again(s)
+    q = torch.full((sum(news), 4, 128), sign * (8.0 if dtype == torch.bfloat16 else 1024.0), dtype=dtype)
+    see = [x if i % 3 else [] for n in news for i, x in enumerate([[i] for i in range(n)])]
+    out = check(s, q, mask_tree(see, [0] * len(see), dev, 1), see, max_q=32, max_kv=544)
+    assert torch.isfinite(out.float()).all()
