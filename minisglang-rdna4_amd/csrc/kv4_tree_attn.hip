@@ -9,7 +9,7 @@
 // times the code's 4 lose one bit at most, 2^-11 of what is left once the middle of the vector's range is taken out; fp16
 // models, whose scores ought to be better than that, have K' = 2 c - 15, exactly, b = 2 m / s + 15, and S times s/2 afterwards.
 // V' = s c + m, rounded once to fp16 (2^-11), times 2^-e with e the largest so far. fp16 models have the codes, exactly, p s
-// rounded instead (times 2^-e, e of the largest step so far) and sum p (m + 7.5 s) beside the product, its middles in fp16: their
+// rounded instead (times 2^-e, e of the largest step so far) and sum p (m + 7.5 s) beside the product, in f32: their
 // output would show the rounding of V' (norm of the error over the output's 3.5e-4, so 3.0e-4; rounding the output 2.1e-4).
 // p is rounded to fp16, and its sum is of the rounded ones: 2^7 and more for the largest score, so that what is lost below
 // fp16's least, 2^-32 of that a token, is nothing over any context. Powers of two change no bits, unless values of a bf16
@@ -44,7 +44,7 @@ struct alignas(32) ScaleTable {
   uint32_t ks[kStep];    // bf16 models: half of K's step, twice, by token
   uint32_t v[8][8];      // bf16 models: V's steps of tokens j and j + 4 of the block (j < 4), and their least values
   float sv[kStep];       // fp16 models: V's steps, in the order of S's rows,
-  uint16_t bv[kStep];    // and the middles m + 7.5 s, in fp16
+  float bv[kStep];       // and the middles m + 7.5 s, which may be past fp16's end
   int ek, ev;
 };
 
@@ -215,7 +215,7 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
         v[8] = f32_to_f16(__builtin_ldexpf(m, -ev_run));
       } else {
         tb.sv[r] = __builtin_ldexpf(s, -ev_run);
-        tb.bv[r] = f32_to_f16(__builtin_fmaf(7.5f, s, m));
+        tb.bv[r] = __builtin_fmaf(7.5f, s, m);
       }
       if (lane == 0) tb.ev = ev_run;
     }
@@ -291,12 +291,11 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
     };
     // of 8 of a lane's 32 values of S
     struct Weights {
-      v8f s;
-      v4w b;
+      v8f s, b;
     };
     auto weights = [&](const ScaleTable& tb, int g) {
       const int at = (g >> 1) * 32 + half * 16 + (g & 1) * 8;
-      return Weights{*reinterpret_cast<const v8f*>(&tb.sv[at]), *reinterpret_cast<const v4w*>(&tb.bv[at])};
+      return Weights{*reinterpret_cast<const v8f*>(&tb.sv[at]), *reinterpret_cast<const v8f*>(&tb.bv[at])};
     };
     auto v_operand = [&](const unsigned char* vc, int f, int d) { return lds_read(vc + v_lane + (2 * f * D + 32 * d) * 16); };
     __syncthreads();
@@ -419,10 +418,8 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
         l = add_pair<kF16>(w, l);
         const Weights& ww = ws[(x >> 2) & 1];
         if (!kFold) {
-          const uint32_t mid = ww.b[x & 3];
-          const v2h h = __builtin_bit_cast(v2h, mid);
-          bo = __builtin_fmaf(a, (float)h.x, bo);
-          bo = __builtin_fmaf(z, (float)h.y, bo);
+          bo = __builtin_fmaf(a, ww.b[(2 * x) & 7], bo);
+          bo = __builtin_fmaf(z, ww.b[(2 * x + 1) & 7], bo);
         }
         pf[x >> 2][x & 3] = kFold ? w : pack16<kF16>(a * ww.s[(2 * x) & 7], z * ww.s[(2 * x + 1) & 7]);
       };

@@ -86,3 +86,34 @@ def test_a_far_maximum_beside_keys_of_zeros(dev, dtype, sign):
     see = [x if i % 3 else [] for n in news for i, x in enumerate([[i] for i in range(n)])]
     out = check(s, q, mask_tree(see, [0] * len(see), dev, 1), see, max_q=32, max_kv=544)
     assert torch.isfinite(out.float()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("end", [65504.0, -65504.0])
+@pytest.mark.parametrize("max_kv", [512, 2000])
+def test_vectors_of_fp16s_last_number(dev, end, max_kv):
+    """Values that are 65504 in all channels, whose range's middle is past fp16's end: in the context, alone or among others, and
+    in a drafted token that some rows do not see, beside which nothing may change."""
+    lens, news = [2000], [40]
+    s = Setup(dev, torch.float16, 128, 1, 64, lens, news, seed=3)
+    s.k[:] = 0
+    s.k[700, 0, 0] = 16
+    s.v[700], s.v[900], s.v[1970] = end, end, end  # 1970: new token 10
+    again(s)
+    q = torch.zeros(40, 4, 128, dtype=torch.float16)
+    q[:, :2, 0] = 64  # a score of 102: token 700 takes all; the other heads weigh all the same
+    see = [[i] if i % 2 else [i, 10] for i in range(40)]
+    see[10] = [10]
+    tree = mask_tree(see, [0] * 40, dev, 2)
+    out, lse = s.attend(q, tree=tree, max_q=40, max_kv=max_kv, sm_scale=0.1, return_lse=True)
+    want, rl, A, C, _ = ref(q, cache_values(s.cache), s.table, s.page, lens, news, see, [0] * 40, 0.1, bounds=True)
+    assert (out[:, :2].cpu() == end).all()  # one key: its value
+    # as test_kv4_tree has it: p s and the sum rounded to fp16, the output's rounding, f32's sums
+    assert ((out.cpu().double() - want).abs() <= 2.0 ** -11 * (C + 0.5 * A + 2 * want.abs()) + 2.0 ** -24).all()
+    assert (lse.cpu().double() - rl).abs().max().item() < 2e-4 + 2.0 ** -11
+    # what no row sees weighs nothing
+    none = [[i] if i != 10 else [] for i in range(40)]
+    a = s.attend(q, tree=mask_tree(none, [0] * 40, dev, 2), max_q=40, max_kv=max_kv, sm_scale=0.1)
+    s.v[1970] = 0
+    again(s)
+    assert torch.equal(a, s.attend(q, tree=mask_tree(none, [0] * 40, dev, 2), max_q=40, max_kv=max_kv, sm_scale=0.1))
