@@ -118,6 +118,7 @@ __device__ __forceinline__ int kv4_page(const Kv4Cache& c, const Kv4Batch& s, in
 struct Span {
   int64_t start;
   int n, cols, len, first_pos;  // new tokens, columns, length, position of the first new token
+  int cut;                      // of a tree: what was taken off the length, and off every position
 };
 template <bool TREE>
 __device__ __forceinline__ Span kv4_span(const Kv4Attn& p, int b) {
@@ -126,9 +127,11 @@ __device__ __forceinline__ Span kv4_span(const Kv4Attn& p, int b) {
   s.cols = s.n * p.G;
   const int64_t cap = (int64_t)p.s.width << p.c.shift;
   const int len = max(p.s.lens[b], 0);  // -2^31 has no position n rows before it
-  // one token past the table's end stands for all of them: its page is missing (of a tree each node has its own)
+  // One token past the table's end stands for all of them: its page is missing. Of a tree each node has its own, behind that
+  // one, and positions move with them: a window that saw some of the missing tokens before the nodes sees the one.
   s.len = len > cap ? (int)min((int64_t)len, cap + (TREE ? s.n + 1 : 1)) : len;
-  s.first_pos = len - s.n;
+  s.cut = TREE ? len - s.len : 0;
+  s.first_pos = len - s.cut - s.n;
   return s;
 }
 // The sequence of the launch's z-th workgroups: the longest first, up to 64 sequences, so that short ones fill the launch's
@@ -149,7 +152,7 @@ __device__ __forceinline__ int kv4_longest(const Kv4Batch& s, int z) {
 // first new one
 __device__ __forceinline__ int tree_from(const Kv4Attn& p, const Span& s, int i) {
   if (!p.window) return 0;
-  const int64_t lo = (int64_t)p.pos[s.start + i] - p.window + 1;
+  const int64_t lo = (int64_t)p.pos[s.start + i] - s.cut - p.window + 1;
   return lo < 0 ? 0 : lo > 0x7fffffff ? 0x7fffffff : (int)lo;
 }
 __device__ __forceinline__ uint32_t tree_bits(const Kv4Attn& p, const Span& s, int i, int at) {

@@ -117,3 +117,36 @@ def test_vectors_of_fp16s_last_number(dev, end, max_kv):
     s.v[1970] = 0
     again(s)
     assert torch.equal(a, s.attend(q, tree=mask_tree(none, [0] * 40, dev, 2), max_q=40, max_kv=max_kv, sm_scale=0.1))
+
+
+# ------------------------------------------------------------------------------------------------
+# GPU: windows
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,width,new", [(64, 1, 1), (64, 2, 3), (128, 2, 30), (256, 3, 20), (128, 40, 70)])
+def test_windows_past_the_table_are_nan(dev, dtype, D, width, new):
+    """A sequence longer than its table: a row of a tree that sees a token past the table is NaN, whatever its window, as a row
+    of a chain is; one that sees none is 0. Beside it a sequence that its table holds."""
+    page = 16
+    cap = width * page
+    rng = random.Random(width)
+    trees = [random_tree(new, rng), random_tree(2, rng)]
+    parents = torch.tensor([p for t in trees for p in t], dtype=torch.int32, device=dev)
+    for past in (0, 1, new, new + 1, new + 2, new + 7, 24, 4000, 2 ** 31 - 1 - cap):
+        s = Setup(dev, dtype, D, 1, page, [cap, min(cap, 13)], [new, 2], seed=width)
+        n = cap + past
+        if n < new:
+            continue
+        s.lens = [n, s.lens[1]]
+        s.d_seq = torch.tensor(s.lens, dtype=torch.int32, device=dev)
+        q = s.q(2)
+        for window in (1, 5, 8, cap + new):
+            for kw in ({}, dict(max_q=new), dict(max_q=1, max_kv=1)):
+                tree = _kv4().kv4_tree(parents, s.d_cu, s.d_seq, max_q=new, window=window)
+                see = [x[-window:] for t in trees for x in lines(t)]
+                check(s, q, tree, see, window, **kw)
+                # rows that see nothing of the new tokens, from positions all over the window
+                see = [x if i % 3 else [] for i, x in enumerate(see)]
+                at = [min(p + rng.randrange(0, 2 * window), 2 ** 31 - 1) for p in tree.positions.tolist()]
+                check(s, q, mask_tree(see, at, dev, tree.mask.shape[1]), see, window, **kw)
