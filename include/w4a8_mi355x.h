@@ -401,8 +401,8 @@ int w4a8_kv4_copy_pages(const void* const* arrays, int64_t caches, int64_t pages
 /* Puts accepted tokens behind the context, in each of several caches of one shape (as above): of sequence b's n new tokens,
  * slot j < kept[b] gets what token keep[b * ldk + j] holds (ascending, so that keep[.][j] >= j; an entry below j or not below n
  * leaves slot j as it is, and so does a page that does not exist). kept is taken between 0 and the smaller of n and most.
- * new_lens (B), where given, receives seq_lens[b] - n + kept; it is not seq_lens. The 8 tokens of a block are one sequence's,
- * as for w4a8_kv4_append. One launch per 64 caches. */
+ * new_lens (B), where given, receives seq_lens[b] - n + kept; it overlaps none of the lists that are read. The 8 tokens of a block
+ * are one sequence's, as for w4a8_kv4_append. One launch per 64 caches. */
 int w4a8_kv4_keep(const void* const* arrays, int64_t caches, int64_t pages, int64_t page_size, int64_t H, int64_t D,
                   const int32_t* table, int64_t ldt, int64_t width, const int32_t* cu, const int32_t* seq_lens, int64_t B,
                   const int32_t* keep, int64_t ldk, int64_t most, const int32_t* kept, int32_t* new_lens, void* stream);

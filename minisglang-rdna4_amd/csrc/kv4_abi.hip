@@ -255,8 +255,12 @@ int w4a8_kv4_keep(const void* const* arrays, int64_t caches, int64_t pages, int6
   if (B == 0) return kOk;
   if (!arrays || !kept || (most > 0 && !keep) || ldk < most)
     return fail(kErrInvalid, "%s: needs the caches' arrays, kept, and keep with a stride of at least its width", who);
-  if (new_lens && new_lens < seq_lens + B && seq_lens < new_lens + B)
-    return fail(kErrInvalid, "%s: new_lens overlaps seq_lens, which every workgroup reads", who);
+  const struct { const int32_t* p; int64_t n; const char* name; } read[] = {
+      {seq_lens, B, "seq_lens"}, {cu, B + 1, "cu"}, {kept, B, "kept"}, {keep, most > 0 ? (B - 1) * ldk + most : 0, "keep"},
+      {table, width > 0 ? (B - 1) * ldt + width : 0, "the page table"}};
+  for (const auto& r : read)
+    if (new_lens && r.p && r.n > 0 && new_lens < r.p + r.n && r.p < new_lens + B)
+      return fail(kErrInvalid, "%s: new_lens overlaps %s, which every workgroup reads", who, r.name);
   if ((rc = distinct(who, arrays, caches))) return rc;
   for (int64_t i = 0; i < caches; i += kKv4Caches) {
     Kv4Caches cs = {};
