@@ -569,8 +569,9 @@ PyObject* kv4_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!ints(parents, 1) || !ints(cu, 1) || !ints(lens, 1) || !PyLong_Check(a[3]) || !PyLong_Check(a[4])) Py_RETURN_NONE;
     const int64_t max_q = PyLong_AsLongLong(a[3]), window = PyLong_AsLongLong(a[4]);
     if (PyErr_Occurred()) return nullptr;
-    const int64_t T = parents->size(0), B = lens->size(0), words = (max_q + 31) / 32;
-    if (max_q < 1 || words > 128 || window < 0 || cu->size(0) != B + 1 || !same_device(*parents, cu, lens)) Py_RETURN_NONE;
+    const int64_t T = parents->size(0), B = lens->size(0);
+    if (max_q < 1 || max_q > 4096 || window < 0 || cu->size(0) != B + 1 || !same_device(*parents, cu, lens)) Py_RETURN_NONE;
+    const int64_t words = (max_q + 31) / 32;
     at::Tensor mask = empty(*parents, {T, words}, at::kInt), pos = empty(*parents, {T}, at::kInt);
     void* st = stream_of(*parents);
     const int rc = unlocked([&] {

@@ -150,3 +150,11 @@ def test_windows_past_the_table_are_nan(dev, dtype, D, width, new):
                 see = [x if i % 3 else [] for i, x in enumerate(see)]
                 at = [min(p + rng.randrange(0, 2 * window), 2 ** 31 - 1) for p in tree.positions.tolist()]
                 check(s, q, mask_tree(see, at, dev, tree.mask.shape[1]), see, window, **kw)
+
+
+@pytest.mark.gpu
+def test_tree_sizes_past_64_bits_are_refused(dev):
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=dev)  # noqa: E731
+    for max_q in (2 ** 63 - 1, 2 ** 62, 4097, 0, -2 ** 63):
+        with pytest.raises(ValueError, match="max_q"):
+            _kv4().kv4_tree(i32(-1, 0), i32(0, 2), i32(5), max_q=max_q)
