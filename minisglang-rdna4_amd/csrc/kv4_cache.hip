@@ -37,8 +37,7 @@ struct Place {
   bool first;
   int left;
 };
-__device__ __forceinline__ bool kv4_place(const Kv4Batch& s, int b, int64_t i, Place& p) {
-  while (b + 1 < s.B && s.cu[b + 1] <= i) ++b;
+__device__ __forceinline__ bool kv4_place_in(const Kv4Batch& s, int b, int64_t i, Place& p) {
   int64_t start;
   int n;
   kv4_rows(s, b, start, n);
@@ -48,6 +47,30 @@ __device__ __forceinline__ bool kv4_place(const Kv4Batch& s, int b, int64_t i, P
   p.pos = (int64_t)s.lens[b] - p.left;
   p.first = i == start;
   return true;
+}
+__device__ __forceinline__ bool kv4_place(const Kv4Batch& s, int b, int64_t i, Place& p) {
+  while (b + 1 < s.B && s.cu[b + 1] <= i) ++b;
+  return kv4_place_in(s, b, i, p);
+}
+// The sequences of the wave's rows i0 .. i0 + ROWS - 1, of which a lane has row lane % ROWS, given the first one's: the next 64
+// sequences are looked at together, since a walk from one to the next is a chain of reads (us, 1100 rows of 8 heads of 128, each
+// of another sequence: 5.0, walked 5.4; 4096 rows 9.9 and 10.4)
+template <int ROWS>
+__device__ __forceinline__ int kv4_sequence_of(const Kv4Batch& s, int b0, int64_t i0, int lane) {
+  const int at = b0 + 1 + lane;
+  const int64_t begins = at < s.B ? s.cu[at] - i0 : ROWS;
+  const int row = (int)(begins < 0 ? 0 : begins < ROWS ? begins : ROWS);  // of the wave's rows, the sequence's first
+  int steps = 0;
+  if (__ballot(row < ROWS))
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const uint64_t later = ~__ballot(row <= r);
+      if ((lane & (ROWS - 1)) == r) steps = later ? __builtin_ctzll(later) : 64;
+    }
+  int b = b0 + steps;
+  if (steps == 64)
+    while (b + 1 < s.B && s.cu[b + 1] <= i0 + (lane & (ROWS - 1))) ++b;
+  return b;
 }
 
 // maximum over the L lanes of a vector
@@ -209,7 +232,8 @@ kv4_read_kernel(Kv4Cache c, Kv4Batch s, int per, uint16_t* __restrict__ k, uint1
   {
     const int64_t i = i0 + (lane & (ROWS - 1));
     Place pl;
-    if (i < s.T && kv4_place(s, b0, i, pl)) {
+    const int b = kv4_sequence_of<ROWS>(s, b0, i0, lane);
+    if (i < s.T && kv4_place_in(s, b, i, pl)) {
       const int page = kv4_page(c, s, pl.b, pl.pos);
       slot = (int)(pl.pos & 7);
       look = page >= 0 ? kv4_block(c, page, 0, (int)(pl.pos & ~(int64_t)7)) : -1;
@@ -288,9 +312,10 @@ int launch_kv4_append(const void* k, int64_t ldk, int64_t hk, const void* v, int
 template <int D, int DT>
 static int read(const Kv4Cache& c, const Kv4Batch& s, uint16_t* k, uint16_t* v, hipStream_t st) {
   constexpr int VP = 512 / D;
-  // few rows (a decode step's, each of another sequence): as many as a wave holds side by side, and a head. us, 64 rows of 8
-  // heads: 3.3, 4.8 with 8 rows a wave
-  const bool few = s.T * c.H <= 8192;
+  // Few rows (a decode step's, each of another sequence): as many as a wave holds side by side, and a head. us with them / with
+  // 8 rows a wave, 8 heads of 128: 64 rows 3.8 / 4.2, 1100 4.5 / 4.6, 1500 4.7 / 4.8, 2048 5.3 / 5.2, 3000 6.4 / 5.9, 8192
+  // 12.2 / 10.5.
+  const bool few = s.T * c.H <= 12288;
   const int rows = few ? VP : 8;
   // as many heads a wave as leave two waves for each place on the card (8192)
   const int64_t groups = (s.T + rows - 1) / rows, most = groups * c.H / 16384;

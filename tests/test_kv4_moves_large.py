@@ -62,6 +62,29 @@ def test_many_rows_are_read_as_few(dev, dtype, D, H, page, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,H,most", [(128, 1, 3), (64, 3, 2), (256, 2, 12), (128, 20, 5)])
+def test_rows_of_many_sequences(dev, D, H, most):
+    """Rows next to each other of different sequences, with more than 64 empty ones between two, rows before and behind all; the
+    bits of each sequence read alone."""
+    rng = random.Random(most)
+    news = [0] * 3 + [rng.choice((0, 1, rng.randrange(0, most))) for _ in range(900)] + [1] + [0] * 64 + [2] + [0] * 150 + [1, 1] + [0] * 70
+    page, B = 16, len(news)
+    lens = [n + rng.randrange(0, 20) if n else 5 for n in news]
+    width = -(-max(lens) // page)
+    c = scaled(dev, 300, page, H, D, torch.bfloat16, H)
+    table = torch.randint(0, 300, (B, width), generator=torch.Generator().manual_seed(1), dtype=torch.int32).to(dev)
+    cu = [3 + sum(news[:i]) for i in range(B + 1)]
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=dev)  # noqa: E731
+    T = cu[-1] + 4
+    got = _kv4().kv4_read(c, table, i32(*cu), i32(*lens), T)
+    for b, n in enumerate(news):
+        if n:
+            want = _kv4().kv4_read(c, table[b:b + 1], i32(0, n), i32(lens[b]), n)
+            for a, w in zip(got, want):
+                assert torch.equal(a[cu[b]:cu[b + 1]].view(torch.int16), w.view(torch.int16)), b
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("page,H,D,layers,n", [(64, 8, 128, 3, 230), (16, 5, 64, 70, 161), (128, 3, 256, 1, 400)])
 def test_many_pages(dev, page, H, D, layers, n):
     """More bytes than the caches hold, to the last of them."""
