@@ -423,10 +423,11 @@ int w4a8_prompt_attention(const void* q, int64_t ldq, int64_t hq, const void* k,
 /* ---- Rotary positions. The first R channels of a head (16 to D, a multiple of 16) are R/2 pairs, channels i and i + R/2, or
  * 2i and 2i + 1 (adjacent); pair i is turned by t = positions[axis[i], token] * f_i:
  *   a' = scale (a cos t - b sin t),  b' = scale (a sin t + b cos t),
- * in f32, rounded once; channels behind R stay. turns[i]: f_i / (2 pi) modulo 1 in units of 2^-64, so that any position's
- * angle is exact to 2^-32 of a turn. positions (axes, T), ldp entries between axes, 32 or 64 bits, signed; axis (R/2) with
- * entries below axes, or null for one axis. q (T, Hq, D) and k (T, Hk, D; Hk may be 0) with strides that are multiples of 8
- * elements; D a multiple of 8 up to 1024. q_out and k_out may be q and k themselves; any other overlap is refused. */
+ * in f32, rounded once; channels behind R stay. turns[i]: f_i / (2 pi) modulo 1 in units of 2^-64; the angle is off by the
+ * position times what turns[i] is off by (2^-65 where it is the nearest) and by 2^-32 of a turn. positions (axes, T), ldp
+ * entries between axes, 32 or 64 bits, signed; axis (R/2) with entries below axes, or null for one axis. q (T, Hq, D) and
+ * k (T, Hk, D; Hk may be 0) with strides that are multiples of 8 elements; D a multiple of 8 up to 1024. q_out and k_out may be
+ * q and k themselves; any other overlap is refused. */
 int w4a8_rotary(const void* q, int64_t ldq, int64_t hq, int64_t Hq, const void* k, int64_t ldk, int64_t hk, int64_t Hk,
                 int dtype, int64_t T, int64_t D, int64_t R, int adjacent, const void* positions, int positions_64,
                 int64_t axes, int64_t ldp, const uint64_t* turns, const int32_t* axis, float scale, void* q_out,

@@ -2,8 +2,8 @@
 // t = position[axis(i)] f_i:   a' = s (a cos t - b sin t),  b' = s (a sin t + b cos t).
 //
 // Angles. Positions are whole numbers, so t in turns is position * (f_i / 2 pi) modulo 1, and with f_i / 2 pi as a
-// fraction of 2^64 that is one 64-bit integer product that overflows as it should: exact for any position, where an f32
-// product is off by 4e-3 at position 131072. Its upper 32 bits are cut into quarters of a turn and a rest within an
+// fraction of 2^64 that is one 64-bit integer product that overflows as it should and rounds nothing: off by the position times
+// the fraction's 2^-65, where an f32 product is off by 4e-3 at position 131072. Its upper 32 bits are cut into quarters of a turn and a rest within an
 // eighth, whose sine and cosine are Taylor's polynomials (to x^9 and x^10: the next terms are below 2e-9 and 2e-10).
 //
 // A thread has one token and one unit of 8 pairs, 16 bytes each of a and b, works its 8 angles out once, and turns that

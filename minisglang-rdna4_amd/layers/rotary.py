@@ -3,8 +3,8 @@ video).
 
 Not a mirror of the reference's layers/rotary.py, which lies outside what this package restates. Pair i of a head's
 first ``rotary_dim`` channels is turned by position[axis of i] * f_i, in f32 and rounded once. Angles are worked out in the
-kernel from whole positions and frequencies as 64-bit fractions of a turn: exact for any position, with no table of sines
-and cosines to keep or to outgrow.
+kernel from whole positions and frequencies as 64-bit fractions of a turn, with no table of sines and cosines to keep or to
+outgrow: off by 2^-32 of a turn, and by 2^-65 for each position from 0 (at 2^31 2^-34, at 2^45 2^-20).
 """
 from __future__ import annotations
 
@@ -22,6 +22,31 @@ engaged = importlib.import_module(f"{_pkg}._hip_engage").engaged
 _MAX_AXES = 8
 
 
+def _two_pi(bits: int) -> int:
+    """2 pi in 2^-bits, to the last place or two: 8 (4 atan(1/5) - atan(1/239)), Machin's sum."""
+    one = 1 << (bits + 16)
+
+    def atan(n: int) -> int:
+        term = one // n
+        total, k = 0, 1
+        while term:
+            total += term // k if k % 4 == 1 else -(term // k)
+            term //= n * n
+            k += 2
+        return total
+
+    return (8 * (4 * atan(5) - atan(239))) >> 16
+
+
+def _turns(freq: float) -> int:
+    """freq / 2 pi modulo 1 in units of 2^-64, to the nearest."""
+    bits = 96 + max(0, math.frexp(freq)[1])
+    n, d = freq.as_integer_ratio()
+    d *= _two_pi(bits)
+    n <<= 64 + bits
+    return ((2 * n + d) // (2 * d)) % (1 << 64)
+
+
 def _rows_ok(t: torch.Tensor) -> bool:
     return t.stride(2) == 1 and all(t.shape[i] <= 1 or t.stride(i) % 8 == 0 for i in (0, 1)) and t.data_ptr() % 16 == 0
 
@@ -30,8 +55,8 @@ class Rotary:
     """Rotary positions for heads of ``head_dim`` channels (a multiple of 8, up to 1024), of which the first ``rotary_dim``
     (default: all; a multiple of 16) turn: pairs are channels i and i + rotary_dim/2, or with ``adjacent`` 2i and 2i + 1.
 
-    Frequencies are base ** (-2i / rotary_dim), or ``inv_freq`` (rotary_dim/2 of them, f64 at best: scaled ones are given this
-    way). ``scale`` multiplies the turned channels (attention factors of scaled frequencies). ``sections``: with several axes
+    Frequencies are base ** (-2i / rotary_dim) in f64, or ``inv_freq`` (rotary_dim/2 of them, f64 at best: scaled ones are given
+    this way). ``scale`` multiplies the turned channels (attention factors of scaled frequencies). ``sections``: with several axes
     of positions, the pairs of each axis, which add up to rotary_dim/2; the first pairs are axis 0's, the next axis 1's, or
     with ``interleaved`` pair i is axis i % axes' while i < axes * sections[i % axes], and else axis 0's."""
 
@@ -61,9 +86,8 @@ class Rotary:
             axis = [i % axes if i < axes * sections[i % axes] else 0 for i in range(pairs)]
         else:
             axis = [a for a, n in enumerate(sections) for _ in range(n)]
-        # turns per position modulo 1, in 2^-64: f / (2 pi) has 53 bits, and the product with the position wraps as it should
-        turns = [round(f / (2.0 * math.pi) * 2.0 ** 64) % (1 << 64) for f in freq]
-        turns = [t - (1 << 64) if t >= 1 << 63 else t for t in turns]
+        # turns per position, whose product with the position wraps as it should; signed, as torch's integers are
+        turns = [(_turns(f) + (1 << 63)) % (1 << 64) - (1 << 63) for f in freq]
         self.head_dim, self.rotary_dim, self.axes = head_dim, rotary_dim, axes
         self.sections, self.adjacent, self.scale = sections, bool(adjacent), float(scale)
         self.turns = torch.tensor(turns, dtype=torch.int64, device=device)
