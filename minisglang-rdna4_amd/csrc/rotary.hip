@@ -7,8 +7,8 @@
 // eighth, whose sine and cosine are Taylor's polynomials (to x^9 and x^10: the next terms are below 2e-9 and 2e-10).
 //
 // A thread has one token and one unit of 8 pairs, 16 bytes each of a and b, works its 8 angles out once, and turns that
-// unit in `per` heads. Bound by memory for prompts (8191 tokens of 40 heads of 128, 168 MB in and out: 40 us, 4.2 TB/s), by the
-// launch for decode (3.5 us).
+// unit in `per` heads. Bound by memory for prompts (8191 tokens of 40 heads of 128, 168 MB in and out: 34 to 40 us, 4.2 to 5
+// TB/s), by the launch for decode (3.5 us).
 #include "rotary.h"
 
 namespace w4a8 {
@@ -144,8 +144,12 @@ int launch_rotary(Rotary& p, int D, int dtype, hipStream_t st) {
   p.per = (int)(rows / 524288 < 1 ? 1 : rows / 524288 > kHeads ? kHeads : rows / 524288);
   const int64_t threads = p.T * ((p.heads + p.per - 1) / p.per) * p.units, wgs = (threads + 255) / 256;
   if (wgs > kMaxGrid) return kErrUnsupported;
-  // us, 168 MB in and out, other rows each time, past the caches / through them: 39.9 / 48.5
-  if (p.T * p.heads * D * 4 > kL2Bytes) launch<true>(p, dtype, dim3((unsigned)wgs), st);
+  // Past the caches where both halves of a head are whole lines of 128 bytes and the rows more than the caches could keep for who
+  // reads them next. us, 40 heads, in and out, other rows each time, past / through the caches (kv4_append behind it in
+  // brackets): 128 channels 42 MB 18.0 / 15.7 (26.9 / 24.5), 84 MB 22.7 / 21.8 (36.0 / 35.1), 106 MB 25.7 / 26.3 (43.0 / 43.0),
+  // 168 MB 33.5 / 39.8 (55.1 / 60.0). Parts of lines are slower past them at any size: 64 channels 168 MB 42.6 / 40.3,
+  // neighbours as pairs 50.3 / 40.8, 96 of 128 channels 50.5 / 49.6.
+  if (!p.adjacent && p.R % 128 == 0 && p.T * p.heads * D * 4 > 3 * kL2Bytes) launch<true>(p, dtype, dim3((unsigned)wgs), st);
   else launch<false>(p, dtype, dim3((unsigned)wgs), st);
   return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }

@@ -1,5 +1,5 @@
-"""Rotary positions far from 0 (layers/rotary.py): the fractions of a turn against pi in whole numbers, on the CPU, and on the GPU
-64-bit positions against exact angles."""
+"""Rotary positions far from 0 and of many rows (layers/rotary.py): the fractions of a turn against pi in whole numbers, on the CPU,
+and on the GPU 64-bit positions against exact angles, and rows that take the way past the caches against the same rows a few at a time."""
 import math
 import random
 from fractions import Fraction
@@ -57,3 +57,23 @@ def test_far_positions(dev, dtype):
     h = 2.0 ** (-8 if dtype == torch.bfloat16 else -11)
     for o in out:
         assert ((o.cpu().double() - want).abs() <= h * want.abs() + tol + 2.0 ** -25).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,R,T", [(128, 128, 5003), (256, 128, 2501), (256, 256, 2600)])
+def test_rows_past_the_caches(dev, dtype, D, R, T):
+    Hq, H = 37, 5
+    assert T * (Hq + H) * D * 4 > 96 << 20
+    g = torch.Generator(device=dev).manual_seed(1)
+    qkv = torch.randn(T, (Hq + 2 * H) * D, generator=g, device=dev).to(dtype)
+    q, k, v = (t.view(T, -1, D) for t in qkv.split([Hq * D, H * D, H * D], dim=1))
+    pos = torch.randint(0, 1 << 20, (T,), generator=g, device=dev)
+    rot = pkg("layers.rotary").Rotary(D, rotary_dim=R, scale=1.25, device=dev)
+    want = [rot.forward(q[i:i + 100], k[i:i + 100], pos[i:i + 100]) for i in range(0, T, 100)]
+    want = tuple(torch.cat(t) for t in zip(*want))
+    got = rot.forward(q, k, pos)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    before = v.clone()
+    rot.forward_inplace(q, k, pos)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, before)
