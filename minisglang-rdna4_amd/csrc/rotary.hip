@@ -149,7 +149,7 @@ int launch_rotary(Rotary& p, int D, int dtype, hipStream_t st) {
   // brackets): 128 channels 42 MB 18.0 / 15.7 (26.9 / 24.5), 84 MB 22.7 / 21.8 (36.0 / 35.1), 106 MB 25.7 / 26.3 (43.0 / 43.0),
   // 168 MB 33.5 / 39.8 (55.1 / 60.0). Parts of lines are slower past them at any size: 64 channels 168 MB 42.6 / 40.3,
   // neighbours as pairs 50.3 / 40.8, 96 of 128 channels 50.5 / 49.6.
-  if (!p.adjacent && p.R % 128 == 0 && p.T * p.heads * D * 4 > 3 * kL2Bytes) launch<true>(p, dtype, dim3((unsigned)wgs), st);
+  if (!p.adjacent && p.R % 128 == 0 && p.T * p.heads * D * 4 > 96 << 20) launch<true>(p, dtype, dim3((unsigned)wgs), st);
   else launch<false>(p, dtype, dim3((unsigned)wgs), st);
   return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;
 }

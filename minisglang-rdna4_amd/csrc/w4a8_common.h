@@ -136,8 +136,8 @@ __device__ __forceinline__ float from_dtype(uint16_t h, int dtype) {
 // `bytes` return 0; the scalar offset is not part of that check.
 typedef unsigned int v4u __attribute__((ext_vector_type(4)));
 
-// 16 bytes of what is read or written once; NT: past the caches, for calls with more of it than the 8 L2s hold
-constexpr int64_t kL2Bytes = 32 << 20;
+// 16 bytes of what is read or written once; NT: past the caches, for calls with so much of it that whoever reads it next
+// would not find it there (the last one holds 256 MB, for what is read as well)
 template <bool NT>
 __device__ __forceinline__ v4u stream_read(const void* p) {
   const v4u* at = reinterpret_cast<const v4u*>(p);

@@ -21,7 +21,8 @@ def scaled(dev, pages, page, H, D, dtype, seed):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("D,H,page,T", [(128, 5, 64, 66003), (64, 7, 16, 80003), (256, 3, 32, 90005), (128, 1, 16, 70001), (64, 5, 128, 1700)])
+@pytest.mark.parametrize("D,H,page,T", [(128, 5, 64, 66003), (64, 7, 16, 80003), (256, 3, 32, 90005), (128, 1, 16, 70001), (64, 5, 128, 1700),
+                                          (128, 5, 64, 140003), (64, 7, 32, 190001), (256, 3, 16, 120005)])
 def test_many_rows_are_read_as_few(dev, dtype, D, H, page, T):
     """The bits of the same rows read a few hundred at a time, each head's own; rows without a page are NaN."""
     lens = [T * 3 // 5, 1, T - T * 3 // 5 - 1]
@@ -85,7 +86,8 @@ def test_rows_of_many_sequences(dev, D, H, most):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("page,H,D,layers,n", [(64, 8, 128, 3, 230), (16, 5, 64, 70, 161), (128, 3, 256, 1, 400)])
+@pytest.mark.parametrize("page,H,D,layers,n", [(64, 8, 128, 3, 230), (16, 5, 64, 70, 161), (128, 3, 256, 1, 400), (64, 8, 128, 3, 701), (16, 5, 64, 70, 461),
+                                                    (128, 3, 256, 1, 1501)])
 def test_many_pages(dev, page, H, D, layers, n):
     """More bytes than the caches hold, to the last of them."""
     pages = 2 * n + 3
