@@ -5,9 +5,9 @@
 // The queries that share a key/value head are columns (column c: query c / G, head h G + c % G), 32 a wave, and the 4 or 8
 // waves of a workgroup share tiles of 64 tokens that are widened to fp16 once, in LDS:
 //   S = b sum(q) + K' Q^T,  p = 2^(S scale - M),  O += V'^T p   (32x32x16 products; tokens, then channels are rows).
-// K' = s (c - 7.5) as s/2 (2 c - 15), b = m + 7.5 s. bf16 models: s comes as s 2^-e, e one for the tile, so that it fits fp16: 8 bits
-// times the code's 4 lose one bit at most, 2^-11 of what is left once the middle of the vector's range is taken out; fp16
-// models, whose scores ought to be better than that, have K' = 2 c - 15, exactly, b = 2 m / s + 15, and S times s/2 afterwards.
+// K' = s (c - 7.5) as s/2 (2 c - 15), b = m + 7.5 s. bf16 models: s comes as s 2^-e, e one for the tile, so that it fits fp16 (one
+// for each token, and S times their difference, where steps of a tile are more than 2^20 apart): 8 bits times the code's 4 lose
+// one bit at most, 2^-11 of what is left once the middle of the vector's range is taken out; fp16 models, whose scores ought to be better than that, have K' = 2 c - 15, exactly, b = 2 m / s + 15, and S times s/2 afterwards.
 // V' = s c + m, rounded once to fp16 (2^-11), times 2^-e with e the largest so far. fp16 models have the codes, exactly, p s
 // rounded instead (times 2^-e, e of the largest step so far) and sum p (m + 7.5 s) beside the product, in f32: their
 // output would show the rounding of V' (norm of the error over the output's 3.5e-4, so 3.0e-4; rounding the output 2.1e-4).
@@ -40,12 +40,12 @@ typedef float v8f __attribute__((ext_vector_type(8)));
 
 struct alignas(32) ScaleTable {
   float b[kStep];        // in the order of S's rows: [32 tokens][half][16 registers]
-  float s[kStep];        // fp16 models: half of K's steps in that order
+  float s[kStep];        // what S is multiplied by, in that order: half of K's steps, of bf16 models, if `apart`, 2^(the token's e - e)
   uint32_t ks[kStep];    // bf16 models: half of K's step, twice, by token
   uint32_t v[8][8];      // bf16 models: V's steps of tokens j and j + 4 of the block (j < 4), and their least values
   float sv[kStep];       // fp16 models: V's steps, in the order of S's rows,
   float bv[kStep];       // and the middles m + 7.5 s, which may be past fp16's end
-  int ek, ev;
+  int ek, ev, apart;
 };
 
 // A word's codes of nibbles j and j + 4 as fp16 numbers, c and 2 c - 15: 1024 with a code in its lowest bits, or a bit higher.
@@ -190,12 +190,17 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
       if (kFold) {
         // the largest step into [2^11, 2^12): times 7.5 it stays in fp16
         // (and least values that no kv4_append gives such a step stay in f32)
-        e = min(max((int)(__float_as_uint(wave_max(in && !bad ? fmaxf(s, fabsf(m0) * 0x1p-14f) : 0.f)) >> 23) - 138, -100), 120);
-        const uint32_t x = (uint32_t)f32_to_f16(__builtin_ldexpf(s, -e - 1));
+        const float size = in && !bad ? fmaxf(s, fabsf(m0) * 0x1p-14f) : 0.f;
+        auto power = [](float x) { return min(max((int)(__float_as_uint(x) >> 23) - 138, -100), 120); };
+        e = power(wave_max(size));
+        // with one e, fp16 has fewer than a step's 8 bits for those 2^24 below the largest: the tokens have an e each then
+        const bool apart = __ballot(size > 0x1p-120f && power(size) < e - 20) != 0;
+        const int own = apart ? power(size) : e;
+        const uint32_t x = (uint32_t)f32_to_f16(__builtin_ldexpf(s, -own - 1));
         tb.ks[lane] = x | (x << 16);
-      }
-      if (kFold) {
-        tb.b[r] = !in ? 0.f : bad ? __builtin_nanf("") : __builtin_ldexpf(c0, -e);
+        tb.b[r] = !in ? 0.f : bad ? __builtin_nanf("") : __builtin_ldexpf(c0, -own);
+        if (apart) tb.s[r] = __builtin_ldexpf(1.f, own - e);
+        if (lane == 0) tb.apart = apart;
       } else {
         // a vector of equal values has no step, and codes of 0: any small one does
         const float s2 = fmaxf(0.5f * s, fmaxf(fabsf(m0) * 0x1p-30f, 0x1p-60f));
@@ -362,7 +367,7 @@ kv4_tree_attn_kernel(const Kv4Attn p) {
         if (!kFold && w >= KS - 2) ws[w & 1] = weights(tb, w & 1);
         in_order();
       }
-      if (!kFold) {
+      if (!kFold || __builtin_amdgcn_readfirstlane(tb.apart)) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
           const float* tsl = &tb.s[kb * 32 + half * 16];

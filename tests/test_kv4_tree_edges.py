@@ -1,6 +1,6 @@
 """Trees of drafted tokens over the 4-bit cache at the edges of what a call may hold: queries, keys and steps whose powers of
-two leave f32's range, maxima that one tile's units cannot hold, sequences longer than their table under a window, values at
-fp16's ends. References and tolerances are test_kv4_tree's."""
+two leave f32's range, keys of all sizes side by side, maxima that one tile's units cannot hold, sequences longer than their
+table under a window, values at fp16's ends. References and tolerances are test_kv4_tree's."""
 import math
 import random
 
@@ -86,6 +86,38 @@ def test_a_far_maximum_beside_keys_of_zeros(dev, dtype, sign):
     see = [x if i % 3 else [] for n in news for i, x in enumerate([[i] for i in range(n)])]
     out = check(s, q, mask_tree(see, [0] * len(see), dev, 1), see, max_q=32, max_kv=544)
     assert torch.isfinite(out.float()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,G", [(128, 4), (64, 2)])
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 25, 2.0 ** 45, 2.0 ** 90])
+@pytest.mark.parametrize("equal", [True, False])
+def test_keys_of_all_sizes_in_one_tile(dev, D, G, size, equal):
+    """Context tokens with keys many times as large as their neighbours', whose scores are so far below those that they weigh
+    nothing, and drafted tokens with such keys that some rows do not see: what the rest weighs is as without them. (All
+    channels alike, a step of 2^-14 of the vector, or not.)"""
+    rng = random.Random(D)
+    lens, news = [700, 130], [40, 33]
+    s = Setup(dev, torch.bfloat16, D, 1, 64, lens, news, seed=13)
+    g = torch.Generator().manual_seed(5)
+    big = torch.zeros(sum(lens), dtype=torch.bool)
+    for b, (n, new) in enumerate(zip(lens, news)):
+        at = sum(lens[:b])
+        big[at:at + n - new:5] = True
+        big[at + n - new:at + n:7] = True
+    s.k[big] = (size * (torch.ones(1) if equal else torch.rand(int(big.sum()), 1, D, generator=g) * 0.5 + 0.75)).to(torch.bfloat16)
+    again(s)
+    q = (s.q(G).float() * 0.5 - 1.0).to(torch.bfloat16)  # the sum of a row's channels is below zero
+    see = [[j for j in x if j % 7] or [1] for n in news for x in lines(random_tree(n, rng))]
+    out = s.attend(q, tree=mask_tree(see, [0] * len(see), dev, 2), max_q=40, max_kv=700).cpu().double()
+    # test_kv4_tree's tolerance, d over the keys that weigh something
+    k, v = cache_values(s.cache)
+    args = (s.table, s.page, lens, news, see, [0] * len(see), D ** -0.5)
+    want, _, A, _, _ = ref(q, (k, v), *args, bounds=True)
+    _, _, _, _, d = ref(q, (torch.where(k.abs().amax(-1, keepdim=True) > size / 2, 0.0, k), v), *args, bounds=True)
+    rest = 2.0 ** -11 * (2.5 * A + want.abs()) + d * (A + want.abs())
+    vmax = s.v.float().abs().max().item()
+    assert ((out - want).abs() <= 2.0 ** -8 * want.abs() + torch.maximum(rest, torch.full_like(rest, 3.5e-4 * vmax)) + 2.0 ** -25).all()
 
 
 @pytest.mark.gpu
