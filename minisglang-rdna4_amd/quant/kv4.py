@@ -331,7 +331,8 @@ def kv4_attention(
     logarithm of each softmax's sum, (T, num_qo_heads) f32.
 
     num_qo_heads is a multiple of the cache's heads. sm_scale defaults to head_dim ** -0.5; it is positive
-    and below 65536, and bf16 queries are below 2^96, cached values' steps below 2^100. causal: a
+    and below 65536, and scores are within f32's range, bf16 queries below 2^96, steps of cached keys below 2^100, of cached values
+    below 2^64 (below 2^100 where none of the sequence's is below 2^-4: the small ones would weigh less). causal: a
     token sees the keys up to its own position; window > 0: only the last ``window`` of those. A row
     that sees no key is 0 (lse -inf). out, where given, may be strided; rows outside cu_q keep what they
     hold there, and are undefined in a fresh output. Rows of out that overlap are refused, and so is an out that
@@ -339,12 +340,14 @@ def kv4_attention(
 
     tree: the new tokens are drafted ones; a token sees the cached context before them and, of them, those that its
     row of ``tree.mask`` names (``causal`` says nothing then). window > 0 counts from ``tree.positions``, among cached
-    tokens: of the new ones the mask alone decides. With more than 64 queries that share a key (max_q times the heads of a
-    group) and no window, bf16 models' values below 2^-29 of their sequence's largest count as 0.
+    tokens: of the new ones the mask alone decides. More than 64 queries that share a key (max_q times the heads of a
+    group) have a kernel of their own where there is no window, heads have up to 128 channels and max_kv is 512 or more: products
+    there are in fp16, errors before the output's rounding are up to four times as large, and bf16 models' values below 2^-29 of
+    their sequence's largest count as 0.
 
     max_q and max_kv, the most new tokens and the greatest length of a sequence, are what the host
-    plans the launch by (default: T rows, and the table's capacity). Too large a bound costs time, too
-    low a one as well; neither changes which keys are read. One launch, and a second that joins the
+    plans the launch by (default: T rows, and the table's capacity): how it is split, and for trees the kernel, whose
+    roundings differ. Too large a bound costs time, too low a one as well; neither changes which keys are read. One launch, and a second that joins the
     parts where the keys are split over workgroups."""
     what = "kv4_attention"
     if sm_scale is None:
