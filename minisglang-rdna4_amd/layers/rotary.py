@@ -8,6 +8,7 @@ outgrow: off by 2^-32 of a turn, and by 2^-65 for each position from 0 (at 2^31 
 """
 from __future__ import annotations
 
+import functools
 import importlib
 import math
 from typing import Sequence
@@ -22,6 +23,7 @@ engaged = importlib.import_module(f"{_pkg}._hip_engage").engaged
 _MAX_AXES = 8
 
 
+@functools.lru_cache(maxsize=None)
 def _two_pi(bits: int) -> int:
     """2 pi in 2^-bits, to the last place or two: 8 (4 atan(1/5) - atan(1/239)), Machin's sum."""
     one = 1 << (bits + 16)
