@@ -134,9 +134,9 @@ __device__ __forceinline__ Span kv4_span(const Kv4Attn& p, int b) {
   s.first_pos = len - s.cut - s.n;
   return s;
 }
-// The sequence of the launch's z-th workgroups: the longest first, up to 64 sequences, so that short ones fill the launch's
-// end (more sequences even themselves out). The whole wave calls. us, in this order / as they come: 48 sequences of up to
-// 26 drafted tokens on up to 8192 193 / 269.
+// The sequence of the launch's z-th workgroups: the longest first, up to 64 sequences (a lane's each), so that short ones fill the
+// launch's end. The whole wave calls. us, in this order / as they come: 48 sequences of up to 26 drafted tokens on up to 8192
+// 193 / 269. More come as the caller has them, and want sorting by who builds the batch: 65 361, sorted 285; 128 627 and 480.
 __device__ __forceinline__ int kv4_longest(const Kv4Batch& s, int z) {
   if (s.B > 64 || s.B == 1) return z;
   const int lane = threadIdx.x & 63;

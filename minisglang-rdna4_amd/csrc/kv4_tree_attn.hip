@@ -7,7 +7,8 @@
 //   S = b sum(q) + K' Q^T,  p = 2^(S scale - M),  O += V'^T p   (32x32x16 products; tokens, then channels are rows).
 // K' = s (c - 7.5) as s/2 (2 c - 15), b = m + 7.5 s. bf16 models: s comes as s 2^-e, e one for the tile, so that it fits fp16 (one
 // for each token, and S times their difference, where steps of a tile are more than 2^20 apart): 8 bits times the code's 4 lose
-// one bit at most, 2^-11 of what is left once the middle of the vector's range is taken out; fp16 models, whose scores ought to be better than that, have K' = 2 c - 15, exactly, b = 2 m / s + 15, and S times s/2 afterwards.
+// one bit at most, 2^-11 of what is left once the middle of the vector's range is taken out; fp16 models, whose scores ought to
+// be better than that, have K' = 2 c - 15, exactly, b = 2 m / s + 15, and S times s/2 afterwards.
 // V' = s c + m, rounded once to fp16 (2^-11), times 2^-e with e the largest so far. fp16 models have the codes, exactly, p s
 // rounded instead (times 2^-e, e of the largest step so far) and sum p (m + 7.5 s) beside the product, in f32: their
 // output would show the rounding of V' (norm of the error over the output's 3.5e-4, so 3.0e-4; rounding the output 2.1e-4).
@@ -24,11 +25,12 @@
 // The scales are unpacked by two of the waves, by turns, a token a lane, into tables. What is read from LDS is read a product
 // or more ahead, exponentials run behind the products of the 16 tokens before them, and the next tile's widening behind the
 // last products: in the compiler's own order each product waited for its operands (14 us more in either case below).
-// us: 48 users' 26 tokens and less on up to 8192 (8 heads of 4 queries, bf16) 191, with kv4_attn_kernel 216; two users' 60
-// tokens on 65536 and less, fp16, 205 (with V' rounded as bf16 models have it 187) / 279, 610 TFLOP/s. Waves without columns
-// only widen: 6 us of the second. No unit is full: of a CU's time vector instructions take 54 %, matrix products 34 %, LDS
-// 40 %; two waves a SIMD, which the accumulators leave room for, do not cover each other's latencies. Tried: the waves of a
-// SIMD half a tile apart, so that one has products while the other has exponentials (no faster).
+// us, this launch alone, under the profiler: 48 users' 26 tokens and less on up to 8192 (8 heads of 4 queries, bf16) 184, with
+// kv4_attn_kernel 216; two users' 60 tokens on 65536 and less, fp16, 205 (with V' rounded as bf16 models have it 187) / 279.
+// Waves without columns only widen: 6 us of the second. No unit is full: of the second's busy cycles vector instructions take
+// 58 %, matrix products 31 %, LDS 43 % (the first's 53, 24, 35); two waves a SIMD, which the accumulators leave room for, do not
+// cover each other's latencies. Tried: the waves of a SIMD half a tile apart, so that one has products while the other has
+// exponentials (no faster).
 #include "kv4.h"
 #include "tile32.h"
 

@@ -18,13 +18,17 @@
 // rounding then weighs values a little differently, and equal values keep their bits. fp16: M is 7 less, so that what is
 // lost below fp16's least, 2^-32 a key of the largest, is nothing over any prompt.
 //
-// Measured: 8192 + 5690 + 3190 tokens, 32 heads on 8 of 128 channels (898 GFLOP), 1.02 ms, 882 TFLOP/s, bf16; heads of 64
-// 754, of 256 857. Bound by power: the matrix units are busy for half of the cycles at 1.75 GHz, and the same cycles take
-// 0.79 ms at 2.2 GHz where all values are 0; products alone, from registers, reach 1.7 PFLOP/s on such values. No
-// exponentials at all would save 6% of the time, no reads of K from LDS 5%, no copies of K and V into LDS 12%.
-// First version 774: S, exponentials and products one after another, 8 waves a workgroup (two workgroups of 4 waves on a CU
-// do not wait for each other: 23 prompts of up to 1999 tokens, heads of 64, 281 -> 234 us). Other steps: blocks of 32 keys
-// whose S is computed while the block before passes through its exponentials (1161 -> 1055 us, heads of 64 762 -> 653), what
+// Measured: 8192 + 5690 + 3190 tokens, 32 heads on 8 of 128 channels (898 GFLOP), 0.88 ms, 1023 TFLOP/s, bf16; heads of 64
+// 904, of 256 925; a window of 1024 802, not causal 1074; 23 prompts of up to 1869 tokens, 24 heads on 8 of 64, 676, fp16 632.
+// Heads of 128 are bound by power: the matrix units are busy for half of the cycles (0.53, vector instructions 0.45), whose clock
+// falls, under the profiler to 1.75 GHz (1.02 ms), and the same cycles take 0.79 ms at 2.2 GHz where all values are 0;
+// products alone, from registers, reach 1.7 PFLOP/s on such values. No exponentials at all would save 6% of the time, no
+// reads of K from LDS 5%, no copies of K and V into LDS 12%. Heads of 64, with twice the exponentials for a product, by
+// vector instructions and products together: 0.63 and 0.37 of the busy cycles, and a SIMD passes little of one beside the
+// other (16 products of a wave take 527 cycles, 128 fma of another 571, both 723).
+// Steps, all under the profiler. First version 774 TFLOP/s: S, exponentials and products one after another, 8 waves a workgroup
+// (two workgroups of 4 waves on a CU do not wait for each other: 23 prompts of up to 1999 tokens, heads of 64, 281 -> 234 us).
+// Other steps: blocks of 32 keys whose S is computed while the block before passes through its exponentials (1161 -> 1055 us, heads of 64 762 -> 653), what
 // is not finite dealt with before the products and not beside them, whose outputs then stay in their registers (-> 1016, 193
 // us). Tried: tiles of 32 keys for all (three waves per SIMD spill, two are no faster, heads of 64 slower: 660 TFLOP/s); 64
 // columns a wave (heads of 64 the same; of 128 take the registers of a SIMD, and half the time goes into moving them).
