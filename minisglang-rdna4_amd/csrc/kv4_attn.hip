@@ -653,11 +653,11 @@ Kv4Plan kv4_plan(int64_t T, int B, int H, int G, int D, int64_t max_q, int64_t m
 
 // A tree's. More than 64 columns, without a window and with a context that is worth its tables, go to kv4_tree_attn_kernel: a
 // workgroup of 8 waves per CU, or two of 4 for up to 128 columns; one round of the card, or two splits where the sequences
-// fill less than that. us, there / in kv4_attn_kernel (8 heads of 4 queries, 128 channels, bf16), 64 and 72 columns: 32 users on 4000
-// 107 / 97 and 115 / 136, 8 on 16000 103 / 93 and 110 / 122, 8 on 512 22 / 18 and 23 / 22, 8 on 300 19 / 16 and 20 / 20. One user
-// breaks even at 16000 only: 72 columns on 512 20 / 16, on 4000 26 / 24, on 16000 39 / 39. The others are kv4_attn_kernel's, and more than 16 columns of few sequences get splits for all of the
-// CUs, of at least 4 tiles: the join is cheap then. us, with it / as above: 13 tokens of 4 heads a group on 2000 16.1 /
-// 17.9, on 30000 46 / 74.
+// fill less than that. us, there / in kv4_attn_kernel (8 heads of 4 queries, 128 channels, bf16), 64 and 72 columns: 32 users on
+// 4000 107 / 97 and 115 / 136, 8 on 16000 103 / 93 and 110 / 122, 8 on 512 22 / 18 and 23 / 22, 8 on 300 19 / 16 and 20 / 20. One
+// user breaks even at 16000 only: 72 columns on 512 20 / 16, on 4000 26 / 24, on 16000 39 / 39. The others are
+// kv4_attn_kernel's, and more than 16 columns of few sequences get splits for all of the CUs, of at least 4 tiles: the join is
+// cheap then. us, with it / as above: 13 tokens of 4 heads a group on 2000 16.1 / 17.9, on 30000 46 / 74.
 Kv4Plan kv4_tree_plan(int64_t T, int B, int H, int G, int D, int64_t window, int64_t max_q, int64_t max_kv) {
   Kv4Plan pl = kv4_plan(T, B, H, G, D, max_q, max_kv);
   if (max_q < (T + B - 1) / B) max_q = (T + B - 1) / B;

@@ -324,8 +324,8 @@ static int read(const Kv4Cache& c, const Kv4Batch& s, uint16_t* k, uint16_t* v, 
   if (wgs > kMaxGrid) return kErrUnsupported;
   const dim3 g((unsigned)wgs), b(256);
   if (few) hipLaunchKernelGGL((kv4_read_kernel<D, DT, VP, false>), g, b, 0, st, c, s, per, k, v);
-  // us, past / through the caches, and with a kernel behind it that reads and writes the rows: 64 MB of rows 15 / 16, 40 / 38; 128 MB 28
-  // / 39, 82 / 75; 256 MB 80 / 73, 151 / 138; 328 MB 95 / 98, 192 / 194; 421 MB 120 / 125, 247 / 265
+  // us, past / through the caches, and with a kernel behind it that reads and writes the rows: 64 MB of rows 15 / 16, 40 / 38;
+  // 128 MB 28 / 39, 82 / 75; 256 MB 80 / 73, 151 / 138; 328 MB 95 / 98, 192 / 194; 421 MB 120 / 125, 247 / 265
   else if (s.T * c.H * D * 4 > 320 << 20) hipLaunchKernelGGL((kv4_read_kernel<D, DT, 8, true>), g, b, 0, st, c, s, per, k, v);
   else hipLaunchKernelGGL((kv4_read_kernel<D, DT, 8, false>), g, b, 0, st, c, s, per, k, v);
   return hipPeekAtLastError() == hipSuccess ? kOk : kErrHip;

@@ -53,8 +53,8 @@ int launch_kv4_copy(const Kv4Caches& cs, int caches, const int32_t* src, const i
   const int64_t parts = (codes + kCopyPart - 1) / kCopyPart, all = 2 * parts + (2 * scales + kCopyPart - 1) / kCopyPart;
   if (n > kMaxGrid || all > 65535) return kErrUnsupported;
   const dim3 g((unsigned)n, (unsigned)all, (unsigned)caches), b(256);
-  // us, bytes in and out, past / through the caches, and with kv4_read behind it: 34 MB 9 / 9, 29 / 24; 68 MB 13 / 16, 52 / 45; 136 MB
-  // 29 / 35, 112 / 108; 207 MB 50 / 51, 157 / 146; 238 MB 57 / 58, 179 / 177; 290 MB 68 / 69, 218 / 220; 373 MB 86 / 87, 274 / 293
+  // us, bytes in and out, past / through the caches, and with kv4_read behind it: 34 MB 9 / 9, 29 / 24; 68 MB 13 / 16, 52 / 45;
+  // 136 MB 29 / 35, 112 / 108; 207 MB 50 / 51, 157 / 146; 238 MB 57 / 58, 179 / 177; 290 MB 68 / 69, 218 / 220; 373 MB 86 / 87, 274 / 293
   if (n * caches * (codes + scales) * 64 > 256 << 20)
     hipLaunchKernelGGL((kv4_copy_kernel<true>), g, b, 0, st, cs, src, dst, (int)pages, (int)parts, (uint32_t)codes, (uint32_t)scales);
   else
